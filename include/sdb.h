@@ -96,6 +96,63 @@ int sdb_mul_mat_gated_supported(const sdb_tensor *w, const sdb_tensor *x, const 
 int sdb_mul_mat_gated(const sdb_tensor *w, const sdb_tensor *x, const sdb_tensor *out, const sdb_chain *chain,
                       void *stream);
 
+/* ---- 4-bit weights --------------------------------------------------------
+ * Extensions of the reference, whose quantized forms quantize an FP16 or FP32
+ * matrix as it is packed (mul_mat.cc:378-381): matrices that ARE 4 bits, as
+ * quantized checkpoints hold them, and linear layers of a few rows on them.
+ *
+ * A matrix of n rows of k numbers, each 4 bits q, with an FP16 scale d and,
+ * with `minimum`, an FP16 minimum m for every `group` (32, 64 or 128)
+ * consecutive numbers of a row (a row's last group may be short):
+ *     value = d (q - 8),      or with `minimum`  value = d q + m.
+ * data: sdb_q4_bytes(k, n, group, minimum) bytes of device memory on a 16-byte
+ * boundary, in a layout of the library's own.  The caller owns it; nothing of
+ * it is kept between calls, so sdb_forget has no part in it. */
+typedef struct sdb_q4 {
+    void *data;
+    int64_t k, n;
+    int32_t group;
+    int32_t minimum;
+} sdb_q4;
+/* 0 for a form that does not exist (k <= 2^24, n <= 2^30). */
+int64_t sdb_q4_bytes(int64_t k, int64_t n, int32_t group, int32_t minimum);
+/* Quantizes w, an FP32 or FP16 matrix [k, n] with contiguous rows, into q:
+ *   symmetric: s the group's number of greatest magnitude (the positive one of
+ *     two), d = f16(s / -8), q = clamp(floor(w / d + 8.5), 0, 15), 8 where d = 0;
+ *   minimum: d = f16((max - min) / 15), m = f16(min),
+ *     q = clamp(floor((w - m) / d + 0.5), 0, 15), 0 where d = 0;
+ * in FP32, each operation rounded; d and m saturate at FP16's range.  A group
+ * that holds an infinity or a NaN stands for NaN. */
+int sdb_q4_quantize(const sdb_tensor *w, const sdb_q4 *q, void *stream);
+/* From 4-bit numbers and their scales: codes [n][(k + 1) / 2] bytes, the even
+ * column in the low half; scales (and minima, else NULL) [n][ceil(k / group)]
+ * FP16, dense. */
+int sdb_q4_import(const void *codes, const void *scales, const void *minima, const sdb_q4 *q, void *stream);
+/* From ggml's blocks of 32 numbers, k a multiple of 32: GGML_TYPE_Q4_0 (no
+ * minimum) or GGML_TYPE_Q4_1 (minimum); rows row_bytes apart. */
+int sdb_q4_from_blocks(const void *blocks, int64_t row_bytes, const sdb_q4 *q, void *stream);
+/* The numbers q stands for into w, an FP32 matrix [k, n] with contiguous rows. */
+int sdb_q4_dequantize(const sdb_q4 *q, const sdb_tensor *w, void *stream);
+
+/* dst[m][n] = sum_k x[m][k] value[n][k], then the chain: sdb_mul_mat for 4-bit
+ * weights and few rows (for hundreds of rows, sdb_q4_dequantize once and
+ * sdb_mul_mat).  x [K, ...] and dst [N, ...] FP32 or FP16, each row contiguous,
+ * rows over dimensions 1..3 at any strides; x and dst do not overlap.  Products
+ * and sums are FP32 whatever the types (x to its last bit), dst rounded once.
+ * A chain's redirect needs an FP32 dst.  No rows: nothing is done.  No device
+ * memory is allocated and none is shared between calls. */
+int sdb_mul_mat_q4_supported(const sdb_q4 *w, const sdb_tensor *x, const sdb_tensor *dst);
+int sdb_mul_mat_q4(const sdb_q4 *w, const sdb_tensor *x, const sdb_tensor *dst, const sdb_chain *chain,
+                   void *stream);
+/* The gated linear layer: out[m][j] = a[m][j] act(b[m][j]), a = x W^T and
+ * b = x V^T (w and gate of one form), the chain applied to both -- its column
+ * coordinate j for a, N + j for b, as sdb_mul_mat_gated's halves -- and no
+ * redirect.  act: GELU (tanh) or SiLU. */
+enum { SDB_GATE_GELU = 0, SDB_GATE_SILU = 1 };
+int sdb_mul_mat_q4_gated_supported(const sdb_q4 *w, const sdb_q4 *gate, const sdb_tensor *x, const sdb_tensor *out);
+int sdb_mul_mat_q4_gated(const sdb_q4 *w, const sdb_q4 *gate, const sdb_tensor *x, const sdb_tensor *out, int32_t act,
+                         const sdb_chain *chain, void *stream);
+
 /* ---- convolutions: GGML_OP_CONV_2D (direct) ------------------------------
  * w [KW, KH, IC, OC] FP16 or FP32, x [W, H, IC, N] FP32, dst [OW, OH, OC, N]
  * FP32; params = {s0, s1, p0, p1, d0, d1} as ggml_conv_2d_direct's op_params.
@@ -180,6 +237,42 @@ int sdb_mul_mat_layer_normed(const sdb_tensor *w, const sdb_tensor *x, const sdb
                              const sdb_chain *norm_chain, const sdb_chain *chain, void *stream);
 int sdb_mul_mat_gated_layer_normed(const sdb_tensor *w, const sdb_tensor *x, const sdb_tensor *out, float eps,
                                    const sdb_chain *norm_chain, const sdb_chain *chain, void *stream);
+
+/* ---- the residual block of a transformer -----------------------------------
+ * An extension of the reference, which computes each of these as a node of its
+ * own: what stands between two blocks of a transformer, in one pass over rows
+ *     h   = keep x + scale gate post(y)
+ *     out = pre(h) (1 + mul) + add
+ * x the residual stream, y a block's output, post the norm after the block, pre
+ * the norm before the next; gate, mul and add modulations.  x may be NULL (no
+ * stream yet: 0) or y (no block yet: post and gate then none); h or out may be
+ * NULL (not wanted; without out no pre, mul, add).  Tensors of one extent
+ * [C, ...], FP32 or FP16, h of x's type and out of y's, rows contiguous at any
+ * strides.  h and out may be the very memory of x or y (same type and strides);
+ * they overlap nothing else.  Arithmetic in FP32, a row's statistics over the
+ * numbers themselves (out is made from h before h is rounded). */
+enum { SDB_NORM_NONE = 0, SDB_NORM_LAYER = 1, SDB_NORM_RMS = 2 };
+/* (v - mean) / sqrt(variance + eps), or v / sqrt(mean of v^2 + eps); then
+ * weight [C] and bias [C], each unless NULL. */
+typedef struct sdb_norm_form {
+    int32_t kind;
+    float eps;
+    const float *weight;
+    const float *bias;
+} sdb_norm_form;
+/* An FP32 operand addressed as a step's (sdb_step): strides in ELEMENTS, 0
+ * along a broadcast dimension; data NULL: none (gate 1, mul 0, add 0). */
+typedef struct sdb_operand {
+    const float *data;
+    int64_t nb[4];
+} sdb_operand;
+typedef struct sdb_residual {
+    float keep, scale;
+    sdb_norm_form post, pre;
+    sdb_operand gate, mul, add;
+} sdb_residual;
+int sdb_residual_norm(const sdb_tensor *x, const sdb_tensor *y, const sdb_tensor *h, const sdb_tensor *out,
+                      const sdb_residual *p, void *stream);
 
 /* ---- the graph's data-movement nodes (device-resident runner) -----------
  * The reference takes only CONV_2D, MUL_MAT, FLASH_ATTN_EXT, GROUP_NORM and

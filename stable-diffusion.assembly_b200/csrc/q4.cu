@@ -1,0 +1,308 @@
+// 4-bit matrices: made from FP16 / FP32 numbers, from 4-bit numbers and group
+// scales, or from ggml's Q4_0 / Q4_1 blocks, and turned back into FP32.
+//
+// All four are one pass over the matrix, a thread to a word of eight columns
+// (q4.cuh), bound by memory.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "../../include/sdb.h"
+#include "q4.cuh"
+#include "runtime.cuh"
+
+namespace sdb {
+
+namespace {
+
+// A thread's word: threads run along k, 16 words a k-block, over the padded matrix.
+struct WordAt {
+    long long row, k0;
+};
+
+__device__ __forceinline__ WordAt word_at(const Q4View& v, long long i) {
+    const long long per_row = static_cast<long long>(v.kblocks) * 16;
+    const long long row = i / per_row;
+    return {row, (i - row * per_row) * 8};
+}
+
+__host__ inline int word_blocks(const Q4View& v) {
+    const long long total = static_cast<long long>(v.tiles) * 16 * v.kblocks * 16;
+    return static_cast<int>(std::min<long long>((total + 255) / 256, 148LL * 32));
+}
+
+__device__ __forceinline__ float saturate_half(float v) { return fminf(fmaxf(v, -65504.0f), 65504.0f); }
+
+// Quantizes eight columns a thread; the extremes of a group come from the
+// group / 8 neighbouring lanes that hold it.  Every step is a rounded FP32
+// operation of its own (no contraction), so that the numbers chosen are those
+// of the formulas:
+//   symmetric  s = the group's number of greatest magnitude (max when both are equal),
+//              d = f16(s / -8), q = clamp(floor(w / d + 8.5), 0, 15), all 8 where d = 0
+//   minimum    d = f16((max - min) / 15), m = f16(min),
+//              q = clamp(floor((w - m) / d + 0.5), 0, 15), all 0 where d = 0
+// d and m saturate at FP16's range.  A group that holds an infinity or a NaN
+// stands for NaN throughout.
+template <typename T, bool MINIMUM>
+__global__ void __launch_bounds__(256) q4_quantize_kernel(const T* __restrict__ w, long long ld, Q4View v) {
+    const long long total = static_cast<long long>(v.tiles) * 16 * v.kblocks * 16;
+    const int lanes = v.group / 8;
+    // A row is a whole number of 16 threads' runs, so a group's lanes leave the loop together.
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+        const WordAt at = word_at(v, i);
+        float x[8];
+        float hi = -INFINITY, lo = INFINITY;
+        bool bad = false;
+        const bool row_in = at.row < v.n;
+        const T* src = w + at.row * ld + at.k0;
+        const bool whole = row_in && at.k0 + 8 <= v.k && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+        if (whole) {
+            if constexpr (sizeof(T) == 4) {
+                const float4 a = __ldg(reinterpret_cast<const float4*>(src));
+                const float4 b = __ldg(reinterpret_cast<const float4*>(src) + 1);
+                x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+                x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+            } else {
+                const uint4 a = __ldg(reinterpret_cast<const uint4*>(src));
+                const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[p]));
+                    x[2 * p] = f.x;
+                    x[2 * p + 1] = f.y;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                x[c] = row_in && at.k0 + c < v.k ? static_cast<float>(src[c]) : 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (row_in && at.k0 + c < v.k) {
+                hi = fmaxf(hi, x[c]);
+                lo = fminf(lo, x[c]);
+                bad |= !(fabsf(x[c]) < INFINITY);
+            }
+        }
+        // The group's own lanes: all of them are in this iteration.
+        const unsigned mask = ((1u << lanes) - 1u) << (threadIdx.x & 31 & ~(lanes - 1));
+        for (int o = 1; o < lanes; o <<= 1) {
+            hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
+            lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
+            bad |= __shfl_xor_sync(mask, static_cast<int>(bad), o) != 0;
+        }
+        const bool empty = hi < lo;  // a group of padding
+        __half dh = __float2half_rn(0.0f), mh = dh;
+        if (!empty) {
+            if (MINIMUM) {
+                dh = __float2half_rn(saturate_half(__fdiv_rn(__fsub_rn(hi, lo), 15.0f)));
+                mh = __float2half_rn(saturate_half(lo));
+            } else {
+                dh = __float2half_rn(saturate_half(__fdiv_rn(hi >= -lo ? hi : lo, -8.0f)));
+            }
+            if (bad) dh = __ushort_as_half(0x7fff);
+        }
+        const float d = __half2float(dh), m = __half2float(mh);
+        uint32_t word = 0;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            float q = MINIMUM ? 0.0f : 8.0f;
+            if (d != 0.0f) {
+                q = MINIMUM ? __fadd_rn(__fdiv_rn(__fsub_rn(x[c], m), d), 0.5f)
+                            : __fadd_rn(__fdiv_rn(x[c], d), 8.5f);
+                q = fminf(fmaxf(floorf(q), 0.0f), 15.0f);
+            }
+            word |= static_cast<uint32_t>(static_cast<int>(q)) << q4_bit(c);
+        }
+        reinterpret_cast<uint32_t*>(v.codes)[q4_word(v, at.row, at.k0)] = word;
+        if (at.k0 % v.group == 0) {
+            const long long s = q4_scale(v, at.row, at.k0);
+            v.scales[s] = dh;
+            if (MINIMUM) v.minima[s] = mh;
+        }
+    }
+}
+
+// 4-bit numbers two a byte (the even column low) and scales [n][groups].
+__global__ void __launch_bounds__(256) q4_import_kernel(const uint8_t* __restrict__ codes, long long code_row,
+                                                        const __half* __restrict__ scales,
+                                                        const __half* __restrict__ minima, long long groups,
+                                                        Q4View v) {
+    const long long total = static_cast<long long>(v.tiles) * 16 * v.kblocks * 16;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+        const WordAt at = word_at(v, i);
+        const bool row_in = at.row < v.n;
+        uint32_t word = 0;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            uint32_t q = minima ? 0 : 8;
+            if (row_in && at.k0 + c < v.k) {
+                const uint32_t b = __ldg(codes + at.row * code_row + (at.k0 + c) / 2);
+                q = (c & 1) ? b >> 4 : b & 15;
+            }
+            word |= q << q4_bit(c);
+        }
+        reinterpret_cast<uint32_t*>(v.codes)[q4_word(v, at.row, at.k0)] = word;
+        if (at.k0 % v.group == 0) {
+            const long long s = q4_scale(v, at.row, at.k0);
+            const bool in = row_in && at.k0 < v.k;
+            const long long from = at.row * groups + at.k0 / v.group;
+            v.scales[s] = in ? scales[from] : __float2half_rn(0.0f);
+            if (minima) v.minima[s] = in ? minima[from] : __float2half_rn(0.0f);
+        }
+    }
+}
+
+// ggml's blocks of 32 numbers: the FP16 scale, with Q4_1 the FP16 minimum,
+// then 16 bytes, byte i numbers i (low) and i + 16 (high).
+__global__ void __launch_bounds__(256) q4_blocks_kernel(const uint8_t* __restrict__ blocks, long long row_bytes,
+                                                        Q4View v) {
+    const int header = v.minima ? 4 : 2, size = header + 16;
+    const long long total = static_cast<long long>(v.tiles) * 16 * v.kblocks * 16;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+        const WordAt at = word_at(v, i);
+        const bool in = at.row < v.n && at.k0 < v.k;
+        const uint8_t* b = blocks + at.row * row_bytes + at.k0 / 32 * size;
+        const int first = static_cast<int>(at.k0) & 31;
+        uint32_t word = 0;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            uint32_t q = v.minima ? 0 : 8;
+            if (in) {
+                const uint32_t two = __ldg(b + header + (first & 15) + c);
+                q = first < 16 ? two & 15 : two >> 4;
+            }
+            word |= q << q4_bit(c);
+        }
+        reinterpret_cast<uint32_t*>(v.codes)[q4_word(v, at.row, at.k0)] = word;
+        if (first == 0) {
+            const long long s = q4_scale(v, at.row, at.k0);
+            uint32_t d = 0, m = 0;
+            if (in) {
+                d = b[0] | static_cast<uint32_t>(b[1]) << 8;
+                if (v.minima) m = b[2] | static_cast<uint32_t>(b[3]) << 8;
+            }
+            v.scales[s] = __ushort_as_half(static_cast<unsigned short>(d));
+            if (v.minima) v.minima[s] = __ushort_as_half(static_cast<unsigned short>(m));
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) q4_dequantize_kernel(Q4View v, float* __restrict__ w, long long ld) {
+    const long long total = v.n * v.kblocks * 16;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+        const WordAt at = word_at(v, i);
+        if (at.k0 >= v.k) continue;
+        const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(v.codes) + q4_word(v, at.row, at.k0));
+        const long long s = q4_scale(v, at.row, at.k0);
+        const float d = __half2float(v.scales[s]);
+        const float m = v.minima ? __half2float(v.minima[s]) : 0.0f;
+        float x[8];
+        // d q and d (q - 8) are exact in FP32 (11 and 4 bits).
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const float code = static_cast<float>(word >> q4_bit(c) & 15u);
+            x[c] = v.minima ? fmaf(d, code, m) : d * (code - 8.0f);
+        }
+        float* dst = w + at.row * ld + at.k0;
+        if (at.k0 + 8 <= v.k && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+            reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+            reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                if (at.k0 + c < v.k) dst[c] = x[c];
+        }
+    }
+}
+
+// A matrix [k, n] with contiguous rows of the 4-bit matrix's extents.
+bool matrix_of(const sdb_tensor* w, const sdb_q4* q, bool f16) {
+    if (w == nullptr || w->data == nullptr) return false;
+    if (w->type != SDB_TYPE_F32 && !(f16 && w->type == SDB_TYPE_F16)) return false;
+    const int64_t es = w->type == SDB_TYPE_F16 ? 2 : 4;
+    return w->ne[0] == q->k && w->ne[1] == q->n && w->ne[2] == 1 && w->ne[3] == 1 && (w->nb[0] == es || w->ne[0] == 1) &&
+           w->nb[1] % es == 0 && (w->ne[1] == 1 || w->nb[1] >= es * w->ne[0]) &&
+           reinterpret_cast<uintptr_t>(w->data) % es == 0;
+}
+
+}  // namespace
+
+}  // namespace sdb
+
+using namespace sdb;
+
+extern "C" {
+
+int64_t sdb_q4_bytes(int64_t k, int64_t n, int32_t group, int32_t minimum) {
+    if (!q4_valid_form(k, n, group, minimum)) return 0;
+    const int64_t blocks = (n + 15) / 16 * ((k + 127) / 128);
+    return blocks * (1024 + 32 * (128 / group) * (minimum ? 2 : 1));
+}
+
+int sdb_q4_quantize(const sdb_tensor* w, const sdb_q4* q, void* stream) {
+    if (!q4_valid(q)) return fail(SDB_INVALID, "sdb_q4_quantize: no such 4-bit matrix");
+    if (!matrix_of(w, q, true))
+        return fail(SDB_INVALID, "sdb_q4_quantize: w must be an FP32 or FP16 matrix [k, n] with contiguous rows");
+    const Q4View v = q4_view(q);
+    const auto st = static_cast<cudaStream_t>(stream);
+    const int blocks = word_blocks(v);
+    if (w->type == SDB_TYPE_F32) {
+        const auto* src = static_cast<const float*>(w->data);
+        if (v.minima) q4_quantize_kernel<float, true><<<blocks, 256, 0, st>>>(src, w->nb[1] / 4, v);
+        else q4_quantize_kernel<float, false><<<blocks, 256, 0, st>>>(src, w->nb[1] / 4, v);
+    } else {
+        const auto* src = static_cast<const __half*>(w->data);
+        if (v.minima) q4_quantize_kernel<__half, true><<<blocks, 256, 0, st>>>(src, w->nb[1] / 2, v);
+        else q4_quantize_kernel<__half, false><<<blocks, 256, 0, st>>>(src, w->nb[1] / 2, v);
+    }
+    count_launch();
+    SDB_CUDA(cudaGetLastError());
+    return SDB_OK;
+}
+
+int sdb_q4_import(const void* codes, const void* scales, const void* minima, const sdb_q4* q, void* stream) {
+    if (!q4_valid(q)) return fail(SDB_INVALID, "sdb_q4_import: no such 4-bit matrix");
+    if (codes == nullptr || scales == nullptr || (minima != nullptr) != (q->minimum != 0) ||
+        reinterpret_cast<uintptr_t>(scales) % 2 != 0 || reinterpret_cast<uintptr_t>(minima) % 2 != 0)
+        return fail(SDB_INVALID, "sdb_q4_import: codes, FP16 scales and (with `minimum`, only then) FP16 minima");
+    const Q4View v = q4_view(q);
+    q4_import_kernel<<<word_blocks(v), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const uint8_t*>(codes), (q->k + 1) / 2, static_cast<const __half*>(scales),
+        static_cast<const __half*>(minima), (q->k + q->group - 1) / q->group, v);
+    count_launch();
+    SDB_CUDA(cudaGetLastError());
+    return SDB_OK;
+}
+
+int sdb_q4_from_blocks(const void* blocks, int64_t row_bytes, const sdb_q4* q, void* stream) {
+    if (!q4_valid(q)) return fail(SDB_INVALID, "sdb_q4_from_blocks: no such 4-bit matrix");
+    if (q->group != 32 || q->k % 32 != 0)
+        return fail(SDB_INVALID, "sdb_q4_from_blocks: ggml's blocks are groups of 32, k a multiple of 32");
+    if (blocks == nullptr || row_bytes < q->k / 32 * (q->minimum ? 20 : 18))
+        return fail(SDB_INVALID, "sdb_q4_from_blocks: no blocks, or rows shorter than k / 32 blocks");
+    const Q4View v = q4_view(q);
+    q4_blocks_kernel<<<word_blocks(v), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const uint8_t*>(blocks), row_bytes, v);
+    count_launch();
+    SDB_CUDA(cudaGetLastError());
+    return SDB_OK;
+}
+
+int sdb_q4_dequantize(const sdb_q4* q, const sdb_tensor* w, void* stream) {
+    if (!q4_valid(q)) return fail(SDB_INVALID, "sdb_q4_dequantize: no such 4-bit matrix");
+    if (!matrix_of(w, q, false))
+        return fail(SDB_INVALID, "sdb_q4_dequantize: w must be an FP32 matrix [k, n] with contiguous rows");
+    const Q4View v = q4_view(q);
+    const long long total = v.n * v.kblocks * 16;
+    const int blocks_n = static_cast<int>(std::min<long long>((total + 255) / 256, 148LL * 32));
+    q4_dequantize_kernel<<<blocks_n, 256, 0, static_cast<cudaStream_t>(stream)>>>(v, static_cast<float*>(w->data),
+                                                                                w->nb[1] / 4);
+    count_launch();
+    SDB_CUDA(cudaGetLastError());
+    return SDB_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,86 @@
+// 4-bit matrices with group scales: the layout that mul_mat_q4 reads.
+//
+// A matrix of n rows of k numbers is held in tiles of 16 rows x 128 columns
+// (rows and columns padded; padding stands for 0), the tiles of 16 rows one
+// after another and each in order of k:
+//   codes   [row tile][k-block][half 2][lane 32][4 words]: lane g * 4 + t of half h
+//           holds row 8 h + g; its word j the eight columns 32 j + 8 t + 0..7,
+//           columns 2 p and 2 p + 1 in bits 4 p and 4 p + 16.  A warp reads a
+//           half tile as one 512-byte run of 16 bytes a lane, and a word's
+//           nibble pairs are the operands of mma.m16n8k16 (rows g and g + 8 of
+//           lane (g, t)) when the columns of x are taken in the same order: a
+//           sum over k may take its terms in any order.
+//   scales  [row tile][k-block][g 8][half 2][128 / group] FP16: what lane (g, t)
+//           needs of a tile is one run of 16, 8 or 4 bytes.
+//   minima  as the scales, present with `minimum`.
+// value = scale (code - 8), or scale code + minimum.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/sdb.h"
+
+namespace sdb {
+
+struct Q4View {
+    uint8_t* codes;
+    __half* scales;
+    __half* minima;   // null: symmetric
+    long long n, k;
+    int tiles;        // of 16 rows
+    int kblocks;      // of 128 columns
+    int group;
+    int ng;           // groups of a k-block: 128 / group
+};
+
+constexpr long long kQ4MaxK = 1LL << 24;
+constexpr long long kQ4MaxN = 1LL << 30;
+
+inline bool q4_valid_form(int64_t k, int64_t n, int32_t group, int32_t minimum) {
+    return k >= 1 && n >= 1 && k <= kQ4MaxK && n <= kQ4MaxN && (group == 32 || group == 64 || group == 128) &&
+           (minimum == 0 || minimum == 1);
+}
+
+// Whether q describes a matrix with memory behind it.
+inline bool q4_valid(const sdb_q4* q) {
+    return q != nullptr && q->data != nullptr && (reinterpret_cast<uintptr_t>(q->data) & 15) == 0 &&
+           q4_valid_form(q->k, q->n, q->group, q->minimum);
+}
+
+inline Q4View q4_view(const sdb_q4* q) {
+    Q4View v{};
+    v.n = q->n;
+    v.k = q->k;
+    v.group = q->group;
+    v.ng = 128 / q->group;
+    v.tiles = static_cast<int>((q->n + 15) / 16);
+    v.kblocks = static_cast<int>((q->k + 127) / 128);
+    const long long blocks = static_cast<long long>(v.tiles) * v.kblocks;
+    v.codes = static_cast<uint8_t*>(q->data);
+    v.scales = reinterpret_cast<__half*>(v.codes + blocks * 1024);
+    v.minima = q->minimum ? v.scales + blocks * 16 * v.ng : nullptr;
+    return v;
+}
+
+// The word of row r's columns k0..k0 + 7 (k0 a multiple of 8), as an index of 32-bit words.
+__host__ __device__ inline long long q4_word(const Q4View& v, long long r, long long k0) {
+    const long long block = (r >> 4) * v.kblocks + (k0 >> 7);
+    const int h = static_cast<int>(r >> 3) & 1, g = static_cast<int>(r) & 7;
+    const int j = static_cast<int>(k0 >> 5) & 3, t = static_cast<int>(k0 >> 3) & 3;
+    return ((block * 2 + h) * 32 + g * 4 + t) * 4 + j;
+}
+
+// The scale (and minimum) of row r's column k.
+__host__ __device__ inline long long q4_scale(const Q4View& v, long long r, long long k) {
+    const long long block = (r >> 4) * v.kblocks + (k >> 7);
+    const int h = static_cast<int>(r >> 3) & 1, g = static_cast<int>(r) & 7;
+    return ((block * 8 + g) * 2 + h) * v.ng + static_cast<int>(k & 127) / v.group;
+}
+
+// The bit of column i (0..7) of a word.
+__host__ __device__ constexpr int q4_bit(int i) { return (i >> 1) * 4 + (i & 1) * 16; }
+
+}  // namespace sdb

@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import weakref
 from pathlib import Path
 from typing import Iterable, Sequence
@@ -42,6 +43,9 @@ EXPORTS = [
     "sdb_concat", "sdb_upscale_nearest", "sdb_timestep_embedding", "sdb_euler_cfg_step", "sdb_soft_max",
     "sdb_coarser_tokens", "sdb_euler_ancestral_cfg_step", "sdb_group_norm_stats", "sdb_conv2d_normed",
     "sdb_mul_mat_normed", "sdb_mul_mat_layer_normed", "sdb_mul_mat_gated_layer_normed",
+    "sdb_q4_bytes", "sdb_q4_quantize", "sdb_q4_import", "sdb_q4_from_blocks", "sdb_q4_dequantize",
+    "sdb_mul_mat_q4_supported", "sdb_mul_mat_q4", "sdb_mul_mat_q4_gated_supported", "sdb_mul_mat_q4_gated",
+    "sdb_residual_norm",
 ]
 
 
@@ -118,6 +122,17 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
         "sdb_mul_mat_normed": (i, [T, T, T, ctypes.POINTER(NormIn), C, vp]),
         "sdb_mul_mat_layer_normed": (i, [T, T, T, ctypes.c_float, C, C, vp]),
         "sdb_mul_mat_gated_layer_normed": (i, [T, T, T, ctypes.c_float, C, C, vp]),
+        # The structs of these come packed as bytes (_packed, Q4.struct, ...), passed by address.
+        "sdb_q4_bytes": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]),
+        "sdb_q4_quantize": (i, [vp, vp, vp]),
+        "sdb_q4_import": (i, [vp, vp, vp, vp, vp]),
+        "sdb_q4_from_blocks": (i, [vp, ctypes.c_int64, vp, vp]),
+        "sdb_q4_dequantize": (i, [vp, vp, vp]),
+        "sdb_mul_mat_q4_supported": (i, [vp, vp, vp]),
+        "sdb_mul_mat_q4": (i, [vp, vp, vp, vp, vp]),
+        "sdb_mul_mat_q4_gated_supported": (i, [vp, vp, vp, vp]),
+        "sdb_mul_mat_q4_gated": (i, [vp, vp, vp, vp, ctypes.c_int32, vp, vp]),
+        "sdb_residual_norm": (i, [vp, vp, vp, vp, vp, vp]),
         "sdb_euler_cfg_step": (i, [vp, vp, vp, ctypes.c_int64, ctypes.c_float, ctypes.c_float, ctypes.c_float,
                                    ctypes.c_float, vp]),
         "sdb_euler_ancestral_cfg_step": (i, [vp, vp, vp, vp, ctypes.c_int64, ctypes.c_float, ctypes.c_float,
@@ -649,3 +664,287 @@ def euler_cfg_step(eps, x, x_in, cfg: float, sigma: float, sigma_next: float, c_
                                   ctypes.c_int64(x.numel()), ctypes.c_float(cfg), ctypes.c_float(sigma),
                                   ctypes.c_float(sigma_next), ctypes.c_float(c_in_next),
                                   ctypes.c_void_p(_stream_ptr(stream))))
+
+
+# ---------------------------------------------------------------- 4-bit weights
+
+# A call of a few microseconds should not wait for its description: the structs of the operators below are
+# packed into bytes in one step each, and the bytes' address is passed.
+_TENSOR = struct.Struct("=i4x4q4qQ")
+_STEP = struct.Struct("=i4xQ4q")
+_CHAIN_TAIL = struct.Struct("=Qi4x")
+_Q4 = struct.Struct("=Q2q2i")
+_NORM_FORM = struct.Struct("=ifQQ")
+_OPERAND = struct.Struct("=Q4q")
+_KEEP_SCALE = struct.Struct("=2f")
+_NO_STEP = _STEP.pack(0, 0, 0, 0, 0, 0)
+_NO_OPERAND = _OPERAND.pack(0, 0, 0, 0, 0)
+
+GATES = {"gelu": 0, "silu": 1}
+NORMS = {"none": 0, "layer": 1, "rms": 2}
+
+
+def _packed(t, what: str) -> bytes:
+    """The sdb_tensor of an FP32 or FP16 CUDA tensor of at most four dimensions, as bytes."""
+    shape, stride = t.shape, t.stride()
+    dtype = str(t.dtype)
+    if dtype == "torch.float32":
+        ty, es = TYPE_F32, 4
+    elif dtype == "torch.float16":
+        ty, es = TYPE_F16, 2
+    else:
+        raise SdbError(INVALID, f"{what}: unsupported dtype {t.dtype}")
+    nd = len(shape)
+    if nd == 2:
+        n0, n1, s0, s1 = shape[1], shape[0], stride[1] * es, stride[0] * es
+        return _TENSOR.pack(ty, n0, n1, 1, 1, s0, s1, s1 * n1, s1 * n1, t.data_ptr())
+    if nd == 0 or nd > 4:
+        raise SdbError(INVALID, f"{what}: one to four dimensions")
+    ne = [shape[nd - 1 - d] if d < nd else 1 for d in range(4)]
+    nb = [stride[nd - 1 - d] * es if d < nd else 0 for d in range(4)]
+    return _TENSOR.pack(ty, *ne, *nb, t.data_ptr())
+
+
+def _packed_chain(chain: Chain | None, out, cols: int):
+    """The sdb_chain of an operation on out's rows, `cols` columns each, as bytes (None: no chain).  Operands
+    that do not reach over the rows are refused: the kernel would read past them."""
+    if chain is None:
+        return None
+    steps = chain.steps
+    if len(steps) > MAX_STEPS:
+        raise SdbError(INVALID, "chain longer than 6 steps")
+    shape = out.shape
+    parts = [struct.pack("=i4x", len(steps))]
+    for kind, t, nb in steps:
+        if t is None:
+            parts.append(_STEP.pack(kind, 0, *nb))
+            continue
+        if min(nb) < 0:
+            raise SdbError(INVALID, "a chain operand's strides are not negative")
+        last = (cols - 1) * nb[0]
+        for d in range(1, len(shape)):
+            last += (shape[-1 - d] - 1) * nb[d]
+        if last >= t.numel() and (out.numel() and
+                                  last >= t.untyped_storage().nbytes() // 4 - t.storage_offset()):
+            raise SdbError(INVALID, "a chain operand ends before the output's rows")
+        parts.append(_STEP.pack(kind, t.data_ptr(), *nb))
+    parts.extend([_NO_STEP] * (MAX_STEPS - len(steps)))
+    r = chain.redirect_tensor
+    if r is not None and (r.dtype != out.dtype or r.shape != shape or r.stride() != out.stride()):
+        raise SdbError(INVALID, "a chain's redirect has the output's type, extents and strides")
+    parts.append(_CHAIN_TAIL.pack(r.data_ptr() if r is not None else 0, 1 if chain.from_redirect else 0))
+    return b"".join(parts)
+
+
+def _chain_tensors(chain: Chain | None) -> list:
+    if chain is None:
+        return []
+    found = [t for _, t, _ in chain.steps if t is not None]
+    return found + [chain.redirect_tensor] if chain.redirect_tensor is not None else found
+
+
+def _on(fn, what: str, tensors, stream, *args) -> None:
+    """Calls fn(*args, stream) with the tensors' device current, on `stream` or that device's current stream."""
+    import torch
+
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index or index < 0:
+            raise SdbError(INVALID, f"{what}: the tensors are not on one CUDA device")
+    if stream is not None and stream.device.index != index:
+        raise SdbError(INVALID, f"{what}: the stream is another device's")
+    if torch.cuda.current_device() == index:
+        s = stream if stream is not None else torch.cuda.current_stream()
+        status = fn(*args, s.cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            s = stream if stream is not None else torch.cuda.current_stream()
+            status = fn(*args, s.cuda_stream)
+    if status != OK:
+        _check(status)
+
+
+class Q4:
+    """A matrix (n, k) of 4-bit numbers with group scales on the device (sdb_q4): value = d (q - 8), or with
+    `minimum` d q + m, an FP16 d (and m) for every `group` numbers of a row.  Made by q4_quantize, q4_import or
+    q4_from_blocks; read by mul_mat_q4 and mul_mat_q4_gated."""
+
+    def __init__(self, n: int, k: int, group: int = 32, minimum: bool = False, device=None):
+        import torch
+
+        size = load().sdb_q4_bytes(k, n, group, 1 if minimum else 0)
+        if size <= 0:
+            raise SdbError(INVALID, f"no 4-bit matrix of {n} x {k} in groups of {group}")
+        self.n, self.k, self.group, self.minimum = n, k, group, bool(minimum)
+        self.data = torch.empty(size, dtype=torch.uint8, device="cuda" if device is None else device)
+        if not self.data.is_cuda:
+            raise SdbError(INVALID, "4-bit matrices are on a CUDA device")
+        self.struct = _Q4.pack(self.data.data_ptr(), k, n, group, 1 if minimum else 0)
+
+    def values(self, out=None, stream=None):
+        """The numbers the matrix stands for, FP32 (n, k) (sdb_q4_dequantize)."""
+        import torch
+
+        if out is None:
+            out = torch.empty(self.n, self.k, dtype=torch.float32, device=self.data.device)
+        _on(load().sdb_q4_dequantize, "Q4.values", (self.data, out), stream, self.struct, _packed(out, "Q4.values"))
+        return out
+
+
+def q4_quantize(w, group: int = 32, minimum: bool = False, stream=None) -> Q4:
+    """w (n, k) FP32 or FP16, rows contiguous, quantized to 4 bits (sdb_q4_quantize)."""
+    if w.dim() != 2:
+        raise SdbError(INVALID, "q4_quantize: a matrix (n, k)")
+    q = Q4(w.shape[0], w.shape[1], group, minimum, w.device)
+    _on(load().sdb_q4_quantize, "q4_quantize", (w, q.data), stream, _packed(w, "q4_quantize"), q.struct)
+    return q
+
+
+def q4_import(codes, scales, minima=None, k: int | None = None, group: int = 32, stream=None) -> Q4:
+    """From 4-bit numbers: codes (n, (k + 1) // 2) uint8, the even column in a byte's low half; scales and minima
+    (n, ceil(k / group)) FP16; k twice the bytes of a row unless given (sdb_q4_import)."""
+    import torch
+
+    k = 2 * codes.shape[-1] if k is None else k
+    n, groups = codes.shape[0], -(-k // group) if group else 0
+    q = Q4(n, k, group, minima is not None, codes.device)
+    if codes.dtype != torch.uint8 or codes.shape != (n, (k + 1) // 2) or not codes.is_contiguous():
+        raise SdbError(INVALID, "q4_import: codes must be dense uint8 (n, (k + 1) // 2)")
+    tensors = [codes, scales, q.data] + ([minima] if minima is not None else [])
+    for t in (scales, minima):
+        if t is not None and (t.dtype != torch.float16 or t.shape != (n, groups) or not t.is_contiguous()):
+            raise SdbError(INVALID, "q4_import: scales and minima must be dense FP16 (n, ceil(k / group))")
+    _on(load().sdb_q4_import, "q4_import", tensors, stream, codes.data_ptr(), scales.data_ptr(),
+        minima.data_ptr() if minima is not None else None, q.struct)
+    return q
+
+
+def q4_from_blocks(blocks, k: int, minimum: bool = False, stream=None) -> Q4:
+    """From ggml's blocks: blocks (n, bytes of a row) uint8, GGML_TYPE_Q4_0 or with `minimum` GGML_TYPE_Q4_1
+    (sdb_q4_from_blocks)."""
+    import torch
+
+    if blocks.dtype != torch.uint8 or blocks.dim() != 2 or blocks.stride(1) != 1:
+        raise SdbError(INVALID, "q4_from_blocks: blocks must be uint8 (n, bytes of a row)")
+    if k % 32 != 0 or blocks.shape[1] < k // 32 * (20 if minimum else 18):
+        raise SdbError(INVALID, "q4_from_blocks: rows are k / 32 whole blocks")
+    q = Q4(blocks.shape[0], k, 32, minimum, blocks.device)
+    _on(load().sdb_q4_from_blocks, "q4_from_blocks", (blocks, q.data), stream, blocks.data_ptr(), blocks.stride(0),
+        q.struct)
+    return q
+
+
+def mul_mat_q4(w: Q4, x, out=None, chain: Chain | None = None, stream=None):
+    """dst[m][n] = sum_k x[m][k] value[n][k], then the chain: w a Q4 (N, K), x (..., K) FP32 or FP16 -> (..., N)
+    of out's type (x's unless out is given).  For a few rows of x."""
+    import torch
+
+    if out is None:
+        out = torch.empty(*x.shape[:-1], w.n, dtype=x.dtype, device=x.device)
+    tensors = [w.data, x, out]
+    if chain is not None:
+        tensors += _chain_tensors(chain)
+    _on(load().sdb_mul_mat_q4, "mul_mat_q4", tensors, stream, w.struct, _packed(x, "mul_mat_q4"),
+        _packed(out, "mul_mat_q4"), _packed_chain(chain, out, w.n))
+    return out
+
+
+def mul_mat_q4_gated(w: Q4, gate: Q4, x, act: str = "gelu", out=None, chain: Chain | None = None, stream=None):
+    """(x W^T) act(x V^T) of two Q4 (N, K), the chain applied to both products as to columns 0..N - 1 and
+    N..2N - 1 of one; act "gelu" or "silu"."""
+    import torch
+
+    if act not in GATES:
+        raise SdbError(INVALID, f"mul_mat_q4_gated: no gate {act!r}")
+    if out is None:
+        out = torch.empty(*x.shape[:-1], w.n, dtype=x.dtype, device=x.device)
+    tensors = [w.data, gate.data, x, out]
+    if chain is not None:
+        tensors += _chain_tensors(chain)
+    _on(load().sdb_mul_mat_q4_gated, "mul_mat_q4_gated", tensors, stream, w.struct, gate.struct,
+        _packed(x, "mul_mat_q4_gated"), _packed(out, "mul_mat_q4_gated"), GATES[act],
+        _packed_chain(chain, out, 2 * w.n))
+    return out
+
+
+# ---------------------------------------------------------------- the residual block
+
+class Norm:
+    """A row's norm (sdb_norm_form): "layer" or "rms", eps, and weight and bias (C,) FP32 or None."""
+
+    def __init__(self, kind: str, eps: float = 1e-5, weight=None, bias=None):
+        if kind not in NORMS:
+            raise SdbError(INVALID, f"no norm {kind!r}")
+        self.kind, self.eps, self.weight, self.bias = kind, eps, weight, bias
+        self.tensors = [t for t in (weight, bias) if t is not None]
+        for t in self.tensors:
+            if str(t.dtype) != "torch.float32" or t.dim() != 1 or not t.is_contiguous():
+                raise SdbError(INVALID, "a norm's weight and bias are dense FP32 (C,)")
+
+    def packed(self, c: int) -> bytes:
+        for t in self.tensors:
+            if t.shape[0] != c:
+                raise SdbError(INVALID, f"a norm of {t.shape[0]} numbers for rows of {c}")
+        return _NORM_FORM.pack(NORMS[self.kind], self.eps,
+                               self.weight.data_ptr() if self.weight is not None else 0,
+                               self.bias.data_ptr() if self.bias is not None else 0)
+
+
+_NO_NORM = _NORM_FORM.pack(0, 0.0, 0, 0)
+
+
+def _packed_operand(t, shape) -> bytes:
+    """An FP32 tensor broadcastable to `shape`, as the bytes of an sdb_operand."""
+    if t is None:
+        return _NO_OPERAND
+    if str(t.dtype) != "torch.float32":
+        raise SdbError(INVALID, "modulations are FP32")
+    nd, od = len(shape), t.dim()
+    if od > nd:
+        raise SdbError(INVALID, "a modulation has more dimensions than the rows")
+    nb = [0, 0, 0, 0]
+    ts, st = t.shape, t.stride()
+    for d in range(od):
+        e = ts[od - 1 - d]
+        if e != 1:
+            if e != shape[nd - 1 - d]:
+                raise SdbError(INVALID, f"a modulation of {tuple(ts)} for rows of {tuple(shape)}")
+            nb[d] = st[od - 1 - d]
+    return _OPERAND.pack(t.data_ptr(), *nb)
+
+
+def residual_norm(x, y, post: Norm | None = None, gate=None, keep: float = 1.0, scale: float = 1.0,
+                  pre: Norm | None = None, mul=None, add=None, h=None, out=None, want_h: bool = True,
+                  want_out: bool = True, stream=None):
+    """h = keep x + scale gate post(y); out = pre(h) (1 + mul) + add.  Returns (h, out).
+
+    x, y (..., C) FP32 or FP16, up to four dimensions, either None; gate, mul and add FP32, broadcastable to
+    them.  h is of x's type, out of y's (of the other's where one is None); h may be x, out may be y (the
+    update in place).  want_h / want_out False: that one is not made (None).
+    """
+    import torch
+
+    ref = x if x is not None else y
+    if ref is None:
+        raise SdbError(INVALID, "residual_norm: neither x nor y")
+    shape = ref.shape
+    if want_h and h is None:
+        h = torch.empty(shape, dtype=ref.dtype, device=ref.device)
+    if want_out and out is None:
+        out = torch.empty(shape, dtype=(y if y is not None else x).dtype, device=ref.device)
+    if not want_h:
+        h = None
+    if not want_out:
+        out = None
+    tensors = [t for t in (ref, y, h, out, gate, mul, add) if t is not None]
+    if post is not None:
+        tensors += post.tensors
+    if pre is not None:
+        tensors += pre.tensors
+    c = shape[-1] if len(shape) else 0
+    params = b"".join((_KEEP_SCALE.pack(keep, scale),
+                       _NO_NORM if post is None else post.packed(c), _NO_NORM if pre is None else pre.packed(c),
+                       _packed_operand(gate, shape), _packed_operand(mul, shape), _packed_operand(add, shape)))
+    _on(load().sdb_residual_norm, "residual_norm", tensors, stream,
+        *(None if t is None else _packed(t, "residual_norm") for t in (x, y, h, out)), params)
+    return h, out

@@ -1,0 +1,435 @@
+"""4-bit matrices and their linear layers against float64.
+
+The matrices: made numbers and scales have to be those of the formulas (restated
+here in numpy, FP32 operation by FP32 operation), bit for bit.  The products:
+sum_k x value in float64 from the numbers the matrix stands for, held to the
+linear layers' bound, oracle.K_B200 of the summed magnitudes.  The kernel takes
+x exactly (its parts sum to it) and every product exactly, so its error is that
+of FP32 sums: a running sum of s terms errs by at most s 2^-23 of the
+magnitudes with sums cut instead of rounded, s at most 8 steps of 16 products
+and three parts in a group of 128, plus the groups joined -- under 1e-6 for the
+random signs of real rows (an error of sqrt(s) steps), for which the bound was
+set.  An FP16 output adds its rounding, 2^-11 of the value (2^-25 below FP16's
+normal numbers).
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import oracle
+from helpers import cuda_tensor, host, rng
+
+pytestmark = pytest.mark.gpu
+
+GROUPS = (32, 64, 128)
+
+
+def made(g, n, k, group, minimum):
+    """4-bit numbers, FP16 scales and minima at random, and the numbers they stand for (float64)."""
+    groups = -(-k // group)
+    q = g.integers(0, 16, (n, k)).astype(np.uint8)
+    scales = ((g.random((n, groups)) + 0.25) * 0.05 * g.choice([-1.0, 1.0], (n, groups))).astype(np.float16)
+    minima = g.standard_normal((n, groups)).astype(np.float16) if minimum else None
+    d = np.repeat(scales.astype(np.float64), group, axis=1)[:, :k]
+    if minimum:
+        values = d * q + np.repeat(minima.astype(np.float64), group, axis=1)[:, :k]
+    else:
+        values = d * (q.astype(np.float64) - 8)
+    return q, scales, minima, values
+
+
+def codes_of(q):
+    n, k = q.shape
+    padded = np.zeros((n, (k + 1) // 2 * 2), dtype=np.uint8)
+    padded[:, :k] = q
+    return padded[:, 0::2] | padded[:, 1::2] << 4
+
+
+def on_device(cuda, q, scales, minima, group):
+    import sdb
+
+    return sdb.q4_import(cuda_tensor(codes_of(q), cuda), cuda_tensor(scales, cuda),
+                         cuda_tensor(minima, cuda) if minima is not None else None, k=q.shape[1], group=group)
+
+
+def quantized(w, group, minimum):
+    """The formulas of sdb_q4_quantize in numpy: FP32 values."""
+    n, k = w.shape
+    w = w.astype(np.float32)
+    out = np.empty((n, k), dtype=np.float32)
+    sat = lambda v: np.clip(v, np.float32(-65504), np.float32(65504)).astype(np.float16).astype(np.float32)
+    for at in range(0, k, group):
+        x = w[:, at:at + group]
+        hi, lo = x.max(axis=1, keepdims=True), x.min(axis=1, keepdims=True)
+        with np.errstate(divide="ignore", invalid="ignore"):
+            if minimum:
+                d, m = sat((hi - lo) / np.float32(15)), sat(lo)
+                q = np.where(d == 0, np.float32(0), np.clip(np.floor((x - m) / d + np.float32(0.5)), 0, 15))
+                out[:, at:at + group] = d * q + m
+            else:
+                d = sat(np.where(hi >= -lo, hi, lo) / np.float32(-8))
+                q = np.where(d == 0, np.float32(8), np.clip(np.floor(x / d + np.float32(8.5)), 0, 15))
+                out[:, at:at + group] = d * (q - np.float32(8))
+    return out
+
+
+# ---------------------------------------------------------------- the matrices
+
+@pytest.mark.parametrize("minimum", [False, True])
+@pytest.mark.parametrize("n,k,group", [(1, 1, 32), (3, 31, 32), (17, 33, 32), (16, 128, 64), (5, 200, 64),
+                                       (40, 640, 128), (33, 1001, 128), (2, 4096, 32)])
+def test_import_stands_for_its_numbers(cuda, n, k, group, minimum):
+    q, scales, minima, values = made(rng(n * k), n, k, group, minimum)
+    got = host(on_device(cuda, q, scales, minima, group).values())
+    np.testing.assert_array_equal(got, values.astype(np.float32))
+
+
+@pytest.mark.parametrize("minimum", [False, True])
+@pytest.mark.parametrize("n,k", [(1, 32), (18, 96), (7, 320), (16, 128)])
+def test_ggml_blocks(cuda, n, k, minimum):
+    """Q4_0 and Q4_1 blocks, rows further apart than their blocks."""
+    import sdb
+
+    q, scales, minima, values = made(rng(n + k), n, k, 32, minimum)
+    size = 20 if minimum else 18
+    rows = np.full((n, k // 32 * size + 6), 0xA5, dtype=np.uint8)
+    for b in range(k // 32):
+        at = b * size
+        rows[:, at:at + 2] = scales[:, b:b + 1].view(np.uint8)
+        if minimum:
+            rows[:, at + 2:at + 4] = minima[:, b:b + 1].view(np.uint8)
+        nib = q[:, b * 32:b * 32 + 32]
+        rows[:, at + size - 16:at + size] = nib[:, :16] | nib[:, 16:] << 4
+    got = host(sdb.q4_from_blocks(cuda_tensor(rows, cuda), k, minimum).values())
+    np.testing.assert_array_equal(got, values.astype(np.float32))
+
+
+@pytest.mark.parametrize("minimum", [False, True])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("n,k,group", [(1, 1, 32), (9, 37, 32), (16, 256, 128), (31, 129, 64), (64, 1280, 64),
+                                       (130, 1000, 128)])
+def test_quantize(cuda, n, k, group, dtype, minimum):
+    import sdb
+
+    g = rng(n + k + group)
+    w = g.standard_normal((n, k)).astype(dtype)
+    w[0, :] = 0  # a row of zeros, then one of a single number, then ties of magnitude
+    if n > 2:
+        w[1, :] = dtype(-0.75)
+        w[2, :] = np.where(np.arange(k) % 2 == 0, dtype(0.5), dtype(-0.5))
+    got = host(sdb.q4_quantize(cuda_tensor(w, cuda), group, minimum).values())
+    np.testing.assert_array_equal(got, quantized(w, group, minimum))
+
+
+def test_quantize_strided_rows_and_extremes(cuda):
+    """A view with rows further apart (odd alignment), numbers past FP16's scales, tiny ones, non-finite groups."""
+    import sdb
+
+    g = rng(5)
+    w = g.standard_normal((6, 101)).astype(np.float32)
+    w[0] *= 1e30
+    w[1] *= 1e-9
+    base = np.zeros((6, 150), dtype=np.float32)
+    base[:, 7:108] = w
+    t = cuda_tensor(base, cuda)[:, 7:108]
+    for minimum in (False, True):
+        got = host(sdb.q4_quantize(t, 32, minimum).values())
+        np.testing.assert_array_equal(got, quantized(w, 32, minimum))
+    w[3, 40], w[4, 0], w[5, 100] = np.nan, np.inf, -np.inf
+    bad = np.zeros((6, 101), dtype=bool)
+    bad[3, 32:64], bad[4, :32], bad[5, 96:] = True, True, True
+    for minimum in (False, True):
+        got = host(sdb.q4_quantize(cuda_tensor(w, cuda), 32, minimum).values())
+        assert np.array_equal(np.isnan(got), bad)
+        clean = np.where(bad, np.float32(1), w)
+        np.testing.assert_array_equal(got[~bad], quantized(clean, 32, minimum)[~bad])
+
+
+def test_values_into_strided_rows(cuda):
+    """Rows further apart than their numbers: what lies between them stays."""
+    import torch
+
+    q, scales, minima, values = made(rng(8), 20, 70, 32, True)
+    out = torch.full((20, 93), 7.0, device=cuda)
+    on_device(cuda, q, scales, minima, 32).values(out=out[:, 11:81])
+    got = host(out)
+    np.testing.assert_array_equal(got[:, 11:81], values.astype(np.float32))
+    assert (got[:, :11] == 7).all() and (got[:, 81:] == 7).all()
+
+
+# ---------------------------------------------------------------- products
+
+def check(got, exact, magnitude, half_out=False):
+    got = np.asarray(got, dtype=np.float64)
+    tol = oracle.K_B200 * np.where(magnitude > 0, magnitude, 1.0)
+    if half_out:
+        tol = tol + 2.0 ** -11 * np.abs(exact) + 2.0 ** -25
+    assert np.isfinite(got).all(), "an output was not written"
+    worst = (np.abs(got - exact) / tol).max()
+    assert worst <= 1.0, f"{worst:.3g} of the bound"
+
+
+def run_linear(cuda, g, rows, k, n, group, minimum, xt=np.float32, ot=np.float32):
+    import sdb
+    import torch
+
+    q, scales, minima, values = made(g, n, k, group, minimum)
+    x = g.standard_normal((rows, k)).astype(xt)
+    x[:, g.random(k) < 0.02] *= xt(20)
+    out = torch.full((rows, n), float("nan"), device=cuda,
+                     dtype=torch.float16 if ot == np.float16 else torch.float32)
+    sdb.mul_mat_q4(on_device(cuda, q, scales, minima, group), cuda_tensor(x, cuda), out=out)
+    exact, mag = oracle.mul_mat_exact(values, x)
+    check(host(out), exact, mag, ot == np.float16)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 7, 8, 9, 16, 17, 24, 31, 32, 33, 64, 65, 77, 129])
+def test_rows(cuda, rows):
+    run_linear(cuda, rng(rows), rows, 320, 130, 32, False)
+    run_linear(cuda, rng(rows + 1), rows, 416, 48, 128, True)
+
+
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("minimum", [False, True])
+@pytest.mark.parametrize("rows", [1, 2, 6, 20])
+@pytest.mark.parametrize("xt,ot", [(np.float32, np.float32), (np.float16, np.float16), (np.float16, np.float32),
+                                   (np.float32, np.float16)])
+def test_forms_and_types(cuda, group, minimum, rows, xt, ot):
+    run_linear(cuda, rng(group + rows), rows, 1000, 72, group, minimum, xt, ot)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 12])
+@pytest.mark.parametrize("k,n", [(1, 1), (2, 17), (31, 16), (33, 15), (127, 31), (128, 16), (129, 33), (255, 1),
+                                 (320, 1280), (1280, 20), (4128, 100), (5000, 9), (11000, 40), (28672, 64),
+                                 (64, 5000)])
+def test_sizes(cuda, k, n, rows):
+    run_linear(cuda, rng(k + n), rows, k, n, 32, True)
+    run_linear(cuda, rng(k + n + 1), rows, k, n, 128, False)
+
+
+def test_wide_and_tall(cuda):
+    run_linear(cuda, rng(1), 1, 4096, 4096, 32, False)
+    run_linear(cuda, rng(2), 2, 1280, 20160, 64, True)
+    run_linear(cuda, rng(3), 40, 28672, 48, 64, True)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 5])
+def test_magnitudes(cuda, rows):
+    """Rows of x from 1e-30 to 1e30 and of mixed magnitudes: the bound holds at every scale."""
+    import sdb
+
+    g = rng(31)
+    q, scales, minima, values = made(g, 50, 300, 64, True)
+    w = on_device(cuda, q, scales, minima, 64)
+    for scale in (1e-30, 1e-6, 1e6, 1e30):
+        x = (g.standard_normal((rows, 300)) * scale * 10.0 ** g.uniform(-3, 3, (rows, 300))).astype(np.float32)
+        exact, mag = oracle.mul_mat_exact(values, x)
+        check(host(sdb.mul_mat_q4(w, cuda_tensor(x, cuda))), exact, mag)
+
+
+@pytest.mark.parametrize("rows", [2, 7])
+def test_a_bad_row_stays_alone(cuda, rows):
+    """Infinities and NaN in one row of x reach that row's outputs and no other."""
+    import sdb
+
+    g = rng(6)
+    q, scales, minima, values = made(g, 40, 200, 32, True)
+    w = on_device(cuda, q, scales, minima, 32)
+    x = g.standard_normal((rows, 200)).astype(np.float32)
+    exact, mag = oracle.mul_mat_exact(values, x)
+    for bad in (np.nan, np.inf, -np.inf):
+        y = x.copy()
+        y[1, 77] = bad
+        got = host(sdb.mul_mat_q4(w, cuda_tensor(y, cuda)))
+        assert not np.isfinite(got[1]).any()
+        keep = [r for r in range(rows) if r != 1]
+        check(got[keep], exact[keep], mag[keep])
+
+
+@pytest.mark.parametrize("rows", [1, 4, 40])
+def test_chain(cuda, rows):
+    """Bias, a scale a column, a residual of the output's shape and SiLU, in order."""
+    import sdb
+
+    g = rng(rows)
+    n, k = 90, 257
+    q, scales, minima, values = made(g, n, k, 32, False)
+    x = g.standard_normal((rows, k)).astype(np.float32)
+    b, s, r = (g.standard_normal(shape).astype(np.float32) for shape in ((n,), (n,), (rows, n)))
+    t = lambda a: cuda_tensor(a, cuda)
+    chain = sdb.Chain().add(t(b)).mul(t(s)).add(t(r)).silu()
+    got = host(sdb.mul_mat_q4(on_device(cuda, q, scales, minima, 32), t(x), chain=chain))
+    exact, mag = oracle.mul_mat_exact(values, x)
+    v = (exact + b) * s.astype(np.float64) + r
+    m = (mag + np.abs(b)) * np.abs(s) + np.abs(r)
+    check(got, v / (1 + np.exp(-v)), 1.1 * m)  # SiLU's slope is at most 1.1
+
+
+@pytest.mark.parametrize("from_redirect", [False, True])
+def test_redirect(cuda, from_redirect):
+    """A residual in its own memory: the sum begins from it, or it is written alone."""
+    import sdb
+    import torch
+
+    g = rng(3)
+    q, scales, minima, values = made(g, 70, 160, 32, False)
+    x, b, r = (g.standard_normal(s).astype(np.float32) for s in ((3, 160), (70,), (3, 70)))
+    out = torch.full((3, 70), 5.0, device=cuda)
+    res = cuda_tensor(r, cuda)
+    sdb.mul_mat_q4(on_device(cuda, q, scales, minima, 32), cuda_tensor(x, cuda), out=out,
+                   chain=sdb.Chain().add(cuda_tensor(b, cuda)).redirect(res, from_redirect))
+    exact, mag = oracle.mul_mat_exact(values, x)
+    check(host(res), exact + b + (r if from_redirect else 0), mag + np.abs(b) + np.abs(r))
+    assert (host(out) == 5).all()
+
+
+@pytest.mark.parametrize("rows", [(2, 3, 1), (1, 5, 2), (2, 2, 9)])
+def test_strides(cuda, rows):
+    """Rows over three dimensions, permuted and further apart, x at an odd element; what lies between stays."""
+    import sdb
+    import torch
+
+    g = rng(9)
+    a, b, c = rows
+    k, n = 200, 33
+    q, scales, minima, values = made(g, n, k, 64, True)
+    x = g.standard_normal((a, b, c, k)).astype(np.float32)
+    base = torch.full((b, a, c, k + 9), 3.0, device=cuda)
+    view = base.permute(1, 0, 2, 3)[..., 3:3 + k]
+    view.copy_(cuda_tensor(x, cuda))
+    whole = torch.full((c, b, a, n + 6), 9.0, device=cuda)
+    out = whole.permute(2, 1, 0, 3)[..., 1:1 + n]
+    bias = g.standard_normal((a, 1, c, n)).astype(np.float32)
+    sdb.mul_mat_q4(on_device(cuda, q, scales, minima, 64), view, out=out, chain=sdb.Chain().add(cuda_tensor(bias, cuda)))
+    exact, mag = oracle.mul_mat_exact(values, x)
+    check(host(out), exact + bias, mag + np.abs(bias))
+    w = host(whole)
+    assert (w[..., :1] == 9).all() and (w[..., 1 + n:] == 9).all()
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("rows,k,half,group,minimum", [(1, 320, 1280, 32, False), (2, 100, 17, 32, True),
+                                                       (5, 1280, 640, 64, True), (9, 777, 50, 128, False),
+                                                       (33, 256, 48, 128, True), (1, 9000, 40, 64, False)])
+@pytest.mark.parametrize("xt,ot", [(np.float32, np.float32), (np.float16, np.float16)])
+def test_gated(cuda, rows, k, half, group, minimum, act, xt, ot):
+    import sdb
+    import torch
+
+    g = rng(rows + k)
+    qa = made(g, half, k, group, minimum)
+    qb = made(g, half, k, group, minimum)
+    x = (g.standard_normal((rows, k)) / np.sqrt(k)).astype(xt)
+    bias = g.standard_normal((2 * half,)).astype(np.float32)
+    out = torch.full((rows, half), float("nan"), device=cuda,
+                     dtype=torch.float16 if ot == np.float16 else torch.float32)
+    sdb.mul_mat_q4_gated(on_device(cuda, *qa[:3], group), on_device(cuda, *qb[:3], group), cuda_tensor(x, cuda), act,
+                         out=out, chain=sdb.Chain().add(cuda_tensor(bias, cuda)))
+    a, ma = oracle.mul_mat_exact(qa[3], x)
+    b, mb = oracle.mul_mat_exact(qb[3], x)
+    a, b, ma, mb = a + bias[:half], b + bias[half:], ma + np.abs(bias[:half]), mb + np.abs(bias[half:])
+    if act == "gelu":
+        act_b = 0.5 * b * (1 + np.tanh(np.sqrt(2 / np.pi) * (b + 0.044715 * b ** 3)))
+    else:
+        act_b = b / (1 + np.exp(-b))
+    # The gate's slope is at most 1.13 (GELU) and 1.1 (SiLU).
+    check(host(out), a * act_b, ma * np.abs(act_b) + np.abs(a) * 1.13 * mb, ot == np.float16)
+
+
+# ---------------------------------------------------------------- use
+
+def test_no_rows(cuda):
+    import sdb
+    import torch
+
+    q, scales, minima, _ = made(rng(1), 8, 64, 32, False)
+    w = on_device(cuda, q, scales, minima, 32)
+    before = sdb.launch_count()
+    out = sdb.mul_mat_q4(w, torch.empty(0, 64, device=cuda))
+    assert out.shape == (0, 8) and sdb.launch_count() == before
+
+
+def test_same_numbers_whatever_the_company(cuda):
+    """A call's result does not turn on chance: twice the same, and on two streams at once."""
+    import sdb
+    import torch
+
+    g = rng(12)
+    q, scales, minima, _ = made(g, 1000, 2048, 32, True)
+    w = on_device(cuda, q, scales, minima, 32)
+    x = [cuda_tensor(g.standard_normal((r, 2048)).astype(np.float32), cuda) for r in (1, 3)]
+    want = [host(sdb.mul_mat_q4(w, v)) for v in x]
+    streams = [torch.cuda.Stream() for _ in x]
+    outs = [[torch.empty(v.shape[0], 1000, device=cuda) for _ in range(20)] for v in x]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for s, v, o in zip(streams, x, outs):
+            sdb.mul_mat_q4(w, v, out=o[i], stream=s)
+    torch.cuda.synchronize()
+    for o, first in zip(outs, want):
+        for t in o:
+            np.testing.assert_array_equal(host(t), first)
+
+
+def test_captured_and_replayed(cuda):
+    """A graph of a gated layer and a projection: replayed on new numbers in the same memory, first call included."""
+    import sdb
+    import torch
+
+    g = rng(13)
+    up = [on_device(cuda, *made(g, 256, 192, 32, False)[:3], 32) for _ in range(2)]
+    down = on_device(cuda, *made(g, 192, 256, 64, True)[:3], 64)
+    x = torch.zeros(2, 192, device=cuda)
+    mid, out = torch.empty(2, 256, device=cuda), torch.empty(2, 192, device=cuda)
+
+    def call():
+        sdb.mul_mat_q4_gated(up[0], up[1], x, out=mid)
+        sdb.mul_mat_q4(down, mid, out=out, chain=sdb.Chain().add(x))
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for _ in range(3):
+        x.copy_(cuda_tensor(g.standard_normal((2, 192)).astype(np.float32), cuda))
+        graph.replay()
+        got = host(out)
+        call()
+        np.testing.assert_array_equal(got, host(out))
+
+
+def test_refusals(cuda):
+    import sdb
+    import torch
+
+    q, scales, minima, _ = made(rng(1), 8, 64, 32, False)
+    w = on_device(cuda, q, scales, minima, 32)
+    x = torch.zeros(2, 64, device=cuda)
+    out = torch.empty(2, 8, device=cuda)
+
+    def refused(status, call):
+        with pytest.raises(sdb.SdbError) as e:
+            call()
+        assert e.value.status == status
+
+    refused(sdb.NOT_SUPPORTED, lambda: sdb.mul_mat_q4(w, torch.zeros(2, 63, device=cuda), out=out))
+    refused(sdb.NOT_SUPPORTED, lambda: sdb.mul_mat_q4(w, x, out=torch.empty(2, 9, device=cuda)))
+    refused(sdb.NOT_SUPPORTED, lambda: sdb.mul_mat_q4(w, x, out=torch.empty(3, 8, device=cuda)))
+    refused(sdb.NOT_SUPPORTED, lambda: sdb.mul_mat_q4(w, torch.zeros(64, 2, device=cuda).t(), out=out))
+    refused(sdb.INVALID, lambda: sdb.mul_mat_q4(w, x.double(), out=out))
+    refused(sdb.INVALID, lambda: sdb.mul_mat_q4(w, x.cpu(), out=out))
+    refused(sdb.INVALID, lambda: sdb.mul_mat_q4(w, x, out=out, chain=sdb.Chain().add(torch.zeros(7, device=cuda))))
+    refused(sdb.INVALID, lambda: sdb.mul_mat_q4(w, x.half(), out=out.half(),
+                                                chain=sdb.Chain().redirect(torch.zeros(2, 8, device=cuda))))
+    refused(sdb.INVALID, lambda: sdb.mul_mat_q4_gated(w, w, x, act="relu"))
+    refused(sdb.INVALID, lambda: sdb.mul_mat_q4_gated(w, w, x, chain=sdb.Chain().add(torch.zeros(8, device=cuda))))
+    refused(sdb.INVALID, lambda: sdb.mul_mat_q4_gated(w, w, x, out=out, chain=sdb.Chain().redirect(out)))
+    other = on_device(cuda, *made(rng(2), 8, 64, 64, False)[:3], 64)
+    refused(sdb.NOT_SUPPORTED, lambda: sdb.mul_mat_q4_gated(w, other, x))
+    refused(sdb.INVALID, lambda: sdb.q4_quantize(torch.zeros(4, 4, 4, device=cuda)))
+    refused(sdb.INVALID, lambda: sdb.q4_quantize(torch.zeros(4, 64, device=cuda), group=48))
+    refused(sdb.INVALID, lambda: sdb.q4_quantize(torch.zeros(64, 4, device=cuda).t()))
+    refused(sdb.INVALID, lambda: w.values(out=torch.empty(8, 64, device=cuda, dtype=torch.float16)))
+    refused(sdb.INVALID, lambda: sdb.q4_import(torch.zeros(4, 16, device=cuda, dtype=torch.uint8),
+                                               torch.zeros(4, 2, device=cuda, dtype=torch.float16)))
+    refused(sdb.INVALID, lambda: sdb.q4_from_blocks(torch.zeros(4, 18, device=cuda, dtype=torch.uint8), 64))
