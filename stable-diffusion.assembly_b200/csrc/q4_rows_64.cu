@@ -1,0 +1,8 @@
+// Linear layers with 4-bit weights in groups of 64 (q4_rows.cuh).
+#include "q4_launch.cuh"
+
+namespace sdb {
+
+template int q4_launch<64>(const Q4Args&, const Q4Plan&, bool, cudaStream_t);
+
+}  // namespace sdb
