@@ -1,6 +1,8 @@
 // The launches of q4_rows.cuh's kernel for one group size (a translation unit each: q4_rows_*.cu).
 #pragma once
 
+#include <atomic>
+
 #include "q4_rows.cuh"
 #include "runtime.cuh"
 
@@ -10,8 +12,15 @@ template <int T, bool PAIRED, bool HALF, bool GATED, int G>
 int q4_launch_form(const Q4Args& a, const Q4Plan& p, cudaStream_t st) {
     using S = Q4Shape<T, PAIRED, HALF, GATED>;
     auto kern = q4_rows_kernel<T, PAIRED, HALF, GATED, G>;
-    const int bytes = S::fixed_bytes() + a.chunk * S::block_bytes(128 / G);
-    SDB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    const int bytes = S::fixed_bytes() + a.chunk * S::block_bytes(a.rows < S::kTokens ? a.rows : S::kTokens, 128 / G);
+    // The kernel's shared-memory limit is raised once on each device (it costs about as much as a launch).
+    static std::atomic<uint64_t> raised{0};
+    int dev = 0;
+    SDB_CUDA(cudaGetDevice(&dev));
+    if (dev >= 64 || !(raised.load(std::memory_order_relaxed) >> dev & 1)) {
+        SDB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kQ4MaxShared));
+        if (dev < 64) raised.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(p.blocks), static_cast<unsigned>(p.chunks));
     cfg.blockDim = dim3(kQ4Threads);

@@ -62,8 +62,8 @@ Q4Plan plan(Q4Args& a, bool half) {
     a.wk_log = a.w.kblocks <= 1 ? 0 : a.w.kblocks <= 2 ? 1 : a.w.kblocks <= 4 ? 2 : 3;
     a.cluster = 1;
     a.range = (a.w.kblocks + a.cluster - 1) / a.cluster;
-    const int products = half || p.form == 0 ? (p.form ? p.form : 1) : 2 * p.form;
-    const int block = 2048 * products + tokens * 4 * (1 + a.w.ng);
+    const int columns = p.form == 0 ? 2 * std::min(a.rows, 4) : 8 * p.form * (half ? 1 : 2);
+    const int block = kQ4Column * columns + tokens * 4 * (1 + a.w.ng);
     const int wk = 1 << a.wk_log;
     a.chunk = std::max(wk, std::min((a.range + wk - 1) / wk * wk, 90 * 1024 / block / wk * wk));
     const int groups = (a.w.tiles + kQ4Warps / wk - 1) / (kQ4Warps / wk);

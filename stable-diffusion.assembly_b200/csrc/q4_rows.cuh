@@ -20,11 +20,13 @@
 //
 // A CTA is eight warps: WR tiles of rows side by side, WK = 8 / WR warps to a
 // tile that share its k-blocks, and up to eight CTAs of a cluster that share
-// them again.  x is split once into shared memory, in the order of the mma's B
-// fragments (8 bytes a lane, 256 a product, 32-byte units permuted so that the
-// stores of a row's k-block meet no bank twice), and stays there for all the
-// row tiles the CTA walks.  Weights go from memory to registers, two k-blocks
-// ahead.  The warps' sums meet in shared memory and are added in one order, so
+// them again.  x is split once into shared memory, each column of the products
+// a run of its eight k-slices' fragments (4 lanes of 8 bytes a slice) and 288
+// bytes to the next column, so that neither a column's stores nor a slice's
+// loads over eight columns meet a bank twice, and stays there for all the row
+// tiles the CTA walks.  A product's unused columns are not stored: their lanes
+// read what lies there and their sums go nowhere.  Weights go from memory to
+// registers, two k-blocks ahead.  The warps' sums meet in shared memory and are added in one order, so
 // a result does not turn on timing; the sums of a cluster's other CTAs are read
 // where they lie.
 #pragma once
@@ -42,6 +44,8 @@ namespace sdb {
 
 constexpr int kQ4Warps = 8;
 constexpr int kQ4Threads = 32 * kQ4Warps;
+constexpr int kQ4MaxShared = 227 * 1024;
+constexpr int kQ4Column = 288;  // bytes of a column's k-block in shared memory: 8 slices x 32, and a step of 8 banks
 
 struct Q4Args {
     Q4View w, gate;            // gate: the gated form's second matrix
@@ -63,36 +67,56 @@ struct Q4Args {
 // What a variant's shared memory holds.
 template <int T, bool PAIRED, bool HALF, bool GATED>
 struct Q4Shape {
-    static constexpr int kTokens = PAIRED ? 4 : 8 * T;           // rows of x of a CTA
-    static constexpr int kProducts = HALF || PAIRED ? T : 2 * T;  // B fragments of a k-slice
+    static constexpr int kTokens = PAIRED ? 4 : 8 * T;            // rows of x of a CTA
+    static constexpr int kProducts = HALF || PAIRED ? T : 2 * T;  // products of a k-slice
     static constexpr int kTiles = GATED ? 2 : 1;
-    static constexpr int kSums = PAIRED ? 2 : 4 * T;             // FP32 sums a lane has of a tile
+    static constexpr int kSums = PAIRED ? 2 : 4 * T;              // FP32 sums a lane has of a tile
     static constexpr int kRedBuffers = T == 1 ? 2 : 1;
     static constexpr int kRedFloats = kQ4Warps * kTiles * kSums * 32;
-    // Bytes of x a k-block: fragments of its 8 slices, the rows' scales, their sums over its groups.
-    static constexpr int block_bytes(int ng) { return 2048 * kProducts + kTokens * 4 * (1 + ng); }
-    static constexpr int fixed_bytes() { return kRedBuffers * kRedFloats * 4 + kTokens * 8; }
+    // Bytes of x a k-block with `tokens` rows: the columns of the products, the rows' scales and their sums
+    // over its groups; and after all k-blocks, what the lanes of unused columns read past the last.
+    static __host__ __device__ constexpr int columns(int tokens) { return PAIRED ? 2 * tokens : 8 * kProducts; }
+    static constexpr int block_bytes(int tokens, int ng) { return kQ4Column * columns(tokens) + kTokens * 4 * (1 + ng); }
+    static constexpr int fixed_bytes() { return kRedBuffers * kRedFloats * 4 + kTokens * 8 + 8 * kQ4Column; }
 };
 
+// c = a b, or c += a b.
+template <bool FIRST>
 __device__ __forceinline__ void q4_mma(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+    if constexpr (FIRST)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%10, %10, %10, %10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(0.0f));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
 
-__device__ __forceinline__ uint32_t q4_low(uint32_t u) {  // nibbles at bits 0 and 16, less 8
-    uint32_t v = (u & 0x000f000fu) | 0x64006400u;
-    const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&v), __half2half2(__ushort_as_half(0x6408)));  // 1032
-    return *reinterpret_cast<const uint32_t*>(&r);
+// u & mask | 0x64006400: two nibbles in the low bits of FP16 numbers from 1024 on.
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t q4_nibbles(uint32_t u) {
+    uint32_t v;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(u), "n"(MASK), "r"(0x64006400u));
+    return v;
 }
 
-__device__ __forceinline__ uint32_t q4_high(uint32_t u) {  // nibbles at bits 4 and 20: 1024 + 16 q
-    uint32_t v = (u & 0x00f000f0u) | 0x64006400u;
-    const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&v), __half2half2(__ushort_as_half(0x2c00)),  // 1 / 16
-                              __half2half2(__ushort_as_half(0xd480)));                                  // -72
-    return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ uint32_t q4_low(uint32_t u) {  // nibbles at bits 0 and 16: 1024 + q, less 1032
+    uint32_t v;
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(v) : "r"(q4_nibbles<0x000f000fu>(u)), "r"(0x64086408u));
+    return v;
+}
+
+__device__ __forceinline__ uint32_t q4_high(uint32_t u) {  // at bits 4 and 20: (1024 + 16 q) / 16, less 72
+    uint32_t v;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;"
+        : "=r"(v)
+        : "r"(q4_nibbles<0x00f000f0u>(u)), "r"(0x2c002c00u), "r"(0xd480d480u));
+    return v;
 }
 
 // Weights pass through: not kept in L1, kept in L2 as any line (a next call may find them there).
@@ -121,43 +145,50 @@ struct Q4Stage {
     uint4 lo, hi;
     uint32_t d[kNg], m[kNg];
 
-    __device__ __forceinline__ void load(const Q4View& w, long long block, int lane) {
-        const uint4* c = reinterpret_cast<const uint4*>(w.codes) + block * 64 + lane;
-        lo = q4_load(c);
-        hi = q4_load(c + 32);
-        const long long at = block * 8 + lane / 4;
-        load_run(d, w.scales, at);
-        if (w.minima) load_run(m, w.minima, at);
-    }
-    static __device__ __forceinline__ void load_run(uint32_t (&r)[kNg], const __half* p, long long at) {
+    static __device__ __forceinline__ void load_run(uint32_t (&r)[kNg], const uint8_t* p) {
         if constexpr (kNg == 4) {
-            const uint4 v = q4_load(reinterpret_cast<const uint4*>(p) + at);
+            const uint4 v = q4_load(reinterpret_cast<const uint4*>(p));
             r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
         } else if constexpr (kNg == 2) {
-            const uint2 v = q4_load(reinterpret_cast<const uint2*>(p) + at);
+            const uint2 v = q4_load(reinterpret_cast<const uint2*>(p));
             r[0] = v.x; r[1] = v.y;
         } else {
-            r[0] = q4_load(reinterpret_cast<const unsigned*>(p) + at);
+            r[0] = q4_load(reinterpret_cast<const unsigned*>(p));
         }
     }
     // Group i's numbers of rows g and g + 8.
     static __device__ __forceinline__ float2 pick(const uint32_t (&r)[kNg], int i) {
-        uint32_t a, b;
-        if constexpr (kNg == 1) {
-            a = r[0] & 0xffffu;
-            b = r[0] >> 16;
-        } else {
-            const int shift = (i & 1) * 16;
-            a = r[i / 2] >> shift & 0xffffu;
-            b = r[kNg / 2 + i / 2] >> shift & 0xffffu;
-        }
-        return {__half2float(__ushort_as_half(static_cast<unsigned short>(a))),
-                __half2float(__ushort_as_half(static_cast<unsigned short>(b)))};
+        if constexpr (kNg == 1) return __half22float2(*reinterpret_cast<const __half2*>(&r[0]));
+        const __half2 a = *reinterpret_cast<const __half2*>(&r[i / 2]);
+        const __half2 b = *reinterpret_cast<const __half2*>(&r[kNg / 2 + i / 2]);
+        return i & 1 ? make_float2(__high2float(a), __high2float(b)) : make_float2(__low2float(a), __low2float(b));
+    }
+};
+
+// Where a lane's next k-block of a matrix lies; steps are counted in k-blocks.
+template <int G>
+struct Q4Walk {
+    const uint8_t *codes, *scales, *minima;
+    __device__ __forceinline__ void start(const Q4View& w, long long block, int lane) {
+        codes = w.codes + block * 1024 + lane * 16;
+        scales = reinterpret_cast<const uint8_t*>(w.scales) + (block * 8 + lane / 4) * (512 / G);
+        minima = w.minima ? reinterpret_cast<const uint8_t*>(w.minima) + (block * 8 + lane / 4) * (512 / G) : nullptr;
+    }
+    __device__ __forceinline__ void step(long long blocks) {
+        codes += blocks * 1024;
+        scales += blocks * (4096 / G);
+        if (minima) minima += blocks * (4096 / G);
+    }
+    __device__ __forceinline__ void load(Q4Stage<G>& s) const {
+        s.lo = q4_load(reinterpret_cast<const uint4*>(codes));
+        s.hi = q4_load(reinterpret_cast<const uint4*>(codes) + 32);
+        Q4Stage<G>::load_run(s.d, scales);
+        if (minima) Q4Stage<G>::load_run(s.m, minima);
     }
 };
 
 // Splits the CTA's rows of x for k-blocks [kb0, kb1) into shared memory: a warp takes a row's k-block, a
-// lane four numbers (columns 4 lane..): slice 2 (lane / 8) + lane % 2, fragment lane (row, lane / 2 % 4).
+// lane four numbers (columns 4 lane..): slice 2 (lane / 8) + lane % 2, and there lane / 2 % 4 of the column.
 template <int T, bool PAIRED, bool HALF, int G>
 __device__ __forceinline__ void q4_split(const Q4Args& a, const long long* row_at, int tokens, int kb0, int kb1,
                                          uint8_t* frags, float* scales, float* sums) {
@@ -165,7 +196,7 @@ __device__ __forceinline__ void q4_split(const Q4Args& a, const long long* row_a
     constexpr int NG = 128 / G;
     const int lane = threadIdx.x & 31;
     const int slice = (lane >> 3) * 2 + (lane & 1), t = (lane >> 1) & 3;
-    const int items = tokens * (kb1 - kb0);
+    const int items = tokens * (kb1 - kb0), block = kQ4Column * S::columns(tokens);
     for (int i = threadIdx.x / 32; i < items; i += kQ4Warps) {
         const int b = i / tokens, m = i - b * tokens;
         const long long k = (kb0 + b) * 128LL + lane * 4;
@@ -193,12 +224,10 @@ __device__ __forceinline__ void q4_split(const Q4Args& a, const long long* row_a
                 for (int c = 0; c < 4; ++c) x[c] = k + c < a.w.k ? p[c] : 0.0f;
             }
         }
-        uint8_t* base = frags + b * (2048 * S::kProducts) + slice * (256 * S::kProducts);
-        auto slot = [&](int product, int col) {
-            return reinterpret_cast<uint2*>(base + product * 256 + ((col * 32 + t * 8) ^ (slice * 32)));
-        };
+        uint8_t* base = frags + b * block + slice * 32 + t * 8;
+        auto slot = [&](int col) { return reinterpret_cast<uint2*>(base + col * kQ4Column); };
         if constexpr (HALF) {
-            *slot(m / 8, m % 8) = raw;
+            *slot(m) = raw;
         } else {
             float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
             for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
@@ -219,11 +248,11 @@ __device__ __forceinline__ void q4_split(const Q4Args& a, const long long* row_a
                 (c ? lo.y : lo.x) = *reinterpret_cast<const uint32_t*>(&l);
             }
             if constexpr (PAIRED) {
-                *slot(0, 2 * m) = hi;
-                *slot(0, 2 * m + 1) = lo;
+                *slot(2 * m) = hi;
+                *slot(2 * m + 1) = lo;
             } else {
-                *slot(m / 8 * 2, m % 8) = hi;
-                *slot(m / 8 * 2 + 1, m % 8) = lo;
+                *slot(m / 8 * 16 + m % 8) = hi;
+                *slot(m / 8 * 16 + m % 8 + 8) = lo;
             }
             if (lane == 0) scales[b * S::kTokens + m] = down;
         }
@@ -265,28 +294,41 @@ __global__ void __launch_bounds__(kQ4Threads, T == 1 ? 2 : 1) q4_rows_kernel(con
     float* red = reinterpret_cast<float*>(smem);
     long long* row_at = reinterpret_cast<long long*>(red + S::kRedBuffers * S::kRedFloats);
     uint8_t* frags = reinterpret_cast<uint8_t*>(row_at + S::kTokens);
-    float* scales = reinterpret_cast<float*>(frags + a.chunk * 2048 * S::kProducts);
+    const int block_bytes = kQ4Column * S::columns(tokens);
+    float* scales = reinterpret_cast<float*>(frags + a.chunk * block_bytes + 8 * kQ4Column);
     float* sums = scales + a.chunk * S::kTokens;
 
+    // The warp's k-blocks in the order they are taken: over its row tiles, kb_begin + wk, + WK, ...  A warp
+    // past the last tile walks the last one again and stores nothing.
     Q4Stage<G> stage[2][S::kTiles];
-    // The warp's k-blocks in the order they are taken: over its row tiles, kb_begin + wk, + WK, ...
-    int load_group = group0, load_kb = kb_begin + wk;
-    if (load_kb >= kb_end) load_group = groups;
-    auto load = [&](int i) {
-        const int tile = load_group * WR + wr;
-        if (load_group < groups && tile < a.w.tiles) {
-            const long long block = static_cast<long long>(tile) * a.w.kblocks + load_kb;
-            stage[i][0].load(a.w, block, lane);
-            if constexpr (GATED) stage[i][1].load(a.gate, block, lane);
+    Q4Walk<G> walk[S::kTiles];
+    const int steps = kb_end - kb_begin > wk ? (kb_end - kb_begin - wk + WK - 1) >> a.wk_log : 0;  // of a tile
+    int load_group = group0, load_step = 0;
+    auto tile_of = [&](int group) { return min(group * WR + wr, a.w.tiles - 1); };
+    {
+        const long long block = static_cast<long long>(tile_of(group0)) * a.w.kblocks + kb_begin + wk;
+        walk[0].start(a.w, block, lane);
+        if constexpr (GATED) walk[1].start(a.gate, block, lane);
+    }
+    auto load = [&](Q4Stage<G> (&to)[S::kTiles]) {
+        if (load_group >= groups) return;
+#pragma unroll
+        for (int i = 0; i < S::kTiles; ++i) walk[i].load(to[i]);
+        long long blocks = WK;
+        if (++load_step == steps) {
+            load_step = 0;
+            const int next = load_group + group_step;
+            if (next < groups)
+                blocks = static_cast<long long>(tile_of(next) - tile_of(load_group)) * a.w.kblocks -
+                         static_cast<long long>(steps - 1) * WK;
+            load_group = next;
         }
-        load_kb += WK;
-        if (load_kb >= kb_end) {
-            load_kb = kb_begin + wk;
-            load_group += group_step;
-        }
+#pragma unroll
+        for (int i = 0; i < S::kTiles; ++i) walk[i].step(blocks);
     };
-    load(0);
-    load(1);
+    if (steps == 0) load_group = groups;
+    load(stage[0]);
+    load(stage[1]);
 
     if (threadIdx.x < tokens) {
         const int m = m0 + threadIdx.x, q = m / a.ne1, i1 = m - q * a.ne1, i3 = q / a.ne2, i2 = q - i3 * a.ne2;
@@ -294,12 +336,119 @@ __global__ void __launch_bounds__(kQ4Threads, T == 1 ? 2 : 1) q4_rows_kernel(con
     }
     __syncthreads();
 
-    const int lane_at = lane * 8;
+    const uint8_t* lane_frags = frags + (lane >> 2) * kQ4Column + (lane & 3) * 8;
+    float acc[S::kTiles][S::kSums];
+    // One k-block, the chunk's at `at`.
+    auto product = [&](const Q4Stage<G> (&st)[S::kTiles], int at) {
+        const uint8_t* f = lane_frags + at * block_bytes;
+        float part[S::kTiles][S::kSums];  // the k-block's sums, in its rows' scales
+        float s[S::kTiles][T][4];         // a group's sums
+        uint32_t w[S::kTiles][2][4];
+#pragma unroll
+        for (int i = 0; i < S::kTiles; ++i) {
+            w[i][0][0] = st[i].lo.x; w[i][0][1] = st[i].lo.y; w[i][0][2] = st[i].lo.z; w[i][0][3] = st[i].lo.w;
+            w[i][1][0] = st[i].hi.x; w[i][1][1] = st[i].hi.y; w[i][1][2] = st[i].hi.z; w[i][1][3] = st[i].hi.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t av[S::kTiles][4];
+#pragma unroll
+                for (int i = 0; i < S::kTiles; ++i) {
+                    const uint32_t u0 = w[i][0][j] >> (8 * h), u1 = w[i][1][j] >> (8 * h);
+                    av[i][0] = q4_low(u0);
+                    av[i][1] = q4_low(u1);
+                    av[i][2] = q4_high(u0);
+                    av[i][3] = q4_high(u1);
+                }
+                const int slice = 2 * j + h;
+#pragma unroll
+                for (int p = 0; p < S::kProducts; ++p) {
+                    const uint2 b = *reinterpret_cast<const uint2*>(f + slice * 32 + p * (8 * kQ4Column));
+                    const int t = HALF || PAIRED ? p : p / 2;
+                    const bool first = j % (4 / NG) == 0 && h == 0 && (HALF || PAIRED || p % 2 == 0);
+#pragma unroll
+                    for (int i = 0; i < S::kTiles; ++i) {
+                        if (first) q4_mma<true>(s[i][t], av[i], b);
+                        else q4_mma<false>(s[i][t], av[i], b);
+                    }
+                }
+            }
+            if ((j + 1) % (4 / NG) != 0) continue;
+            const int g = (j + 1) / (4 / NG) - 1;
+#pragma unroll
+            for (int i = 0; i < S::kTiles; ++i) {
+                const float2 d = Q4Stage<G>::pick(st[i].d, g);
+                auto join = [&](int c, float scale, float v) {
+                    part[i][c] = g == 0 ? scale * v : fmaf(scale, v, part[i][c]);
+                };
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    if constexpr (PAIRED) {
+                        join(0, d.x, s[i][0][0] + s[i][0][1]);
+                        join(1, d.y, s[i][0][2] + s[i][0][3]);
+                    } else {
+                        join(4 * t, d.x, s[i][t][0]);
+                        join(4 * t + 1, d.x, s[i][t][1]);
+                        join(4 * t + 2, d.y, s[i][t][2]);
+                        join(4 * t + 3, d.y, s[i][t][3]);
+                    }
+                }
+            }
+            if (a.w.minima) {
+                const float* xs = sums + (at * NG + g) * S::kTokens;
+#pragma unroll
+                for (int i = 0; i < S::kTiles; ++i) {
+                    const float2 d = Q4Stage<G>::pick(st[i].d, g), mn = Q4Stage<G>::pick(st[i].m, g);
+                    const float o0 = fmaf(8.0f, d.x, mn.x), o1 = fmaf(8.0f, d.y, mn.y);
+                    if constexpr (PAIRED) {
+                        const float v = xs[lane & 3];
+                        acc[i][0] = fmaf(o0, v, acc[i][0]);
+                        acc[i][1] = fmaf(o1, v, acc[i][1]);
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < T; ++t) {
+                            const float2 v = *reinterpret_cast<const float2*>(xs + t * 8 + (lane & 3) * 2);
+                            acc[i][4 * t] = fmaf(o0, v.x, acc[i][4 * t]);
+                            acc[i][4 * t + 1] = fmaf(o0, v.y, acc[i][4 * t + 1]);
+                            acc[i][4 * t + 2] = fmaf(o1, v.x, acc[i][4 * t + 2]);
+                            acc[i][4 * t + 3] = fmaf(o1, v.y, acc[i][4 * t + 3]);
+                        }
+                    }
+                }
+            }
+        }
+        const float* xs = scales + at * S::kTokens;
+#pragma unroll
+        for (int i = 0; i < S::kTiles; ++i) {
+            if constexpr (HALF) {
+#pragma unroll
+                for (int c = 0; c < S::kSums; ++c) acc[i][c] += part[i][c];
+            } else if constexpr (PAIRED) {
+                const float v = xs[lane & 3];
+                acc[i][0] = fmaf(v, part[i][0], acc[i][0]);
+                acc[i][1] = fmaf(v, part[i][1], acc[i][1]);
+            } else {
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    const float2 v = *reinterpret_cast<const float2*>(xs + t * 8 + (lane & 3) * 2);
+                    acc[i][4 * t] = fmaf(v.x, part[i][4 * t], acc[i][4 * t]);
+                    acc[i][4 * t + 1] = fmaf(v.y, part[i][4 * t + 1], acc[i][4 * t + 1]);
+                    acc[i][4 * t + 2] = fmaf(v.x, part[i][4 * t + 2], acc[i][4 * t + 2]);
+                    acc[i][4 * t + 3] = fmaf(v.y, part[i][4 * t + 3], acc[i][4 * t + 3]);
+                }
+            }
+        }
+    };
+
     bool held = false;  // the one chunk of x is in shared memory
     int parity = 0;
     for (int group = group0; group < groups; group += group_step) {
-        float acc[S::kTiles][S::kSums] = {};
-        const bool tile_in = group * WR + wr < a.w.tiles;
+#pragma unroll
+        for (int i = 0; i < S::kTiles; ++i)
+#pragma unroll
+            for (int c = 0; c < S::kSums; ++c) acc[i][c] = 0.0f;
         for (int kc = kb_begin; kc < kb_end; kc += a.chunk) {
             const int kc_end = min(kc + a.chunk, kb_end);
             if (!held) {
@@ -308,111 +457,18 @@ __global__ void __launch_bounds__(kQ4Threads, T == 1 ? 2 : 1) q4_rows_kernel(con
                 __syncthreads();
                 held = a.chunk >= kb_end - kb_begin;
             }
-            for (int kb = kc + wk; kb < kc_end; kb += WK) {
-                if (tile_in) {
-                    const int at = kb - kc;
-                    const uint8_t* f = frags + at * (2048 * S::kProducts);
-                    float part[S::kTiles][S::kSums] = {};   // the k-block's sums, in its rows' scales
-                    float s[S::kTiles][T][4] = {};          // a group's sums
-                    uint32_t w[S::kTiles][2][4];
-#pragma unroll
-                    for (int i = 0; i < S::kTiles; ++i) {
-                        const Q4Stage<G>& st = stage[0][i];
-                        w[i][0][0] = st.lo.x; w[i][0][1] = st.lo.y; w[i][0][2] = st.lo.z; w[i][0][3] = st.lo.w;
-                        w[i][1][0] = st.hi.x; w[i][1][1] = st.hi.y; w[i][1][2] = st.hi.z; w[i][1][3] = st.hi.w;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            uint32_t av[S::kTiles][4];
-#pragma unroll
-                            for (int i = 0; i < S::kTiles; ++i) {
-                                const uint32_t u0 = w[i][0][j] >> (8 * h), u1 = w[i][1][j] >> (8 * h);
-                                av[i][0] = q4_low(u0);
-                                av[i][1] = q4_low(u1);
-                                av[i][2] = q4_high(u0);
-                                av[i][3] = q4_high(u1);
-                            }
-                            const int slice = 2 * j + h;
-#pragma unroll
-                            for (int p = 0; p < S::kProducts; ++p) {
-                                const uint2 b = *reinterpret_cast<const uint2*>(
-                                    f + slice * (256 * S::kProducts) + p * 256 + (lane_at ^ (slice * 32)));
-#pragma unroll
-                                for (int i = 0; i < S::kTiles; ++i) q4_mma(s[i][HALF || PAIRED ? p : p / 2], av[i], b);
-                            }
-                        }
-                        if ((j + 1) % (4 / NG) == 0) {
-                            const int g = (j + 1) / (4 / NG) - 1;
-#pragma unroll
-                            for (int i = 0; i < S::kTiles; ++i) {
-                                const float2 d = Q4Stage<G>::pick(stage[0][i].d, g);
-#pragma unroll
-                                for (int t = 0; t < T; ++t) {
-                                    if constexpr (PAIRED) {
-                                        part[i][0] = fmaf(d.x, s[i][t][0] + s[i][t][1], part[i][0]);
-                                        part[i][1] = fmaf(d.y, s[i][t][2] + s[i][t][3], part[i][1]);
-                                    } else {
-                                        part[i][4 * t] = fmaf(d.x, s[i][t][0], part[i][4 * t]);
-                                        part[i][4 * t + 1] = fmaf(d.x, s[i][t][1], part[i][4 * t + 1]);
-                                        part[i][4 * t + 2] = fmaf(d.y, s[i][t][2], part[i][4 * t + 2]);
-                                        part[i][4 * t + 3] = fmaf(d.y, s[i][t][3], part[i][4 * t + 3]);
-                                    }
-                                    s[i][t][0] = s[i][t][1] = s[i][t][2] = s[i][t][3] = 0.0f;
-                                }
-                            }
-                            if (a.w.minima) {
-                                const float* xs = sums + (at * NG + g) * S::kTokens;
-#pragma unroll
-                                for (int i = 0; i < S::kTiles; ++i) {
-                                    const float2 d = Q4Stage<G>::pick(stage[0][i].d, g);
-                                    const float2 mn = Q4Stage<G>::pick(stage[0][i].m, g);
-                                    const float o0 = fmaf(8.0f, d.x, mn.x), o1 = fmaf(8.0f, d.y, mn.y);
-                                    if constexpr (PAIRED) {
-                                        const float v = xs[lane & 3];
-                                        acc[i][0] = fmaf(o0, v, acc[i][0]);
-                                        acc[i][1] = fmaf(o1, v, acc[i][1]);
-                                    } else {
-#pragma unroll
-                                        for (int t = 0; t < T; ++t) {
-                                            const float2 v =
-                                                *reinterpret_cast<const float2*>(xs + t * 8 + (lane & 3) * 2);
-                                            acc[i][4 * t] = fmaf(o0, v.x, acc[i][4 * t]);
-                                            acc[i][4 * t + 1] = fmaf(o0, v.y, acc[i][4 * t + 1]);
-                                            acc[i][4 * t + 2] = fmaf(o1, v.x, acc[i][4 * t + 2]);
-                                            acc[i][4 * t + 3] = fmaf(o1, v.y, acc[i][4 * t + 3]);
-                                        }
-                                    }
-                                }
-                            }
-                        }
-                    }
-                    const float* xs = scales + at * S::kTokens;
-#pragma unroll
-                    for (int i = 0; i < S::kTiles; ++i) {
-                        if constexpr (HALF) {
-#pragma unroll
-                            for (int c = 0; c < S::kSums; ++c) acc[i][c] += part[i][c];
-                        } else if constexpr (PAIRED) {
-                            const float v = xs[lane & 3];
-                            acc[i][0] = fmaf(v, part[i][0], acc[i][0]);
-                            acc[i][1] = fmaf(v, part[i][1], acc[i][1]);
-                        } else {
-#pragma unroll
-                            for (int t = 0; t < T; ++t) {
-                                const float2 v = *reinterpret_cast<const float2*>(xs + t * 8 + (lane & 3) * 2);
-                                acc[i][4 * t] = fmaf(v.x, part[i][4 * t], acc[i][4 * t]);
-                                acc[i][4 * t + 1] = fmaf(v.y, part[i][4 * t + 1], acc[i][4 * t + 1]);
-                                acc[i][4 * t + 2] = fmaf(v.x, part[i][4 * t + 2], acc[i][4 * t + 2]);
-                                acc[i][4 * t + 3] = fmaf(v.y, part[i][4 * t + 3], acc[i][4 * t + 3]);
-                            }
-                        }
-                    }
-                }
+            int at = wk;
+            for (; at + WK < kc_end - kc; at += 2 * WK) {
+                product(stage[0], at);
+                load(stage[0]);
+                product(stage[1], at + WK);
+                load(stage[1]);
+            }
+            if (at < kc_end - kc) {
+                product(stage[0], at);
 #pragma unroll
                 for (int i = 0; i < S::kTiles; ++i) stage[0][i] = stage[1][i];
-                load(1);
+                load(stage[1]);
             }
         }
 

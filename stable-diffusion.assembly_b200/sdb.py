@@ -687,17 +687,21 @@ NORMS = {"none": 0, "layer": 1, "rms": 2}
 def _packed(t, what: str) -> bytes:
     """The sdb_tensor of an FP32 or FP16 CUDA tensor of at most four dimensions, as bytes."""
     shape, stride = t.shape, t.stride()
-    dtype = str(t.dtype)
-    if dtype == "torch.float32":
-        ty, es = TYPE_F32, 4
-    elif dtype == "torch.float16":
-        ty, es = TYPE_F16, 2
-    else:
+    es = t.element_size()
+    if not t.is_floating_point() or (es != 4 and (es != 2 or str(t.dtype) != "torch.float16")):
         raise SdbError(INVALID, f"{what}: unsupported dtype {t.dtype}")
+    ty = TYPE_F32 if es == 4 else TYPE_F16
     nd = len(shape)
     if nd == 2:
-        n0, n1, s0, s1 = shape[1], shape[0], stride[1] * es, stride[0] * es
-        return _TENSOR.pack(ty, n0, n1, 1, 1, s0, s1, s1 * n1, s1 * n1, t.data_ptr())
+        n1, n0 = shape
+        s1, s0 = stride
+        s1 *= es
+        return _TENSOR.pack(ty, n0, n1, 1, 1, s0 * es, s1, s1 * n1, s1 * n1, t.data_ptr())
+    if nd == 3:
+        n2, n1, n0 = shape
+        s2, s1, s0 = stride
+        s2 *= es
+        return _TENSOR.pack(ty, n0, n1, n2, 1, s0 * es, s1 * es, s2, s2 * n2, t.data_ptr())
     if nd == 0 or nd > 4:
         raise SdbError(INVALID, f"{what}: one to four dimensions")
     ne = [shape[nd - 1 - d] if d < nd else 1 for d in range(4)]
@@ -705,15 +709,31 @@ def _packed(t, what: str) -> bytes:
     return _TENSOR.pack(ty, *ne, *nb, t.data_ptr())
 
 
-def _packed_chain(chain: Chain | None, out, cols: int):
+def _chain_tensors(chain: Chain | None) -> tuple:
+    """The tensors of a chain: its operands, then its redirect."""
+    if chain is None:
+        return ()
+    found = [t for _, t, _ in chain.steps if t is not None]
+    if chain.redirect_tensor is not None:
+        found.append(chain.redirect_tensor)
+    return tuple(found)
+
+
+def _packed_chain(chain: Chain | None, tensors: tuple, out, cols: int):
     """The sdb_chain of an operation on out's rows, `cols` columns each, as bytes (None: no chain).  Operands
     that do not reach over the rows are refused: the kernel would read past them."""
     if chain is None:
         return None
+    # A chain that is used again as it was is not described again.
+    shape = out.shape
+    key = (len(chain.steps), chain.from_redirect, cols, shape, out.stride(), out.dtype,
+           [t.data_ptr() for t in tensors])
+    kept = chain.__dict__.get("_described")
+    if kept is not None and kept[0] == key:
+        return kept[1]
     steps = chain.steps
     if len(steps) > MAX_STEPS:
         raise SdbError(INVALID, "chain longer than 6 steps")
-    shape = out.shape
     parts = [struct.pack("=i4x", len(steps))]
     for kind, t, nb in steps:
         if t is None:
@@ -733,33 +753,48 @@ def _packed_chain(chain: Chain | None, out, cols: int):
     if r is not None and (r.dtype != out.dtype or r.shape != shape or r.stride() != out.stride()):
         raise SdbError(INVALID, "a chain's redirect has the output's type, extents and strides")
     parts.append(_CHAIN_TAIL.pack(r.data_ptr() if r is not None else 0, 1 if chain.from_redirect else 0))
-    return b"".join(parts)
+    packed = b"".join(parts)
+    chain._described = (key, packed)
+    return packed
 
 
-def _chain_tensors(chain: Chain | None) -> list:
-    if chain is None:
-        return []
-    found = [t for _, t, _ in chain.steps if t is not None]
-    return found + [chain.redirect_tensor] if chain.redirect_tensor is not None else found
+_raw_stream = None  # device index -> the address of its current stream
+_raw_device = None  # the current device's index
+
+
+def _find_raw() -> None:
+    """The two lookups a call makes, without the Python objects of torch.cuda.current_stream() (3 of a call's
+    8 microseconds on the host) where this torch offers that."""
+    global _raw_stream, _raw_device
+    import torch
+
+    torch.cuda.init()
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _on(fn, what: str, tensors, stream, *args) -> None:
     """Calls fn(*args, stream) with the tensors' device current, on `stream` or that device's current stream."""
-    import torch
-
     index = tensors[0].get_device()
     for t in tensors:
         if t.get_device() != index or index < 0:
             raise SdbError(INVALID, f"{what}: the tensors are not on one CUDA device")
-    if stream is not None and stream.device.index != index:
+    if _raw_stream is None:
+        _find_raw()
+    if stream is None:
+        address = _raw_stream(index)
+    elif stream.device.index != index:
         raise SdbError(INVALID, f"{what}: the stream is another device's")
-    if torch.cuda.current_device() == index:
-        s = stream if stream is not None else torch.cuda.current_stream()
-        status = fn(*args, s.cuda_stream)
     else:
+        address = stream.cuda_stream
+    if _raw_device() == index:
+        status = fn(*args, address)
+    else:
+        import torch
+
         with torch.cuda.device(index):
-            s = stream if stream is not None else torch.cuda.current_stream()
-            status = fn(*args, s.cuda_stream)
+            status = fn(*args, address)
     if status != OK:
         _check(status)
 
@@ -841,11 +876,9 @@ def mul_mat_q4(w: Q4, x, out=None, chain: Chain | None = None, stream=None):
 
     if out is None:
         out = torch.empty(*x.shape[:-1], w.n, dtype=x.dtype, device=x.device)
-    tensors = [w.data, x, out]
-    if chain is not None:
-        tensors += _chain_tensors(chain)
-    _on(load().sdb_mul_mat_q4, "mul_mat_q4", tensors, stream, w.struct, _packed(x, "mul_mat_q4"),
-        _packed(out, "mul_mat_q4"), _packed_chain(chain, out, w.n))
+    extra = _chain_tensors(chain)
+    _on((_lib or load()).sdb_mul_mat_q4, "mul_mat_q4", (w.data, x, out, *extra), stream, w.struct,
+        _packed(x, "mul_mat_q4"), _packed(out, "mul_mat_q4"), _packed_chain(chain, extra, out, w.n))
     return out
 
 
@@ -858,12 +891,10 @@ def mul_mat_q4_gated(w: Q4, gate: Q4, x, act: str = "gelu", out=None, chain: Cha
         raise SdbError(INVALID, f"mul_mat_q4_gated: no gate {act!r}")
     if out is None:
         out = torch.empty(*x.shape[:-1], w.n, dtype=x.dtype, device=x.device)
-    tensors = [w.data, gate.data, x, out]
-    if chain is not None:
-        tensors += _chain_tensors(chain)
-    _on(load().sdb_mul_mat_q4_gated, "mul_mat_q4_gated", tensors, stream, w.struct, gate.struct,
-        _packed(x, "mul_mat_q4_gated"), _packed(out, "mul_mat_q4_gated"), GATES[act],
-        _packed_chain(chain, out, 2 * w.n))
+    extra = _chain_tensors(chain)
+    _on((_lib or load()).sdb_mul_mat_q4_gated, "mul_mat_q4_gated", (w.data, gate.data, x, out, *extra), stream,
+        w.struct, gate.struct, _packed(x, "mul_mat_q4_gated"), _packed(out, "mul_mat_q4_gated"), GATES[act],
+        _packed_chain(chain, extra, out, 2 * w.n))
     return out
 
 
@@ -882,12 +913,17 @@ class Norm:
                 raise SdbError(INVALID, "a norm's weight and bias are dense FP32 (C,)")
 
     def packed(self, c: int) -> bytes:
-        for t in self.tensors:
-            if t.shape[0] != c:
-                raise SdbError(INVALID, f"a norm of {t.shape[0]} numbers for rows of {c}")
-        return _NORM_FORM.pack(NORMS[self.kind], self.eps,
-                               self.weight.data_ptr() if self.weight is not None else 0,
-                               self.bias.data_ptr() if self.bias is not None else 0)
+        """The sdb_norm_form for rows of c numbers."""
+        w = b = 0
+        if self.weight is not None:
+            w = self.weight.data_ptr()
+            if self.weight.shape[0] != c:
+                raise SdbError(INVALID, f"a norm of {self.weight.shape[0]} numbers for rows of {c}")
+        if self.bias is not None:
+            b = self.bias.data_ptr()
+            if self.bias.shape[0] != c:
+                raise SdbError(INVALID, f"a norm of {self.bias.shape[0]} numbers for rows of {c}")
+        return _NORM_FORM.pack(NORMS[self.kind], self.eps, w, b)
 
 
 _NO_NORM = _NORM_FORM.pack(0, 0.0, 0, 0)
@@ -897,13 +933,13 @@ def _packed_operand(t, shape) -> bytes:
     """An FP32 tensor broadcastable to `shape`, as the bytes of an sdb_operand."""
     if t is None:
         return _NO_OPERAND
-    if str(t.dtype) != "torch.float32":
+    if t.element_size() != 4 or not t.is_floating_point():
         raise SdbError(INVALID, "modulations are FP32")
-    nd, od = len(shape), t.dim()
-    if od > nd:
-        raise SdbError(INVALID, "a modulation has more dimensions than the rows")
     nb = [0, 0, 0, 0]
     ts, st = t.shape, t.stride()
+    nd, od = len(shape), len(ts)
+    if od > nd:
+        raise SdbError(INVALID, "a modulation has more dimensions than the rows")
     for d in range(od):
         e = ts[od - 1 - d]
         if e != 1:
@@ -922,20 +958,18 @@ def residual_norm(x, y, post: Norm | None = None, gate=None, keep: float = 1.0, 
     them.  h is of x's type, out of y's (of the other's where one is None); h may be x, out may be y (the
     update in place).  want_h / want_out False: that one is not made (None).
     """
-    import torch
-
     ref = x if x is not None else y
     if ref is None:
         raise SdbError(INVALID, "residual_norm: neither x nor y")
     shape = ref.shape
-    if want_h and h is None:
-        h = torch.empty(shape, dtype=ref.dtype, device=ref.device)
-    if want_out and out is None:
-        out = torch.empty(shape, dtype=(y if y is not None else x).dtype, device=ref.device)
     if not want_h:
         h = None
+    elif h is None:
+        h = ref.new_empty(shape)
     if not want_out:
         out = None
+    elif out is None:
+        out = (y if y is not None else x).new_empty(shape)
     tensors = [t for t in (ref, y, h, out, gate, mul, add) if t is not None]
     if post is not None:
         tensors += post.tensors
@@ -945,6 +979,8 @@ def residual_norm(x, y, post: Norm | None = None, gate=None, keep: float = 1.0, 
     params = b"".join((_KEEP_SCALE.pack(keep, scale),
                        _NO_NORM if post is None else post.packed(c), _NO_NORM if pre is None else pre.packed(c),
                        _packed_operand(gate, shape), _packed_operand(mul, shape), _packed_operand(add, shape)))
-    _on(load().sdb_residual_norm, "residual_norm", tensors, stream,
-        *(None if t is None else _packed(t, "residual_norm") for t in (x, y, h, out)), params)
+    what = "residual_norm"
+    _on((_lib or load()).sdb_residual_norm, what, tensors, stream,
+        _packed(x, what) if x is not None else None, _packed(y, what) if y is not None else None,
+        _packed(h, what) if h is not None else None, _packed(out, what) if out is not None else None, params)
     return h, out
