@@ -137,7 +137,7 @@ int sdb_q4_dequantize(const sdb_q4 *q, const sdb_tensor *w, void *stream);
 /* dst[m][n] = sum_k x[m][k] value[n][k], then the chain: sdb_mul_mat for 4-bit
  * weights and few rows (for hundreds of rows, sdb_q4_dequantize once and
  * sdb_mul_mat).  x [K, ...] and dst [N, ...] FP32 or FP16, each row contiguous,
- * rows over dimensions 1..3 at any strides; x and dst do not overlap.  Products
+ * rows (at most 2^20) over dimensions 1..3 at any strides; x and dst do not overlap.  Products
  * and sums are FP32 whatever the types (x to its last bit), dst rounded once.
  * A chain's redirect needs an FP32 dst.  No rows: nothing is done.  No device
  * memory is allocated and none is shared between calls. */

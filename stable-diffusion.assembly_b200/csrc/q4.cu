@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const T* __restrict__ 
             }
             word |= static_cast<uint32_t>(static_cast<int>(q)) << q4_bit(c);
         }
-        reinterpret_cast<uint32_t*>(v.codes)[q4_word(v, at.row, at.k0)] = word;
+        reinterpret_cast<uint32_t*>(v.codes)[q4_word(v, at.row, at.k0)] = word ^ 0x88888888u;
         if (at.k0 % v.group == 0) {
             const long long s = q4_scale(v, at.row, at.k0);
             v.scales[s] = dh;
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(256) q4_import_kernel(const uint8_t* __restric
             }
             word |= q << q4_bit(c);
         }
-        reinterpret_cast<uint32_t*>(v.codes)[q4_word(v, at.row, at.k0)] = word;
+        reinterpret_cast<uint32_t*>(v.codes)[q4_word(v, at.row, at.k0)] = word ^ 0x88888888u;
         if (at.k0 % v.group == 0) {
             const long long s = q4_scale(v, at.row, at.k0);
             const bool in = row_in && at.k0 < v.k;
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(256) q4_blocks_kernel(const uint8_t* __restric
             }
             word |= q << q4_bit(c);
         }
-        reinterpret_cast<uint32_t*>(v.codes)[q4_word(v, at.row, at.k0)] = word;
+        reinterpret_cast<uint32_t*>(v.codes)[q4_word(v, at.row, at.k0)] = word ^ 0x88888888u;
         if (first == 0) {
             const long long s = q4_scale(v, at.row, at.k0);
             uint32_t d = 0, m = 0;
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(256) q4_dequantize_kernel(Q4View v, float* __r
     for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
         const WordAt at = word_at(v, i);
         if (at.k0 >= v.k) continue;
-        const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(v.codes) + q4_word(v, at.row, at.k0));
+        const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(v.codes) + q4_word(v, at.row, at.k0)) ^ 0x88888888u;
         const long long s = q4_scale(v, at.row, at.k0);
         const float d = __half2float(v.scales[s]);
         const float m = v.minima ? __half2float(v.minima[s]) : 0.0f;

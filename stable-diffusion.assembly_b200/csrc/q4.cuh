@@ -5,11 +5,12 @@
 // after another and each in order of k:
 //   codes   [row tile][k-block][half 2][lane 32][4 words]: lane g * 4 + t of half h
 //           holds row 8 h + g; its word j the eight columns 32 j + 8 t + 0..7,
-//           columns 2 p and 2 p + 1 in bits 4 p and 4 p + 16.  A warp reads a
-//           half tile as one 512-byte run of 16 bytes a lane, and a word's
-//           nibble pairs are the operands of mma.m16n8k16 (rows g and g + 8 of
-//           lane (g, t)) when the columns of x are taken in the same order: a
-//           sum over k may take its terms in any order.
+//           columns i and i + 4 (i < 4) in byte i, low and high, each as code - 8
+//           in four bits, so that a nibble at the top of a byte is 16 (code - 8).
+//           A warp reads a half tile as one 512-byte run of 16 bytes a lane, and
+//           a word's low and high nibbles are operands of mma.m16n8k32 (rows g
+//           and g + 8 of lane (g, t)) when the columns of x are taken in the
+//           same order: a sum over k may take its terms in any order.
 //   scales  [row tile][k-block][g 8][half 2][128 / group] FP16: what lane (g, t)
 //           needs of a tile is one run of 16, 8 or 4 bytes.
 //   minima  as the scales, present with `minimum`.
@@ -81,6 +82,6 @@ __host__ __device__ inline long long q4_scale(const Q4View& v, long long r, long
 }
 
 // The bit of column i (0..7) of a word.
-__host__ __device__ constexpr int q4_bit(int i) { return (i >> 1) * 4 + (i & 1) * 16; }
+__host__ __device__ constexpr int q4_bit(int i) { return (i & 3) * 8 + (i >> 2) * 4; }
 
 }  // namespace sdb

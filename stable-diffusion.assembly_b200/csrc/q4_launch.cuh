@@ -1,6 +1,7 @@
 // The launches of q4_rows.cuh's kernel for one group size (a translation unit each: q4_rows_*.cu).
 #pragma once
 
+#include <algorithm>
 #include <atomic>
 
 #include "q4_rows.cuh"
@@ -8,11 +9,9 @@
 
 namespace sdb {
 
-template <int T, bool PAIRED, bool HALF, bool GATED, int G>
-int q4_launch_form(const Q4Args& a, const Q4Plan& p, cudaStream_t st) {
-    using S = Q4Shape<T, PAIRED, HALF, GATED>;
-    auto kern = q4_rows_kernel<T, PAIRED, HALF, GATED, G>;
-    const int bytes = S::fixed_bytes() + a.chunk * S::block_bytes(a.rows < S::kTokens ? a.rows : S::kTokens, 128 / G);
+template <class F, int G>
+int q4_launch_form(const Q4Args& args, const Q4Plan& p, cudaStream_t st) {
+    auto kern = q4_rows_kernel<F, G>;
     // The kernel's shared-memory limit is raised once on each device (it costs about as much as a launch).
     static std::atomic<uint64_t> raised{0};
     int dev = 0;
@@ -21,10 +20,26 @@ int q4_launch_form(const Q4Args& a, const Q4Plan& p, cudaStream_t st) {
         SDB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kQ4MaxShared));
         if (dev < 64) raised.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
+    Q4Args a = args;
+    a.cluster = p.cluster;
+    a.range = (a.w.kblocks + a.cluster - 1) / a.cluster;
+    // The k-blocks of x held at a time: all of the CTA's, or the multiple of WK that fits.
+    const int fixed = q4_fixed_bytes<F, G>(a.w.minima != nullptr);
+    const int block = F::block_bytes(std::min(a.rows, F::kTokens), 128 / G);
+    const int fit = (p.shared - fixed) / block;
+    int wk_log = p.wk_log;
+    while ((1 << wk_log) > F::kWarps || (wk_log > 0 && (1 << wk_log) > fit)) --wk_log;
+    const int wk = 1 << wk_log;
+    if (fit < wk) return fail(SDB_CUDA_ERROR, "mul_mat_q4: shared memory");
+    a.wk_log = wk_log;
+    a.chunk = std::min((a.range + wk - 1) / wk, fit / wk) * wk;
+    const int wr = F::kWarps / wk, groups = (a.w.tiles + wr - 1) / wr;
+    const int blocks = std::min(groups, std::max(1, current_sm_count() / a.cluster)) * a.cluster;
+    const int runs = (a.rows + F::kTokens - 1) / F::kTokens;  // of x's rows
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(p.blocks), static_cast<unsigned>(p.chunks));
-    cfg.blockDim = dim3(kQ4Threads);
-    cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(runs));
+    cfg.blockDim = dim3(32 * F::kWarps);
+    cfg.dynamicSmemBytes = static_cast<size_t>(fixed + a.chunk * block);
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -37,20 +52,21 @@ int q4_launch_form(const Q4Args& a, const Q4Plan& p, cudaStream_t st) {
     return SDB_OK;
 }
 
-template <bool HALF, bool GATED, int G>
+template <bool GATED, int G>
 int q4_launch_rows(const Q4Args& a, const Q4Plan& p, cudaStream_t st) {
-    if constexpr (!HALF)
-        if (p.form == 0) return q4_launch_form<1, true, HALF, GATED, G>(a, p, st);
-    if (p.form <= 1) return q4_launch_form<1, false, HALF, GATED, G>(a, p, st);
-    if (p.form == 2) return q4_launch_form<2, false, HALF, GATED, G>(a, p, st);
-    return q4_launch_form<4, false, HALF, GATED, G>(a, p, st);
+    if (p.form == 2) return q4_launch_form<Q4Digits<1, GATED>, G>(a, p, st);
+    if (p.form == 4) return q4_launch_form<Q4Digits<2, GATED>, G>(a, p, st);
+    if (p.form == 8) return q4_launch_form<Q4Digits<4, GATED>, G>(a, p, st);
+    if (p.form == 16)
+        return a.x_half ? q4_launch_form<Q4Halves<2, true, GATED>, G>(a, p, st)
+                        : q4_launch_form<Q4Halves<2, false, GATED>, G>(a, p, st);
+    return a.x_half ? q4_launch_form<Q4Halves<4, true, GATED>, G>(a, p, st)
+                    : q4_launch_form<Q4Halves<4, false, GATED>, G>(a, p, st);
 }
 
 template <int G>
-int q4_launch(const Q4Args& a, const Q4Plan& p, bool half, cudaStream_t st) {
-    const bool gated = a.gate.codes != nullptr;
-    if (half) return gated ? q4_launch_rows<true, true, G>(a, p, st) : q4_launch_rows<true, false, G>(a, p, st);
-    return gated ? q4_launch_rows<false, true, G>(a, p, st) : q4_launch_rows<false, false, G>(a, p, st);
+int q4_launch(const Q4Args& a, const Q4Plan& p, cudaStream_t st) {
+    return a.gate.codes ? q4_launch_rows<true, G>(a, p, st) : q4_launch_rows<false, G>(a, p, st);
 }
 
 }  // namespace sdb

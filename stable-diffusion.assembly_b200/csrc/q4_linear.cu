@@ -31,8 +31,8 @@ bool product_shapes(const sdb_q4* w, const sdb_tensor* x, const sdb_tensor* dst)
     if (x->ne[0] != w->k || dst->ne[0] != w->n) return false;
     for (int d = 1; d < 4; ++d)
         if (dst->ne[d] != x->ne[d] || (dst->ne[d] > 1 && dst->nb[d] == 0)) return false;
-    // Rows as 32-bit numbers; each extent on its own first, so that the product cannot overflow.
-    const int64_t limit = 1LL << 30;
+    // A grid's second dimension counts runs of rows; each extent on its own first, so that no product overflows.
+    const int64_t limit = 1LL << 20;
     if (x->ne[1] > limit || x->ne[2] > limit || x->ne[3] > limit) return false;
     const double rows = static_cast<double>(x->ne[1]) * x->ne[2] * x->ne[3];
     if (rows > static_cast<double>(limit)) return false;
@@ -52,22 +52,13 @@ bool chain_ok(const sdb_chain* c, const sdb_tensor* dst, bool gated) {
     return c->redirect == nullptr || (!gated && dst->type == SDB_TYPE_F32);
 }
 
-// Cuts the product: the rows of x a CTA takes (a form), the warps and CTAs that share a tile's k-blocks, the
-// k-blocks of x in shared memory at a time and the grid.
-Q4Plan plan(Q4Args& a, bool half) {
+// Cuts the product: the rows of x a CTA takes (a form), the warps and CTAs that share a tile's k-blocks.
+Q4Plan plan(const Q4Args& a) {
     Q4Plan p{};
-    p.form = !half && a.rows <= 4 ? 0 : a.rows <= 8 ? 1 : a.rows <= 16 ? 2 : 4;
-    const int tokens = p.form == 0 ? 4 : 8 * p.form;
-    p.chunks = (a.rows + tokens - 1) / tokens;
-    a.wk_log = a.w.kblocks <= 1 ? 0 : a.w.kblocks <= 2 ? 1 : a.w.kblocks <= 4 ? 2 : 3;
-    a.cluster = 1;
-    a.range = (a.w.kblocks + a.cluster - 1) / a.cluster;
-    const int columns = p.form == 0 ? 2 * std::min(a.rows, 4) : 8 * p.form * (half ? 1 : 2);
-    const int block = kQ4Column * columns + tokens * 4 * (1 + a.w.ng);
-    const int wk = 1 << a.wk_log;
-    a.chunk = std::max(wk, std::min((a.range + wk - 1) / wk * wk, 90 * 1024 / block / wk * wk));
-    const int groups = (a.w.tiles + kQ4Warps / wk - 1) / (kQ4Warps / wk);
-    p.blocks = std::min(groups, current_sm_count() * 2) * a.cluster;
+    p.form = a.rows <= 2 ? 2 : a.rows <= 4 ? 4 : a.rows <= 8 ? 8 : a.rows <= 16 ? 16 : 32;
+    p.wk_log = 3;
+    p.cluster = 1;
+    p.shared = kQ4MaxShared;
     return p;
 }
 
@@ -81,6 +72,7 @@ int run(const sdb_q4* w, const sdb_q4* gate, const sdb_tensor* x, const sdb_tens
     const bool half = x->type == SDB_TYPE_F16;
     const int es = half ? 2 : 4;
     a.y_half = dst->type == SDB_TYPE_F16;
+    a.x_half = half;
     a.x_vec = reinterpret_cast<uintptr_t>(x->data) % (4 * es) == 0;
     for (int d = 0; d < 3; ++d) {
         a.xnb[d] = x->nb[d + 1] / es;
@@ -93,10 +85,10 @@ int run(const sdb_q4* w, const sdb_q4* gate, const sdb_tensor* x, const sdb_tens
     a.act = act;
     a.chain = make_chain(chain);
     if (a.rows == 0) return SDB_OK;
-    const Q4Plan p = plan(a, half);
-    if (w->group == 32) return q4_launch<32>(a, p, half, st);
-    if (w->group == 64) return q4_launch<64>(a, p, half, st);
-    return q4_launch<128>(a, p, half, st);
+    const Q4Plan p = plan(a);
+    if (w->group == 32) return q4_launch<32>(a, p, st);
+    if (w->group == 64) return q4_launch<64>(a, p, st);
+    return q4_launch<128>(a, p, st);
 }
 
 }  // namespace

@@ -4,31 +4,39 @@
 //   S = sum_{k in g} (q[n][k] - 8) x[m][k]
 //
 // The weights' bytes are the work: each is read once for up to 32 rows of x.
-// The 16 weight rows of a tile are the M of mma.m16n8k16 and the rows of x its
-// N, so that one instruction turns 8 bytes a lane into sums for 8 columns; S
-// is summed over one group by the tensor core, from zero, and joins the FP32
-// sum with the group's scale.  q - 8 is exact in FP16 (0x6400 | q is 1024 + q;
-// a subtraction, or for a nibble four bits up a multiply-add, leaves q - 8).
+// The 16 weight rows of a tile are the M of an mma and the rows of x its N; S
+// is summed over one group by the tensor core, from zero, and joins FP32 sums
+// with the group's scale.  x is taken whole in one of two forms:
 //
-// FP32 rows of x are made FP16 pairs: a row's 128 numbers of a k-block are
-// scaled by a power of two that brings the greatest just under 2^15, x = hi + lo
-// with both FP16 -- off by 2^-24 of x at most, or 2^-40 of the k-block's
-// greatest number -- and the sum over the k-block is scaled back.  So the
-// products see x whole at any magnitude.  With up to four rows hi and lo are
-// two columns of one product (PAIRED), else two products.  FP16 rows are taken
-// as they are.
+// Digits (up to 8 rows).  A row's 128 numbers of a k-block are scaled by a
+//   power of two to integers below 2^30 -- off by 2^-31 of the k-block's
+//   greatest number at most, an FP32 number within 2^7 of it is whole -- and
+//   written as four signed base-256 digits, four columns of an integer product
+//   (m16n8k32, s8 x s8).  A nibble at the top of its byte is the operand
+//   16 (q - 8): three instructions unpack eight weights.  The sum is exact; it
+//   starts from 0x4b400000, so that its bits, read as FP32, are 1.5 * 2^23 + 16 S,
+//   and one subtraction makes it a number (|16 S| <= 2^21).  A k-block that
+//   holds an infinity or a NaN makes its row's sums NaN.
+// Halves (more rows, where the digits' four columns a row cost more than the
+//   unpacking saves).  The k-block is scaled so that its greatest number comes
+//   just under 2^15, x = hi + lo in FP16 -- off by 2^-24 of x at most, or 2^-40
+//   of the greatest -- two columns of FP16 products (m16n8k16; FP16 rows are one
+//   column, as they are).  q - 8 is exact in FP16 (0x6400 | q is 1024 + q; a
+//   subtraction, or for a nibble four bits up a multiply-add, leaves q - 8).
 //
-// A CTA is eight warps: WR tiles of rows side by side, WK = 8 / WR warps to a
-// tile that share its k-blocks, and up to eight CTAs of a cluster that share
-// them again.  x is split once into shared memory, each column of the products
-// a run of its eight k-slices' fragments (4 lanes of 8 bytes a slice) and 288
-// bytes to the next column, so that neither a column's stores nor a slice's
-// loads over eight columns meet a bank twice, and stays there for all the row
-// tiles the CTA walks.  A product's unused columns are not stored: their lanes
-// read what lies there and their sums go nowhere.  Weights go from memory to
-// registers, two k-blocks ahead.  The warps' sums meet in shared memory and are added in one order, so
-// a result does not turn on timing; the sums of a cluster's other CTAs are read
-// where they lie.
+// A CTA is 8 or 16 warps: WR tiles of rows side by side, WK warps to a tile
+// that share its k-blocks, and up to eight CTAs of a cluster that share them
+// again.  x is split once into shared memory, each column of the products a run
+// of its k-slices' fragments and 32 bytes more than a multiple of 128 to the
+// next column, so that neither a column's stores nor a slice's loads over eight
+// columns meet a bank twice, and stays there for all the row tiles the CTA
+// walks.  A product's unused columns are not stored: their lanes read what lies
+// there and their sums go nowhere.  Weights go from memory to a ring of
+// kRing k-blocks a warp in shared memory by asynchronous copies, which
+// wait for nothing but the warp's own reads.
+// The warps' sums meet in shared memory and are added in one order, so a result
+// does not turn on timing; the sums of a cluster's other CTAs are read where
+// they lie.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -42,10 +50,7 @@
 
 namespace sdb {
 
-constexpr int kQ4Warps = 8;
-constexpr int kQ4Threads = 32 * kQ4Warps;
 constexpr int kQ4MaxShared = 227 * 1024;
-constexpr int kQ4Column = 288;  // bytes of a column's k-block in shared memory: 8 slices x 32, and a step of 8 banks
 
 struct Q4Args {
     Q4View w, gate;            // gate: the gated form's second matrix
@@ -54,7 +59,7 @@ struct Q4Args {
     long long xnb[3], ynb[3];  // strides of rows in elements (dims 1..3)
     int ne1, ne2;
     int rows;                  // of x
-    int x_vec;                 // x's runs of four numbers are aligned
+    int x_half, x_vec;         // FP16 rows; their runs of four numbers are aligned
     int y_half;                // FP16 output
     int act;                   // SDB_GATE_*
     int wk_log;                // WK = 1 << wk_log
@@ -64,97 +69,48 @@ struct Q4Args {
     Chain chain;
 };
 
-// What a variant's shared memory holds.
-template <int T, bool PAIRED, bool HALF, bool GATED>
-struct Q4Shape {
-    static constexpr int kTokens = PAIRED ? 4 : 8 * T;            // rows of x of a CTA
-    static constexpr int kProducts = HALF || PAIRED ? T : 2 * T;  // products of a k-slice
-    static constexpr int kTiles = GATED ? 2 : 1;
-    static constexpr int kSums = PAIRED ? 2 : 4 * T;              // FP32 sums a lane has of a tile
-    static constexpr int kRedBuffers = T == 1 ? 2 : 1;
-    static constexpr int kRedFloats = kQ4Warps * kTiles * kSums * 32;
-    // Bytes of x a k-block with `tokens` rows: the columns of the products, the rows' scales and their sums
-    // over its groups; and after all k-blocks, what the lanes of unused columns read past the last.
-    static __host__ __device__ constexpr int columns(int tokens) { return PAIRED ? 2 * tokens : 8 * kProducts; }
-    static constexpr int block_bytes(int tokens, int ng) { return kQ4Column * columns(tokens) + kTokens * 4 * (1 + ng); }
-    static constexpr int fixed_bytes() { return kRedBuffers * kRedFloats * 4 + kTokens * 8 + 8 * kQ4Column; }
+// A row of x and of the output: where they begin, the output's coordinates.
+struct Q4Row {
+    long long x_at, y_at;
+    int i1, i2, i3, pad;
 };
 
-// c = a b, or c += a b.
-template <bool FIRST>
-__device__ __forceinline__ void q4_mma(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
-    if constexpr (FIRST)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%10, %10, %10, %10};"
-            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(0.0f));
+// BYTES of a lane's own, from global to shared memory, in the background.
+template <int BYTES>
+__device__ __forceinline__ void q4_copy(uint32_t to, const void* from) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
     else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
 }
 
-// u & mask | 0x64006400: two nibbles in the low bits of FP16 numbers from 1024 on.
-template <uint32_t MASK>
-__device__ __forceinline__ uint32_t q4_nibbles(uint32_t u) {
-    uint32_t v;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(u), "n"(MASK), "r"(0x64006400u));
-    return v;
-}
-
-__device__ __forceinline__ uint32_t q4_low(uint32_t u) {  // nibbles at bits 0 and 16: 1024 + q, less 1032
-    uint32_t v;
-    asm("sub.f16x2 %0, %1, %2;" : "=r"(v) : "r"(q4_nibbles<0x000f000fu>(u)), "r"(0x64086408u));
-    return v;
-}
-
-__device__ __forceinline__ uint32_t q4_high(uint32_t u) {  // at bits 4 and 20: (1024 + 16 q) / 16, less 72
-    uint32_t v;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;"
-        : "=r"(v)
-        : "r"(q4_nibbles<0x00f000f0u>(u)), "r"(0x2c002c00u), "r"(0xd480d480u));
-    return v;
-}
-
-// Weights pass through: not kept in L1, kept in L2 as any line (a next call may find them there).
-__device__ __forceinline__ uint4 q4_load(const uint4* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint2 q4_load(const uint2* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ unsigned q4_load(const unsigned* p) {
-    unsigned v;
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
-    return v;
-}
-
-// A k-block of a row tile as a lane holds it: the words of rows g and g + 8, the scales, the minima.
+// A k-block of a row tile as a lane holds it: the words of rows g and g + 8, the scales, the minima; and its
+// place in the ring: 32 lanes' words of rows g, of rows g + 8, then eight runs of scales, each for four lanes,
+// and as many of minima.
 template <int G>
 struct Q4Stage {
     static constexpr int kNg = 128 / G;
+    static constexpr int kRun = 4 * kNg;  // bytes of a lane's scales: rows g and g + 8
+    static __host__ __device__ constexpr int bytes(bool minima) { return 1024 + 8 * kRun * (minima ? 2 : 1); }
     uint4 lo, hi;
     uint32_t d[kNg], m[kNg];
 
-    static __device__ __forceinline__ void load_run(uint32_t (&r)[kNg], const uint8_t* p) {
+    static __device__ __forceinline__ void run(uint32_t (&r)[kNg], const uint8_t* p) {
         if constexpr (kNg == 4) {
-            const uint4 v = q4_load(reinterpret_cast<const uint4*>(p));
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
             r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
         } else if constexpr (kNg == 2) {
-            const uint2 v = q4_load(reinterpret_cast<const uint2*>(p));
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
             r[0] = v.x; r[1] = v.y;
         } else {
-            r[0] = q4_load(reinterpret_cast<const unsigned*>(p));
+            r[0] = *reinterpret_cast<const uint32_t*>(p);
         }
+    }
+    __device__ __forceinline__ void read(const uint8_t* slot, int lane, bool minima) {
+        lo = *reinterpret_cast<const uint4*>(slot + lane * 16);
+        hi = *reinterpret_cast<const uint4*>(slot + 512 + lane * 16);
+        run(d, slot + 1024 + lane / 4 * kRun);
+        if (minima) run(m, slot + 1024 + 8 * kRun + lane / 4 * kRun);
     }
     // Group i's numbers of rows g and g + 8.
     static __device__ __forceinline__ float2 pick(const uint32_t (&r)[kNg], int i) {
@@ -179,173 +135,416 @@ struct Q4Walk {
         scales += blocks * (4096 / G);
         if (minima) minima += blocks * (4096 / G);
     }
-    __device__ __forceinline__ void load(Q4Stage<G>& s) const {
-        s.lo = q4_load(reinterpret_cast<const uint4*>(codes));
-        s.hi = q4_load(reinterpret_cast<const uint4*>(codes) + 32);
-        Q4Stage<G>::load_run(s.d, scales);
-        if (minima) Q4Stage<G>::load_run(s.m, minima);
+    __device__ __forceinline__ void load(uint32_t slot, int lane) const {
+        constexpr int run = Q4Stage<G>::kRun;
+        q4_copy<16>(slot + lane * 16, codes);
+        q4_copy<16>(slot + 512 + lane * 16, codes + 512);
+        if (lane % 4 == 0) {
+            q4_copy<run>(slot + 1024 + lane / 4 * run, scales);
+            if (minima) q4_copy<run>(slot + 1024 + 8 * run + lane / 4 * run, minima);
+        }
     }
 };
 
-// Splits the CTA's rows of x for k-blocks [kb0, kb1) into shared memory: a warp takes a row's k-block, a
-// lane four numbers (columns 4 lane..): slice 2 (lane / 8) + lane % 2, and there lane / 2 % 4 of the column.
-template <int T, bool PAIRED, bool HALF, int G>
-__device__ __forceinline__ void q4_split(const Q4Args& a, const long long* row_at, int tokens, int kb0, int kb1,
-                                         uint8_t* frags, float* scales, float* sums) {
-    using S = Q4Shape<T, PAIRED, HALF, false>;
-    constexpr int NG = 128 / G;
-    const int lane = threadIdx.x & 31;
-    const int slice = (lane >> 3) * 2 + (lane & 1), t = (lane >> 1) & 3;
-    const int items = tokens * (kb1 - kb0), block = kQ4Column * S::columns(tokens);
-    for (int i = threadIdx.x / 32; i < items; i += kQ4Warps) {
-        const int b = i / tokens, m = i - b * tokens;
-        const long long k = (kb0 + b) * 128LL + lane * 4;
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        uint2 raw = make_uint2(0, 0);
-        if constexpr (HALF) {
-            const __half* p = static_cast<const __half*>(a.x) + row_at[m] + k;
-            if (a.x_vec && k + 4 <= a.w.k) {
-                raw = __ldg(reinterpret_cast<const uint2*>(p));
-            } else {
-                unsigned short h[4];
-                for (int c = 0; c < 4; ++c) h[c] = k + c < a.w.k ? __half_as_ushort(p[c]) : 0;
-                raw.x = h[0] | static_cast<uint32_t>(h[1]) << 16;
-                raw.y = h[2] | static_cast<uint32_t>(h[3]) << 16;
-            }
-            const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&raw.x));
-            const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
-            x[0] = f0.x; x[1] = f0.y; x[2] = f1.x; x[3] = f1.y;
+// Four numbers of a row from column k on, zeros past the row's end.
+__device__ __forceinline__ float4 q4_four(const Q4Args& a, long long at, int k) {
+    const int cols = static_cast<int>(a.w.k);
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (a.x_half) {
+        const __half* p = static_cast<const __half*>(a.x) + at + k;
+        if (a.x_vec && k + 4 <= cols) {
+            const uint2 r = __ldg(reinterpret_cast<const uint2*>(p));
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.x));
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
+            x = make_float4(f.x, f.y, h.x, h.y);
         } else {
-            const float* p = static_cast<const float*>(a.x) + row_at[m] + k;
-            if (a.x_vec && k + 4 <= a.w.k) {
-                const float4 f = __ldg(reinterpret_cast<const float4*>(p));
-                x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
-            } else {
-                for (int c = 0; c < 4; ++c) x[c] = k + c < a.w.k ? p[c] : 0.0f;
-            }
+            if (k < cols) x.x = __half2float(p[0]);
+            if (k + 1 < cols) x.y = __half2float(p[1]);
+            if (k + 2 < cols) x.z = __half2float(p[2]);
+            if (k + 3 < cols) x.w = __half2float(p[3]);
         }
-        uint8_t* base = frags + b * block + slice * 32 + t * 8;
-        auto slot = [&](int col) { return reinterpret_cast<uint2*>(base + col * kQ4Column); };
-        if constexpr (HALF) {
-            *slot(m) = raw;
+    } else {
+        const float* p = static_cast<const float*>(a.x) + at + k;
+        if (a.x_vec && k + 4 <= cols) {
+            x = __ldg(reinterpret_cast<const float4*>(p));
         } else {
-            float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-            // top < 2^(e - 126), e its exponent field: scaled by 2^(141 - e) it is below 2^15.  The field of
-            // that power is 268 - e, kept a normal number's; infinities (and NaN, which fmaxf passes over)
-            // stay what they are.
-            const int e = static_cast<int>(__float_as_uint(top) >> 23);
-            const int f = min(268 - e, 253);
+            if (k < cols) x.x = p[0];
+            if (k + 1 < cols) x.y = p[1];
+            if (k + 2 < cols) x.z = p[2];
+            if (k + 3 < cols) x.w = p[3];
+        }
+    }
+    return x;
+}
+
+// Splits x: item i is row i % tokens of k-block i / tokens of [kb0, kb1), a warp takes an item and a lane its
+// columns 4 lane .. 4 lane + 3: split(k-block, row, x).  The numbers are read kAhead items before they are
+// split; the loop has one copy of the splitting, whose instructions a CTA mostly passes once.
+template <int WARPS, class Split>
+__device__ __forceinline__ void q4_items(const Q4Args& a, const Q4Row* rows, int tokens, int kb0, int kb1, Split split) {
+    constexpr int kAhead = 3;
+    const int lane = threadIdx.x & 31, first = threadIdx.x / 32, items = tokens * (kb1 - kb0);
+    const unsigned inverse = 0xffffffffu / static_cast<unsigned>(tokens) + 1;  // i / tokens = high(i inverse), tokens > 1
+    float4 x[kAhead];
+    int b[kAhead], m[kAhead];
+#pragma unroll 1
+    for (int i = first - kAhead * WARPS; i < items; i += WARPS) {
+        if (i >= 0) split(b[0], m[0], x[0]);
+#pragma unroll
+        for (int u = 0; u + 1 < kAhead; ++u) {
+            x[u] = x[u + 1];
+            b[u] = b[u + 1];
+            m[u] = m[u + 1];
+        }
+        const int next = i + kAhead * WARPS;
+        if (next < items) {
+            constexpr int u = kAhead - 1;
+            b[u] = tokens == 1 ? next : static_cast<int>(__umulhi(static_cast<unsigned>(next), inverse));
+            m[u] = next - b[u] * tokens;
+            x[u] = q4_four(a, rows[m[u]].x_at, (kb0 + b[u]) * 128 + lane * 4);
+        }
+    }
+}
+
+// The greatest magnitude of a warp's numbers, as FP32 bits (a NaN's bits are greater than an infinity's).
+__device__ __forceinline__ uint32_t q4_top(float4 x) {
+    const uint32_t a = max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu);
+    const uint32_t b = max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu);
+    return __reduce_max_sync(~0u, max(a, b));
+}
+
+// The sums of a warp's numbers over its groups of G, in every lane.
+template <int G>
+__device__ __forceinline__ float q4_group_sum(float4 x) {
+    float s = (x.x + x.y) + (x.z + x.w);
+#pragma unroll
+    for (int o = 1; o < G / 4; o <<= 1) s += __shfl_xor_sync(~0u, s, o);
+    return s;
+}
+
+// Two FP32 numbers an instruction.
+__device__ __forceinline__ uint64_t q4_pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 q4_unpair(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t q4_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t q4_mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t q4_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// ---- x as digits: NT products of eight columns, 2 NT rows of x
+
+template <int NT, bool GATED_>
+struct Q4Digits {
+    static constexpr bool GATED = GATED_;
+    static constexpr int kTokens = 2 * NT;
+    static constexpr int kTiles = GATED ? 2 : 1;
+    static constexpr int kLaneSums = NT;         // of a tile, joined over the digits
+    static constexpr int kWarps = NT <= 2 && !GATED ? 16 : 8;
+    static constexpr int kRing = 4;              // k-blocks of a warp on their way
+    static constexpr int kColumn = 160;          // bytes: 4 slices x 32, and a step of 8 banks
+
+    // Shared memory of `chunk` k-blocks: the columns; each column's factor; each row's sums over the groups.
+    static __host__ __device__ int columns(int tokens) { return 4 * tokens; }
+    static __host__ __device__ int block_bytes(int tokens, int ng) {
+        return columns(tokens) * (kColumn + 4) + kTokens * 4 * ng;
+    }
+    static constexpr int kTail = 8 * NT * (kColumn + 4);  // what the lanes of unused columns read past the last
+    uint8_t* frags;
+    float* factors;
+    float* sums;
+    int cols;
+    __device__ __forceinline__ Q4Digits(const Q4Args& a, uint8_t* x, int tokens) {
+        cols = columns(tokens);
+        frags = x;
+        factors = reinterpret_cast<float*>(x + (a.chunk * cols + 8 * NT) * kColumn);
+        sums = factors + a.chunk * cols + 8 * NT;
+    }
+
+    // A column's digits of a k-block are a run of 128 bytes, a lane's four numbers a word of it.
+    template <int G>
+    __device__ __forceinline__ void split(const Q4Args& a, const Q4Row* rows, int tokens, int kb0, int kb1) const {
+        constexpr int NG = 128 / G;
+        const int lane = threadIdx.x & 31;
+        q4_items<kWarps>(a, rows, tokens, kb0, kb1, [&](int b, int m, float4 x) {
+            // top < 2^(e - 126), e its exponent field: 2^(156 - e) x is below 2^30.  The power's field is
+            // 283 - e, kept a normal number's.
+            const int e = static_cast<int>(q4_top(x) >> 23), f = min(283 - e, 253);
             const float up = __uint_as_float(static_cast<uint32_t>(f) << 23);
-            const float down = __uint_as_float(static_cast<uint32_t>(254 - f) << 23);
-            uint2 hi, lo;
-            for (int c = 0; c < 4; c += 2) {
-                const float u = x[c] * up, v = x[c + 1] * up;
-                const __half2 h = __floats2half2_rn(u, v);
-                const float2 r = __half22float2(h);
-                const __half2 l = __floats2half2_rn(u - r.x, v - r.y);
-                (c ? hi.y : hi.x) = *reinterpret_cast<const uint32_t*>(&h);
-                (c ? lo.y : lo.x) = *reinterpret_cast<const uint32_t*>(&l);
+            // v = sum of digits 256^p: adding 128 to each of the lower three makes them v's bytes.
+            auto digits = [&](float n) {
+                return (static_cast<uint32_t>(__float2int_rn(n * up)) + 0x00808080u) ^ 0x00808080u;
+            };
+            const uint32_t v0 = digits(x.x), v1 = digits(x.y), v2 = digits(x.z), v3 = digits(x.w);
+            const uint32_t l01 = __byte_perm(v0, v1, 0x5140), l23 = __byte_perm(v2, v3, 0x5140);
+            const uint32_t h01 = __byte_perm(v0, v1, 0x7362), h23 = __byte_perm(v2, v3, 0x7362);
+            uint32_t* to = reinterpret_cast<uint32_t*>(frags + (b * cols + 4 * m) * kColumn) + lane;
+            to[0] = __byte_perm(l01, l23, 0x5410);
+            to[kColumn / 4] = __byte_perm(l01, l23, 0x7632);
+            to[kColumn / 2] = __byte_perm(h01, h23, 0x5410);
+            to[kColumn / 4 * 3] = __byte_perm(h01, h23, 0x7632);
+            if (lane < 4) {  // digit p's factor: 2^(8 p) of the scale's inverse, and the weights' 1 / 16
+                const float down = __uint_as_float(static_cast<uint32_t>(254 - f + 8 * lane) << 23) * 0.0625f;
+                factors[b * cols + 4 * m + lane] = e == 255 ? __uint_as_float(0x7fffffffu) : down;
             }
-            if constexpr (PAIRED) {
-                *slot(2 * m) = hi;
-                *slot(2 * m + 1) = lo;
-            } else {
-                *slot(m / 8 * 16 + m % 8) = hi;
-                *slot(m / 8 * 16 + m % 8 + 8) = lo;
+            if (a.w.minima) {
+                const float s = q4_group_sum<G>(x);
+                if (lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
             }
-            if (lane == 0) scales[b * S::kTokens + m] = down;
-        }
-        if (a.w.minima) {
-            float s = (x[0] + x[1]) + (x[2] + x[3]);
-            for (int o = 1; o < G / 4; o <<= 1) s += __shfl_xor_sync(~0u, s, o);
-            if (lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * S::kTokens + m] = s;
-        }
+        });
     }
-}
 
-// One output element: the chain, the gate, the store.
-__device__ __forceinline__ void q4_finish(const Q4Args& a, int m, long long n, float v, float g, bool gated) {
-    const int q = m / a.ne1, i1 = m - q * a.ne1, i3 = q / a.ne2, i2 = q - i3 * a.ne2;
-    const long long at = n + i1 * a.ynb[0] + i2 * a.ynb[1] + i3 * a.ynb[2];
-    if (a.chain.from_redirect) v += static_cast<const float*>(a.y)[at];
-    v = apply_chain(a.chain, v, n, i1, i2, i3);
-    if (gated) {
-        g = apply_chain(a.chain, g, a.w.n + n, i1, i2, i3);
-        v *= a.act == SDB_GATE_SILU ? silu(g) : gelu(g);
-    }
-    if (a.y_half) static_cast<__half*>(a.y)[at] = __float2half_rn(v);
-    else static_cast<float*>(a.y)[at] = v;
-}
-
-template <int T, bool PAIRED, bool HALF, bool GATED, int G>
-__global__ void __launch_bounds__(kQ4Threads, T == 1 ? 2 : 1) q4_rows_kernel(const __grid_constant__ Q4Args a) {
-    using S = Q4Shape<T, PAIRED, HALF, GATED>;
-    constexpr int NG = 128 / G;
-    extern __shared__ __align__(16) uint8_t smem[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    const int wk = warp & ((1 << a.wk_log) - 1), wr = warp >> a.wk_log, WK = 1 << a.wk_log, WR = kQ4Warps >> a.wk_log;
-    const int rank = blockIdx.x % a.cluster;
-    const int groups = (a.w.tiles + WR - 1) / WR;                  // of WR row tiles
-    const int group0 = blockIdx.x / a.cluster, group_step = gridDim.x / a.cluster;
-    const int m0 = blockIdx.y * S::kTokens, tokens = min(S::kTokens, a.rows - m0);
-    const int kb_begin = rank * a.range, kb_end = min(kb_begin + a.range, a.w.kblocks);
-
-    float* red = reinterpret_cast<float*>(smem);
-    long long* row_at = reinterpret_cast<long long*>(red + S::kRedBuffers * S::kRedFloats);
-    uint8_t* frags = reinterpret_cast<uint8_t*>(row_at + S::kTokens);
-    const int block_bytes = kQ4Column * S::columns(tokens);
-    float* scales = reinterpret_cast<float*>(frags + a.chunk * block_bytes + 8 * kQ4Column);
-    float* sums = scales + a.chunk * S::kTokens;
-
-    // The warp's k-blocks in the order they are taken: over its row tiles, kb_begin + wk, + WK, ...  A warp
-    // past the last tile walks the last one again and stores nothing.
-    Q4Stage<G> stage[2][S::kTiles];
-    Q4Walk<G> walk[S::kTiles];
-    const int steps = kb_end - kb_begin > wk ? (kb_end - kb_begin - wk + WK - 1) >> a.wk_log : 0;  // of a tile
-    int load_group = group0, load_step = 0;
-    auto tile_of = [&](int group) { return min(group * WR + wr, a.w.tiles - 1); };
-    {
-        const long long block = static_cast<long long>(tile_of(group0)) * a.w.kblocks + kb_begin + wk;
-        walk[0].start(a.w, block, lane);
-        if constexpr (GATED) walk[1].start(a.gate, block, lane);
-    }
-    auto load = [&](Q4Stage<G> (&to)[S::kTiles]) {
-        if (load_group >= groups) return;
+    uint64_t acc[kTiles][NT][2];  // columns 2 t and 2 t + 1 of rows g, g + 8
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < S::kTiles; ++i) walk[i].load(to[i]);
-        long long blocks = WK;
-        if (++load_step == steps) {
-            load_step = 0;
-            const int next = load_group + group_step;
-            if (next < groups)
-                blocks = static_cast<long long>(tile_of(next) - tile_of(load_group)) * a.w.kblocks -
-                         static_cast<long long>(steps - 1) * WK;
-            load_group = next;
-        }
+        for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-        for (int i = 0; i < S::kTiles; ++i) walk[i].step(blocks);
-    };
-    if (steps == 0) load_group = groups;
-    load(stage[0]);
-    load(stage[1]);
-
-    if (threadIdx.x < tokens) {
-        const int m = m0 + threadIdx.x, q = m / a.ne1, i1 = m - q * a.ne1, i3 = q / a.ne2, i2 = q - i3 * a.ne2;
-        row_at[threadIdx.x] = i1 * a.xnb[0] + i2 * a.xnb[1] + i3 * a.xnb[2];
+            for (int t = 0; t < NT; ++t) acc[i][t][0] = acc[i][t][1] = 0;
     }
-    __syncthreads();
 
-    const uint8_t* lane_frags = frags + (lane >> 2) * kQ4Column + (lane & 3) * 8;
-    float acc[S::kTiles][S::kSums];
+    // c = a b + (first, first, first, first), or c += a b.
+    template <bool FIRST>
+    static __device__ __forceinline__ void mma(int (&c)[4], const uint32_t (&a)[4], uint2 b) {
+        if constexpr (FIRST)
+            asm volatile(
+                "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                "{%10, %10, %10, %10};"
+                : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(0x4b400000));
+        else
+            asm volatile(
+                "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                "{%0, %1, %2, %3};"
+                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+    }
+
     // One k-block, the chunk's at `at`.
-    auto product = [&](const Q4Stage<G> (&st)[S::kTiles], int at) {
-        const uint8_t* f = lane_frags + at * block_bytes;
-        float part[S::kTiles][S::kSums];  // the k-block's sums, in its rows' scales
-        float s[S::kTiles][T][4];         // a group's sums
-        uint32_t w[S::kTiles][2][4];
+    template <int G>
+    __device__ __forceinline__ void product(const Q4Stage<G> (&st)[kTiles], int at, bool minima) {
+        constexpr int NG = 128 / G, SL = 4 / NG;  // slices of 32 a group
+        const int lane = threadIdx.x & 31;
+        const uint8_t* f = frags + at * (cols * kColumn) + (lane >> 2) * kColumn + (lane & 3) * 8;
+        const uint64_t magic = q4_pair(-12582912.0f, -12582912.0f);
+        uint64_t part[kTiles][NT][2];  // the k-block's sums, in its rows' scales
+        uint32_t w[kTiles][2][4];
 #pragma unroll
-        for (int i = 0; i < S::kTiles; ++i) {
+        for (int i = 0; i < kTiles; ++i) {
+            w[i][0][0] = st[i].lo.x; w[i][0][1] = st[i].lo.y; w[i][0][2] = st[i].lo.z; w[i][0][3] = st[i].lo.w;
+            w[i][1][0] = st[i].hi.x; w[i][1][1] = st[i].hi.y; w[i][1][2] = st[i].hi.z; w[i][1][3] = st[i].hi.w;
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            uint32_t av[kTiles][SL][4];
+            uint64_t d0[kTiles], d1[kTiles];
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+                for (int s = 0; s < SL; ++s) {
+                    const uint32_t u0 = w[i][0][g * SL + s], u1 = w[i][1][g * SL + s];
+                    av[i][s][0] = u0 << 4 & 0xf0f0f0f0u;
+                    av[i][s][1] = u1 << 4 & 0xf0f0f0f0u;
+                    av[i][s][2] = u0 & 0xf0f0f0f0u;
+                    av[i][s][3] = u1 & 0xf0f0f0f0u;
+                }
+                const float2 d = Q4Stage<G>::pick(st[i].d, g);
+                d0[i] = q4_pair(d.x, d.x);
+                d1[i] = q4_pair(d.y, d.y);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                uint2 b[SL];
+#pragma unroll
+                for (int s = 0; s < SL; ++s)
+                    b[s] = *reinterpret_cast<const uint2*>(f + t * (8 * kColumn) + (g * SL + s) * 32);
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) {
+                    int c[4];
+                    mma<true>(c, av[i][0], b[0]);
+#pragma unroll
+                    for (int s = 1; s < SL; ++s) mma<false>(c, av[i][s], b[s]);
+                    const uint64_t v0 = q4_add2(q4_pair(__int_as_float(c[0]), __int_as_float(c[1])), magic);
+                    const uint64_t v1 = q4_add2(q4_pair(__int_as_float(c[2]), __int_as_float(c[3])), magic);
+                    part[i][t][0] = g == 0 ? q4_mul2(d0[i], v0) : q4_fma2(d0[i], v0, part[i][t][0]);
+                    part[i][t][1] = g == 0 ? q4_mul2(d1[i], v1) : q4_fma2(d1[i], v1, part[i][t][1]);
+                }
+            }
+            if (minima) {
+                // (m + 8 d) sum x, to one of a row's four columns: the even lanes' first.
+                const float* xs = sums + (at * NG + g) * kTokens + (lane >> 1 & 1);
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) {
+                    const float2 d = Q4Stage<G>::pick(st[i].d, g), mn = Q4Stage<G>::pick(st[i].m, g);
+                    const float o0 = lane & 1 ? 0.0f : fmaf(8.0f, d.x, mn.x);
+                    const float o1 = lane & 1 ? 0.0f : fmaf(8.0f, d.y, mn.y);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const float v = xs[2 * t];
+                        acc[i][t][0] = q4_fma2(q4_pair(o0, 0.0f), q4_pair(v, 0.0f), acc[i][t][0]);
+                        acc[i][t][1] = q4_fma2(q4_pair(o1, 0.0f), q4_pair(v, 0.0f), acc[i][t][1]);
+                    }
+                }
+            }
+        }
+        const float* factor = factors + at * cols + (lane & 3) * 2;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const uint64_t v = *reinterpret_cast<const uint64_t*>(factor + t * 8);
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+                acc[i][t][0] = q4_fma2(v, part[i][t][0], acc[i][t][0]);
+                acc[i][t][1] = q4_fma2(v, part[i][t][1], acc[i][t][1]);
+            }
+        }
+    }
+
+    // The lane's sum c of tile i: row lane / 4 (lane odd: + 8) of row 2 c + (lane / 2) % 2 of x.
+    __device__ __forceinline__ float lane_sum(int i, int c) const {
+        const float2 a = q4_unpair(acc[i][c][0]), b = q4_unpair(acc[i][c][1]);
+        float u = a.x + a.y, v = b.x + b.y;  // two digits of the four
+        u += __shfl_xor_sync(~0u, u, 1);
+        v += __shfl_xor_sync(~0u, v, 1);
+        return threadIdx.x & 1 ? v : u;
+    }
+    static __device__ __forceinline__ int row_of(int c, int lane) { return (lane >> 2) + 8 * (lane & 1); }
+    static __device__ __forceinline__ int token_of(int c, int lane) { return 2 * c + (lane >> 1 & 1); }
+};
+
+// ---- x as FP16 halves: T products of eight rows of x, HALF: FP16 rows as they are
+
+// (u & MASK) ^ FLIP: two nibbles, code - 8 in four bits, made codes in FP16 numbers from 1024 on.
+template <uint32_t MASK, uint32_t FLIP>
+__device__ __forceinline__ uint32_t q4_nibbles(uint32_t u) {
+    uint32_t v;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(v) : "r"(u), "n"(MASK), "r"(FLIP));
+    return v;
+}
+
+__device__ __forceinline__ uint32_t q4_low(uint32_t u) {  // nibbles at bits 0 and 16: 1024 + q, less 1032
+    uint32_t v;
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(v) : "r"(q4_nibbles<0x000f000fu, 0x64086408u>(u)), "r"(0x64086408u));
+    return v;
+}
+
+__device__ __forceinline__ uint32_t q4_high(uint32_t u) {  // at bits 4 and 20: (1024 + 16 q) / 16, less 72
+    uint32_t v;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;"
+        : "=r"(v)
+        : "r"(q4_nibbles<0x00f000f0u, 0x64806480u>(u)), "r"(0x2c002c00u), "r"(0xd480d480u));
+    return v;
+}
+
+// c = a b, or c += a b.
+template <bool FIRST>
+__device__ __forceinline__ void q4_mma(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
+    if constexpr (FIRST)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%10, %10, %10, %10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(0.0f));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+}
+
+template <int T, bool HALF, bool GATED_>
+struct Q4Halves {
+    static constexpr bool GATED = GATED_;
+    static constexpr int kTokens = 8 * T;
+    static constexpr int kTiles = GATED ? 2 : 1;
+    static constexpr int kLaneSums = 4 * T;
+    static constexpr int kProducts = HALF ? T : 2 * T;
+    static constexpr int kWarps = 8;
+    static constexpr int kRing = GATED ? 3 : 4;
+    static constexpr int kColumn = 288;  // bytes: 8 slices x 32, and a step of 8 banks
+
+    static __host__ __device__ int block_bytes(int, int ng) {
+        return 8 * kProducts * kColumn + kTokens * 4 * (1 + ng);
+    }
+    static constexpr int kTail = 0;
+    uint8_t* frags;
+    float* scales;  // of a row's k-block
+    float* sums;    // of a row's groups
+    __device__ __forceinline__ Q4Halves(const Q4Args& a, uint8_t* x, int) {
+        frags = x;
+        scales = reinterpret_cast<float*>(x + a.chunk * (8 * kProducts * kColumn));
+        sums = scales + a.chunk * kTokens;
+    }
+
+    // A lane's four numbers are columns 0..3 or 4..7 of the run of eight that lane t = lane / 2 % 4 of a fragment
+    // holds: a word of slice 2 (lane / 8), the even columns, and one of the next, the odd ones, of hi (a column
+    // of product 2 i) and of lo (the same column of product 2 i + 1); FP16 rows have no lo.
+    template <int G>
+    __device__ __forceinline__ void split(const Q4Args& a, const Q4Row* rows, int tokens, int kb0, int kb1) const {
+        constexpr int NG = 128 / G;
+        const int lane = threadIdx.x & 31;
+        q4_items<kWarps>(a, rows, tokens, kb0, kb1, [&](int b, int m, float4 x) {
+            uint8_t* to = frags + (b * (8 * kProducts) + (HALF ? m : m / 8 * 16 + m % 8)) * kColumn + (lane >> 3) * 64 +
+                          (lane >> 1 & 3) * 8 + (lane & 1) * 4;
+            if constexpr (HALF) {
+                *reinterpret_cast<__half2*>(to) = __floats2half2_rn(x.x, x.z);
+                *reinterpret_cast<__half2*>(to + 32) = __floats2half2_rn(x.y, x.w);
+            } else {
+                // top < 2^(e - 126), e its exponent field: scaled by 2^(141 - e) it is below 2^15.  The power's
+                // field is 268 - e, kept a normal number's; infinities and NaN stay what they are.
+                const int e = static_cast<int>(q4_top(x) >> 23), f = min(268 - e, 253);
+                const float up = __uint_as_float(static_cast<uint32_t>(f) << 23);
+                auto put = [&](float u, float v, int at) {
+                    const __half2 hi = __floats2half2_rn(u, v);
+                    const float2 r = __half22float2(hi);
+                    *reinterpret_cast<__half2*>(to + at) = hi;
+                    *reinterpret_cast<__half2*>(to + 8 * kColumn + at) = __floats2half2_rn(u - r.x, v - r.y);
+                };
+                put(x.x * up, x.z * up, 0);
+                put(x.y * up, x.w * up, 32);
+                if (lane == 0) scales[b * kTokens + m] = __uint_as_float(static_cast<uint32_t>(254 - f) << 23);
+            }
+            if (a.w.minima) {
+                const float s = q4_group_sum<G>(x);
+                if (lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
+            }
+        });
+    }
+
+    float acc[kTiles][kLaneSums];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+            for (int c = 0; c < kLaneSums; ++c) acc[i][c] = 0.0f;
+    }
+
+    template <int G>
+    __device__ __forceinline__ void product(const Q4Stage<G> (&st)[kTiles], int at, bool minima) {
+        constexpr int NG = 128 / G;
+        const int lane = threadIdx.x & 31;
+        const uint8_t* f = frags + at * (8 * kProducts * kColumn) + (lane >> 2) * kColumn + (lane & 3) * 8;
+        float part[kTiles][kLaneSums];  // the k-block's sums, in its rows' scales
+        float s[kTiles][T][4];          // a group's sums
+        uint32_t w[kTiles][2][4];
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
             w[i][0][0] = st[i].lo.x; w[i][0][1] = st[i].lo.y; w[i][0][2] = st[i].lo.z; w[i][0][3] = st[i].lo.w;
             w[i][1][0] = st[i].hi.x; w[i][1][1] = st[i].hi.y; w[i][1][2] = st[i].hi.z; w[i][1][3] = st[i].hi.w;
         }
@@ -353,23 +552,22 @@ __global__ void __launch_bounds__(kQ4Threads, T == 1 ? 2 : 1) q4_rows_kernel(con
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                uint32_t av[S::kTiles][4];
+                uint32_t av[kTiles][4];
 #pragma unroll
-                for (int i = 0; i < S::kTiles; ++i) {
+                for (int i = 0; i < kTiles; ++i) {
                     const uint32_t u0 = w[i][0][j] >> (8 * h), u1 = w[i][1][j] >> (8 * h);
                     av[i][0] = q4_low(u0);
                     av[i][1] = q4_low(u1);
                     av[i][2] = q4_high(u0);
                     av[i][3] = q4_high(u1);
                 }
-                const int slice = 2 * j + h;
 #pragma unroll
-                for (int p = 0; p < S::kProducts; ++p) {
-                    const uint2 b = *reinterpret_cast<const uint2*>(f + slice * 32 + p * (8 * kQ4Column));
-                    const int t = HALF || PAIRED ? p : p / 2;
-                    const bool first = j % (4 / NG) == 0 && h == 0 && (HALF || PAIRED || p % 2 == 0);
+                for (int p = 0; p < kProducts; ++p) {
+                    const uint2 b = *reinterpret_cast<const uint2*>(f + (2 * j + h) * 32 + p * (8 * kColumn));
+                    const int t = HALF ? p : p / 2;
+                    const bool first = j % (4 / NG) == 0 && h == 0 && (HALF || p % 2 == 0);
 #pragma unroll
-                    for (int i = 0; i < S::kTiles; ++i) {
+                    for (int i = 0; i < kTiles; ++i) {
                         if (first) q4_mma<true>(s[i][t], av[i], b);
                         else q4_mma<false>(s[i][t], av[i], b);
                     }
@@ -378,153 +576,216 @@ __global__ void __launch_bounds__(kQ4Threads, T == 1 ? 2 : 1) q4_rows_kernel(con
             if ((j + 1) % (4 / NG) != 0) continue;
             const int g = (j + 1) / (4 / NG) - 1;
 #pragma unroll
-            for (int i = 0; i < S::kTiles; ++i) {
+            for (int i = 0; i < kTiles; ++i) {
                 const float2 d = Q4Stage<G>::pick(st[i].d, g);
-                auto join = [&](int c, float scale, float v) {
-                    part[i][c] = g == 0 ? scale * v : fmaf(scale, v, part[i][c]);
-                };
 #pragma unroll
-                for (int t = 0; t < T; ++t) {
-                    if constexpr (PAIRED) {
-                        join(0, d.x, s[i][0][0] + s[i][0][1]);
-                        join(1, d.y, s[i][0][2] + s[i][0][3]);
-                    } else {
-                        join(4 * t, d.x, s[i][t][0]);
-                        join(4 * t + 1, d.x, s[i][t][1]);
-                        join(4 * t + 2, d.y, s[i][t][2]);
-                        join(4 * t + 3, d.y, s[i][t][3]);
-                    }
+                for (int c = 0; c < kLaneSums; ++c) {
+                    const float scale = c & 2 ? d.y : d.x, v = s[i][c / 4][c % 4];
+                    part[i][c] = g == 0 ? scale * v : fmaf(scale, v, part[i][c]);
                 }
             }
-            if (a.w.minima) {
-                const float* xs = sums + (at * NG + g) * S::kTokens;
+            if (minima) {
+                const float* xs = sums + (at * NG + g) * kTokens + (lane & 3) * 2;
 #pragma unroll
-                for (int i = 0; i < S::kTiles; ++i) {
+                for (int i = 0; i < kTiles; ++i) {
                     const float2 d = Q4Stage<G>::pick(st[i].d, g), mn = Q4Stage<G>::pick(st[i].m, g);
                     const float o0 = fmaf(8.0f, d.x, mn.x), o1 = fmaf(8.0f, d.y, mn.y);
-                    if constexpr (PAIRED) {
-                        const float v = xs[lane & 3];
-                        acc[i][0] = fmaf(o0, v, acc[i][0]);
-                        acc[i][1] = fmaf(o1, v, acc[i][1]);
-                    } else {
 #pragma unroll
-                        for (int t = 0; t < T; ++t) {
-                            const float2 v = *reinterpret_cast<const float2*>(xs + t * 8 + (lane & 3) * 2);
-                            acc[i][4 * t] = fmaf(o0, v.x, acc[i][4 * t]);
-                            acc[i][4 * t + 1] = fmaf(o0, v.y, acc[i][4 * t + 1]);
-                            acc[i][4 * t + 2] = fmaf(o1, v.x, acc[i][4 * t + 2]);
-                            acc[i][4 * t + 3] = fmaf(o1, v.y, acc[i][4 * t + 3]);
-                        }
+                    for (int t = 0; t < T; ++t) {
+                        const float2 v = *reinterpret_cast<const float2*>(xs + t * 8);
+                        acc[i][4 * t] = fmaf(o0, v.x, acc[i][4 * t]);
+                        acc[i][4 * t + 1] = fmaf(o0, v.y, acc[i][4 * t + 1]);
+                        acc[i][4 * t + 2] = fmaf(o1, v.x, acc[i][4 * t + 2]);
+                        acc[i][4 * t + 3] = fmaf(o1, v.y, acc[i][4 * t + 3]);
                     }
                 }
             }
         }
-        const float* xs = scales + at * S::kTokens;
+        const float* xs = scales + at * kTokens + (lane & 3) * 2;
 #pragma unroll
-        for (int i = 0; i < S::kTiles; ++i) {
-            if constexpr (HALF) {
+        for (int t = 0; t < T; ++t) {
+            const float2 v = HALF ? make_float2(1.0f, 1.0f) : *reinterpret_cast<const float2*>(xs + t * 8);
 #pragma unroll
-                for (int c = 0; c < S::kSums; ++c) acc[i][c] += part[i][c];
-            } else if constexpr (PAIRED) {
-                const float v = xs[lane & 3];
-                acc[i][0] = fmaf(v, part[i][0], acc[i][0]);
-                acc[i][1] = fmaf(v, part[i][1], acc[i][1]);
-            } else {
+            for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-                for (int t = 0; t < T; ++t) {
-                    const float2 v = *reinterpret_cast<const float2*>(xs + t * 8 + (lane & 3) * 2);
-                    acc[i][4 * t] = fmaf(v.x, part[i][4 * t], acc[i][4 * t]);
-                    acc[i][4 * t + 1] = fmaf(v.y, part[i][4 * t + 1], acc[i][4 * t + 1]);
-                    acc[i][4 * t + 2] = fmaf(v.x, part[i][4 * t + 2], acc[i][4 * t + 2]);
-                    acc[i][4 * t + 3] = fmaf(v.y, part[i][4 * t + 3], acc[i][4 * t + 3]);
-                }
-            }
+                for (int c = 0; c < 4; ++c)
+                    acc[i][4 * t + c] = fmaf(c & 1 ? v.y : v.x, part[i][4 * t + c], acc[i][4 * t + c]);
         }
+    }
+
+    __device__ __forceinline__ float lane_sum(int i, int c) const { return acc[i][c]; }
+    static __device__ __forceinline__ int row_of(int c, int lane) { return (lane >> 2) + 4 * (c & 2); }
+    static __device__ __forceinline__ int token_of(int c, int lane) { return c / 4 * 8 + (lane & 3) * 2 + (c & 1); }
+};
+
+// ---- the kernel
+
+// One output element: the chain, the gate, the store.
+__device__ __forceinline__ void q4_finish(const Q4Args& a, const Q4Row& row, long long n, float v, float g, bool gated) {
+    const long long at = row.y_at + n;
+    if (a.chain.from_redirect) v += static_cast<const float*>(a.y)[at];
+    v = apply_chain(a.chain, v, n, row.i1, row.i2, row.i3);
+    if (gated) {
+        g = apply_chain(a.chain, g, a.w.n + n, row.i1, row.i2, row.i3);
+        v *= a.act == SDB_GATE_SILU ? silu(g) : gelu(g);
+    }
+    if (a.y_half) static_cast<__half*>(a.y)[at] = __float2half_rn(v);
+    else static_cast<float*>(a.y)[at] = v;
+}
+
+// The warps' sums: two buffers where they are small.
+template <class F>
+constexpr int q4_red_floats() { return F::kWarps * F::kTiles * F::kLaneSums * 32; }
+template <class F>
+constexpr int q4_red_buffers() { return F::kLaneSums <= 4 ? 2 : 1; }
+
+// Shared memory but for the k-blocks of x.
+template <class F, int G>
+int q4_fixed_bytes(bool minima) {
+    return q4_red_buffers<F>() * q4_red_floats<F>() * 4 + F::kTokens * static_cast<int>(sizeof(Q4Row)) +
+           F::kWarps * F::kRing * F::kTiles * Q4Stage<G>::bytes(minima) + F::kTail;
+}
+
+template <class F, int G>
+__global__ void __launch_bounds__(32 * F::kWarps, 1) q4_rows_kernel(const __grid_constant__ Q4Args a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const int WK = 1 << a.wk_log, WR = F::kWarps >> a.wk_log, wk = warp & (WK - 1), wr = warp >> a.wk_log;
+    const int rank = a.cluster > 1 ? blockIdx.x % a.cluster : 0;
+    const int groups = (a.w.tiles + WR - 1) / WR;  // of WR row tiles
+    const int group0 = a.cluster > 1 ? blockIdx.x / a.cluster : blockIdx.x;
+    const int group_step = a.cluster > 1 ? gridDim.x / a.cluster : gridDim.x;
+    const int m0 = blockIdx.y * F::kTokens, tokens = min(F::kTokens, a.rows - m0);
+    const int kb_begin = rank * a.range, kb_end = min(kb_begin + a.range, a.w.kblocks);
+    const bool minima = a.w.minima != nullptr;
+
+    float* red = reinterpret_cast<float*>(smem);
+    Q4Row* rows = reinterpret_cast<Q4Row*>(red + q4_red_buffers<F>() * q4_red_floats<F>());
+    const int slot_bytes = Q4Stage<G>::bytes(minima), turn_bytes = F::kTiles * slot_bytes;
+    uint8_t* ring = reinterpret_cast<uint8_t*>(rows + F::kTokens) + warp * (F::kRing * turn_bytes);
+    F form(a, reinterpret_cast<uint8_t*>(rows + F::kTokens) + F::kWarps * F::kRing * turn_bytes, tokens);
+
+    // The warp's k-blocks in the order they are taken: over its row tiles, kb_begin + wk, + WK, ...  A warp
+    // past the last tile walks the last one again and stores nothing.
+    Q4Walk<G> walk[F::kTiles];
+    const int steps = kb_end - kb_begin > wk ? (kb_end - kb_begin - wk + WK - 1) >> a.wk_log : 0;  // of a tile
+    int load_group = group0, load_step = 0;
+    auto tile_of = [&](int group) { return min(group * WR + wr, a.w.tiles - 1); };
+    {
+        const long long block = static_cast<long long>(tile_of(group0)) * a.w.kblocks + kb_begin + wk;
+        walk[0].start(a.w, block, lane);
+        if constexpr (F::GATED) walk[1].start(a.gate, block, lane);
+    }
+    auto load = [&](int turn) {
+        if (load_group < groups) {
+            const uint32_t slot = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + turn * turn_bytes;
+#pragma unroll
+            for (int i = 0; i < F::kTiles; ++i) walk[i].load(slot + i * slot_bytes, lane);
+            long long blocks = WK;
+            if (++load_step == steps) {
+                load_step = 0;
+                const int next = load_group + group_step;
+                if (next < groups)
+                    blocks = static_cast<long long>(tile_of(next) - tile_of(load_group)) * a.w.kblocks -
+                             static_cast<long long>(steps - 1) * WK;
+                load_group = next;
+            }
+#pragma unroll
+            for (int i = 0; i < F::kTiles; ++i) walk[i].step(blocks);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    if (steps == 0) load_group = groups;
+#pragma unroll 1
+    for (int turn = 0; turn < F::kRing - 1; ++turn) load(turn);
+
+    if (threadIdx.x < tokens) {
+        const int m = m0 + threadIdx.x, q = m / a.ne1, i1 = m - q * a.ne1, i3 = q / a.ne2, i2 = q - i3 * a.ne2;
+        rows[threadIdx.x] = {i1 * a.xnb[0] + i2 * a.xnb[1] + i3 * a.xnb[2],
+                             i1 * a.ynb[0] + i2 * a.ynb[1] + i3 * a.ynb[2], i1, i2, i3, 0};
+    }
+    __syncthreads();
 
     bool held = false;  // the one chunk of x is in shared memory
-    int parity = 0;
+    int parity = 0, turn = 0;
+#pragma unroll 1
     for (int group = group0; group < groups; group += group_step) {
-#pragma unroll
-        for (int i = 0; i < S::kTiles; ++i)
-#pragma unroll
-            for (int c = 0; c < S::kSums; ++c) acc[i][c] = 0.0f;
+        form.clear();
+#pragma unroll 1
         for (int kc = kb_begin; kc < kb_end; kc += a.chunk) {
             const int kc_end = min(kc + a.chunk, kb_end);
             if (!held) {
                 if (kc != kb_begin || group != group0) __syncthreads();  // the chunk before has been read
-                q4_split<T, PAIRED, HALF, G>(a, row_at, tokens, kc, kc_end, frags, scales, sums);
+                form.template split<G>(a, rows, tokens, kc, kc_end);
                 __syncthreads();
                 held = a.chunk >= kb_end - kb_begin;
             }
-            int at = wk;
-            for (; at + WK < kc_end - kc; at += 2 * WK) {
-                product(stage[0], at);
-                load(stage[0]);
-                product(stage[1], at + WK);
-                load(stage[1]);
-            }
-            if (at < kc_end - kc) {
-                product(stage[0], at);
+#pragma unroll 1
+            for (int at = wk; at < kc_end - kc; at += WK) {
+                // The oldest of the ring's k-blocks has come, to every lane; the place filled next is the one that
+                // all lanes have read before this.
+                asm volatile("cp.async.wait_group %0;" ::"n"(F::kRing - 2) : "memory");
+                __syncwarp();
+                Q4Stage<G> stage[F::kTiles];
 #pragma unroll
-                for (int i = 0; i < S::kTiles; ++i) stage[0][i] = stage[1][i];
-                load(stage[1]);
+                for (int i = 0; i < F::kTiles; ++i)
+                    stage[i].read(ring + turn * turn_bytes + i * slot_bytes, lane, minima);
+                load((turn + F::kRing - 1) % F::kRing);
+                turn = (turn + 1) % F::kRing;
+                form.template product<G>(stage, at, minima);
             }
         }
 
-        // The warps' sums: [warp][tile][sum][lane].
-        float* mine = red + parity * S::kRedFloats;
+        // The warps' sums: [sum][tile][warp][lane].  Of two buffers, the one written next has been read by
+        // every thread before the barrier in between.
+        float* mine = red + parity * q4_red_floats<F>();
+        if constexpr (q4_red_buffers<F>() == 2) parity ^= 1;
 #pragma unroll
-        for (int i = 0; i < S::kTiles; ++i)
+        for (int c = 0; c < F::kLaneSums; ++c)
 #pragma unroll
-            for (int c = 0; c < S::kSums; ++c) mine[((warp * S::kTiles + i) * S::kSums + c) * 32 + lane] = acc[i][c];
+            for (int i = 0; i < F::kTiles; ++i)
+                mine[((c * F::kTiles + i) * F::kWarps + warp) * 32 + lane] = form.lane_sum(i, c);
         if (a.cluster > 1) cooperative_groups::this_cluster().sync();
         else __syncthreads();
-        // An output's sums lie WK (of each CTA) apart; a cluster's CTAs share the outputs.
-        const int outs = WR * 16 * tokens;
-        for (int o = threadIdx.x * a.cluster + rank; o < outs; o += kQ4Threads * a.cluster) {
-            const int r = o & 15, q = o >> 4, m = q / WR, tw = q - m * WR;
-            const long long n = (static_cast<long long>(group) * WR + tw) * 16 + r;
-            if (n >= a.w.n) continue;
-            int c, l;
-            if constexpr (PAIRED) {
-                c = r >> 3;
-                l = (r & 7) * 4 + m;
-            } else {
-                c = (m >> 3) * 4 + (r >> 3) * 2 + (m & 1);
-                l = (r & 7) * 4 + ((m & 7) >> 1);
-            }
+        // A warp finishes a sum of a tile; a cluster's CTAs share them.
+#pragma unroll 1
+        for (int o = warp * a.cluster + rank; o < F::kLaneSums * WR; o += F::kWarps * a.cluster) {
+            const int c = o / WR, tw = o - c * WR;
+            const int m = F::token_of(c, lane);
+            const long long n = (static_cast<long long>(group) * WR + tw) * 16 + F::row_of(c, lane);
+            if (m >= tokens || n >= a.w.n) continue;
             float v[2] = {0.0f, 0.0f};
+#pragma unroll 1
             for (int k = 0; k < a.cluster; ++k) {
-                const float* from =
-                    a.cluster > 1 ? cooperative_groups::this_cluster().map_shared_rank(mine, k) : mine;
+                const float* from = a.cluster > 1 ? cooperative_groups::this_cluster().map_shared_rank(mine, k) : mine;
+#pragma unroll 4
                 for (int j = 0; j < WK; ++j) {
 #pragma unroll
-                    for (int i = 0; i < S::kTiles; ++i)
-                        v[i] += from[(((tw * WK + j) * S::kTiles + i) * S::kSums + c) * 32 + l];
+                    for (int i = 0; i < F::kTiles; ++i)
+                        v[i] += from[((c * F::kTiles + i) * F::kWarps + tw * WK + j) * 32 + lane];
                 }
             }
-            q4_finish(a, m0 + m, n, v[0], v[1], GATED);
+            q4_finish(a, rows[m], n, v[0], v[1], F::GATED);
         }
-        if constexpr (S::kRedBuffers == 2) {
-            parity ^= 1;  // the buffer is written again after the next barrier
-        } else {
+        if constexpr (q4_red_buffers<F>() == 1) {
             if (a.cluster > 1) cooperative_groups::this_cluster().sync();
             else __syncthreads();
         }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (a.cluster > 1) cooperative_groups::this_cluster().sync();  // the others have read this CTA's sums
 }
 
-// How a product is cut: see q4_linear.cu.
+// How a product is cut (q4_linear.cu).
 struct Q4Plan {
-    int form;      // 0: PAIRED; else T = 1, 2 or 4
-    int blocks;    // grid x
-    int chunks;    // grid y: rows of x in runs of the form's tokens
+    int form;      // rows of x a CTA takes: 2, 4 or 8 in digits; 16 or 32 in halves
+    int wk_log;    // warps that share a row tile's k-blocks (fewer where their k-blocks of x do not fit)
+    int cluster;   // CTAs that do
+    int shared;    // bytes of shared memory a CTA may take
 };
 
-// Launches the kernel for FP16 or FP32 rows, plain or gated, groups of G; cudaGetLastError() says how it went.
+// Launches the kernel for rows in FP16 or FP32, plain or gated, groups of G.
 template <int G>
-int q4_launch(const Q4Args& a, const Q4Plan& p, bool half, cudaStream_t st);
+int q4_launch(const Q4Args& a, const Q4Plan& p, cudaStream_t st);
 
 }  // namespace sdb

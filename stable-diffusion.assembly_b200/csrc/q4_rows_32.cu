@@ -3,6 +3,6 @@
 
 namespace sdb {
 
-template int q4_launch<32>(const Q4Args&, const Q4Plan&, bool, cudaStream_t);
+template int q4_launch<32>(const Q4Args&, const Q4Plan&, cudaStream_t);
 
 }  // namespace sdb
