@@ -38,7 +38,7 @@ int q4_launch_form(const Q4Args& args, const Q4Plan& p, cudaStream_t st) {
     const int runs = (a.rows + F::kTokens - 1) / F::kTokens;  // of x's rows
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(runs));
-    cfg.blockDim = dim3(32 * F::kWarps);
+    cfg.blockDim = dim3(q4_threads<F>());
     cfg.dynamicSmemBytes = static_cast<size_t>(fixed + a.chunk * block);
     cfg.stream = st;
     cudaLaunchAttribute attr{};

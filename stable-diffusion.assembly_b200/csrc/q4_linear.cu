@@ -81,6 +81,7 @@ int run(const sdb_q4* w, const sdb_q4* gate, const sdb_tensor* x, const sdb_tens
     }
     a.ne1 = static_cast<int>(x->ne[1]);
     a.ne2 = static_cast<int>(x->ne[2]);
+    a.flat = x->ne[2] == 1 && x->ne[3] == 1;
     a.rows = static_cast<int>(x->ne[1] * x->ne[2] * x->ne[3]);
     a.act = act;
     a.chain = make_chain(chain);

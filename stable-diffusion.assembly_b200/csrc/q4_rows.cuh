@@ -59,6 +59,7 @@ struct Q4Args {
     long long xnb[3], ynb[3];  // strides of rows in elements (dims 1..3)
     int ne1, ne2;
     int rows;                  // of x
+    int flat;                  // rows along dimension 1 alone
     int x_half, x_vec;         // FP16 rows; their runs of four numbers are aligned
     int y_half;                // FP16 output
     int act;                   // SDB_GATE_*
@@ -69,10 +70,20 @@ struct Q4Args {
     Chain chain;
 };
 
-// A row of x and of the output: where they begin, the output's coordinates.
+// Row m's coordinates along dimensions 1..3.
 struct Q4Row {
-    long long x_at, y_at;
-    int i1, i2, i3, pad;
+    int i1, i2, i3;
+    __device__ __forceinline__ Q4Row(const Q4Args& a, int m) : i1(m), i2(0), i3(0) {
+        if (!a.flat) {
+            const int q = m / a.ne1;
+            i1 = m - q * a.ne1;
+            i3 = q / a.ne2;
+            i2 = q - i3 * a.ne2;
+        }
+    }
+    __device__ __forceinline__ long long at(const long long (&nb)[3]) const {
+        return i1 * nb[0] + i2 * nb[1] + i3 * nb[2];
+    }
 };
 
 // BYTES of a lane's own, from global to shared memory, in the background.
@@ -178,31 +189,35 @@ __device__ __forceinline__ float4 q4_four(const Q4Args& a, long long at, int k) 
 }
 
 // Splits x: item i is row i % tokens of k-block i / tokens of [kb0, kb1), a warp takes an item and a lane its
-// columns 4 lane .. 4 lane + 3: split(k-block, row, x).  The numbers are read kAhead items before they are
-// split; the loop has one copy of the splitting, whose instructions a CTA mostly passes once.
-template <int WARPS, class Split>
-__device__ __forceinline__ void q4_items(const Q4Args& a, const Q4Row* rows, int tokens, int kb0, int kb1, Split split) {
-    constexpr int kAhead = 3;
-    const int lane = threadIdx.x & 31, first = threadIdx.x / 32, items = tokens * (kb1 - kb0);
+// columns 4 lane .. 4 lane + 3: split(k-block, row, x).  Two items at a time, whose chains of dependent steps
+// overlap, and the next two read before; between() once the first are on their way.  (One copy of the loop's
+// code: a CTA passes it a few times, and the first pass waits for its instructions.)
+template <int WARPS, class Between, class Split>
+__device__ __forceinline__ void q4_items(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Between between,
+                                         Split split) {
+    const int lane = threadIdx.x & 31, items = tokens * (kb1 - kb0);
     const unsigned inverse = 0xffffffffu / static_cast<unsigned>(tokens) + 1;  // i / tokens = high(i inverse), tokens > 1
-    float4 x[kAhead];
-    int b[kAhead], m[kAhead];
+    float4 x[2];
+    int b[2], m[2];
+    auto read = [&](int i, int u) {
+        b[u] = tokens == 1 ? i : static_cast<int>(__umulhi(static_cast<unsigned>(i), inverse));
+        m[u] = i - b[u] * tokens;
+        if (i < items) x[u] = q4_four(a, Q4Row(a, m0 + m[u]).at(a.xnb), (kb0 + b[u]) * 128 + lane * 4);
+    };
+    int i = threadIdx.x / 32;
+    read(i, 0);
+    read(i + WARPS, 1);
+    between();
 #pragma unroll 1
-    for (int i = first - kAhead * WARPS; i < items; i += WARPS) {
-        if (i >= 0) split(b[0], m[0], x[0]);
-#pragma unroll
-        for (int u = 0; u + 1 < kAhead; ++u) {
-            x[u] = x[u + 1];
-            b[u] = b[u + 1];
-            m[u] = m[u + 1];
-        }
-        const int next = i + kAhead * WARPS;
-        if (next < items) {
-            constexpr int u = kAhead - 1;
-            b[u] = tokens == 1 ? next : static_cast<int>(__umulhi(static_cast<unsigned>(next), inverse));
-            m[u] = next - b[u] * tokens;
-            x[u] = q4_four(a, rows[m[u]].x_at, (kb0 + b[u]) * 128 + lane * 4);
-        }
+    while (i < items) {
+        const float4 x0 = x[0], x1 = x[1];
+        const int b0 = b[0], b1 = b[1], r0 = m[0], r1 = m[1];
+        const bool two = i + WARPS < items;
+        i += 2 * WARPS;
+        read(i, 0);
+        read(i + WARPS, 1);
+        split(b0, r0, x0, true);
+        split(b1, r1, x1, two);  // without a second item: computed on what is there and not stored
     }
 }
 
@@ -259,6 +274,7 @@ struct Q4Digits {
     static constexpr int kLaneSums = NT;         // of a tile, joined over the digits
     static constexpr int kWarps = NT <= 2 && !GATED ? 16 : 8;
     static constexpr int kRing = 4;              // k-blocks of a warp on their way
+    static constexpr bool kFinisher = NT <= 2;   // a warp of its own finishes the sums
     static constexpr int kColumn = 160;          // bytes: 4 slices x 32, and a step of 8 banks
 
     // Shared memory of `chunk` k-blocks: the columns; each column's factor; each row's sums over the groups.
@@ -279,11 +295,11 @@ struct Q4Digits {
     }
 
     // A column's digits of a k-block are a run of 128 bytes, a lane's four numbers a word of it.
-    template <int G>
-    __device__ __forceinline__ void split(const Q4Args& a, const Q4Row* rows, int tokens, int kb0, int kb1) const {
+    template <int G, class Between>
+    __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Between between) const {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
-        q4_items<kWarps>(a, rows, tokens, kb0, kb1, [&](int b, int m, float4 x) {
+        q4_items<kWarps>(a, m0, tokens, kb0, kb1, between, [&](int b, int m, float4 x, bool store) {
             // top < 2^(e - 126), e its exponent field: 2^(156 - e) x is below 2^30.  The power's field is
             // 283 - e, kept a normal number's.
             const int e = static_cast<int>(q4_top(x) >> 23), f = min(283 - e, 253);
@@ -295,18 +311,20 @@ struct Q4Digits {
             const uint32_t v0 = digits(x.x), v1 = digits(x.y), v2 = digits(x.z), v3 = digits(x.w);
             const uint32_t l01 = __byte_perm(v0, v1, 0x5140), l23 = __byte_perm(v2, v3, 0x5140);
             const uint32_t h01 = __byte_perm(v0, v1, 0x7362), h23 = __byte_perm(v2, v3, 0x7362);
-            uint32_t* to = reinterpret_cast<uint32_t*>(frags + (b * cols + 4 * m) * kColumn) + lane;
-            to[0] = __byte_perm(l01, l23, 0x5410);
-            to[kColumn / 4] = __byte_perm(l01, l23, 0x7632);
-            to[kColumn / 2] = __byte_perm(h01, h23, 0x5410);
-            to[kColumn / 4 * 3] = __byte_perm(h01, h23, 0x7632);
-            if (lane < 4) {  // digit p's factor: 2^(8 p) of the scale's inverse, and the weights' 1 / 16
+            if (store) {
+                uint32_t* to = reinterpret_cast<uint32_t*>(frags + (b * cols + 4 * m) * kColumn) + lane;
+                to[0] = __byte_perm(l01, l23, 0x5410);
+                to[kColumn / 4] = __byte_perm(l01, l23, 0x7632);
+                to[kColumn / 2] = __byte_perm(h01, h23, 0x5410);
+                to[kColumn / 4 * 3] = __byte_perm(h01, h23, 0x7632);
+            }
+            if (store && lane < 4) {  // digit p's factor: 2^(8 p) of the scale's inverse, and the weights' 1 / 16
                 const float down = __uint_as_float(static_cast<uint32_t>(254 - f + 8 * lane) << 23) * 0.0625f;
                 factors[b * cols + 4 * m + lane] = e == 255 ? __uint_as_float(0x7fffffffu) : down;
             }
             if (a.w.minima) {
                 const float s = q4_group_sum<G>(x);
-                if (lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
+                if (store && lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
             }
         });
     }
@@ -477,6 +495,7 @@ struct Q4Halves {
     static constexpr int kProducts = HALF ? T : 2 * T;
     static constexpr int kWarps = 8;
     static constexpr int kRing = GATED ? 3 : 4;
+    static constexpr bool kFinisher = false;
     static constexpr int kColumn = 288;  // bytes: 8 slices x 32, and a step of 8 banks
 
     static __host__ __device__ int block_bytes(int, int ng) {
@@ -495,16 +514,18 @@ struct Q4Halves {
     // A lane's four numbers are columns 0..3 or 4..7 of the run of eight that lane t = lane / 2 % 4 of a fragment
     // holds: a word of slice 2 (lane / 8), the even columns, and one of the next, the odd ones, of hi (a column
     // of product 2 i) and of lo (the same column of product 2 i + 1); FP16 rows have no lo.
-    template <int G>
-    __device__ __forceinline__ void split(const Q4Args& a, const Q4Row* rows, int tokens, int kb0, int kb1) const {
+    template <int G, class Between>
+    __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Between between) const {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
-        q4_items<kWarps>(a, rows, tokens, kb0, kb1, [&](int b, int m, float4 x) {
+        q4_items<kWarps>(a, m0, tokens, kb0, kb1, between, [&](int b, int m, float4 x, bool store) {
             uint8_t* to = frags + (b * (8 * kProducts) + (HALF ? m : m / 8 * 16 + m % 8)) * kColumn + (lane >> 3) * 64 +
                           (lane >> 1 & 3) * 8 + (lane & 1) * 4;
             if constexpr (HALF) {
-                *reinterpret_cast<__half2*>(to) = __floats2half2_rn(x.x, x.z);
-                *reinterpret_cast<__half2*>(to + 32) = __floats2half2_rn(x.y, x.w);
+                if (store) {
+                    *reinterpret_cast<__half2*>(to) = __floats2half2_rn(x.x, x.z);
+                    *reinterpret_cast<__half2*>(to + 32) = __floats2half2_rn(x.y, x.w);
+                }
             } else {
                 // top < 2^(e - 126), e its exponent field: scaled by 2^(141 - e) it is below 2^15.  The power's
                 // field is 268 - e, kept a normal number's; infinities and NaN stay what they are.
@@ -513,16 +534,19 @@ struct Q4Halves {
                 auto put = [&](float u, float v, int at) {
                     const __half2 hi = __floats2half2_rn(u, v);
                     const float2 r = __half22float2(hi);
-                    *reinterpret_cast<__half2*>(to + at) = hi;
-                    *reinterpret_cast<__half2*>(to + 8 * kColumn + at) = __floats2half2_rn(u - r.x, v - r.y);
+                    const __half2 lo = __floats2half2_rn(u - r.x, v - r.y);
+                    if (store) {
+                        *reinterpret_cast<__half2*>(to + at) = hi;
+                        *reinterpret_cast<__half2*>(to + 8 * kColumn + at) = lo;
+                    }
                 };
                 put(x.x * up, x.z * up, 0);
                 put(x.y * up, x.w * up, 32);
-                if (lane == 0) scales[b * kTokens + m] = __uint_as_float(static_cast<uint32_t>(254 - f) << 23);
+                if (store && lane == 0) scales[b * kTokens + m] = __uint_as_float(static_cast<uint32_t>(254 - f) << 23);
             }
             if (a.w.minima) {
                 const float s = q4_group_sum<G>(x);
-                if (lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
+                if (store && lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
             }
         });
     }
@@ -621,8 +645,9 @@ struct Q4Halves {
 // ---- the kernel
 
 // One output element: the chain, the gate, the store.
-__device__ __forceinline__ void q4_finish(const Q4Args& a, const Q4Row& row, long long n, float v, float g, bool gated) {
-    const long long at = row.y_at + n;
+__device__ __forceinline__ void q4_finish(const Q4Args& a, int m, long long n, float v, float g, bool gated) {
+    const Q4Row row(a, m);
+    const long long at = row.at(a.ynb) + n;
     if (a.chain.from_redirect) v += static_cast<const float*>(a.y)[at];
     v = apply_chain(a.chain, v, n, row.i1, row.i2, row.i3);
     if (gated) {
@@ -639,17 +664,21 @@ constexpr int q4_red_floats() { return F::kWarps * F::kTiles * F::kLaneSums * 32
 template <class F>
 constexpr int q4_red_buffers() { return F::kLaneSums <= 4 ? 2 : 1; }
 
+template <class F>
+constexpr int q4_threads() { return 32 * (F::kWarps + (F::kFinisher ? 1 : 0)); }
+
 // Shared memory but for the k-blocks of x.
 template <class F, int G>
 int q4_fixed_bytes(bool minima) {
-    return q4_red_buffers<F>() * q4_red_floats<F>() * 4 + F::kTokens * static_cast<int>(sizeof(Q4Row)) +
-           F::kWarps * F::kRing * F::kTiles * Q4Stage<G>::bytes(minima) + F::kTail;
+    return q4_red_buffers<F>() * q4_red_floats<F>() * 4 + F::kWarps * F::kRing * F::kTiles * Q4Stage<G>::bytes(minima) +
+           F::kTail;
 }
 
 template <class F, int G>
-__global__ void __launch_bounds__(32 * F::kWarps, 1) q4_rows_kernel(const __grid_constant__ Q4Args a) {
+__global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __grid_constant__ Q4Args a) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const bool worker = !F::kFinisher || warp < F::kWarps;
     const int WK = 1 << a.wk_log, WR = F::kWarps >> a.wk_log, wk = warp & (WK - 1), wr = warp >> a.wk_log;
     const int rank = a.cluster > 1 ? blockIdx.x % a.cluster : 0;
     const int groups = (a.w.tiles + WR - 1) / WR;  // of WR row tiles
@@ -660,22 +689,17 @@ __global__ void __launch_bounds__(32 * F::kWarps, 1) q4_rows_kernel(const __grid
     const bool minima = a.w.minima != nullptr;
 
     float* red = reinterpret_cast<float*>(smem);
-    Q4Row* rows = reinterpret_cast<Q4Row*>(red + q4_red_buffers<F>() * q4_red_floats<F>());
     const int slot_bytes = Q4Stage<G>::bytes(minima), turn_bytes = F::kTiles * slot_bytes;
-    uint8_t* ring = reinterpret_cast<uint8_t*>(rows + F::kTokens) + warp * (F::kRing * turn_bytes);
-    F form(a, reinterpret_cast<uint8_t*>(rows + F::kTokens) + F::kWarps * F::kRing * turn_bytes, tokens);
+    uint8_t* rings = reinterpret_cast<uint8_t*>(red + q4_red_buffers<F>() * q4_red_floats<F>());
+    uint8_t* ring = rings + warp * (F::kRing * turn_bytes);
+    F form(a, rings + F::kWarps * F::kRing * turn_bytes, tokens);
 
     // The warp's k-blocks in the order they are taken: over its row tiles, kb_begin + wk, + WK, ...  A warp
     // past the last tile walks the last one again and stores nothing.
     Q4Walk<G> walk[F::kTiles];
     const int steps = kb_end - kb_begin > wk ? (kb_end - kb_begin - wk + WK - 1) >> a.wk_log : 0;  // of a tile
-    int load_group = group0, load_step = 0;
+    int load_group = steps ? group0 : groups, load_step = 0;
     auto tile_of = [&](int group) { return min(group * WR + wr, a.w.tiles - 1); };
-    {
-        const long long block = static_cast<long long>(tile_of(group0)) * a.w.kblocks + kb_begin + wk;
-        walk[0].start(a.w, block, lane);
-        if constexpr (F::GATED) walk[1].start(a.gate, block, lane);
-    }
     auto load = [&](int turn) {
         if (load_group < groups) {
             const uint32_t slot = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + turn * turn_bytes;
@@ -695,16 +719,14 @@ __global__ void __launch_bounds__(32 * F::kWarps, 1) q4_rows_kernel(const __grid
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (steps == 0) load_group = groups;
+    auto start = [&] {
+        const long long block = static_cast<long long>(tile_of(group0)) * a.w.kblocks + kb_begin + wk;
+        walk[0].start(a.w, block, lane);
+        if constexpr (F::GATED) walk[1].start(a.gate, block, lane);
 #pragma unroll 1
-    for (int turn = 0; turn < F::kRing - 1; ++turn) load(turn);
-
-    if (threadIdx.x < tokens) {
-        const int m = m0 + threadIdx.x, q = m / a.ne1, i1 = m - q * a.ne1, i3 = q / a.ne2, i2 = q - i3 * a.ne2;
-        rows[threadIdx.x] = {i1 * a.xnb[0] + i2 * a.xnb[1] + i3 * a.xnb[2],
-                             i1 * a.ynb[0] + i2 * a.ynb[1] + i3 * a.ynb[2], i1, i2, i3, 0};
-    }
-    __syncthreads();
+        for (int turn = 0; turn < F::kRing - 1; ++turn) load(turn);
+    };
+    bool started = false;
 
     bool held = false;  // the one chunk of x is in shared memory
     int parity = 0, turn = 0;
@@ -715,11 +737,16 @@ __global__ void __launch_bounds__(32 * F::kWarps, 1) q4_rows_kernel(const __grid
         for (int kc = kb_begin; kc < kb_end; kc += a.chunk) {
             const int kc_end = min(kc + a.chunk, kb_end);
             if (!held) {
-                if (kc != kb_begin || group != group0) __syncthreads();  // the chunk before has been read
-                form.template split<G>(a, rows, tokens, kc, kc_end);
+                if (started) __syncthreads();  // the chunk before has been read
+                if (worker)
+                    form.template split<G>(a, m0, tokens, kc, kc_end, [&] {
+                        if (!started) start();
+                    });
+                started = true;
                 __syncthreads();
                 held = a.chunk >= kb_end - kb_begin;
             }
+            if (!worker) continue;
 #pragma unroll 1
             for (int at = wk; at < kc_end - kc; at += WK) {
                 // The oldest of the ring's k-blocks has come, to every lane; the place filled next is the one that
@@ -740,32 +767,40 @@ __global__ void __launch_bounds__(32 * F::kWarps, 1) q4_rows_kernel(const __grid
         // every thread before the barrier in between.
         float* mine = red + parity * q4_red_floats<F>();
         if constexpr (q4_red_buffers<F>() == 2) parity ^= 1;
+        if (worker) {
 #pragma unroll
-        for (int c = 0; c < F::kLaneSums; ++c)
+            for (int c = 0; c < F::kLaneSums; ++c)
 #pragma unroll
-            for (int i = 0; i < F::kTiles; ++i)
-                mine[((c * F::kTiles + i) * F::kWarps + warp) * 32 + lane] = form.lane_sum(i, c);
+                for (int i = 0; i < F::kTiles; ++i)
+                    mine[((c * F::kTiles + i) * F::kWarps + warp) * 32 + lane] = form.lane_sum(i, c);
+        }
         if (a.cluster > 1) cooperative_groups::this_cluster().sync();
         else __syncthreads();
-        // A warp finishes a sum of a tile; a cluster's CTAs share them.
+        // A warp finishes a sum of a tile, all warps or one that does nothing else, while the others go on; a
+        // cluster's CTAs share them.
+        const int item0 = F::kFinisher ? (worker ? F::kLaneSums * WR : 0) : warp, item_step = F::kFinisher ? 1 : F::kWarps;
 #pragma unroll 1
-        for (int o = warp * a.cluster + rank; o < F::kLaneSums * WR; o += F::kWarps * a.cluster) {
-            const int c = o / WR, tw = o - c * WR;
+        for (int o = item0 * a.cluster + rank; o < F::kLaneSums * WR; o += item_step * a.cluster) {
+            const int tw = o & (WR - 1), c = o / WR;
             const int m = F::token_of(c, lane);
             const long long n = (static_cast<long long>(group) * WR + tw) * 16 + F::row_of(c, lane);
             if (m >= tokens || n >= a.w.n) continue;
             float v[2] = {0.0f, 0.0f};
-#pragma unroll 1
-            for (int k = 0; k < a.cluster; ++k) {
-                const float* from = a.cluster > 1 ? cooperative_groups::this_cluster().map_shared_rank(mine, k) : mine;
+            const int at = (c * F::kTiles * F::kWarps + tw * WK) * 32 + lane;
+            auto join = [&](const float* from) {
 #pragma unroll 4
                 for (int j = 0; j < WK; ++j) {
 #pragma unroll
-                    for (int i = 0; i < F::kTiles; ++i)
-                        v[i] += from[((c * F::kTiles + i) * F::kWarps + tw * WK + j) * 32 + lane];
+                    for (int i = 0; i < F::kTiles; ++i) v[i] += from[at + (i * F::kWarps + j) * 32];
                 }
+            };
+            if (a.cluster > 1) {
+#pragma unroll 4
+                for (int k = 0; k < a.cluster; ++k) join(cooperative_groups::this_cluster().map_shared_rank(mine, k));
+            } else {
+                join(mine);
             }
-            q4_finish(a, rows[m], n, v[0], v[1], F::GATED);
+            q4_finish(a, m0 + m, n, v[0], v[1], F::GATED);
         }
         if constexpr (q4_red_buffers<F>() == 1) {
             if (a.cluster > 1) cooperative_groups::this_cluster().sync();
