@@ -116,11 +116,11 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const T* __restrict__ 
             }
             word |= static_cast<uint32_t>(static_cast<int>(q)) << q4_bit(c);
         }
-        reinterpret_cast<uint32_t*>(v.codes)[q4_word(v, at.row, at.k0)] = word ^ 0x88888888u;
+        *q4_word(v, at.row, at.k0) = word ^ 0x88888888u;
         if (at.k0 % v.group == 0) {
-            const long long s = q4_scale(v, at.row, at.k0);
-            v.scales[s] = dh;
-            if (MINIMUM) v.minima[s] = mh;
+            __half* s = q4_scale(v, at.row, at.k0);
+            *s = dh;
+            if (MINIMUM) s[16 * v.ng] = mh;
         }
     }
 }
@@ -144,13 +144,13 @@ __global__ void __launch_bounds__(256) q4_import_kernel(const uint8_t* __restric
             }
             word |= q << q4_bit(c);
         }
-        reinterpret_cast<uint32_t*>(v.codes)[q4_word(v, at.row, at.k0)] = word ^ 0x88888888u;
+        *q4_word(v, at.row, at.k0) = word ^ 0x88888888u;
         if (at.k0 % v.group == 0) {
-            const long long s = q4_scale(v, at.row, at.k0);
+            __half* s = q4_scale(v, at.row, at.k0);
             const bool in = row_in && at.k0 < v.k;
             const long long from = at.row * groups + at.k0 / v.group;
-            v.scales[s] = in ? scales[from] : __float2half_rn(0.0f);
-            if (minima) v.minima[s] = in ? minima[from] : __float2half_rn(0.0f);
+            *s = in ? scales[from] : __float2half_rn(0.0f);
+            if (minima) s[16 * v.ng] = in ? minima[from] : __float2half_rn(0.0f);
         }
     }
 }
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(256) q4_import_kernel(const uint8_t* __restric
 // then 16 bytes, byte i numbers i (low) and i + 16 (high).
 __global__ void __launch_bounds__(256) q4_blocks_kernel(const uint8_t* __restrict__ blocks, long long row_bytes,
                                                         Q4View v) {
-    const int header = v.minima ? 4 : 2, size = header + 16;
+    const int header = v.minimum ? 4 : 2, size = header + 16;
     const long long total = static_cast<long long>(v.tiles) * 16 * v.kblocks * 16;
     for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
         const WordAt at = word_at(v, i);
@@ -169,23 +169,23 @@ __global__ void __launch_bounds__(256) q4_blocks_kernel(const uint8_t* __restric
         uint32_t word = 0;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            uint32_t q = v.minima ? 0 : 8;
+            uint32_t q = v.minimum ? 0 : 8;
             if (in) {
                 const uint32_t two = __ldg(b + header + (first & 15) + c);
                 q = first < 16 ? two & 15 : two >> 4;
             }
             word |= q << q4_bit(c);
         }
-        reinterpret_cast<uint32_t*>(v.codes)[q4_word(v, at.row, at.k0)] = word ^ 0x88888888u;
+        *q4_word(v, at.row, at.k0) = word ^ 0x88888888u;
         if (first == 0) {
-            const long long s = q4_scale(v, at.row, at.k0);
+            __half* s = q4_scale(v, at.row, at.k0);
             uint32_t d = 0, m = 0;
             if (in) {
                 d = b[0] | static_cast<uint32_t>(b[1]) << 8;
-                if (v.minima) m = b[2] | static_cast<uint32_t>(b[3]) << 8;
+                if (v.minimum) m = b[2] | static_cast<uint32_t>(b[3]) << 8;
             }
-            v.scales[s] = __ushort_as_half(static_cast<unsigned short>(d));
-            if (v.minima) v.minima[s] = __ushort_as_half(static_cast<unsigned short>(m));
+            *s = __ushort_as_half(static_cast<unsigned short>(d));
+            if (v.minimum) s[16 * v.ng] = __ushort_as_half(static_cast<unsigned short>(m));
         }
     }
 }
@@ -195,16 +195,16 @@ __global__ void __launch_bounds__(256) q4_dequantize_kernel(Q4View v, float* __r
     for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
         const WordAt at = word_at(v, i);
         if (at.k0 >= v.k) continue;
-        const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(v.codes) + q4_word(v, at.row, at.k0)) ^ 0x88888888u;
-        const long long s = q4_scale(v, at.row, at.k0);
-        const float d = __half2float(v.scales[s]);
-        const float m = v.minima ? __half2float(v.minima[s]) : 0.0f;
+        const uint32_t word = __ldg(q4_word(v, at.row, at.k0)) ^ 0x88888888u;
+        const __half* s = q4_scale(v, at.row, at.k0);
+        const float d = __half2float(s[0]);
+        const float m = v.minimum ? __half2float(s[16 * v.ng]) : 0.0f;
         float x[8];
         // d q and d (q - 8) are exact in FP32 (11 and 4 bits).
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
             const float code = static_cast<float>(word >> q4_bit(c) & 15u);
-            x[c] = v.minima ? fmaf(d, code, m) : d * (code - 8.0f);
+            x[c] = v.minimum ? fmaf(d, code, m) : d * (code - 8.0f);
         }
         float* dst = w + at.row * ld + at.k0;
         if (at.k0 + 8 <= v.k && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
@@ -217,6 +217,10 @@ __global__ void __launch_bounds__(256) q4_dequantize_kernel(Q4View v, float* __r
         }
     }
 }
+
+// What every maker of a matrix does first: the products' error word is allocated with the matrix, not by a first
+// product that a stream capture records.
+void prepare_device() { device_error_word(); }
 
 // A matrix [k, n] with contiguous rows of the 4-bit matrix's extents.
 bool matrix_of(const sdb_tensor* w, const sdb_q4* q, bool f16) {
@@ -246,16 +250,17 @@ int sdb_q4_quantize(const sdb_tensor* w, const sdb_q4* q, void* stream) {
     if (!q4_valid(q)) return fail(SDB_INVALID, "sdb_q4_quantize: no such 4-bit matrix");
     if (!matrix_of(w, q, true))
         return fail(SDB_INVALID, "sdb_q4_quantize: w must be an FP32 or FP16 matrix [k, n] with contiguous rows");
+    prepare_device();
     const Q4View v = q4_view(q);
     const auto st = static_cast<cudaStream_t>(stream);
     const int blocks = word_blocks(v);
     if (w->type == SDB_TYPE_F32) {
         const auto* src = static_cast<const float*>(w->data);
-        if (v.minima) q4_quantize_kernel<float, true><<<blocks, 256, 0, st>>>(src, w->nb[1] / 4, v);
+        if (v.minimum) q4_quantize_kernel<float, true><<<blocks, 256, 0, st>>>(src, w->nb[1] / 4, v);
         else q4_quantize_kernel<float, false><<<blocks, 256, 0, st>>>(src, w->nb[1] / 4, v);
     } else {
         const auto* src = static_cast<const __half*>(w->data);
-        if (v.minima) q4_quantize_kernel<__half, true><<<blocks, 256, 0, st>>>(src, w->nb[1] / 2, v);
+        if (v.minimum) q4_quantize_kernel<__half, true><<<blocks, 256, 0, st>>>(src, w->nb[1] / 2, v);
         else q4_quantize_kernel<__half, false><<<blocks, 256, 0, st>>>(src, w->nb[1] / 2, v);
     }
     count_launch();
@@ -268,6 +273,7 @@ int sdb_q4_import(const void* codes, const void* scales, const void* minima, con
     if (codes == nullptr || scales == nullptr || (minima != nullptr) != (q->minimum != 0) ||
         reinterpret_cast<uintptr_t>(scales) % 2 != 0 || reinterpret_cast<uintptr_t>(minima) % 2 != 0)
         return fail(SDB_INVALID, "sdb_q4_import: codes, FP16 scales and (with `minimum`, only then) FP16 minima");
+    prepare_device();
     const Q4View v = q4_view(q);
     q4_import_kernel<<<word_blocks(v), 256, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const uint8_t*>(codes), (q->k + 1) / 2, static_cast<const __half*>(scales),
@@ -283,6 +289,7 @@ int sdb_q4_from_blocks(const void* blocks, int64_t row_bytes, const sdb_q4* q, v
         return fail(SDB_INVALID, "sdb_q4_from_blocks: ggml's blocks are groups of 32, k a multiple of 32");
     if (blocks == nullptr || row_bytes < q->k / 32 * (q->minimum ? 20 : 18))
         return fail(SDB_INVALID, "sdb_q4_from_blocks: no blocks, or rows shorter than k / 32 blocks");
+    prepare_device();
     const Q4View v = q4_view(q);
     q4_blocks_kernel<<<word_blocks(v), 256, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const uint8_t*>(blocks), row_bytes, v);

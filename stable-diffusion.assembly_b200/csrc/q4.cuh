@@ -2,17 +2,17 @@
 //
 // A matrix of n rows of k numbers is held in tiles of 16 rows x 128 columns
 // (rows and columns padded; padding stands for 0), the tiles of 16 rows one
-// after another and each in order of k:
-//   codes   [row tile][k-block][half 2][lane 32][4 words]: lane g * 4 + t of half h
-//           holds row 8 h + g; its word j the eight columns 32 j + 8 t + 0..7,
-//           columns i and i + 4 (i < 4) in byte i, low and high, each as code - 8
-//           in four bits, so that a nibble at the top of a byte is 16 (code - 8).
-//           A warp reads a half tile as one 512-byte run of 16 bytes a lane, and
-//           a word's low and high nibbles are operands of mma.m16n8k32 (rows g
+// after another and each in order of k, so that any run of a row tile's
+// k-blocks is one run of memory.  A tile is
+//   codes   [half 2][lane 32][4 words]: lane g * 4 + t of half h holds row
+//           8 h + g; its word j the eight columns 32 j + 8 t + 0..7, columns i
+//           and i + 4 (i < 4) in byte i, low and high, each as code - 8 in four
+//           bits, so that a nibble at the top of a byte is 16 (code - 8).  A
+//           word's low and high nibbles are operands of mma.m16n8k32 (rows g
 //           and g + 8 of lane (g, t)) when the columns of x are taken in the
 //           same order: a sum over k may take its terms in any order.
-//   scales  [row tile][k-block][g 8][half 2][128 / group] FP16: what lane (g, t)
-//           needs of a tile is one run of 16, 8 or 4 bytes.
+//   scales  [g 8][half 2][128 / group] FP16: what lane (g, t) needs of a tile
+//           is one run of 16, 8 or 4 bytes.
 //   minima  as the scales, present with `minimum`.
 // value = scale (code - 8), or scale code + minimum.
 #pragma once
@@ -27,14 +27,14 @@
 namespace sdb {
 
 struct Q4View {
-    uint8_t* codes;
-    __half* scales;
-    __half* minima;   // null: symmetric
+    uint8_t* data;
     long long n, k;
     int tiles;        // of 16 rows
     int kblocks;      // of 128 columns
     int group;
     int ng;           // groups of a k-block: 128 / group
+    int minimum;
+    int block;        // bytes of a tile
 };
 
 constexpr long long kQ4MaxK = 1LL << 24;
@@ -59,26 +59,27 @@ inline Q4View q4_view(const sdb_q4* q) {
     v.ng = 128 / q->group;
     v.tiles = static_cast<int>((q->n + 15) / 16);
     v.kblocks = static_cast<int>((q->k + 127) / 128);
-    const long long blocks = static_cast<long long>(v.tiles) * v.kblocks;
-    v.codes = static_cast<uint8_t*>(q->data);
-    v.scales = reinterpret_cast<__half*>(v.codes + blocks * 1024);
-    v.minima = q->minimum ? v.scales + blocks * 16 * v.ng : nullptr;
+    v.minimum = q->minimum;
+    v.block = 1024 + 32 * v.ng * (q->minimum ? 2 : 1);
+    v.data = static_cast<uint8_t*>(q->data);
     return v;
 }
 
-// The word of row r's columns k0..k0 + 7 (k0 a multiple of 8), as an index of 32-bit words.
-__host__ __device__ inline long long q4_word(const Q4View& v, long long r, long long k0) {
-    const long long block = (r >> 4) * v.kblocks + (k0 >> 7);
-    const int h = static_cast<int>(r >> 3) & 1, g = static_cast<int>(r) & 7;
-    const int j = static_cast<int>(k0 >> 5) & 3, t = static_cast<int>(k0 >> 3) & 3;
-    return ((block * 2 + h) * 32 + g * 4 + t) * 4 + j;
+__host__ __device__ inline uint8_t* q4_tile(const Q4View& v, long long r, long long k) {
+    return v.data + ((r >> 4) * v.kblocks + (k >> 7)) * v.block;
 }
 
-// The scale (and minimum) of row r's column k.
-__host__ __device__ inline long long q4_scale(const Q4View& v, long long r, long long k) {
-    const long long block = (r >> 4) * v.kblocks + (k >> 7);
+// The word of row r's columns k0..k0 + 7 (k0 a multiple of 8).
+__host__ __device__ inline uint32_t* q4_word(const Q4View& v, long long r, long long k0) {
     const int h = static_cast<int>(r >> 3) & 1, g = static_cast<int>(r) & 7;
-    return ((block * 8 + g) * 2 + h) * v.ng + static_cast<int>(k & 127) / v.group;
+    const int j = static_cast<int>(k0 >> 5) & 3, t = static_cast<int>(k0 >> 3) & 3;
+    return reinterpret_cast<uint32_t*>(q4_tile(v, r, k0)) + (h * 32 + g * 4 + t) * 4 + j;
+}
+
+// The scale of row r's column k; its minimum, if any, lies 16 ng numbers on.
+__host__ __device__ inline __half* q4_scale(const Q4View& v, long long r, long long k) {
+    const int h = static_cast<int>(r >> 3) & 1, g = static_cast<int>(r) & 7;
+    return reinterpret_cast<__half*>(q4_tile(v, r, k) + 1024) + (g * 2 + h) * v.ng + static_cast<int>(k & 127) / v.group;
 }
 
 // The bit of column i (0..7) of a word.

@@ -24,7 +24,7 @@ int q4_launch_form(const Q4Args& args, const Q4Plan& p, cudaStream_t st) {
     a.cluster = p.cluster;
     a.range = (a.w.kblocks + a.cluster - 1) / a.cluster;
     // The k-blocks of x held at a time: all of the CTA's, or the multiple of WK that fits.
-    const int fixed = q4_fixed_bytes<F, G>(a.w.minima != nullptr);
+    const int fixed = q4_fixed_bytes<F, G>(a.w.block);
     const int block = F::block_bytes(std::min(a.rows, F::kTokens), 128 / G);
     const int fit = (p.shared - fixed) / block;
     int wk_log = p.wk_log;
@@ -66,7 +66,7 @@ int q4_launch_rows(const Q4Args& a, const Q4Plan& p, cudaStream_t st) {
 
 template <int G>
 int q4_launch(const Q4Args& a, const Q4Plan& p, cudaStream_t st) {
-    return a.gate.codes ? q4_launch_rows<true, G>(a, p, st) : q4_launch_rows<false, G>(a, p, st);
+    return a.gate.data ? q4_launch_rows<true, G>(a, p, st) : q4_launch_rows<false, G>(a, p, st);
 }
 
 }  // namespace sdb

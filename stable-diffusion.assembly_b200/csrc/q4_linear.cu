@@ -84,6 +84,7 @@ int run(const sdb_q4* w, const sdb_q4* gate, const sdb_tensor* x, const sdb_tens
     a.flat = x->ne[2] == 1 && x->ne[3] == 1;
     a.rows = static_cast<int>(x->ne[1] * x->ne[2] * x->ne[3]);
     a.act = act;
+    a.err = device_error_word();
     a.chain = make_chain(chain);
     if (a.rows == 0) return SDB_OK;
     const Q4Plan p = plan(a);

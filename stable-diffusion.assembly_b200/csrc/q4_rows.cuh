@@ -32,8 +32,9 @@
 // columns meet a bank twice, and stays there for all the row tiles the CTA
 // walks.  A product's unused columns are not stored: their lanes read what lies
 // there and their sums go nowhere.  Weights go from memory to a ring of
-// kRing k-blocks a warp in shared memory by asynchronous copies, which
-// wait for nothing but the warp's own reads.
+// kRing places a warp in shared memory, by bulk copies of kRun k-blocks that
+// one lane issues: they take few issue slots and no registers, and wait for
+// nothing but the warp's own reads.
 // The warps' sums meet in shared memory and are added in one order, so a result
 // does not turn on timing; the sums of a cluster's other CTAs are read where
 // they lie.
@@ -46,6 +47,7 @@
 #include <cstdint>
 
 #include "chain.cuh"
+#include "ptx.cuh"
 #include "q4.cuh"
 
 namespace sdb {
@@ -67,6 +69,7 @@ struct Q4Args {
     int cluster;               // CTAs that share a tile's k-blocks
     int range;                 // k-blocks of a CTA (the last of a cluster may have fewer)
     int chunk;                 // k-blocks of x held at a time, a multiple of WK
+    unsigned* err;             // the device error word
     Chain chain;
 };
 
@@ -86,23 +89,11 @@ struct Q4Row {
     }
 };
 
-// BYTES of a lane's own, from global to shared memory, in the background.
-template <int BYTES>
-__device__ __forceinline__ void q4_copy(uint32_t to, const void* from) {
-    if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
-}
-
-// A k-block of a row tile as a lane holds it: the words of rows g and g + 8, the scales, the minima; and its
-// place in the ring: 32 lanes' words of rows g, of rows g + 8, then eight runs of scales, each for four lanes,
-// and as many of minima.
+// A tile of weights (q4.cuh) as a lane holds it: the words of rows g and g + 8, the scales, the minima.
 template <int G>
 struct Q4Stage {
     static constexpr int kNg = 128 / G;
     static constexpr int kRun = 4 * kNg;  // bytes of a lane's scales: rows g and g + 8
-    static __host__ __device__ constexpr int bytes(bool minima) { return 1024 + 8 * kRun * (minima ? 2 : 1); }
     uint4 lo, hi;
     uint32_t d[kNg], m[kNg];
 
@@ -117,11 +108,11 @@ struct Q4Stage {
             r[0] = *reinterpret_cast<const uint32_t*>(p);
         }
     }
-    __device__ __forceinline__ void read(const uint8_t* slot, int lane, bool minima) {
-        lo = *reinterpret_cast<const uint4*>(slot + lane * 16);
-        hi = *reinterpret_cast<const uint4*>(slot + 512 + lane * 16);
-        run(d, slot + 1024 + lane / 4 * kRun);
-        if (minima) run(m, slot + 1024 + 8 * kRun + lane / 4 * kRun);
+    __device__ __forceinline__ void read(const uint8_t* tile, int lane, bool minima) {
+        lo = *reinterpret_cast<const uint4*>(tile + lane * 16);
+        hi = *reinterpret_cast<const uint4*>(tile + 512 + lane * 16);
+        run(d, tile + 1024 + lane / 4 * kRun);
+        if (minima) run(m, tile + 1024 + 8 * kRun + lane / 4 * kRun);
     }
     // Group i's numbers of rows g and g + 8.
     static __device__ __forceinline__ float2 pick(const uint32_t (&r)[kNg], int i) {
@@ -129,31 +120,6 @@ struct Q4Stage {
         const __half2 a = *reinterpret_cast<const __half2*>(&r[i / 2]);
         const __half2 b = *reinterpret_cast<const __half2*>(&r[kNg / 2 + i / 2]);
         return i & 1 ? make_float2(__high2float(a), __high2float(b)) : make_float2(__low2float(a), __low2float(b));
-    }
-};
-
-// Where a lane's next k-block of a matrix lies; steps are counted in k-blocks.
-template <int G>
-struct Q4Walk {
-    const uint8_t *codes, *scales, *minima;
-    __device__ __forceinline__ void start(const Q4View& w, long long block, int lane) {
-        codes = w.codes + block * 1024 + lane * 16;
-        scales = reinterpret_cast<const uint8_t*>(w.scales) + (block * 8 + lane / 4) * (512 / G);
-        minima = w.minima ? reinterpret_cast<const uint8_t*>(w.minima) + (block * 8 + lane / 4) * (512 / G) : nullptr;
-    }
-    __device__ __forceinline__ void step(long long blocks) {
-        codes += blocks * 1024;
-        scales += blocks * (4096 / G);
-        if (minima) minima += blocks * (4096 / G);
-    }
-    __device__ __forceinline__ void load(uint32_t slot, int lane) const {
-        constexpr int run = Q4Stage<G>::kRun;
-        q4_copy<16>(slot + lane * 16, codes);
-        q4_copy<16>(slot + 512 + lane * 16, codes + 512);
-        if (lane % 4 == 0) {
-            q4_copy<run>(slot + 1024 + lane / 4 * run, scales);
-            if (minima) q4_copy<run>(slot + 1024 + 8 * run + lane / 4 * run, minima);
-        }
     }
 };
 
@@ -273,7 +239,7 @@ struct Q4Digits {
     static constexpr int kTiles = GATED ? 2 : 1;
     static constexpr int kLaneSums = NT;         // of a tile, joined over the digits
     static constexpr int kWarps = NT <= 2 && !GATED ? 16 : 8;
-    static constexpr int kRing = 4;              // k-blocks of a warp on their way
+    static constexpr int kRun = 2, kRing = 3;    // k-blocks of a copy; copies of a warp on their way
     static constexpr bool kFinisher = NT <= 2;   // a warp of its own finishes the sums
     static constexpr int kColumn = 160;          // bytes: 4 slices x 32, and a step of 8 banks
 
@@ -322,7 +288,7 @@ struct Q4Digits {
                 const float down = __uint_as_float(static_cast<uint32_t>(254 - f + 8 * lane) << 23) * 0.0625f;
                 factors[b * cols + 4 * m + lane] = e == 255 ? __uint_as_float(0x7fffffffu) : down;
             }
-            if (a.w.minima) {
+            if (a.w.minimum) {
                 const float s = q4_group_sum<G>(x);
                 if (store && lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
             }
@@ -494,7 +460,7 @@ struct Q4Halves {
     static constexpr int kLaneSums = 4 * T;
     static constexpr int kProducts = HALF ? T : 2 * T;
     static constexpr int kWarps = 8;
-    static constexpr int kRing = GATED ? 3 : 4;
+    static constexpr int kRun = 1, kRing = GATED ? 3 : 4;
     static constexpr bool kFinisher = false;
     static constexpr int kColumn = 288;  // bytes: 8 slices x 32, and a step of 8 banks
 
@@ -544,7 +510,7 @@ struct Q4Halves {
                 put(x.y * up, x.w * up, 32);
                 if (store && lane == 0) scales[b * kTokens + m] = __uint_as_float(static_cast<uint32_t>(254 - f) << 23);
             }
-            if (a.w.minima) {
+            if (a.w.minimum) {
                 const float s = q4_group_sum<G>(x);
                 if (store && lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
             }
@@ -669,8 +635,8 @@ constexpr int q4_threads() { return 32 * (F::kWarps + (F::kFinisher ? 1 : 0)); }
 
 // Shared memory but for the k-blocks of x.
 template <class F, int G>
-int q4_fixed_bytes(bool minima) {
-    return q4_red_buffers<F>() * q4_red_floats<F>() * 4 + F::kWarps * F::kRing * F::kTiles * Q4Stage<G>::bytes(minima) +
+int q4_fixed_bytes(int block) {
+    return q4_red_buffers<F>() * q4_red_floats<F>() * 4 + F::kWarps * F::kRing * (F::kTiles * F::kRun * block + 8) + 16 +
            F::kTail;
 }
 
@@ -686,50 +652,73 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
     const int group_step = a.cluster > 1 ? gridDim.x / a.cluster : gridDim.x;
     const int m0 = blockIdx.y * F::kTokens, tokens = min(F::kTokens, a.rows - m0);
     const int kb_begin = rank * a.range, kb_end = min(kb_begin + a.range, a.w.kblocks);
-    const bool minima = a.w.minima != nullptr;
+    const bool minima = a.w.minimum != 0;
 
     float* red = reinterpret_cast<float*>(smem);
-    const int slot_bytes = Q4Stage<G>::bytes(minima), turn_bytes = F::kTiles * slot_bytes;
+    const int block = 1024 + 4096 / G * (minima ? 2 : 1);  // bytes of a tile, a.w.block
+    const int place_bytes = F::kTiles * F::kRun * block;
     uint8_t* rings = reinterpret_cast<uint8_t*>(red + q4_red_buffers<F>() * q4_red_floats<F>());
-    uint8_t* ring = rings + warp * (F::kRing * turn_bytes);
-    F form(a, rings + F::kWarps * F::kRing * turn_bytes, tokens);
+    uint8_t* ring = rings + warp * (F::kRing * place_bytes);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(rings + F::kWarps * F::kRing * place_bytes);
+    volatile int* abort = reinterpret_cast<volatile int*>(bars + F::kWarps * F::kRing);
+    F form(a, reinterpret_cast<uint8_t*>(bars + F::kWarps * F::kRing) + 16, tokens);
+    bars += warp * F::kRing;
 
-    // The warp's k-blocks in the order they are taken: over its row tiles, kb_begin + wk, + WK, ...  A warp
-    // past the last tile walks the last one again and stores nothing.
-    Q4Walk<G> walk[F::kTiles];
-    const int steps = kb_end - kb_begin > wk ? (kb_end - kb_begin - wk + WK - 1) >> a.wk_log : 0;  // of a tile
-    int load_group = steps ? group0 : groups, load_step = 0;
-    auto tile_of = [&](int group) { return min(group * WR + wr, a.w.tiles - 1); };
-    auto load = [&](int turn) {
-        if (load_group < groups) {
-            const uint32_t slot = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + turn * turn_bytes;
-#pragma unroll
-            for (int i = 0; i < F::kTiles; ++i) walk[i].load(slot + i * slot_bytes, lane);
-            long long blocks = WK;
-            if (++load_step == steps) {
-                load_step = 0;
-                const int next = load_group + group_step;
-                if (next < groups)
-                    blocks = static_cast<long long>(tile_of(next) - tile_of(load_group)) * a.w.kblocks -
-                             static_cast<long long>(steps - 1) * WK;
-                load_group = next;
+    // The warp's k-blocks in the order they are taken: for each of its row tiles and each chunk of x, the wk'th
+    // run of the chunk's k-blocks.  A warp past the last tile walks the last one again and stores nothing.
+    struct Walk {
+        int group, kc, kb, stop;
+    };
+    auto enter = [&](Walk& w) {  // the run of (group, kc), or of the first after it that is not empty
+        for (;;) {
+            const int len = min(a.chunk, kb_end - w.kc), per = (len + WK - 1) >> a.wk_log;
+            w.kb = w.kc + wk * per;
+            w.stop = min(w.kb + per, w.kc + len);
+            if (w.kb < w.stop) return;
+            w.kc += a.chunk;
+            if (w.kc >= kb_end) {
+                w.kc = kb_begin;
+                w.group += group_step;
+                if (w.group >= groups) return;
             }
-#pragma unroll
-            for (int i = 0; i < F::kTiles; ++i) walk[i].step(blocks);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    Walk ahead{kb_begin < kb_end ? group0 : groups, kb_begin, 0, 0};
+    auto load = [&](int place) {  // lane 0: the next run of up to kRun k-blocks
+        if (ahead.group >= groups) return;
+        const int count = min(F::kRun, ahead.stop - ahead.kb);
+        const long long first = static_cast<long long>(min(ahead.group * WR + wr, a.w.tiles - 1)) * a.w.kblocks + ahead.kb;
+        mbar_arrive_expect_tx(bars + place, F::kTiles * count * block);
+        bulk_load(ring + place * place_bytes, a.w.data + first * block, count * block, bars + place);
+        if constexpr (F::GATED)
+            bulk_load(ring + place * place_bytes + F::kRun * block, a.gate.data + first * block, count * block, bars + place);
+        ahead.kb += count;
+        if (ahead.kb >= ahead.stop) {
+            ahead.kc += a.chunk;
+            if (ahead.kc >= kb_end) {
+                ahead.kc = kb_begin;
+                ahead.group += group_step;
+            }
+            if (ahead.group < groups) enter(ahead);
+        }
     };
     auto start = [&] {
-        const long long block = static_cast<long long>(tile_of(group0)) * a.w.kblocks + kb_begin + wk;
-        walk[0].start(a.w, block, lane);
-        if constexpr (F::GATED) walk[1].start(a.gate, block, lane);
+        if (lane == 0) {
+            *abort = 0;
+            for (int i = 0; i < F::kRing; ++i) mbar_init(bars + i, 1);
+            fence_barrier_init();
+            if (ahead.group < groups) enter(ahead);
 #pragma unroll 1
-        for (int turn = 0; turn < F::kRing - 1; ++turn) load(turn);
+            for (int i = 0; i < F::kRing; ++i) load(i);
+        }
+        __syncwarp();
     };
     bool started = false;
 
     bool held = false;  // the one chunk of x is in shared memory
-    int parity = 0, turn = 0;
+    bool lost = false;  // a bounded wait ran out
+    int parity = 0, place = 0;
+    uint32_t phase = 0;
 #pragma unroll 1
     for (int group = group0; group < groups; group += group_step) {
         form.clear();
@@ -746,20 +735,31 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
                 __syncthreads();
                 held = a.chunk >= kb_end - kb_begin;
             }
-            if (!worker) continue;
+            if (!worker || lost) continue;
+            const int per = (kc_end - kc + WK - 1) >> a.wk_log;
+            const int stop = min(wk * per + per, kc_end - kc);
 #pragma unroll 1
-            for (int at = wk; at < kc_end - kc; at += WK) {
-                // The oldest of the ring's k-blocks has come, to every lane; the place filled next is the one that
-                // all lanes have read before this.
-                asm volatile("cp.async.wait_group %0;" ::"n"(F::kRing - 2) : "memory");
-                __syncwarp();
-                Q4Stage<G> stage[F::kTiles];
+            for (int at = wk * per; at < stop; at += F::kRun) {
+                if (!lost) lost = !mbar_wait(bars + place, phase, abort, a.err);
+                if (__any_sync(~0u, lost)) {  // the copies did not come: no more are waited for, no sums made
+                    lost = true;
+                    break;
+                }
+#pragma unroll 1
+                for (int i = 0; i < F::kRun; ++i) {
+                    if (i && at + i >= stop) break;
+                    Q4Stage<G> stage[F::kTiles];
 #pragma unroll
-                for (int i = 0; i < F::kTiles; ++i)
-                    stage[i].read(ring + turn * turn_bytes + i * slot_bytes, lane, minima);
-                load((turn + F::kRing - 1) % F::kRing);
-                turn = (turn + 1) % F::kRing;
-                form.template product<G>(stage, at, minima);
+                    for (int t = 0; t < F::kTiles; ++t)
+                        stage[t].read(ring + place * place_bytes + (t * F::kRun + i) * block, lane, minima);
+                    form.template product<G>(stage, at + i, minima);
+                }
+                __syncwarp();  // every lane has read the place that is filled again
+                if (lane == 0) load(place);
+                if (++place == F::kRing) {
+                    place = 0;
+                    phase ^= 1;
+                }
             }
         }
 
@@ -807,7 +807,10 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
             else __syncthreads();
         }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (lost) {  // copies may still be on their way into this CTA's memory: wait for them, with a limit again
+        for (int i = 0; i < F::kRing; ++i) 
+            mbar_wait_quiet(bars + (place + i) % F::kRing, i < F::kRing - place ? phase : phase ^ 1, kWaitLimitNs);
+    }
     if (a.cluster > 1) cooperative_groups::this_cluster().sync();  // the others have read this CTA's sums
 }
 
