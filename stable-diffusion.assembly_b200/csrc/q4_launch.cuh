@@ -21,20 +21,25 @@ int q4_launch_form(const Q4Args& args, const Q4Plan& p, cudaStream_t st) {
         if (dev < 64) raised.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
     Q4Args a = args;
-    a.cluster = p.cluster;
-    a.range = (a.w.kblocks + a.cluster - 1) / a.cluster;
+    const int cluster = 1 << p.cluster_log;
+    a.cluster_log = static_cast<uint8_t>(p.cluster_log);
+    a.range = (a.kblocks + cluster - 1) / cluster;
     // The k-blocks of x held at a time: all of the CTA's, or the multiple of WK that fits.
-    const int fixed = q4_fixed_bytes<F, G>(a.w.block);
-    const int block = F::block_bytes(std::min(a.rows, F::kTokens), 128 / G);
+    const int rows = std::min(a.rows, F::kTokens);
+    a.inverse = rows > 1 ? 0xffffffffu / static_cast<unsigned>(rows) + 1 : 0;
+    const int fixed = q4_fixed_bytes<F>(1024 + 4096 / G * (a.minimum ? 2 : 1));
+    const int block = F::block_bytes(rows, 128 / G);
     const int fit = (p.shared - fixed) / block;
     int wk_log = p.wk_log;
     while ((1 << wk_log) > F::kWarps || (wk_log > 0 && (1 << wk_log) > fit)) --wk_log;
-    const int wk = 1 << wk_log;
+    const int wk = 1 << wk_log, wr = F::kWarps / wk;
     if (fit < wk) return fail(SDB_CUDA_ERROR, "mul_mat_q4: shared memory");
-    a.wk_log = wk_log;
-    a.chunk = std::min((a.range + wk - 1) / wk, fit / wk) * wk;
-    const int wr = F::kWarps / wk, groups = (a.w.tiles + wr - 1) / wr;
-    const int blocks = std::min(groups, std::max(1, current_sm_count() / a.cluster)) * a.cluster;
+    a.wk_log = static_cast<uint8_t>(wk_log);
+    a.wr_log = 0;
+    while ((1 << a.wr_log) < wr) ++a.wr_log;
+    a.chunk = std::min(a.range, fit / wk * wk);
+    a.groups = (a.tiles + wr - 1) / wr;
+    const int blocks = std::min(a.groups, std::max(1, current_sm_count() / cluster)) * cluster;
     const int runs = (a.rows + F::kTokens - 1) / F::kTokens;  // of x's rows
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(runs));
@@ -43,10 +48,10 @@ int q4_launch_form(const Q4Args& args, const Q4Plan& p, cudaStream_t st) {
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = static_cast<unsigned>(a.cluster);
+    attr.val.clusterDim.x = static_cast<unsigned>(cluster);
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = a.cluster > 1 ? 1 : 0;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
     SDB_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
     count_launch();
     return SDB_OK;
@@ -66,7 +71,7 @@ int q4_launch_rows(const Q4Args& a, const Q4Plan& p, cudaStream_t st) {
 
 template <int G>
 int q4_launch(const Q4Args& a, const Q4Plan& p, cudaStream_t st) {
-    return a.gate.data ? q4_launch_rows<true, G>(a, p, st) : q4_launch_rows<false, G>(a, p, st);
+    return a.gate ? q4_launch_rows<true, G>(a, p, st) : q4_launch_rows<false, G>(a, p, st);
 }
 
 }  // namespace sdb

@@ -57,22 +57,27 @@ Q4Plan plan(const Q4Args& a) {
     Q4Plan p{};
     p.form = a.rows <= 2 ? 2 : a.rows <= 4 ? 4 : a.rows <= 8 ? 8 : a.rows <= 16 ? 16 : 32;
     p.wk_log = 3;
-    p.cluster = 1;
+    p.cluster_log = 0;
     p.shared = kQ4MaxShared;
     return p;
 }
 
 int run(const sdb_q4* w, const sdb_q4* gate, const sdb_tensor* x, const sdb_tensor* dst, int act,
         const sdb_chain* chain, cudaStream_t st) {
+    const Q4View v = q4_view(w);
     Q4Args a{};
-    a.w = q4_view(w);
-    if (gate) a.gate = q4_view(gate);
+    a.w = v.data;
+    a.gate = gate ? static_cast<const uint8_t*>(gate->data) : nullptr;
+    a.tiles = v.tiles;
+    a.kblocks = v.kblocks;
+    a.minimum = static_cast<uint8_t>(v.minimum);
+    a.k = static_cast<int>(v.k);
+    a.n = static_cast<int>(v.n);
     a.x = x->data;
     a.y = chain && chain->redirect ? chain->redirect : dst->data;
-    const bool half = x->type == SDB_TYPE_F16;
-    const int es = half ? 2 : 4;
+    a.x_half = x->type == SDB_TYPE_F16;
+    const int es = a.x_half ? 2 : 4;
     a.y_half = dst->type == SDB_TYPE_F16;
-    a.x_half = half;
     a.x_vec = reinterpret_cast<uintptr_t>(x->data) % (4 * es) == 0;
     for (int d = 0; d < 3; ++d) {
         a.xnb[d] = x->nb[d + 1] / es;

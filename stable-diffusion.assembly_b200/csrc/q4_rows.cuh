@@ -24,20 +24,21 @@
 //   column, as they are).  q - 8 is exact in FP16 (0x6400 | q is 1024 + q; a
 //   subtraction, or for a nibble four bits up a multiply-add, leaves q - 8).
 //
-// A CTA is 8 or 16 warps: WR tiles of rows side by side, WK warps to a tile
-// that share its k-blocks, and up to eight CTAs of a cluster that share them
-// again.  x is split once into shared memory, each column of the products a run
-// of its k-slices' fragments and 32 bytes more than a multiple of 128 to the
-// next column, so that neither a column's stores nor a slice's loads over eight
-// columns meet a bank twice, and stays there for all the row tiles the CTA
-// walks.  A product's unused columns are not stored: their lanes read what lies
-// there and their sums go nowhere.  Weights go from memory to a ring of
-// kRing places a warp in shared memory, by bulk copies of kRun k-blocks that
-// one lane issues: they take few issue slots and no registers, and wait for
-// nothing but the warp's own reads.
-// The warps' sums meet in shared memory and are added in one order, so a result
-// does not turn on timing; the sums of a cluster's other CTAs are read where
-// they lie.
+// A CTA has 8 or 16 working warps: WR tiles of rows side by side, WK warps to a
+// tile that share its k-blocks, and up to eight CTAs of a cluster that share
+// them again.  x is split once into shared memory, each column of the products
+// a run of its k-slices' fragments and 32 bytes more than a multiple of 128 to
+// the next column, so that neither a column's stores nor a slice's loads over
+// eight columns meet a bank twice, and stays there for all the row tiles the
+// CTA walks.  A product's unused columns are not stored: their lanes read what
+// lies there and their sums go nowhere.  A further warp brings the weights: a
+// round, kRun k-blocks for every working warp, is one bulk copy for each of the
+// WR tiles into one of kRing places, announced by an mbarrier and refilled when
+// the working warps have said by another that they have read it.  The working
+// warps' sums meet in shared memory and are added in one order, so a result does
+// not turn on timing; the sums of a cluster's other CTAs are read where they
+// lie.  Where there are few sums, one more warp finishes them (chain, gate,
+// store) while the others go on.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -54,22 +55,32 @@ namespace sdb {
 
 constexpr int kQ4MaxShared = 227 * 1024;
 
+// The parameters, in the order of their first use: a launch's parameters come from memory a line at a time, and
+// what a CTA needs before its first copies is within two lines.
 struct Q4Args {
-    Q4View w, gate;            // gate: the gated form's second matrix
-    const void* x;
-    void* y;
-    long long xnb[3], ynb[3];  // strides of rows in elements (dims 1..3)
-    int ne1, ne2;
-    int rows;                  // of x
-    int flat;                  // rows along dimension 1 alone
-    int x_half, x_vec;         // FP16 rows; their runs of four numbers are aligned
-    int y_half;                // FP16 output
-    int act;                   // SDB_GATE_*
-    int wk_log;                // WK = 1 << wk_log
-    int cluster;               // CTAs that share a tile's k-blocks
+    const uint8_t* w;          // tiles (q4.cuh)
+    const uint8_t* gate;       // the gated form's second matrix
+    int tiles, kblocks;        // of 16 rows; of 128 columns
+    int groups;                // of WR row tiles
     int range;                 // k-blocks of a CTA (the last of a cluster may have fewer)
-    int chunk;                 // k-blocks of x held at a time, a multiple of WK
+    int chunk;                 // k-blocks of x held at a time, a multiple of WK unless all of them
+    uint8_t wk_log, wr_log;    // WK = 1 << wk_log warps to a tile, WR = 1 << wr_log tiles
+    uint8_t cluster_log;       // CTAs that share a tile's k-blocks
+    uint8_t minimum;
+    const void* x;
+    long long xnb[3];          // strides of rows in elements (dims 1..3)
+    int k;
+    int rows;                  // of x
+    unsigned inverse;          // i / rows a CTA takes = high(i inverse), for CTAs with as many as there are
+    uint8_t flat;              // rows along dimension 1 alone
+    uint8_t x_half, x_vec;     // FP16 rows; their runs of four numbers are aligned
+    uint8_t y_half;            // FP16 output
+    int ne1, ne2;
     unsigned* err;             // the device error word
+    void* y;
+    long long ynb[3];
+    int n;
+    int act;                   // SDB_GATE_*
     Chain chain;
 };
 
@@ -125,7 +136,7 @@ struct Q4Stage {
 
 // Four numbers of a row from column k on, zeros past the row's end.
 __device__ __forceinline__ float4 q4_four(const Q4Args& a, long long at, int k) {
-    const int cols = static_cast<int>(a.w.k);
+    const int cols = a.k;
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (a.x_half) {
         const __half* p = static_cast<const __half*>(a.x) + at + k;
@@ -156,24 +167,23 @@ __device__ __forceinline__ float4 q4_four(const Q4Args& a, long long at, int k) 
 
 // Splits x: item i is row i % tokens of k-block i / tokens of [kb0, kb1), a warp takes an item and a lane its
 // columns 4 lane .. 4 lane + 3: split(k-block, row, x).  Two items at a time, whose chains of dependent steps
-// overlap, and the next two read before; between() once the first are on their way.  (One copy of the loop's
-// code: a CTA passes it a few times, and the first pass waits for its instructions.)
-template <int WARPS, class Between, class Split>
-__device__ __forceinline__ void q4_items(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Between between,
-                                         Split split) {
+// overlap, and the next two read before.  (One copy of the loop's code: a CTA passes it a few times, and the
+// first pass waits for its instructions.)
+template <int WARPS, int ROWS, class Split>
+__device__ __forceinline__ void q4_items(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Split split) {
     const int lane = threadIdx.x & 31, items = tokens * (kb1 - kb0);
-    const unsigned inverse = 0xffffffffu / static_cast<unsigned>(tokens) + 1;  // i / tokens = high(i inverse), tokens > 1
     float4 x[2];
     int b[2], m[2];
     auto read = [&](int i, int u) {
-        b[u] = tokens == 1 ? i : static_cast<int>(__umulhi(static_cast<unsigned>(i), inverse));
+        b[u] = i;
+        if (tokens > 1)
+            b[u] = tokens == min(a.rows, ROWS) ? static_cast<int>(__umulhi(static_cast<unsigned>(i), a.inverse)) : i / tokens;
         m[u] = i - b[u] * tokens;
         if (i < items) x[u] = q4_four(a, Q4Row(a, m0 + m[u]).at(a.xnb), (kb0 + b[u]) * 128 + lane * 4);
     };
     int i = threadIdx.x / 32;
     read(i, 0);
     read(i + WARPS, 1);
-    between();
 #pragma unroll 1
     while (i < items) {
         const float4 x0 = x[0], x1 = x[1];
@@ -239,7 +249,7 @@ struct Q4Digits {
     static constexpr int kTiles = GATED ? 2 : 1;
     static constexpr int kLaneSums = NT;         // of a tile, joined over the digits
     static constexpr int kWarps = NT <= 2 && !GATED ? 16 : 8;
-    static constexpr int kRun = 2, kRing = 3;    // k-blocks of a copy; copies of a warp on their way
+    static constexpr int kRun = 2, kRing = 3;    // k-blocks of a warp a round; rounds on their way
     static constexpr bool kFinisher = NT <= 2;   // a warp of its own finishes the sums
     static constexpr int kColumn = 160;          // bytes: 4 slices x 32, and a step of 8 banks
 
@@ -261,11 +271,11 @@ struct Q4Digits {
     }
 
     // A column's digits of a k-block are a run of 128 bytes, a lane's four numbers a word of it.
-    template <int G, class Between>
-    __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Between between) const {
+    template <int G>
+    __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1) const {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
-        q4_items<kWarps>(a, m0, tokens, kb0, kb1, between, [&](int b, int m, float4 x, bool store) {
+        q4_items<kWarps, kTokens>(a, m0, tokens, kb0, kb1, [&](int b, int m, float4 x, bool store) {
             // top < 2^(e - 126), e its exponent field: 2^(156 - e) x is below 2^30.  The power's field is
             // 283 - e, kept a normal number's.
             const int e = static_cast<int>(q4_top(x) >> 23), f = min(283 - e, 253);
@@ -288,7 +298,7 @@ struct Q4Digits {
                 const float down = __uint_as_float(static_cast<uint32_t>(254 - f + 8 * lane) << 23) * 0.0625f;
                 factors[b * cols + 4 * m + lane] = e == 255 ? __uint_as_float(0x7fffffffu) : down;
             }
-            if (a.w.minimum) {
+            if (a.minimum) {
                 const float s = q4_group_sum<G>(x);
                 if (store && lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
             }
@@ -480,11 +490,11 @@ struct Q4Halves {
     // A lane's four numbers are columns 0..3 or 4..7 of the run of eight that lane t = lane / 2 % 4 of a fragment
     // holds: a word of slice 2 (lane / 8), the even columns, and one of the next, the odd ones, of hi (a column
     // of product 2 i) and of lo (the same column of product 2 i + 1); FP16 rows have no lo.
-    template <int G, class Between>
-    __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Between between) const {
+    template <int G>
+    __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1) const {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
-        q4_items<kWarps>(a, m0, tokens, kb0, kb1, between, [&](int b, int m, float4 x, bool store) {
+        q4_items<kWarps, kTokens>(a, m0, tokens, kb0, kb1, [&](int b, int m, float4 x, bool store) {
             uint8_t* to = frags + (b * (8 * kProducts) + (HALF ? m : m / 8 * 16 + m % 8)) * kColumn + (lane >> 3) * 64 +
                           (lane >> 1 & 3) * 8 + (lane & 1) * 4;
             if constexpr (HALF) {
@@ -510,7 +520,7 @@ struct Q4Halves {
                 put(x.y * up, x.w * up, 32);
                 if (store && lane == 0) scales[b * kTokens + m] = __uint_as_float(static_cast<uint32_t>(254 - f) << 23);
             }
-            if (a.w.minimum) {
+            if (a.minimum) {
                 const float s = q4_group_sum<G>(x);
                 if (store && lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
             }
@@ -617,7 +627,7 @@ __device__ __forceinline__ void q4_finish(const Q4Args& a, int m, long long n, f
     if (a.chain.from_redirect) v += static_cast<const float*>(a.y)[at];
     v = apply_chain(a.chain, v, n, row.i1, row.i2, row.i3);
     if (gated) {
-        g = apply_chain(a.chain, g, a.w.n + n, row.i1, row.i2, row.i3);
+        g = apply_chain(a.chain, g, a.n + n, row.i1, row.i2, row.i3);
         v *= a.act == SDB_GATE_SILU ? silu(g) : gelu(g);
     }
     if (a.y_half) static_cast<__half*>(a.y)[at] = __float2half_rn(v);
@@ -631,12 +641,12 @@ template <class F>
 constexpr int q4_red_buffers() { return F::kLaneSums <= 4 ? 2 : 1; }
 
 template <class F>
-constexpr int q4_threads() { return 32 * (F::kWarps + (F::kFinisher ? 1 : 0)); }
+constexpr int q4_threads() { return 32 * (F::kWarps + 1 + (F::kFinisher ? 1 : 0)); }
 
-// Shared memory but for the k-blocks of x.
-template <class F, int G>
+// Shared memory but for the k-blocks of x; `block` the bytes of a tile.
+template <class F>
 int q4_fixed_bytes(int block) {
-    return q4_red_buffers<F>() * q4_red_floats<F>() * 4 + F::kWarps * F::kRing * (F::kTiles * F::kRun * block + 8) + 16 +
+    return q4_red_buffers<F>() * q4_red_floats<F>() * 4 + F::kRing * (F::kWarps * F::kTiles * F::kRun * block + 16) + 16 +
            F::kTail;
 }
 
@@ -644,79 +654,64 @@ template <class F, int G>
 __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __grid_constant__ Q4Args a) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    const bool worker = !F::kFinisher || warp < F::kWarps;
-    const int WK = 1 << a.wk_log, WR = F::kWarps >> a.wk_log, wk = warp & (WK - 1), wr = warp >> a.wk_log;
-    const int rank = a.cluster > 1 ? blockIdx.x % a.cluster : 0;
-    const int groups = (a.w.tiles + WR - 1) / WR;  // of WR row tiles
-    const int group0 = a.cluster > 1 ? blockIdx.x / a.cluster : blockIdx.x;
-    const int group_step = a.cluster > 1 ? gridDim.x / a.cluster : gridDim.x;
+    const bool worker = warp < F::kWarps, bringer = warp == F::kWarps;
+    const int WK = 1 << a.wk_log, wk = warp & (WK - 1), wr = warp >> a.wk_log, round_blocks = F::kRun << a.wk_log;
+    const int cluster = 1 << a.cluster_log, rank = blockIdx.x & (cluster - 1);
+    const int groups = a.groups, group0 = blockIdx.x >> a.cluster_log, group_step = gridDim.x >> a.cluster_log;
+    const int kb_begin = rank * a.range, kb_end = min(kb_begin + a.range, a.kblocks);
     const int m0 = blockIdx.y * F::kTokens, tokens = min(F::kTokens, a.rows - m0);
-    const int kb_begin = rank * a.range, kb_end = min(kb_begin + a.range, a.w.kblocks);
-    const bool minima = a.w.minimum != 0;
+    const bool minima = a.minimum != 0;
+    const int block = 1024 + 4096 / G * (minima ? 2 : 1);  // bytes of a tile
+    const int place_bytes = F::kWarps * F::kTiles * F::kRun * block;
 
     float* red = reinterpret_cast<float*>(smem);
-    const int block = 1024 + 4096 / G * (minima ? 2 : 1);  // bytes of a tile, a.w.block
-    const int place_bytes = F::kTiles * F::kRun * block;
-    uint8_t* rings = reinterpret_cast<uint8_t*>(red + q4_red_buffers<F>() * q4_red_floats<F>());
-    uint8_t* ring = rings + warp * (F::kRing * place_bytes);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(rings + F::kWarps * F::kRing * place_bytes);
-    volatile int* abort = reinterpret_cast<volatile int*>(bars + F::kWarps * F::kRing);
-    F form(a, reinterpret_cast<uint8_t*>(bars + F::kWarps * F::kRing) + 16, tokens);
-    bars += warp * F::kRing;
+    uint8_t* ring = reinterpret_cast<uint8_t*>(red + q4_red_buffers<F>() * q4_red_floats<F>());
+    uint64_t* full = reinterpret_cast<uint64_t*>(ring + F::kRing * place_bytes);
+    uint64_t* empty = full + F::kRing;
+    volatile int* abort = reinterpret_cast<volatile int*>(empty + F::kRing);
+    F form(a, reinterpret_cast<uint8_t*>(empty + F::kRing) + 16, tokens);
 
-    // The warp's k-blocks in the order they are taken: for each of its row tiles and each chunk of x, the wk'th
-    // run of the chunk's k-blocks.  A warp past the last tile walks the last one again and stores nothing.
-    struct Walk {
-        int group, kc, kb, stop;
-    };
-    auto enter = [&](Walk& w) {  // the run of (group, kc), or of the first after it that is not empty
-        for (;;) {
-            const int len = min(a.chunk, kb_end - w.kc), per = (len + WK - 1) >> a.wk_log;
-            w.kb = w.kc + wk * per;
-            w.stop = min(w.kb + per, w.kc + len);
-            if (w.kb < w.stop) return;
-            w.kc += a.chunk;
-            if (w.kc >= kb_end) {
-                w.kc = kb_begin;
-                w.group += group_step;
-                if (w.group >= groups) return;
+    // The rounds in order: over the row tiles, the chunks of x and their k-blocks.
+    int next_group = group0, next_kc = kb_begin, next_kb = kb_begin, brought = 0;
+    auto bring = [&](int place) {  // the bringer's warp: the next round
+        if (next_group >= groups) return;
+        const int kc_end = min(next_kc + a.chunk, kb_end), count = min(round_blocks, kc_end - next_kb);
+        if (lane == 0) mbar_arrive_expect_tx(full + place, (F::kTiles << a.wr_log) * count * block);
+        __syncwarp();
+        if (lane < F::kTiles << a.wr_log) {
+            const int tile = min((next_group << a.wr_log) + (lane & ((1 << a.wr_log) - 1)), a.tiles - 1);
+            const uint8_t* from = F::GATED && lane >> a.wr_log ? a.gate : a.w;
+            bulk_load(ring + place * place_bytes + lane * (round_blocks * block),
+                      from + (static_cast<long long>(tile) * a.kblocks + next_kb) * block, count * block, full + place);
+        }
+        ++brought;
+        next_kb += count;
+        if (next_kb == kc_end) {
+            next_kc = kc_end;
+            if (kc_end == kb_end) {
+                next_kc = kb_begin;
+                next_group += group_step;
             }
+            next_kb = next_kc;
         }
     };
-    Walk ahead{kb_begin < kb_end ? group0 : groups, kb_begin, 0, 0};
-    auto load = [&](int place) {  // lane 0: the next run of up to kRun k-blocks
-        if (ahead.group >= groups) return;
-        const int count = min(F::kRun, ahead.stop - ahead.kb);
-        const long long first = static_cast<long long>(min(ahead.group * WR + wr, a.w.tiles - 1)) * a.w.kblocks + ahead.kb;
-        mbar_arrive_expect_tx(bars + place, F::kTiles * count * block);
-        bulk_load(ring + place * place_bytes, a.w.data + first * block, count * block, bars + place);
-        if constexpr (F::GATED)
-            bulk_load(ring + place * place_bytes + F::kRun * block, a.gate.data + first * block, count * block, bars + place);
-        ahead.kb += count;
-        if (ahead.kb >= ahead.stop) {
-            ahead.kc += a.chunk;
-            if (ahead.kc >= kb_end) {
-                ahead.kc = kb_begin;
-                ahead.group += group_step;
-            }
-            if (ahead.group < groups) enter(ahead);
-        }
-    };
-    auto start = [&] {
+    if (bringer) {
         if (lane == 0) {
             *abort = 0;
-            for (int i = 0; i < F::kRing; ++i) mbar_init(bars + i, 1);
+            for (int i = 0; i < F::kRing; ++i) {
+                mbar_init(full + i, 1);
+                mbar_init(empty + i, F::kWarps);
+            }
             fence_barrier_init();
-            if (ahead.group < groups) enter(ahead);
-#pragma unroll 1
-            for (int i = 0; i < F::kRing; ++i) load(i);
         }
         __syncwarp();
-    };
-    bool started = false;
+        if (kb_begin < kb_end)
+#pragma unroll 1
+            for (int i = 0; i < F::kRing; ++i) bring(i);
+    }
 
-    bool held = false;  // the one chunk of x is in shared memory
-    bool lost = false;  // a bounded wait ran out
+    bool started = false, held = false;  // a chunk of x, the only one, is in shared memory
+    bool lost = false;                   // a bounded wait ran out
     int parity = 0, place = 0;
     uint32_t phase = 0;
 #pragma unroll 1
@@ -727,35 +722,39 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
             const int kc_end = min(kc + a.chunk, kb_end);
             if (!held) {
                 if (started) __syncthreads();  // the chunk before has been read
-                if (worker)
-                    form.template split<G>(a, m0, tokens, kc, kc_end, [&] {
-                        if (!started) start();
-                    });
+                if (worker) form.template split<G>(a, m0, tokens, kc, kc_end);
                 started = true;
                 __syncthreads();
                 held = a.chunk >= kb_end - kb_begin;
             }
-            if (!worker || lost) continue;
-            const int per = (kc_end - kc + WK - 1) >> a.wk_log;
-            const int stop = min(wk * per + per, kc_end - kc);
+            if (!worker && !bringer) continue;
 #pragma unroll 1
-            for (int at = wk * per; at < stop; at += F::kRun) {
-                if (!lost) lost = !mbar_wait(bars + place, phase, abort, a.err);
-                if (__any_sync(~0u, lost)) {  // the copies did not come: no more are waited for, no sums made
-                    lost = true;
-                    break;
-                }
-#pragma unroll 1
-                for (int i = 0; i < F::kRun; ++i) {
-                    if (i && at + i >= stop) break;
-                    Q4Stage<G> stage[F::kTiles];
+            for (int kb = kc; kb < kc_end && !lost; kb += round_blocks) {
+                // A wait that runs out ends the rounds for this warp and, by the abort flag, for the others; the
+                // barriers are still met.
+                lost = __any_sync(~0u, !mbar_wait((bringer ? empty : full) + place, phase, abort, a.err));
+                if (lost) break;
+                if (bringer) {
+                    bring(place);
+                } else {
+                    const int at = kb - kc + wk * F::kRun;
+                    const uint8_t* tiles = ring + place * place_bytes + warp * (F::kRun * block);
+                    auto one = [&](int i) {
+                        Q4Stage<G> stage[F::kTiles];
 #pragma unroll
-                    for (int t = 0; t < F::kTiles; ++t)
-                        stage[t].read(ring + place * place_bytes + (t * F::kRun + i) * block, lane, minima);
-                    form.template product<G>(stage, at + i, minima);
+                        for (int t = 0; t < F::kTiles; ++t)
+                            stage[t].read(tiles + t * (F::kWarps * F::kRun * block) + i * block, lane, minima);
+                        form.template product<G>(stage, at + i, minima);
+                    };
+                    if (F::kRun == 2 && at + 1 < kc_end - kc) {  // two k-blocks' chains of products side by side
+                        one(0);
+                        one(1);
+                    } else if (at < kc_end - kc) {
+                        one(0);
+                    }
+                    __syncwarp();  // every lane has read its part
+                    if (lane == 0) mbar_arrive(empty + place);
                 }
-                __syncwarp();  // every lane has read the place that is filled again
-                if (lane == 0) load(place);
                 if (++place == F::kRing) {
                     place = 0;
                     phase ^= 1;
@@ -774,17 +773,18 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
                 for (int i = 0; i < F::kTiles; ++i)
                     mine[((c * F::kTiles + i) * F::kWarps + warp) * 32 + lane] = form.lane_sum(i, c);
         }
-        if (a.cluster > 1) cooperative_groups::this_cluster().sync();
+        if (cluster > 1) cooperative_groups::this_cluster().sync();
         else __syncthreads();
-        // A warp finishes a sum of a tile, all warps or one that does nothing else, while the others go on; a
-        // cluster's CTAs share them.
-        const int item0 = F::kFinisher ? (worker ? F::kLaneSums * WR : 0) : warp, item_step = F::kFinisher ? 1 : F::kWarps;
+        // A warp finishes a sum of a tile: the working warps, or the one that does nothing else.  A cluster's CTAs
+        // share the sums.
+        const int items = F::kLaneSums << a.wr_log, item_step = F::kFinisher ? 1 : F::kWarps;
+        const int item0 = F::kFinisher ? (worker || bringer ? items : 0) : worker ? warp : items;
 #pragma unroll 1
-        for (int o = item0 * a.cluster + rank; o < F::kLaneSums * WR; o += item_step * a.cluster) {
-            const int tw = o & (WR - 1), c = o / WR;
+        for (int o = (item0 << a.cluster_log) + rank; o < items; o += item_step << a.cluster_log) {
+            const int c = o >> a.wr_log, tw = o - (c << a.wr_log);
             const int m = F::token_of(c, lane);
-            const long long n = (static_cast<long long>(group) * WR + tw) * 16 + F::row_of(c, lane);
-            if (m >= tokens || n >= a.w.n) continue;
+            const long long n = ((static_cast<long long>(group) << a.wr_log) + tw) * 16 + F::row_of(c, lane);
+            if (m >= tokens || n >= a.n) continue;
             float v[2] = {0.0f, 0.0f};
             const int at = (c * F::kTiles * F::kWarps + tw * WK) * 32 + lane;
             auto join = [&](const float* from) {
@@ -794,31 +794,30 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
                     for (int i = 0; i < F::kTiles; ++i) v[i] += from[at + (i * F::kWarps + j) * 32];
                 }
             };
-            if (a.cluster > 1) {
+            if (cluster > 1) {
 #pragma unroll 4
-                for (int k = 0; k < a.cluster; ++k) join(cooperative_groups::this_cluster().map_shared_rank(mine, k));
+                for (int k = 0; k < cluster; ++k) join(cooperative_groups::this_cluster().map_shared_rank(mine, k));
             } else {
                 join(mine);
             }
             q4_finish(a, m0 + m, n, v[0], v[1], F::GATED);
         }
         if constexpr (q4_red_buffers<F>() == 1) {
-            if (a.cluster > 1) cooperative_groups::this_cluster().sync();
+            if (cluster > 1) cooperative_groups::this_cluster().sync();
             else __syncthreads();
         }
     }
-    if (lost) {  // copies may still be on their way into this CTA's memory: wait for them, with a limit again
-        for (int i = 0; i < F::kRing; ++i) 
-            mbar_wait_quiet(bars + (place + i) % F::kRing, i < F::kRing - place ? phase : phase ^ 1, kWaitLimitNs);
-    }
-    if (a.cluster > 1) cooperative_groups::this_cluster().sync();  // the others have read this CTA's sums
+    if (bringer && lost)  // copies may still be on their way into this CTA's memory: wait for them, with a limit
+        for (int i = max(0, brought - F::kRing); i < brought; ++i)
+            mbar_wait_quiet(full + i % F::kRing, i / F::kRing & 1, kWaitLimitNs);
+    if (cluster > 1) cooperative_groups::this_cluster().sync();  // the others have read this CTA's sums
 }
 
 // How a product is cut (q4_linear.cu).
 struct Q4Plan {
     int form;      // rows of x a CTA takes: 2, 4 or 8 in digits; 16 or 32 in halves
     int wk_log;    // warps that share a row tile's k-blocks (fewer where their k-blocks of x do not fit)
-    int cluster;   // CTAs that do
+    int cluster_log;  // CTAs that do
     int shared;    // bytes of shared memory a CTA may take
 };
 
