@@ -134,66 +134,74 @@ struct Q4Stage {
     }
 };
 
-// Four numbers of a row from column k on, zeros past the row's end.
-__device__ __forceinline__ float4 q4_four(const Q4Args& a, long long at, int k) {
-    const int cols = a.k;
-    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (a.x_half) {
-        const __half* p = static_cast<const __half*>(a.x) + at + k;
-        if (a.x_vec && k + 4 <= cols) {
-            const uint2 r = __ldg(reinterpret_cast<const uint2*>(p));
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.x));
-            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
-            x = make_float4(f.x, f.y, h.x, h.y);
-        } else {
-            if (k < cols) x.x = __half2float(p[0]);
-            if (k + 1 < cols) x.y = __half2float(p[1]);
-            if (k + 2 < cols) x.z = __half2float(p[2]);
-            if (k + 3 < cols) x.w = __half2float(p[3]);
-        }
-    } else {
-        const float* p = static_cast<const float*>(a.x) + at + k;
-        if (a.x_vec && k + 4 <= cols) {
-            x = __ldg(reinterpret_cast<const float4*>(p));
-        } else {
-            if (k < cols) x.x = p[0];
-            if (k + 1 < cols) x.y = p[1];
-            if (k + 2 < cols) x.z = p[2];
-            if (k + 3 < cols) x.w = p[3];
+// Splitting x: item i is row i % tokens of k-block i / tokens of a chunk, a warp takes an item and a lane its
+// columns 4 lane .. 4 lane + 3.  The numbers come first, all items' at once and in the background, into the very
+// columns that take their fragments -- a lane's four into slot(k-block, row), 16 bytes (8, FP16, with HALF_SLOT) --
+// in a short loop: what a CTA does once costs it the fetching of the instructions more than their work.
+struct Q4Items {
+    int first, items, tokens;
+    unsigned inverse;  // i / tokens = high(i inverse), where known and tokens > 1
+    __device__ __forceinline__ Q4Items(const Q4Args& a, int tokens_, int blocks, int rows)
+        : first(threadIdx.x / 32), items(tokens_ * blocks), tokens(tokens_),
+          inverse(tokens_ == min(a.rows, rows) ? a.inverse : 0xffffffffu / static_cast<unsigned>(tokens_) + 1) {}
+    __device__ __forceinline__ int block(int i) const {
+        return tokens == 1 ? i : static_cast<int>(__umulhi(static_cast<unsigned>(i), inverse));
+    }
+};
+
+template <int WARPS, bool HALF_SLOT, class Slot>
+__device__ __forceinline__ void q4_fetch(const Q4Args& a, const Q4Items& it, int m0, int kb0, Slot slot) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int i = it.first; i < it.items; i += WARPS) {
+        const int b = it.block(i), m = i - b * it.tokens, k = (kb0 + b) * 128 + lane * 4;
+        const long long at = Q4Row(a, m0 + m).at(a.xnb) + k;
+        uint8_t* to = slot(b, m);
+        const uint32_t to32 = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+        if (a.x_vec && k + 4 <= a.k) {
+            if (a.x_half)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to32), "l"(static_cast<const __half*>(a.x) + at)
+                             : "memory");
+            else if constexpr (!HALF_SLOT)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to32), "l"(static_cast<const float*>(a.x) + at)
+                             : "memory");
+        } else if (a.x_half) {
+            for (int c = 0; c < 4; ++c)
+                reinterpret_cast<__half*>(to)[c] =
+                    k + c < a.k ? static_cast<const __half*>(a.x)[at + c] : __ushort_as_half(0);
+        } else if constexpr (!HALF_SLOT) {
+            for (int c = 0; c < 4; ++c)
+                reinterpret_cast<float*>(to)[c] = k + c < a.k ? static_cast<const float*>(a.x)[at + c] : 0.0f;
         }
     }
-    return x;
 }
 
-// Splits x: item i is row i % tokens of k-block i / tokens of [kb0, kb1), a warp takes an item and a lane its
-// columns 4 lane .. 4 lane + 3: split(k-block, row, x).  Two items at a time, whose chains of dependent steps
-// overlap, and the next two read before.  (One copy of the loop's code: a CTA passes it a few times, and the
-// first pass waits for its instructions.)
-template <int WARPS, int ROWS, class Split>
-__device__ __forceinline__ void q4_items(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Split split) {
-    const int lane = threadIdx.x & 31, items = tokens * (kb1 - kb0);
-    float4 x[2];
-    int b[2], m[2];
-    auto read = [&](int i, int u) {
-        b[u] = i;
-        if (tokens > 1)
-            b[u] = tokens == min(a.rows, ROWS) ? static_cast<int>(__umulhi(static_cast<unsigned>(i), a.inverse)) : i / tokens;
-        m[u] = i - b[u] * tokens;
-        if (i < items) x[u] = q4_four(a, Q4Row(a, m0 + m[u]).at(a.xnb), (kb0 + b[u]) * 128 + lane * 4);
-    };
-    int i = threadIdx.x / 32;
-    read(i, 0);
-    read(i + WARPS, 1);
+// A lane's four numbers out of its slot.
+template <bool HALF_SLOT>
+__device__ __forceinline__ float4 q4_slot(const Q4Args& a, const uint8_t* from) {
+    if (HALF_SLOT || a.x_half) {
+        const uint2 r = *reinterpret_cast<const uint2*>(from);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.x));
+        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
+        return make_float4(f.x, f.y, h.x, h.y);
+    }
+    return *reinterpret_cast<const float4*>(from);
+}
+
+// split(k-block, row, x, store) of a warp's items, two at a time, whose chains of dependent steps overlap.
+template <int WARPS, bool HALF_SLOT, class Slot, class Split>
+__device__ __forceinline__ void q4_split(const Q4Args& a, const Q4Items& it, Slot slot, Split split) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 1
-    while (i < items) {
-        const float4 x0 = x[0], x1 = x[1];
-        const int b0 = b[0], b1 = b[1], r0 = m[0], r1 = m[1];
-        const bool two = i + WARPS < items;
-        i += 2 * WARPS;
-        read(i, 0);
-        read(i + WARPS, 1);
+    for (int i = it.first; i < it.items; i += 2 * WARPS) {
+        // Without a second item the first one's is computed again and not stored.
+        const bool two = i + WARPS < it.items;
+        const int j = two ? i + WARPS : i, b0 = it.block(i), b1 = it.block(j);
+        const int r0 = i - b0 * it.tokens, r1 = j - b1 * it.tokens;
+        const float4 x0 = q4_slot<HALF_SLOT>(a, slot(b0, r0)), x1 = q4_slot<HALF_SLOT>(a, slot(b1, r1));
+        __syncwarp();  // every lane has its numbers: the fragments may take their places
         split(b0, r0, x0, true);
-        split(b1, r1, x1, two);  // without a second item: computed on what is there and not stored
+        split(b1, r1, x1, two);
     }
 }
 
@@ -271,11 +279,18 @@ struct Q4Digits {
     }
 
     // A column's digits of a k-block are a run of 128 bytes, a lane's four numbers a word of it.
-    template <int G>
-    __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1) const {
+    // read() once the numbers are on their way.
+    template <int G, class Read>
+    __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Read read) const {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
-        q4_items<kWarps, kTokens>(a, m0, tokens, kb0, kb1, [&](int b, int m, float4 x, bool store) {
+        const Q4Items it(a, tokens, kb1 - kb0, kTokens);
+        auto slot = [&](int b, int m) {
+            return frags + (b * cols + 4 * m + (lane >> 3)) * kColumn + (lane & 7) * 16;
+        };
+        q4_fetch<kWarps, false>(a, it, m0, kb0, slot);
+        read();
+        q4_split<kWarps, false>(a, it, slot, [&](int b, int m, float4 x, bool store) {
             // top < 2^(e - 126), e its exponent field: 2^(156 - e) x is below 2^30.  The power's field is
             // 283 - e, kept a normal number's.
             const int e = static_cast<int>(q4_top(x) >> 23), f = min(283 - e, 253);
@@ -490,13 +505,21 @@ struct Q4Halves {
     // A lane's four numbers are columns 0..3 or 4..7 of the run of eight that lane t = lane / 2 % 4 of a fragment
     // holds: a word of slice 2 (lane / 8), the even columns, and one of the next, the odd ones, of hi (a column
     // of product 2 i) and of lo (the same column of product 2 i + 1); FP16 rows have no lo.
-    template <int G>
-    __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1) const {
+    template <int G, class Read>
+    __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Read read) const {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
-        q4_items<kWarps, kTokens>(a, m0, tokens, kb0, kb1, [&](int b, int m, float4 x, bool store) {
-            uint8_t* to = frags + (b * (8 * kProducts) + (HALF ? m : m / 8 * 16 + m % 8)) * kColumn + (lane >> 3) * 64 +
-                          (lane >> 1 & 3) * 8 + (lane & 1) * 4;
+        const Q4Items it(a, tokens, kb1 - kb0, kTokens);
+        auto column = [&](int b, int m) {
+            return frags + (b * (8 * kProducts) + (HALF ? m : m / 8 * 16 + m % 8)) * kColumn;
+        };
+        auto slot = [&](int b, int m) {
+            return HALF ? column(b, m) + lane * 8 : column(b, m) + (lane >> 4) * (8 * kColumn) + (lane & 15) * 16;
+        };
+        q4_fetch<kWarps, HALF>(a, it, m0, kb0, slot);
+        read();
+        q4_split<kWarps, HALF>(a, it, slot, [&](int b, int m, float4 x, bool store) {
+            uint8_t* to = column(b, m) + (lane >> 3) * 64 + (lane >> 1 & 3) * 8 + (lane & 1) * 4;
             if constexpr (HALF) {
                 if (store) {
                     *reinterpret_cast<__half2*>(to) = __floats2half2_rn(x.x, x.z);
@@ -705,9 +728,12 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
             fence_barrier_init();
         }
         __syncwarp();
-        if (kb_begin < kb_end)
+        if (kb_begin < kb_end) {
+            // After the working warps' first reads of x, which would else queue behind all of this.
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * (F::kWarps + 1)) : "memory");
 #pragma unroll 1
             for (int i = 0; i < F::kRing; ++i) bring(i);
+        }
     }
 
     bool started = false, held = false;  // a chunk of x, the only one, is in shared memory
@@ -722,7 +748,10 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
             const int kc_end = min(kc + a.chunk, kb_end);
             if (!held) {
                 if (started) __syncthreads();  // the chunk before has been read
-                if (worker) form.template split<G>(a, m0, tokens, kc, kc_end);
+                if (worker)
+                    form.template split<G>(a, m0, tokens, kc, kc_end, [&] {
+                        if (!started) asm volatile("bar.arrive 1, %0;" ::"n"(32 * (F::kWarps + 1)) : "memory");
+                    });
                 started = true;
                 __syncthreads();
                 held = a.chunk >= kb_end - kb_begin;
