@@ -26,7 +26,6 @@ int q4_launch_form(const Q4Args& args, const Q4Plan& p, cudaStream_t st) {
     a.range = (a.kblocks + cluster - 1) / cluster;
     // The k-blocks of x held at a time: all of the CTA's, or the multiple of WK that fits.
     const int rows = std::min(a.rows, F::kTokens);
-    a.inverse = rows > 1 ? 0xffffffffu / static_cast<unsigned>(rows) + 1 : 0;
     const int fixed = q4_fixed_bytes<F>(1024 + 4096 / G * (a.minimum ? 2 : 1));
     const int block = F::block_bytes(rows, 128 / G);
     const int fit = (p.shared - fixed) / block;

@@ -71,7 +71,6 @@ struct Q4Args {
     long long xnb[3];          // strides of rows in elements (dims 1..3)
     int k;
     int rows;                  // of x
-    unsigned inverse;          // i / rows a CTA takes = high(i inverse), for CTAs with as many as there are
     uint8_t flat;              // rows along dimension 1 alone
     uint8_t x_half, x_vec;     // FP16 rows; their runs of four numbers are aligned
     uint8_t y_half;            // FP16 output
@@ -134,44 +133,57 @@ struct Q4Stage {
     }
 };
 
-// Splitting x: item i is row i % tokens of k-block i / tokens of a chunk, a warp takes an item and a lane its
-// columns 4 lane .. 4 lane + 3.  The numbers come first, all items' at once and in the background, into the very
+// Splitting x: a warp takes a row's k-blocks, a lane columns 4 lane .. 4 lane + 3 of each.  With fewer rows than
+// warps, warps / rows of them share a row.  The numbers come first, all of them in the background, into the very
 // columns that take their fragments -- a lane's four into slot(k-block, row), 16 bytes (8, FP16, with HALF_SLOT) --
-// in a short loop: what a CTA does once costs it the fetching of the instructions more than their work.
+// in short loops of running addresses: what a CTA does once costs it the latency of its instructions.
 struct Q4Items {
-    int first, items, tokens;
-    unsigned inverse;  // i / tokens = high(i inverse), where known and tokens > 1
-    __device__ __forceinline__ Q4Items(const Q4Args& a, int tokens_, int blocks, int rows)
-        : first(threadIdx.x / 32), items(tokens_ * blocks), tokens(tokens_),
-          inverse(tokens_ == min(a.rows, rows) ? a.inverse : 0xffffffffu / static_cast<unsigned>(tokens_) + 1) {}
-    __device__ __forceinline__ int block(int i) const {
-        return tokens == 1 ? i : static_cast<int>(__umulhi(static_cast<unsigned>(i), inverse));
+    int row, row_step, block, block_step;
+    __device__ __forceinline__ Q4Items(int warps, int tokens) : row(threadIdx.x / 32), row_step(warps), block(0), block_step(1) {
+        if (tokens < warps) {
+            block_step = tokens == 1 ? warps : warps / tokens;
+            block = tokens == 1 ? row : row / tokens;
+            row -= block * tokens;
+            if (block >= block_step) row = tokens;  // a warp too many
+        }
     }
 };
 
-template <int WARPS, bool HALF_SLOT, class Slot>
-__device__ __forceinline__ void q4_fetch(const Q4Args& a, const Q4Items& it, int m0, int kb0, Slot slot) {
+template <bool HALF_SLOT, class Slot>
+__device__ __forceinline__ void q4_fetch(const Q4Args& a, const Q4Items& it, int m0, int tokens, int kb0, int blocks,
+                                         Slot slot) {
     const int lane = threadIdx.x & 31;
 #pragma unroll 1
-    for (int i = it.first; i < it.items; i += WARPS) {
-        const int b = it.block(i), m = i - b * it.tokens, k = (kb0 + b) * 128 + lane * 4;
+    for (int m = it.row; m < tokens; m += it.row_step) {
+        int k = (kb0 + it.block) * 128 + lane * 4;
         const long long at = Q4Row(a, m0 + m).at(a.xnb) + k;
-        uint8_t* to = slot(b, m);
-        const uint32_t to32 = static_cast<uint32_t>(__cvta_generic_to_shared(to));
-        if (a.x_vec && k + 4 <= a.k) {
-            if (a.x_half)
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to32), "l"(static_cast<const __half*>(a.x) + at)
-                             : "memory");
-            else if constexpr (!HALF_SLOT)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to32), "l"(static_cast<const float*>(a.x) + at)
-                             : "memory");
-        } else if (a.x_half) {
-            for (int c = 0; c < 4; ++c)
-                reinterpret_cast<__half*>(to)[c] =
-                    k + c < a.k ? static_cast<const __half*>(a.x)[at + c] : __ushort_as_half(0);
+        uint8_t* to = slot(it.block, m);
+        const int to_step = static_cast<int>(slot(it.block_step, 0) - slot(0, 0));
+        if (a.x_half) {
+            const __half* from = static_cast<const __half*>(a.x) + at;
+#pragma unroll 2
+            for (int b = it.block; b < blocks; b += it.block_step) {
+                if (a.x_vec && k + 4 <= a.k)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+                else
+                    for (int c = 0; c < 4; ++c)
+                        reinterpret_cast<__half*>(to)[c] = k + c < a.k ? from[c] : __ushort_as_half(0);
+                from += it.block_step * 128;
+                k += it.block_step * 128;
+                to += to_step;
+            }
         } else if constexpr (!HALF_SLOT) {
-            for (int c = 0; c < 4; ++c)
-                reinterpret_cast<float*>(to)[c] = k + c < a.k ? static_cast<const float*>(a.x)[at + c] : 0.0f;
+            const float* from = static_cast<const float*>(a.x) + at;
+#pragma unroll 2
+            for (int b = it.block; b < blocks; b += it.block_step) {
+                if (a.x_vec && k + 4 <= a.k)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+                else
+                    for (int c = 0; c < 4; ++c) reinterpret_cast<float*>(to)[c] = k + c < a.k ? from[c] : 0.0f;
+                from += it.block_step * 128;
+                k += it.block_step * 128;
+                to += to_step;
+            }
         }
     }
 }
@@ -189,20 +201,20 @@ __device__ __forceinline__ float4 q4_slot(const Q4Args& a, const uint8_t* from) 
 }
 
 // split(k-block, row, x, store) of a warp's items, two at a time, whose chains of dependent steps overlap.
-template <int WARPS, bool HALF_SLOT, class Slot, class Split>
-__device__ __forceinline__ void q4_split(const Q4Args& a, const Q4Items& it, Slot slot, Split split) {
-    asm volatile("cp.async.wait_all;" ::: "memory");
+template <bool HALF_SLOT, class Slot, class Split>
+__device__ __forceinline__ void q4_split(const Q4Args& a, const Q4Items& it, int tokens, int blocks, Slot slot, Split split) {
 #pragma unroll 1
-    for (int i = it.first; i < it.items; i += 2 * WARPS) {
-        // Without a second item the first one's is computed again and not stored.
-        const bool two = i + WARPS < it.items;
-        const int j = two ? i + WARPS : i, b0 = it.block(i), b1 = it.block(j);
-        const int r0 = i - b0 * it.tokens, r1 = j - b1 * it.tokens;
-        const float4 x0 = q4_slot<HALF_SLOT>(a, slot(b0, r0)), x1 = q4_slot<HALF_SLOT>(a, slot(b1, r1));
-        __syncwarp();  // every lane has its numbers: the fragments may take their places
-        split(b0, r0, x0, true);
-        split(b1, r1, x1, two);
-    }
+    for (int m = it.row; m < tokens; m += it.row_step)
+#pragma unroll 1
+        for (int b = it.block; b < blocks; b += 2 * it.block_step) {
+            // Without a second item the first one's is computed again and not stored.
+            const bool two = b + it.block_step < blocks;
+            const int c = two ? b + it.block_step : b;
+            const float4 x0 = q4_slot<HALF_SLOT>(a, slot(b, m)), x1 = q4_slot<HALF_SLOT>(a, slot(c, m));
+            __syncwarp();  // every lane has its numbers: the fragments may take their places
+            split(b, m, x0, true);
+            split(c, m, x1, two);
+        }
 }
 
 // The greatest magnitude of a warp's numbers, as FP32 bits (a NaN's bits are greater than an infinity's).
@@ -284,13 +296,14 @@ struct Q4Digits {
     __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Read read) const {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
-        const Q4Items it(a, tokens, kb1 - kb0, kTokens);
+        const Q4Items it(kWarps, tokens);
         auto slot = [&](int b, int m) {
             return frags + (b * cols + 4 * m + (lane >> 3)) * kColumn + (lane & 7) * 16;
         };
-        q4_fetch<kWarps, false>(a, it, m0, kb0, slot);
+        q4_fetch<false>(a, it, m0, tokens, kb0, kb1 - kb0, slot);
         read();
-        q4_split<kWarps, false>(a, it, slot, [&](int b, int m, float4 x, bool store) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        q4_split<false>(a, it, tokens, kb1 - kb0, slot, [&](int b, int m, float4 x, bool store) {
             // top < 2^(e - 126), e its exponent field: 2^(156 - e) x is below 2^30.  The power's field is
             // 283 - e, kept a normal number's.
             const int e = static_cast<int>(q4_top(x) >> 23), f = min(283 - e, 253);
@@ -509,16 +522,17 @@ struct Q4Halves {
     __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Read read) const {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
-        const Q4Items it(a, tokens, kb1 - kb0, kTokens);
+        const Q4Items it(kWarps, tokens);
         auto column = [&](int b, int m) {
             return frags + (b * (8 * kProducts) + (HALF ? m : m / 8 * 16 + m % 8)) * kColumn;
         };
         auto slot = [&](int b, int m) {
             return HALF ? column(b, m) + lane * 8 : column(b, m) + (lane >> 4) * (8 * kColumn) + (lane & 15) * 16;
         };
-        q4_fetch<kWarps, HALF>(a, it, m0, kb0, slot);
+        q4_fetch<HALF>(a, it, m0, tokens, kb0, kb1 - kb0, slot);
         read();
-        q4_split<kWarps, HALF>(a, it, slot, [&](int b, int m, float4 x, bool store) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        q4_split<HALF>(a, it, tokens, kb1 - kb0, slot, [&](int b, int m, float4 x, bool store) {
             uint8_t* to = column(b, m) + (lane >> 3) * 64 + (lane >> 1 & 3) * 8 + (lane & 1) * 4;
             if constexpr (HALF) {
                 if (store) {
