@@ -21,22 +21,27 @@ int q4_launch_form(const Q4Args& args, const Q4Plan& p, cudaStream_t st) {
         if (dev < 64) raised.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
     Q4Args a = args;
-    const int cluster = 1 << p.cluster_log;
-    a.cluster_log = static_cast<uint8_t>(p.cluster_log);
-    a.range = (a.kblocks + cluster - 1) / cluster;
-    // The k-blocks of x held at a time: all of the CTA's, or the multiple of WK that fits.
-    const int rows = std::min(a.rows, F::kTokens);
     const int fixed = q4_fixed_bytes<F>(1024 + 4096 / G * (a.minimum ? 2 : 1));
-    const int block = F::block_bytes(rows, 128 / G);
-    const int fit = (p.shared - fixed) / block;
-    int wk_log = p.wk_log;
+    const int block = F::block_bytes(std::min(a.rows, F::kTokens), 128 / G);
+    const int fit = (p.shared - fixed) / block;  // k-blocks of x that fit
+    // All of a CTA's k-blocks of x are held where a cluster of up to eight brings them down to what fits: else x is
+    // split again for every tile (28672 -> 8192, one row: two CTAs 31 us, one 67).
+    int wk_log = p.wk_log, cluster_log = p.cluster_log;
+    while (cluster_log < 3 && ((a.kblocks - 1) >> cluster_log) + 1 > fit) {
+        ++cluster_log;
+        if (wk_log > 0) --wk_log;
+    }
+    const int cluster = 1 << cluster_log;
+    a.cluster_log = static_cast<uint8_t>(cluster_log);
+    a.range = (a.kblocks + cluster - 1) / cluster;
     while ((1 << wk_log) > F::kWarps || (wk_log > 0 && (1 << wk_log) > fit)) --wk_log;
     const int wk = 1 << wk_log, wr = F::kWarps / wk;
     if (fit < wk) return fail(SDB_CUDA_ERROR, "mul_mat_q4: shared memory");
     a.wk_log = static_cast<uint8_t>(wk_log);
     a.wr_log = 0;
     while ((1 << a.wr_log) < wr) ++a.wr_log;
-    a.chunk = std::min(a.range, fit / wk * wk);
+    // The k-blocks of x held at a time: all of the CTA's, or the multiple of WK that fits.
+    a.chunk = std::min(a.range, a.range <= fit ? a.range : fit / wk * wk);
     a.groups = (a.tiles + wr - 1) / wr;
     const int blocks = std::min(a.groups, std::max(1, current_sm_count() / cluster)) * cluster;
     const int runs = (a.rows + F::kTokens - 1) / F::kTokens;  // of x's rows
