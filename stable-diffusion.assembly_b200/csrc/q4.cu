@@ -1,7 +1,7 @@
 // 4-bit matrices: made from FP16 / FP32 numbers, from 4-bit numbers and group
 // scales, or from ggml's Q4_0 / Q4_1 blocks, and turned back into FP32.
 //
-// All four are one pass over the matrix, a thread to a word of eight columns
+// All four are one pass over the matrix, a lane to a word of eight columns
 // (q4.cuh), bound by memory.
 #include <cuda_runtime.h>
 
@@ -16,21 +16,19 @@ namespace sdb {
 
 namespace {
 
-// A thread's word: threads run along k, 16 words a k-block, over the padded matrix.
+// A warp takes 1024 columns of a row, four runs of 256, a lane a word of eight columns of each: no division to
+// find them, and four loads on their way.
+constexpr int kRuns = 4;
+
+__host__ inline dim3 word_grid(const Q4View& v, long long rows) {
+    return dim3(static_cast<unsigned>((rows + 7) / 8), static_cast<unsigned>((v.kblocks + 7) / 8));
+}
+
 struct WordAt {
     long long row, k0;
+    __device__ __forceinline__ WordAt(int run)
+        : row(blockIdx.x * 8LL + threadIdx.x / 32), k0(blockIdx.y * 1024LL + run * 256 + (threadIdx.x & 31) * 8) {}
 };
-
-__device__ __forceinline__ WordAt word_at(const Q4View& v, long long i) {
-    const long long per_row = static_cast<long long>(v.kblocks) * 16;
-    const long long row = i / per_row;
-    return {row, (i - row * per_row) * 8};
-}
-
-__host__ inline int word_blocks(const Q4View& v) {
-    const long long total = static_cast<long long>(v.tiles) * 16 * v.kblocks * 16;
-    return static_cast<int>(std::min<long long>((total + 255) / 256, 148LL * 32));
-}
 
 __device__ __forceinline__ float saturate_half(float v) { return fminf(fmaxf(v, -65504.0f), 65504.0f); }
 
@@ -46,18 +44,14 @@ __device__ __forceinline__ float saturate_half(float v) { return fminf(fmaxf(v, 
 // stands for NaN throughout.
 template <typename T, bool MINIMUM>
 __global__ void __launch_bounds__(256) q4_quantize_kernel(const T* __restrict__ w, long long ld, Q4View v) {
-    const long long total = static_cast<long long>(v.tiles) * 16 * v.kblocks * 16;
     const int lanes = v.group / 8;
-    // A row is a whole number of 16 threads' runs, so a group's lanes leave the loop together.
-    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-        const WordAt at = word_at(v, i);
-        float x[8];
-        float hi = -INFINITY, lo = INFINITY;
-        bool bad = false;
-        const bool row_in = at.row < v.n;
+    float xs[kRuns][8];
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r) {
+        const WordAt at(r);
+        float (&x)[8] = xs[r];
         const T* src = w + at.row * ld + at.k0;
-        const bool whole = row_in && at.k0 + 8 <= v.k && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-        if (whole) {
+        if (at.row < v.n && at.k0 + 8 <= v.k && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
             if constexpr (sizeof(T) == 4) {
                 const float4 a = __ldg(reinterpret_cast<const float4*>(src));
                 const float4 b = __ldg(reinterpret_cast<const float4*>(src) + 1);
@@ -76,17 +70,25 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const T* __restrict__ 
         } else {
 #pragma unroll
             for (int c = 0; c < 8; ++c)
-                x[c] = row_in && at.k0 + c < v.k ? static_cast<float>(src[c]) : 0.0f;
+                x[c] = at.row < v.n && at.k0 + c < v.k ? static_cast<float>(src[c]) : 0.0f;
         }
+    }
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r) {
+        const WordAt at(r);
+        if (at.k0 >= v.kblocks * 128LL) break;  // whole groups of lanes leave together: k-blocks are 16 lanes
+        const float (&x)[8] = xs[r];
+        float hi = -INFINITY, lo = INFINITY;
+        bool bad = false;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            if (row_in && at.k0 + c < v.k) {
+            if (at.row < v.n && at.k0 + c < v.k) {
                 hi = fmaxf(hi, x[c]);
                 lo = fminf(lo, x[c]);
                 bad |= !(fabsf(x[c]) < INFINITY);
             }
         }
-        // The group's own lanes: all of them are in this iteration.
+        // The group's own lanes: all of them are here.
         const unsigned mask = ((1u << lanes) - 1u) << (threadIdx.x & 31 & ~(lanes - 1));
         for (int o = 1; o < lanes; o <<= 1) {
             hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
@@ -100,7 +102,7 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const T* __restrict__ 
                 dh = __float2half_rn(saturate_half(__fdiv_rn(__fsub_rn(hi, lo), 15.0f)));
                 mh = __float2half_rn(saturate_half(lo));
             } else {
-                dh = __float2half_rn(saturate_half(__fdiv_rn(hi >= -lo ? hi : lo, -8.0f)));
+                dh = __float2half_rn(saturate_half((hi >= -lo ? hi : lo) * -0.125f));  // s / -8: exact but for the lowest
             }
             if (bad) dh = __ushort_as_half(0x7fff);
         }
@@ -130,9 +132,9 @@ __global__ void __launch_bounds__(256) q4_import_kernel(const uint8_t* __restric
                                                         const __half* __restrict__ scales,
                                                         const __half* __restrict__ minima, long long groups,
                                                         Q4View v) {
-    const long long total = static_cast<long long>(v.tiles) * 16 * v.kblocks * 16;
-    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-        const WordAt at = word_at(v, i);
+    for (int r = 0; r < kRuns; ++r) {
+        const WordAt at(r);
+        if (at.k0 >= v.kblocks * 128LL) break;
         const bool row_in = at.row < v.n;
         uint32_t word = 0;
 #pragma unroll
@@ -160,9 +162,9 @@ __global__ void __launch_bounds__(256) q4_import_kernel(const uint8_t* __restric
 __global__ void __launch_bounds__(256) q4_blocks_kernel(const uint8_t* __restrict__ blocks, long long row_bytes,
                                                         Q4View v) {
     const int header = v.minimum ? 4 : 2, size = header + 16;
-    const long long total = static_cast<long long>(v.tiles) * 16 * v.kblocks * 16;
-    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-        const WordAt at = word_at(v, i);
+    for (int r = 0; r < kRuns; ++r) {
+        const WordAt at(r);
+        if (at.k0 >= v.kblocks * 128LL) break;
         const bool in = at.row < v.n && at.k0 < v.k;
         const uint8_t* b = blocks + at.row * row_bytes + at.k0 / 32 * size;
         const int first = static_cast<int>(at.k0) & 31;
@@ -191,10 +193,10 @@ __global__ void __launch_bounds__(256) q4_blocks_kernel(const uint8_t* __restric
 }
 
 __global__ void __launch_bounds__(256) q4_dequantize_kernel(Q4View v, float* __restrict__ w, long long ld) {
-    const long long total = v.n * v.kblocks * 16;
-    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-        const WordAt at = word_at(v, i);
-        if (at.k0 >= v.k) continue;
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r) {
+        const WordAt at(r);
+        if (at.row >= v.n || at.k0 >= v.k) continue;
         const uint32_t word = __ldg(q4_word(v, at.row, at.k0)) ^ 0x88888888u;
         const __half* s = q4_scale(v, at.row, at.k0);
         const float d = __half2float(s[0]);
@@ -253,7 +255,7 @@ int sdb_q4_quantize(const sdb_tensor* w, const sdb_q4* q, void* stream) {
     prepare_device();
     const Q4View v = q4_view(q);
     const auto st = static_cast<cudaStream_t>(stream);
-    const int blocks = word_blocks(v);
+    const dim3 blocks = word_grid(v, v.tiles * 16LL);
     if (w->type == SDB_TYPE_F32) {
         const auto* src = static_cast<const float*>(w->data);
         if (v.minimum) q4_quantize_kernel<float, true><<<blocks, 256, 0, st>>>(src, w->nb[1] / 4, v);
@@ -275,7 +277,7 @@ int sdb_q4_import(const void* codes, const void* scales, const void* minima, con
         return fail(SDB_INVALID, "sdb_q4_import: codes, FP16 scales and (with `minimum`, only then) FP16 minima");
     prepare_device();
     const Q4View v = q4_view(q);
-    q4_import_kernel<<<word_blocks(v), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+    q4_import_kernel<<<word_grid(v, v.tiles * 16LL), 256, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const uint8_t*>(codes), (q->k + 1) / 2, static_cast<const __half*>(scales),
         static_cast<const __half*>(minima), (q->k + q->group - 1) / q->group, v);
     count_launch();
@@ -291,7 +293,7 @@ int sdb_q4_from_blocks(const void* blocks, int64_t row_bytes, const sdb_q4* q, v
         return fail(SDB_INVALID, "sdb_q4_from_blocks: no blocks, or rows shorter than k / 32 blocks");
     prepare_device();
     const Q4View v = q4_view(q);
-    q4_blocks_kernel<<<word_blocks(v), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+    q4_blocks_kernel<<<word_grid(v, v.tiles * 16LL), 256, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const uint8_t*>(blocks), row_bytes, v);
     count_launch();
     SDB_CUDA(cudaGetLastError());
@@ -303,9 +305,7 @@ int sdb_q4_dequantize(const sdb_q4* q, const sdb_tensor* w, void* stream) {
     if (!matrix_of(w, q, false))
         return fail(SDB_INVALID, "sdb_q4_dequantize: w must be an FP32 matrix [k, n] with contiguous rows");
     const Q4View v = q4_view(q);
-    const long long total = v.n * v.kblocks * 16;
-    const int blocks_n = static_cast<int>(std::min<long long>((total + 255) / 256, 148LL * 32));
-    q4_dequantize_kernel<<<blocks_n, 256, 0, static_cast<cudaStream_t>(stream)>>>(v, static_cast<float*>(w->data),
+    q4_dequantize_kernel<<<word_grid(v, v.n), 256, 0, static_cast<cudaStream_t>(stream)>>>(v, static_cast<float*>(w->data),
                                                                                 w->nb[1] / 4);
     count_launch();
     SDB_CUDA(cudaGetLastError());

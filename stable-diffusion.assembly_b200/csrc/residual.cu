@@ -4,10 +4,13 @@
 // post and pre are nothing, a LayerNorm or an RMS norm of the row; gate, mul
 // and add are operands of the output's extents or broadcast along any of them.
 //
-// A CTA per row. The mean of a LayerNorm comes from a first sum, the variance
-// from the sum of d^2 about that float mean less the square of d's own mean
-// (d = v - mean), so that rows far from 0 lose nothing. Sums are FP32 in a
-// thread (a thread's share of a row) and across threads.
+// Bound by memory: x and y are read once and h and out written once, the row's
+// numbers in registers in between, both statistics and the normalisations from
+// there -- a warp a row up to 1280 numbers, a CTA up to 16384 (residual_kernel);
+// wider rows are read again for each pass (residual_rows_kernel).  The mean of a
+// LayerNorm comes from a first sum, the variance from the sum of d^2 about that
+// float mean less the square of d's own mean (d = v - mean), so that rows far
+// from 0 lose nothing; sums are FP32, a thread's share of a row and a tree.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -149,6 +152,184 @@ __global__ void __launch_bounds__(kRowThreads) residual_rows_kernel(const Residu
     }
 }
 
+// ---- rows in registers
+
+// Four numbers at p[0..3] (16 or 8 bytes at a time); plain loads, since h and out may be the same memory.
+__device__ __forceinline__ float4 get4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 get4(const __half* p) {
+    const uint2 r = *reinterpret_cast<const uint2*>(p);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ void put4(float* p, const float (&v)[4]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void put4(__half* p, const float (&v)[4]) {
+    const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// The sum over the T threads of a row, in all of them; *buffer alternates, so that a sum's partial sums are not
+// overwritten before every warp has read them.
+template <int T>
+__device__ __forceinline__ float2 row_sum(float2 v, int* buffer) {
+    for (int o = 16; o; o >>= 1) {
+        v.x += __shfl_xor_sync(~0u, v.x, o);
+        v.y += __shfl_xor_sync(~0u, v.y, o);
+    }
+    if constexpr (T > 32) {
+        __shared__ float2 part[2][T / 32];
+        float2* p = part[*buffer];
+        *buffer ^= 1;
+        if ((threadIdx.x & 31) == 0) p[threadIdx.x / 32] = v;
+        __syncthreads();
+        v = p[0];
+#pragma unroll
+        for (int w = 1; w < T / 32; ++w) {
+            v.x += p[w].x;
+            v.y += p[w].y;
+        }
+    }
+    return v;
+}
+
+// T threads a row (32: eight rows a CTA), 4 V numbers a thread: with VEC, runs of four (rows of a multiple of four
+// numbers, aligned), else one by one.  A thread's numbers lie T (runs) apart.
+template <typename TX, typename TY, int V, int T, bool VEC>
+__global__ void __launch_bounds__(T == 32 ? 256 : T) residual_kernel(const __grid_constant__ ResidualArgs a) {
+    const int t = T == 32 ? threadIdx.x & 31 : threadIdx.x;
+    constexpr int kRows = T == 32 ? 8 : 1;
+    int buffer = 0;
+    auto at = [&](int v, int e) { return VEC ? (v * T + t) * 4 + e : (v * 4 + e) * T + t; };
+    for (long long row = blockIdx.x * static_cast<long long>(kRows) + (T == 32 ? threadIdx.x / 32 : 0); row < a.rows;
+         row += gridDim.x * static_cast<long long>(kRows)) {
+        const int q = static_cast<int>(row) / static_cast<int>(a.ne1), i1 = static_cast<int>(row) - q * static_cast<int>(a.ne1);
+        const int i3 = q / static_cast<int>(a.ne2), i2 = q - i3 * static_cast<int>(a.ne2);
+        auto base = [&](const long long (&nb)[3]) { return i1 * nb[0] + i2 * nb[1] + i3 * nb[2]; };
+        float h[V][4], u[V][4];
+        auto load = [&](float (&to)[V][4], const auto* p) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if constexpr (VEC) {
+                    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (at(v, 0) < a.c) f = get4(p + at(v, 0));
+                    to[v][0] = f.x; to[v][1] = f.y; to[v][2] = f.z; to[v][3] = f.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) to[v][e] = at(v, e) < a.c ? get(p, at(v, e)) : 0.0f;
+                }
+            }
+        };
+        // f(v, e, operand's number) over the row, the operand's numbers nb apart.
+        auto with = [&](const float* p, long long nb, auto f) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float o[4];
+                if (VEC && nb == 1 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+                    float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (at(v, 0) < a.c) w = __ldg(reinterpret_cast<const float4*>(p + at(v, 0)));
+                    o[0] = w.x; o[1] = w.y; o[2] = w.z; o[3] = w.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = at(v, e) < a.c ? __ldg(p + at(v, e) * nb) : 0.0f;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f(v, e, o[e]);
+            }
+        };
+        auto normalise = [&](const NormForm& n, float (&to)[V][4]) {
+            if (n.kind == SDB_NORM_NONE) return;
+            const float inv = 1.0f / static_cast<float>(a.c);
+            float2 s{0.0f, 0.0f};
+            float shift = 0.0f;
+            if (n.kind == SDB_NORM_LAYER) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) s.x += (to[v][0] + to[v][1]) + (to[v][2] + to[v][3]);
+                const float mean = row_sum<T>(s, &buffer).x * inv;
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) to[v][e] = at(v, e) < a.c ? to[v][e] - mean : 0.0f;
+                s.x = 0.0f;
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s.x += to[v][e];
+                    s.y = fmaf(to[v][e], to[v][e], s.y);
+                }
+            s = row_sum<T>(s, &buffer);
+            if (n.kind == SDB_NORM_LAYER) shift = s.x * inv;
+            const float rstd = 1.0f / sqrtf(fmaxf(s.y * inv - shift * shift, 0.0f) + n.eps);
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) to[v][e] = (to[v][e] - shift) * rstd;
+            if (n.weight) with(n.weight, 1, [&](int v, int e, float w) { to[v][e] *= w; });
+            if (n.bias) with(n.bias, 1, [&](int v, int e, float b) { to[v][e] += b; });
+        };
+        auto store = [&](auto* p, const float (&from)[V][4]) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if constexpr (VEC) {
+                    if (at(v, 0) < a.c) put4(p + at(v, 0), from[v]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (at(v, e) < a.c) put(p, at(v, e), from[v][e]);
+                }
+            }
+        };
+        auto operand = [&](const Operand& o) { return o.data + i1 * o.nb[1] + i2 * o.nb[2] + i3 * o.nb[3]; };
+
+        if (a.y) load(u, static_cast<const TY*>(a.y) + base(a.ynb));
+        if (a.x) load(h, static_cast<const TX*>(a.x) + base(a.xnb));
+        if (a.y) {
+            normalise(a.post, u);
+            if (a.gate.data) with(operand(a.gate), a.gate.nb[0], [&](int v, int e, float g) { u[v][e] *= g; });
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float s = a.x ? a.keep * h[v][e] : 0.0f;
+                if (a.y) s = fmaf(a.scale, u[v][e], s);
+                h[v][e] = s;
+            }
+        if (a.h) store(static_cast<TX*>(a.h) + base(a.hnb), h);
+        if (a.out) {
+            normalise(a.pre, h);
+            if (a.mul.data) with(operand(a.mul), a.mul.nb[0], [&](int v, int e, float m) { h[v][e] *= 1.0f + m; });
+            if (a.add.data) with(operand(a.add), a.add.nb[0], [&](int v, int e, float m) { h[v][e] += m; });
+            store(static_cast<TY*>(a.out) + base(a.onb), h);
+        }
+    }
+}
+
+template <typename TX, typename TY, int V, int T>
+void launch_rows(const ResidualArgs& a, bool vec, cudaStream_t st) {
+    constexpr int rows = T == 32 ? 8 : 1, threads = T == 32 ? 256 : T;
+    const unsigned blocks = static_cast<unsigned>(std::min<long long>((a.rows + rows - 1) / rows, 1LL << 20));
+    if (vec) residual_kernel<TX, TY, V, T, true><<<blocks, threads, 0, st>>>(a);
+    else residual_kernel<TX, TY, V, T, false><<<blocks, threads, 0, st>>>(a);
+}
+
+template <typename TX, typename TY>
+void launch(const ResidualArgs& a, bool vec, cudaStream_t st) {
+    if (a.c <= 256) launch_rows<TX, TY, 2, 32>(a, vec, st);
+    else if (a.c <= 640) launch_rows<TX, TY, 5, 32>(a, vec, st);
+    else if (a.c <= 1280) launch_rows<TX, TY, 10, 32>(a, vec, st);
+    else if (a.c <= 2048) launch_rows<TX, TY, 2, 256>(a, vec, st);
+    else if (a.c <= 4096) launch_rows<TX, TY, 4, 256>(a, vec, st);
+    else if (a.c <= 8192) launch_rows<TX, TY, 4, 512>(a, vec, st);
+    else if (a.c <= 16384) launch_rows<TX, TY, 8, 512>(a, vec, st);
+    else
+        residual_rows_kernel<TX, TY>
+            <<<static_cast<unsigned>(std::min<long long>(a.rows, 148LL * 32)), kRowThreads, 0, st>>>(a);
+}
+
 bool rows_of(const sdb_tensor* t, bool written) {
     if (t->type != SDB_TYPE_F32 && t->type != SDB_TYPE_F16) return false;
     const int64_t es = t->type == SDB_TYPE_F16 ? 2 : 4;
@@ -238,11 +419,18 @@ extern "C" int sdb_residual_norm(const sdb_tensor* x, const sdb_tensor* y, const
     const sdb_tensor* ty = y ? y : out;
     const bool xh = tx && tx->type == SDB_TYPE_F16, yh = ty && ty->type == SDB_TYPE_F16;
     const auto st = static_cast<cudaStream_t>(stream);
-    const int blocks = static_cast<int>(std::min<long long>(a.rows, 148LL * 32));
-    if (xh && yh) residual_rows_kernel<__half, __half><<<blocks, kRowThreads, 0, st>>>(a);
-    else if (xh) residual_rows_kernel<__half, float><<<blocks, kRowThreads, 0, st>>>(a);
-    else if (yh) residual_rows_kernel<float, __half><<<blocks, kRowThreads, 0, st>>>(a);
-    else residual_rows_kernel<float, float><<<blocks, kRowThreads, 0, st>>>(a);
+    bool vec = a.c % 4 == 0;
+    for (const sdb_tensor* t : {x, y, h, out}) {
+        if (t == nullptr) continue;
+        const int64_t run = t->type == SDB_TYPE_F16 ? 8 : 16;
+        if (reinterpret_cast<uintptr_t>(t->data) % run != 0) vec = false;
+        for (int d = 1; d < 4; ++d)
+            if (t->ne[d] > 1 && t->nb[d] % run != 0) vec = false;
+    }
+    if (xh && yh) launch<__half, __half>(a, vec, st);
+    else if (xh) launch<__half, float>(a, vec, st);
+    else if (yh) launch<float, __half>(a, vec, st);
+    else launch<float, float>(a, vec, st);
     count_launch();
     SDB_CUDA(cudaGetLastError());
     return SDB_OK;
