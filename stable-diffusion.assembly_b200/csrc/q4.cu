@@ -102,21 +102,37 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const T* __restrict__ 
                 dh = __float2half_rn(saturate_half(__fdiv_rn(__fsub_rn(hi, lo), 15.0f)));
                 mh = __float2half_rn(saturate_half(lo));
             } else {
-                dh = __float2half_rn(saturate_half((hi >= -lo ? hi : lo) * -0.125f));  // s / -8: exact but for the lowest
+                dh = __float2half_rn(saturate_half((hi >= -lo ? hi : lo) * -0.125f));  // s / -8
             }
             if (bad) dh = __ushort_as_half(0x7fff);
         }
         const float d = __half2float(dh), m = __half2float(mh);
-        uint32_t word = 0;
+        // With 1 / d for the division, t is off by under 3e-6: where that is far from the next integer the number
+        // is the formula's; else (one word in thousands) the word is made again by true divisions.  t is clamped
+        // first, and 2^23 + t rounded towards zero ends in its floor.
+        constexpr float add = MINIMUM ? 0.5f : 8.5f;
+        uint32_t word = MINIMUM ? 0u : 0x88888888u;
+        if (d != 0.0f) {
+            const float inverse = __fdiv_rn(1.0f, d);
+            bool near = !(fabsf(inverse) < INFINITY);
+            word = 0;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            float q = MINIMUM ? 0.0f : 8.0f;
-            if (d != 0.0f) {
-                q = MINIMUM ? __fadd_rn(__fdiv_rn(__fsub_rn(x[c], m), d), 0.5f)
-                            : __fadd_rn(__fdiv_rn(x[c], d), 8.5f);
-                q = fminf(fmaxf(floorf(q), 0.0f), 15.0f);
+            for (int c = 0; c < 8; ++c) {
+                const float n = MINIMUM ? __fsub_rn(x[c], m) : x[c];
+                const float t = fminf(fmaxf(__fadd_rn(__fmul_rn(n, inverse), add), 0.0f), 15.5f);
+                const float f = __fadd_rz(t, 8388608.0f);
+                near |= fabsf(t - (f - 8388608.0f) - 0.5f) > 0.4999f;
+                word |= (__float_as_uint(f) & 15u) << q4_bit(c);
             }
-            word |= static_cast<uint32_t>(static_cast<int>(q)) << q4_bit(c);
+            if (near) {
+                word = 0;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const float n = MINIMUM ? __fsub_rn(x[c], m) : x[c];
+                    const float q = fminf(fmaxf(floorf(__fadd_rn(__fdiv_rn(n, d), add)), 0.0f), 15.0f);
+                    word |= static_cast<uint32_t>(static_cast<int>(q)) << q4_bit(c);
+                }
+            }
         }
         *q4_word(v, at.row, at.k0) = word ^ 0x88888888u;
         if (at.k0 % v.group == 0) {
@@ -192,30 +208,50 @@ __global__ void __launch_bounds__(256) q4_blocks_kernel(const uint8_t* __restric
     }
 }
 
+// A run's numbers cross shared memory, so that a store's lanes write neighbours.
 __global__ void __launch_bounds__(256) q4_dequantize_kernel(Q4View v, float* __restrict__ w, long long ld) {
+    __shared__ __align__(16) float turned[8][256];
+    float* own = turned[threadIdx.x / 32];
+    const int lane = threadIdx.x & 31;
+    uint32_t words[kRuns];
+    float ds[kRuns], ms[kRuns];
 #pragma unroll
     for (int r = 0; r < kRuns; ++r) {
         const WordAt at(r);
-        if (at.row >= v.n || at.k0 >= v.k) continue;
-        const uint32_t word = __ldg(q4_word(v, at.row, at.k0)) ^ 0x88888888u;
-        const __half* s = q4_scale(v, at.row, at.k0);
-        const float d = __half2float(s[0]);
-        const float m = v.minimum ? __half2float(s[16 * v.ng]) : 0.0f;
+        words[r] = 0x88888888u;
+        ds[r] = ms[r] = 0.0f;
+        if (at.row < v.n && at.k0 < v.k) {
+            words[r] = __ldg(q4_word(v, at.row, at.k0)) ^ 0x88888888u;
+            const __half* s = q4_scale(v, at.row, at.k0);
+            ds[r] = __half2float(s[0]);
+            if (v.minimum) ms[r] = __half2float(s[16 * v.ng]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r) {
+        const WordAt at(r);
+        const long long first = at.k0 - lane * 8;  // the warp's run
+        if (at.row >= v.n || first >= v.k) break;
         float x[8];
         // d q and d (q - 8) are exact in FP32 (11 and 4 bits).
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            const float code = static_cast<float>(word >> q4_bit(c) & 15u);
-            x[c] = v.minimum ? fmaf(d, code, m) : d * (code - 8.0f);
+            const float code = static_cast<float>(words[r] >> q4_bit(c) & 15u);
+            x[c] = v.minimum ? fmaf(ds[r], code, ms[r]) : ds[r] * (code - 8.0f);
         }
-        float* dst = w + at.row * ld + at.k0;
-        if (at.k0 + 8 <= v.k && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-            reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
-            reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        __syncwarp();  // the run before has been read
+        reinterpret_cast<float4*>(own)[lane * 2] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(own)[lane * 2 + 1] = make_float4(x[4], x[5], x[6], x[7]);
+        __syncwarp();
+        float* dst = w + at.row * ld + first;
+        if (first + 256 <= v.k && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                reinterpret_cast<float4*>(dst)[i * 32 + lane] = reinterpret_cast<const float4*>(own)[i * 32 + lane];
         } else {
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-                if (at.k0 + c < v.k) dst[c] = x[c];
+            for (int i = 0; i < 8; ++i)
+                if (first + i * 32 + lane < v.k) dst[i * 32 + lane] = own[i * 32 + lane];
         }
     }
 }

@@ -6,7 +6,7 @@
 //
 // Bound by memory: x and y are read once and h and out written once, the row's
 // numbers in registers in between, both statistics and the normalisations from
-// there -- a warp a row up to 1280 numbers, a CTA up to 16384 (residual_kernel);
+// there -- a warp a row up to 512 numbers, a CTA up to 16384 (residual_kernel);
 // wider rows are read again for each pass (residual_rows_kernel).  The mean of a
 // LayerNorm comes from a first sum, the variance from the sum of d^2 about that
 // float mean less the square of d's own mean (d = v - mean), so that rows far
@@ -319,9 +319,9 @@ void launch_rows(const ResidualArgs& a, bool vec, cudaStream_t st) {
 template <typename TX, typename TY>
 void launch(const ResidualArgs& a, bool vec, cudaStream_t st) {
     if (a.c <= 256) launch_rows<TX, TY, 2, 32>(a, vec, st);
-    else if (a.c <= 640) launch_rows<TX, TY, 5, 32>(a, vec, st);
-    else if (a.c <= 1280) launch_rows<TX, TY, 10, 32>(a, vec, st);
-    else if (a.c <= 2048) launch_rows<TX, TY, 2, 256>(a, vec, st);
+    else if (a.c <= 512) launch_rows<TX, TY, 4, 32>(a, vec, st);
+    else if (a.c <= 1280) launch_rows<TX, TY, 5, 64>(a, vec, st);
+    else if (a.c <= 2048) launch_rows<TX, TY, 4, 128>(a, vec, st);
     else if (a.c <= 4096) launch_rows<TX, TY, 4, 256>(a, vec, st);
     else if (a.c <= 8192) launch_rows<TX, TY, 4, 512>(a, vec, st);
     else if (a.c <= 16384) launch_rows<TX, TY, 8, 512>(a, vec, st);
