@@ -24,11 +24,10 @@ __host__ inline dim3 word_grid(const Q4View& v, long long rows) {
     return dim3(static_cast<unsigned>((rows + 7) / 8), static_cast<unsigned>((v.kblocks + 7) / 8));
 }
 
-struct WordAt {
-    long long row, k0;
-    __device__ __forceinline__ WordAt(int run)
-        : row(blockIdx.x * 8LL + threadIdx.x / 32), k0(blockIdx.y * 1024LL + run * 256 + (threadIdx.x & 31) * 8) {}
-};
+__device__ __forceinline__ long long word_row() { return blockIdx.x * 8LL + threadIdx.x / 32; }
+__device__ __forceinline__ int word_column(int run) {
+    return static_cast<int>(blockIdx.y) * 1024 + run * 256 + (threadIdx.x & 31) * 8;
+}
 
 __device__ __forceinline__ float saturate_half(float v) { return fminf(fmaxf(v, -65504.0f), 65504.0f); }
 
@@ -44,14 +43,16 @@ __device__ __forceinline__ float saturate_half(float v) { return fminf(fmaxf(v, 
 // stands for NaN throughout.
 template <typename T, bool MINIMUM>
 __global__ void __launch_bounds__(256) q4_quantize_kernel(const T* __restrict__ w, long long ld, Q4View v) {
-    const int lanes = v.group / 8;
+    const int lanes = v.group / 8, k = static_cast<int>(v.k);
+    const long long row = word_row();
+    const Q4RowAt to(v, row);
     float xs[kRuns][8];
 #pragma unroll
     for (int r = 0; r < kRuns; ++r) {
-        const WordAt at(r);
+        const int k0 = word_column(r), cols = row < v.n ? k - k0 : 0;
         float (&x)[8] = xs[r];
-        const T* src = w + at.row * ld + at.k0;
-        if (at.row < v.n && at.k0 + 8 <= v.k && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+        const T* src = w + row * ld + k0;
+        if (cols >= 8 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
             if constexpr (sizeof(T) == 4) {
                 const float4 a = __ldg(reinterpret_cast<const float4*>(src));
                 const float4 b = __ldg(reinterpret_cast<const float4*>(src) + 1);
@@ -68,33 +69,32 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const T* __restrict__ 
                 }
             }
         } else {
+            // Past the row's end its last number again, which changes neither extreme.
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-                x[c] = at.row < v.n && at.k0 + c < v.k ? static_cast<float>(src[c]) : 0.0f;
+            for (int c = 0; c < 8; ++c) x[c] = cols > 0 ? static_cast<float>(src[min(c, cols - 1)]) : 0.0f;
         }
     }
 #pragma unroll
     for (int r = 0; r < kRuns; ++r) {
-        const WordAt at(r);
-        if (at.k0 >= v.kblocks * 128LL) break;  // whole groups of lanes leave together: k-blocks are 16 lanes
+        const int k0 = word_column(r);
+        if (k0 >= v.kblocks * 128) break;  // whole groups of lanes leave together: k-blocks are 16 lanes
+        const bool in = row < v.n && k0 < k;
         const float (&x)[8] = xs[r];
-        float hi = -INFINITY, lo = INFINITY;
-        bool bad = false;
+        float hi = in ? x[0] : -INFINITY, lo = in ? x[0] : INFINITY, zero = 0.0f;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            if (at.row < v.n && at.k0 + c < v.k) {
-                hi = fmaxf(hi, x[c]);
-                lo = fminf(lo, x[c]);
-                bad |= !(fabsf(x[c]) < INFINITY);
-            }
+            hi = in ? fmaxf(hi, x[c]) : hi;
+            lo = in ? fminf(lo, x[c]) : lo;
+            zero = fmaf(x[c], 0.0f, zero);  // NaN from an infinity or a NaN
         }
         // The group's own lanes: all of them are here.
         const unsigned mask = ((1u << lanes) - 1u) << (threadIdx.x & 31 & ~(lanes - 1));
         for (int o = 1; o < lanes; o <<= 1) {
             hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
             lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
-            bad |= __shfl_xor_sync(mask, static_cast<int>(bad), o) != 0;
+            zero += __shfl_xor_sync(mask, zero, o);
         }
+        const bool bad = zero != 0.0f;
         const bool empty = hi < lo;  // a group of padding
         __half dh = __float2half_rn(0.0f), mh = dh;
         if (!empty) {
@@ -134,9 +134,9 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const T* __restrict__ 
                 }
             }
         }
-        *q4_word(v, at.row, at.k0) = word ^ 0x88888888u;
-        if (at.k0 % v.group == 0) {
-            __half* s = q4_scale(v, at.row, at.k0);
+        *to.word(k0) = word ^ 0x88888888u;
+        if ((k0 & (v.group - 1)) == 0) {
+            __half* s = to.scale(k0);
             *s = dh;
             if (MINIMUM) s[16 * v.ng] = mh;
         }
@@ -148,9 +148,15 @@ __global__ void __launch_bounds__(256) q4_import_kernel(const uint8_t* __restric
                                                         const __half* __restrict__ scales,
                                                         const __half* __restrict__ minima, long long groups,
                                                         Q4View v) {
+    struct {
+        long long row;
+        int k0;
+    } at;
+    at.row = word_row();
+    const Q4RowAt to(v, at.row);
     for (int r = 0; r < kRuns; ++r) {
-        const WordAt at(r);
-        if (at.k0 >= v.kblocks * 128LL) break;
+        at.k0 = word_column(r);
+        if (at.k0 >= v.kblocks * 128) break;
         const bool row_in = at.row < v.n;
         uint32_t word = 0;
 #pragma unroll
@@ -162,9 +168,9 @@ __global__ void __launch_bounds__(256) q4_import_kernel(const uint8_t* __restric
             }
             word |= q << q4_bit(c);
         }
-        *q4_word(v, at.row, at.k0) = word ^ 0x88888888u;
+        *to.word(at.k0) = word ^ 0x88888888u;
         if (at.k0 % v.group == 0) {
-            __half* s = q4_scale(v, at.row, at.k0);
+            __half* s = to.scale(at.k0);
             const bool in = row_in && at.k0 < v.k;
             const long long from = at.row * groups + at.k0 / v.group;
             *s = in ? scales[from] : __float2half_rn(0.0f);
@@ -178,9 +184,15 @@ __global__ void __launch_bounds__(256) q4_import_kernel(const uint8_t* __restric
 __global__ void __launch_bounds__(256) q4_blocks_kernel(const uint8_t* __restrict__ blocks, long long row_bytes,
                                                         Q4View v) {
     const int header = v.minimum ? 4 : 2, size = header + 16;
+    struct {
+        long long row;
+        int k0;
+    } at;
+    at.row = word_row();
+    const Q4RowAt to(v, at.row);
     for (int r = 0; r < kRuns; ++r) {
-        const WordAt at(r);
-        if (at.k0 >= v.kblocks * 128LL) break;
+        at.k0 = word_column(r);
+        if (at.k0 >= v.kblocks * 128) break;
         const bool in = at.row < v.n && at.k0 < v.k;
         const uint8_t* b = blocks + at.row * row_bytes + at.k0 / 32 * size;
         const int first = static_cast<int>(at.k0) & 31;
@@ -194,9 +206,9 @@ __global__ void __launch_bounds__(256) q4_blocks_kernel(const uint8_t* __restric
             }
             word |= q << q4_bit(c);
         }
-        *q4_word(v, at.row, at.k0) = word ^ 0x88888888u;
+        *to.word(at.k0) = word ^ 0x88888888u;
         if (first == 0) {
-            __half* s = q4_scale(v, at.row, at.k0);
+            __half* s = to.scale(at.k0);
             uint32_t d = 0, m = 0;
             if (in) {
                 d = b[0] | static_cast<uint32_t>(b[1]) << 8;
@@ -213,25 +225,27 @@ __global__ void __launch_bounds__(256) q4_dequantize_kernel(Q4View v, float* __r
     __shared__ __align__(16) float turned[8][256];
     float* own = turned[threadIdx.x / 32];
     const int lane = threadIdx.x & 31;
+    const long long row = word_row();
+    const Q4RowAt from(v, row);
+    const int k = static_cast<int>(v.k);
     uint32_t words[kRuns];
     float ds[kRuns], ms[kRuns];
 #pragma unroll
     for (int r = 0; r < kRuns; ++r) {
-        const WordAt at(r);
-        words[r] = 0x88888888u;
+        const int k0 = word_column(r);
+        words[r] = 0;
         ds[r] = ms[r] = 0.0f;
-        if (at.row < v.n && at.k0 < v.k) {
-            words[r] = __ldg(q4_word(v, at.row, at.k0)) ^ 0x88888888u;
-            const __half* s = q4_scale(v, at.row, at.k0);
+        if (row < v.n && k0 < k) {
+            words[r] = __ldg(from.word(k0)) ^ 0x88888888u;
+            const __half* s = from.scale(k0);
             ds[r] = __half2float(s[0]);
             if (v.minimum) ms[r] = __half2float(s[16 * v.ng]);
         }
     }
 #pragma unroll
     for (int r = 0; r < kRuns; ++r) {
-        const WordAt at(r);
-        const long long first = at.k0 - lane * 8;  // the warp's run
-        if (at.row >= v.n || first >= v.k) break;
+        const int first = word_column(r) - lane * 8;  // the warp's run
+        if (row >= v.n || first >= k) break;
         float x[8];
         // d q and d (q - 8) are exact in FP32 (11 and 4 bits).
 #pragma unroll
@@ -243,15 +257,15 @@ __global__ void __launch_bounds__(256) q4_dequantize_kernel(Q4View v, float* __r
         reinterpret_cast<float4*>(own)[lane * 2] = make_float4(x[0], x[1], x[2], x[3]);
         reinterpret_cast<float4*>(own)[lane * 2 + 1] = make_float4(x[4], x[5], x[6], x[7]);
         __syncwarp();
-        float* dst = w + at.row * ld + first;
-        if (first + 256 <= v.k && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+        float* dst = w + row * ld + first;
+        if (first + 256 <= k && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 reinterpret_cast<float4*>(dst)[i * 32 + lane] = reinterpret_cast<const float4*>(own)[i * 32 + lane];
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (first + i * 32 + lane < v.k) dst[i * 32 + lane] = own[i * 32 + lane];
+                if (first + i * 32 + lane < k) dst[i * 32 + lane] = own[i * 32 + lane];
         }
     }
 }

@@ -1,7 +1,8 @@
 // 4-bit matrices with group scales: the layout that mul_mat_q4 reads.
 //
 // A matrix of n rows of k numbers is held in tiles of 16 rows x 128 columns
-// (rows and columns padded; padding stands for 0), the tiles of 16 rows one
+// (rows and columns padded: padded rows and groups stand for 0, the columns
+// that fill up a short group meet zeros of x), the tiles of 16 rows one
 // after another and each in order of k, so that any run of a row tile's
 // k-blocks is one run of memory.  A tile is
 //   codes   [half 2][lane 32][4 words]: lane g * 4 + t of half h holds row
@@ -65,22 +66,29 @@ inline Q4View q4_view(const sdb_q4* q) {
     return v;
 }
 
-__host__ __device__ inline uint8_t* q4_tile(const Q4View& v, long long r, long long k) {
-    return v.data + ((r >> 4) * v.kblocks + (k >> 7)) * v.block;
-}
-
-// The word of row r's columns k0..k0 + 7 (k0 a multiple of 8).
-__host__ __device__ inline uint32_t* q4_word(const Q4View& v, long long r, long long k0) {
-    const int h = static_cast<int>(r >> 3) & 1, g = static_cast<int>(r) & 7;
-    const int j = static_cast<int>(k0 >> 5) & 3, t = static_cast<int>(k0 >> 3) & 3;
-    return reinterpret_cast<uint32_t*>(q4_tile(v, r, k0)) + (h * 32 + g * 4 + t) * 4 + j;
-}
-
-// The scale of row r's column k; its minimum, if any, lies 16 ng numbers on.
-__host__ __device__ inline __half* q4_scale(const Q4View& v, long long r, long long k) {
-    const int h = static_cast<int>(r >> 3) & 1, g = static_cast<int>(r) & 7;
-    return reinterpret_cast<__half*>(q4_tile(v, r, k) + 1024) + (g * 2 + h) * v.ng + static_cast<int>(k & 127) / v.group;
-}
+// A row of the matrix.
+struct Q4RowAt {
+    uint8_t* base;  // of its row tile
+    int word0, scale0, block, ng, group_log;
+    __device__ __forceinline__ Q4RowAt(const Q4View& v, long long r) {
+        const int h = static_cast<int>(r >> 3) & 1, g = static_cast<int>(r) & 7;
+        base = v.data + (r >> 4) * v.kblocks * v.block;
+        word0 = (h * 32 + g * 4) * 16;
+        scale0 = 1024 + (g * 2 + h) * v.ng * 2;
+        block = v.block;
+        ng = v.ng;
+        group_log = v.ng == 4 ? 5 : v.ng == 2 ? 6 : 7;
+    }
+    // The word of columns k0..k0 + 7 (k0 a multiple of 8).
+    __device__ __forceinline__ uint32_t* word(int k0) const {
+        return reinterpret_cast<uint32_t*>(base + static_cast<long long>(k0 >> 7) * block + word0 + (k0 >> 3 & 3) * 16 +
+                                           (k0 >> 5 & 3) * 4);
+    }
+    // The scale of column k; its minimum, if any, lies 16 ng numbers on.
+    __device__ __forceinline__ __half* scale(int k) const {
+        return reinterpret_cast<__half*>(base + static_cast<long long>(k >> 7) * block + scale0 + ((k & 127) >> group_log) * 2);
+    }
+};
 
 // The bit of column i (0..7) of a word.
 __host__ __device__ constexpr int q4_bit(int i) { return (i & 3) * 8 + (i >> 2) * 4; }
