@@ -67,14 +67,14 @@ Q4Plan plan(const Q4Args& a) {
     p.form = a.rows <= 2 ? 2 : a.rows <= 4 ? 4 : a.rows <= 8 ? 8 : a.rows <= 16 ? 16 : 32;
     p.shared = kQ4MaxShared;
     const bool gated = a.gate != nullptr;
-    const int warps = p.form <= 4 && !gated ? 16 : 8, runs = (a.rows + p.form - 1) / p.form;
+    const int warps = (p.form <= 4 || p.form == 16) && !gated ? 16 : 8, runs = (a.rows + p.form - 1) / p.form;
     if (p.form <= 4) {
         p.wk_log = 3;
     } else if (a.kblocks >= 16) {
         p.cluster_log = gated ? 1 : 2;
         p.wk_log = gated && p.form == 8 ? 1 : 0;
     } else {
-        p.wk_log = p.form == 32 ? 0 : 1;
+        p.wk_log = p.form == 8 || (gated && p.form == 16) ? 1 : 0;
     }
     while ((warps >> p.wk_log) > 1 &&
            (static_cast<long long>(a.tiles / (warps >> p.wk_log)) << p.cluster_log) * runs < current_sm_count() / 2)

@@ -497,7 +497,7 @@ struct Q4Halves {
     static constexpr int kTiles = GATED ? 2 : 1;
     static constexpr int kLaneSums = 4 * T;
     static constexpr int kProducts = HALF ? T : 2 * T;
-    static constexpr int kWarps = 8;
+    static constexpr int kWarps = T == 2 && !GATED ? 16 : 8;
     static constexpr int kRun = 1, kRing = GATED ? 3 : 4;
     static constexpr bool kFinisher = false;
     static constexpr int kColumn = 288;  // bytes: 8 slices x 32, and a step of 8 banks
