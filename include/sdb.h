@@ -139,7 +139,8 @@ int sdb_q4_dequantize(const sdb_q4 *q, const sdb_tensor *w, void *stream);
  * sdb_mul_mat).  x [K, ...] and dst [N, ...] FP32 or FP16, each row contiguous,
  * rows (at most 2^20) over dimensions 1..3 at any strides; x and dst do not overlap.  Products
  * and sums are FP32 whatever the types (x to its last bit), dst rounded once.
- * A chain's redirect needs an FP32 dst.  No rows: nothing is done.  No device
+ * A row of x that holds an infinity or a NaN gives numbers that are not finite,
+ * and no other row does.  A chain's redirect needs an FP32 dst.  No rows: nothing is done.  No device
  * memory is allocated and none is shared between calls. */
 int sdb_mul_mat_q4_supported(const sdb_q4 *w, const sdb_tensor *x, const sdb_tensor *dst);
 int sdb_mul_mat_q4(const sdb_q4 *w, const sdb_tensor *x, const sdb_tensor *dst, const sdb_chain *chain,

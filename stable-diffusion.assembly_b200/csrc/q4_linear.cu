@@ -56,25 +56,25 @@ bool chain_ok(const sdb_chain* c, const sdb_tensor* dst, bool gated) {
 //
 // With up to four rows x is cheap and the weights are all: eight warps share a tile, so that a round is a long
 // run of memory (8192 -> 28672, one row: 29.9 us; four warps 32.7, sixteen 31.1).  With more rows a CTA spends as
-// long on splitting x as on its products: the CTAs of a cluster split it between them instead, a warp a tile
-// (4096 -> 4096, 8 rows: four CTAs and one warp a tile 10.1 us, two and two 11.5, one and eight 24; 32 rows 21.0,
-// 28.1, 74), but for short rows (1280 -> 20160, 16 rows: two warps and no cluster 24.4, a cluster of two 27.1) and
-// for two matrices, whose sums take the registers (4096 -> 11008, 8 rows: two CTAs and two warps 28.4, four and one
-// 39.0).  And where the tiles leave most SMs idle, more warps share one (5120 -> 1280, one row: sixteen 5.7 us,
-// eight 6.7).
+// long on splitting x as on its products: the CTAs of a cluster split it between them, and few warps share a tile
+// (32 rows of 4096 -> 4096: four CTAs and one warp a tile 21.0 us, two and two 28.1, one and eight 74), but not
+// short rows (1280 -> 20160, 16 rows: no cluster and one warp a tile 20.7, two 22.9, a cluster of two and one 27;
+// 8 rows: no cluster and four warps 16.7, two 17.3), and two matrices, whose sums take the registers, less so
+// (4096 -> 11008, 8 rows: two CTAs and two warps 28.4, four and one 39.0).  And where the tiles leave most SMs
+// idle, more warps share one (5120 -> 1280, one row: sixteen 5.7 us, eight 6.7).
 Q4Plan plan(const Q4Args& a) {
     Q4Plan p{};
     p.form = a.rows <= 2 ? 2 : a.rows <= 4 ? 4 : a.rows <= 8 ? 8 : a.rows <= 16 ? 16 : 32;
     p.shared = kQ4MaxShared;
     const bool gated = a.gate != nullptr;
-    const int warps = (p.form <= 4 || p.form == 16) && !gated ? 16 : 8, runs = (a.rows + p.form - 1) / p.form;
+    const int warps = p.form <= 16 && !gated ? 16 : 8, runs = (a.rows + p.form - 1) / p.form;
     if (p.form <= 4) {
         p.wk_log = 3;
     } else if (a.kblocks >= 16) {
         p.cluster_log = gated ? 1 : 2;
         p.wk_log = gated && p.form == 8 ? 1 : 0;
     } else {
-        p.wk_log = p.form == 8 || (gated && p.form == 16) ? 1 : 0;
+        p.wk_log = p.form == 8 ? (gated ? 1 : 2) : gated && p.form == 16 ? 1 : 0;
     }
     while ((warps >> p.wk_log) > 1 &&
            (static_cast<long long>(a.tiles / (warps >> p.wk_log)) << p.cluster_log) * runs < current_sm_count() / 2)

@@ -268,8 +268,8 @@ struct Q4Digits {
     static constexpr int kTokens = 2 * NT;
     static constexpr int kTiles = GATED ? 2 : 1;
     static constexpr int kLaneSums = NT;         // of a tile, joined over the digits
-    static constexpr int kWarps = NT <= 2 && !GATED ? 16 : 8;
-    static constexpr int kRun = 2, kRing = 3;    // k-blocks of a warp a round; rounds on their way
+    static constexpr int kWarps = !GATED ? 16 : 8;
+    static constexpr int kRun = NT <= 2 ? 2 : 1, kRing = 3;    // k-blocks of a warp a round; rounds on their way
     static constexpr bool kFinisher = NT <= 2;   // a warp of its own finishes the sums
     static constexpr int kColumn = 160;          // bytes: 4 slices x 32, and a step of 8 banks
 

@@ -308,6 +308,60 @@ def test_strides(cuda, rows):
     assert (w[..., :1] == 9).all() and (w[..., 1 + n:] == 9).all()
 
 
+@pytest.mark.parametrize("xt", [np.float32, np.float16])
+@pytest.mark.parametrize("rows", [1, 3, 6, 12, 20])
+def test_alignments(cuda, rows, xt):
+    """Rows that begin at every alignment and lie any number of elements apart, k a multiple of 4 and not."""
+    import sdb
+
+    g = rng(rows)
+    for k, offset, apart in ((260, 0, 0), (260, 4, 4), (260, 2, 2), (260, 1, 3), (257, 0, 7), (130, 8, 6)):
+        q, scales, minima, values = made(g, 40, k, 32, True)
+        x = g.standard_normal((rows, k)).astype(xt)
+        base = np.full((rows, offset + k + apart), 1e4, dtype=xt)
+        base[:, offset:offset + k] = x
+        view = cuda_tensor(base, cuda)[:, offset:offset + k]
+        exact, mag = oracle.mul_mat_exact(values, x)
+        got = sdb.mul_mat_q4(on_device(cuda, q, scales, minima, 32), view)
+        check(host(got), exact, mag, xt == np.float16)
+
+
+def test_one_dimension(cuda):
+    """A single row as a vector, in and out; rows of one image each over the third dimension."""
+    import sdb
+
+    g = rng(4)
+    q, scales, minima, values = made(g, 33, 96, 32, False)
+    w = on_device(cuda, q, scales, minima, 32)
+    x = g.standard_normal((96,)).astype(np.float32)
+    exact, mag = oracle.mul_mat_exact(values, x)
+    out = sdb.mul_mat_q4(w, cuda_tensor(x, cuda))
+    assert out.shape == (33,)
+    check(host(out), exact, mag)
+    x = g.standard_normal((3, 1, 96)).astype(np.float32)
+    exact, mag = oracle.mul_mat_exact(values, x)
+    check(host(sdb.mul_mat_q4(w, cuda_tensor(x, cuda))), exact, mag)
+
+
+def test_infinities_with_many_rows(cuda):
+    """The halves' form too keeps a bad row alone: 12 and 40 rows, FP32 and FP16."""
+    import sdb
+
+    g = rng(16)
+    q, scales, minima, values = made(g, 48, 300, 64, False)
+    w = on_device(cuda, q, scales, minima, 64)
+    for rows in (12, 40):
+        for xt in (np.float32, np.float16):
+            x = g.standard_normal((rows, 300)).astype(xt)
+            exact, mag = oracle.mul_mat_exact(values, x)
+            y = x.copy()
+            y[3, 5], y[9, 299] = np.inf, np.nan
+            got = host(sdb.mul_mat_q4(w, cuda_tensor(y, cuda)))
+            keep = [r for r in range(rows) if r not in (3, 9)]
+            assert not np.isfinite(got[[3, 9]]).any()
+            check(got[keep], exact[keep], mag[keep], xt == np.float16)
+
+
 @pytest.mark.parametrize("act", ["gelu", "silu"])
 @pytest.mark.parametrize("rows,k,half,group,minimum", [(1, 320, 1280, 32, False), (2, 100, 17, 32, True),
                                                        (5, 1280, 640, 64, True), (9, 777, 50, 128, False),

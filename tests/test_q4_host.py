@@ -75,6 +75,9 @@ def test_products_not_taken(sdb):
                 (w, tensor(sdb, [64, 1 << 62, 4, 1], nb=[4, 4, 4, 4]), tensor(sdb, [8, 1 << 62, 4, 1], nb=[4] * 4))):
         assert lib.sdb_mul_mat_q4_supported(*bad) == 0
         assert lib.sdb_mul_mat_q4(*bad, None, None) == sdb.NOT_SUPPORTED
+    many = 1 << 20
+    assert lib.sdb_mul_mat_q4_supported(w, tensor(sdb, [64, many]), tensor(sdb, [8, many])) == 1
+    assert lib.sdb_mul_mat_q4_supported(w, tensor(sdb, [64, many + 1]), tensor(sdb, [8, many + 1])) == 0
     assert lib.sdb_mul_mat_q4_gated_supported(w, q4(sdb, 64, 8, 64), x, y) == 0
     assert lib.sdb_mul_mat_q4_gated_supported(w, q4(sdb, 64, 8, minimum=1), x, y) == 0
     assert lib.sdb_mul_mat_q4_gated_supported(w, q4(sdb, 64, 16), x, y) == 0
