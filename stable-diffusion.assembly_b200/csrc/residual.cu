@@ -197,7 +197,9 @@ __device__ __forceinline__ float2 row_sum(float2 v, int* buffer) {
 // T threads a row (32: eight rows a CTA), 4 V numbers a thread: with VEC, runs of four (rows of a multiple of four
 // numbers, aligned), else one by one.  A thread's numbers lie T (runs) apart.
 template <typename TX, typename TY, int V, int T, bool VEC>
-__global__ void __launch_bounds__(T == 32 ? 256 : T) residual_kernel(const __grid_constant__ ResidualArgs a) {
+// Registers for 1024 threads an SM: 64 a thread (rows of 8193 to 16384 numbers: 128), more rows at once being worth
+// more than the few words that spill (8 x 4096 x 320 35.7 us, unbounded 40.0; 2 x 4096 x 1280 30.1 and 30.8).
+__global__ void __launch_bounds__(T == 32 ? 256 : T, (V == 8 ? 512 : 1024) / (T == 32 ? 256 : T)) residual_kernel(const __grid_constant__ ResidualArgs a) {
     const int t = T == 32 ? threadIdx.x & 31 : threadIdx.x;
     constexpr int kRows = T == 32 ? 8 : 1;
     int buffer = 0;
@@ -208,34 +210,52 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) residual_kernel(const __gri
         const int i3 = q / static_cast<int>(a.ne2), i2 = q - i3 * static_cast<int>(a.ne2);
         auto base = [&](const long long (&nb)[3]) { return i1 * nb[0] + i2 * nb[1] + i3 * nb[2]; };
         float h[V][4], u[V][4];
+        // f(v, e) for the thread's numbers, a run that ends the row early passed over as a whole.
+        auto each = [&](auto f) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if constexpr (VEC) {
+                    if (at(v, 0) < a.c) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) f(v, e);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (at(v, e) < a.c) f(v, e);
+                }
+            }
+        };
         auto load = [&](float (&to)[V][4], const auto* p) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 if constexpr (VEC) {
-                    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (at(v, 0) < a.c) f = get4(p + at(v, 0));
-                    to[v][0] = f.x; to[v][1] = f.y; to[v][2] = f.z; to[v][3] = f.w;
+                    if (at(v, 0) < a.c) {
+                        const float4 f = get4(p + at(v, 0));
+                        to[v][0] = f.x; to[v][1] = f.y; to[v][2] = f.z; to[v][3] = f.w;
+                    }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) to[v][e] = at(v, e) < a.c ? get(p, at(v, e)) : 0.0f;
+                    for (int e = 0; e < 4; ++e)
+                        if (at(v, e) < a.c) to[v][e] = get(p, at(v, e));
                 }
             }
         };
         // f(v, e, operand's number) over the row, the operand's numbers nb apart.
         auto with = [&](const float* p, long long nb, auto f) {
+            if (VEC && nb == 1 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float o[4];
-                if (VEC && nb == 1 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-                    float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (at(v, 0) < a.c) w = __ldg(reinterpret_cast<const float4*>(p + at(v, 0)));
-                    o[0] = w.x; o[1] = w.y; o[2] = w.z; o[3] = w.w;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = at(v, e) < a.c ? __ldg(p + at(v, e) * nb) : 0.0f;
+                for (int v = 0; v < V; ++v) {
+                    if (at(v, 0) < a.c) {
+                        const float4 o = __ldg(reinterpret_cast<const float4*>(p + at(v, 0)));
+                        f(v, 0, o.x);
+                        f(v, 1, o.y);
+                        f(v, 2, o.z);
+                        f(v, 3, o.w);
+                    }
                 }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) f(v, e, o[e]);
+            } else {
+                each([&](int v, int e) { f(v, e, __ldg(p + at(v, e) * nb)); });
             }
         };
         auto normalise = [&](const NormForm& n, float (&to)[V][4]) {
@@ -244,29 +264,21 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) residual_kernel(const __gri
             float2 s{0.0f, 0.0f};
             float shift = 0.0f;
             if (n.kind == SDB_NORM_LAYER) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) s.x += (to[v][0] + to[v][1]) + (to[v][2] + to[v][3]);
+                each([&](int v, int e) { s.x += to[v][e]; });
                 const float mean = row_sum<T>(s, &buffer).x * inv;
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) to[v][e] = at(v, e) < a.c ? to[v][e] - mean : 0.0f;
                 s.x = 0.0f;
-            }
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                each([&](int v, int e) {
+                    to[v][e] -= mean;
                     s.x += to[v][e];
                     s.y = fmaf(to[v][e], to[v][e], s.y);
-                }
+                });
+            } else {
+                each([&](int v, int e) { s.y = fmaf(to[v][e], to[v][e], s.y); });
+            }
             s = row_sum<T>(s, &buffer);
             if (n.kind == SDB_NORM_LAYER) shift = s.x * inv;
             const float rstd = 1.0f / sqrtf(fmaxf(s.y * inv - shift * shift, 0.0f) + n.eps);
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) to[v][e] = (to[v][e] - shift) * rstd;
+            each([&](int v, int e) { to[v][e] = (to[v][e] - shift) * rstd; });
             if (n.weight) with(n.weight, 1, [&](int v, int e, float w) { to[v][e] *= w; });
             if (n.bias) with(n.bias, 1, [&](int v, int e, float b) { to[v][e] += b; });
         };
@@ -290,14 +302,11 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) residual_kernel(const __gri
             normalise(a.post, u);
             if (a.gate.data) with(operand(a.gate), a.gate.nb[0], [&](int v, int e, float g) { u[v][e] *= g; });
         }
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float s = a.x ? a.keep * h[v][e] : 0.0f;
-                if (a.y) s = fmaf(a.scale, u[v][e], s);
-                h[v][e] = s;
-            }
+        each([&](int v, int e) {
+            float s = a.x ? a.keep * h[v][e] : 0.0f;
+            if (a.y) s = fmaf(a.scale, u[v][e], s);
+            h[v][e] = s;
+        });
         if (a.h) store(static_cast<TX*>(a.h) + base(a.hnb), h);
         if (a.out) {
             normalise(a.pre, h);
