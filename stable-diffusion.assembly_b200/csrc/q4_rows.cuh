@@ -305,12 +305,13 @@ struct Q4Digits {
         asm volatile("cp.async.wait_all;" ::: "memory");
         q4_split<false>(a, it, tokens, kb1 - kb0, slot, [&](int b, int m, float4 x, bool store) {
             // top < 2^(e - 126), e its exponent field: 2^(156 - e) x is below 2^30.  The power's field is
-            // 283 - e, kept a normal number's.
-            const int e = static_cast<int>(q4_top(x) >> 23), f = min(283 - e, 253);
+            // 283 - e, kept a normal number's; of the smallest numbers a second power is what is missing.
+            const int e = static_cast<int>(q4_top(x) >> 23), f = min(283 - e, 253), more = 283 - e - f;
             const float up = __uint_as_float(static_cast<uint32_t>(f) << 23);
+            const float up_more = __uint_as_float(static_cast<uint32_t>(127 + more) << 23);
             // v = sum of digits 256^p: adding 128 to each of the lower three makes them v's bytes.
             auto digits = [&](float n) {
-                return (static_cast<uint32_t>(__float2int_rn(n * up)) + 0x00808080u) ^ 0x00808080u;
+                return (static_cast<uint32_t>(__float2int_rn(n * up * up_more)) + 0x00808080u) ^ 0x00808080u;
             };
             const uint32_t v0 = digits(x.x), v1 = digits(x.y), v2 = digits(x.z), v3 = digits(x.w);
             const uint32_t l01 = __byte_perm(v0, v1, 0x5140), l23 = __byte_perm(v2, v3, 0x5140);
@@ -323,7 +324,8 @@ struct Q4Digits {
                 to[kColumn / 4 * 3] = __byte_perm(h01, h23, 0x7632);
             }
             if (store && lane < 4) {  // digit p's factor: 2^(8 p) of the scale's inverse, and the weights' 1 / 16
-                const float down = __uint_as_float(static_cast<uint32_t>(254 - f + 8 * lane) << 23) * 0.0625f;
+                const float down = __uint_as_float(static_cast<uint32_t>(254 - f + 8 * lane) << 23) * 0.0625f *
+                                   __uint_as_float(static_cast<uint32_t>(127 - more) << 23);
                 factors[b * cols + 4 * m + lane] = e == 255 ? __uint_as_float(0x7fffffffu) : down;
             }
             if (a.minimum) {

@@ -726,8 +726,8 @@ def _packed_chain(chain: Chain | None, tensors: tuple, out, cols: int):
         return None
     # A chain that is used again as it was is not described again.
     shape = out.shape
-    key = (len(chain.steps), chain.from_redirect, cols, shape, out.stride(), out.dtype,
-           [t.data_ptr() for t in tensors])
+    key = (chain.from_redirect, cols, shape, out.stride(), out.dtype, [(kind, *nb) for kind, _, nb in chain.steps],
+           [(t.data_ptr(), t.numel()) for t in tensors])
     kept = chain.__dict__.get("_described")
     if kept is not None and kept[0] == key:
         return kept[1]

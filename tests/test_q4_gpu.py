@@ -214,15 +214,16 @@ def test_wide_and_tall(cuda):
     run_linear(cuda, rng(3), 40, 28672, 48, 64, True)
 
 
-@pytest.mark.parametrize("rows", [1, 2, 5])
+@pytest.mark.parametrize("rows", [1, 2, 5, 12, 20])
 def test_magnitudes(cuda, rows):
-    """Rows of x from 1e-30 to 1e30 and of mixed magnitudes: the bound holds at every scale."""
+    """Rows of x from 1e-36 (numbers below the normal ones among them) to 1e30 and of mixed magnitudes: the bound
+    holds at every scale."""
     import sdb
 
     g = rng(31)
     q, scales, minima, values = made(g, 50, 300, 64, True)
     w = on_device(cuda, q, scales, minima, 64)
-    for scale in (1e-30, 1e-6, 1e6, 1e30):
+    for scale in (1e-36, 1e-30, 1e-6, 1e6, 1e30):
         x = (g.standard_normal((rows, 300)) * scale * 10.0 ** g.uniform(-3, 3, (rows, 300))).astype(np.float32)
         exact, mag = oracle.mul_mat_exact(values, x)
         check(host(sdb.mul_mat_q4(w, cuda_tensor(x, cuda))), exact, mag)
@@ -450,6 +451,27 @@ def test_captured_and_replayed(cuda):
         got = host(out)
         call()
         np.testing.assert_array_equal(got, host(out))
+
+
+def test_a_chain_used_again_and_changed(cuda):
+    """A chain's description follows what is done to it between calls."""
+    import sdb
+
+    g = rng(21)
+    q, scales, minima, values = made(g, 24, 64, 32, False)
+    w = on_device(cuda, q, scales, minima, 32)
+    x = g.standard_normal((2, 64)).astype(np.float32)
+    a, b = (g.standard_normal((24,)).astype(np.float32) for _ in range(2))
+    exact, mag = oracle.mul_mat_exact(values, x)
+    chain = sdb.Chain().add(cuda_tensor(a, cuda))
+    t = cuda_tensor(x, cuda)
+    for _ in range(2):
+        check(host(sdb.mul_mat_q4(w, t, chain=chain)), exact + a, mag + np.abs(a))
+    chain.mul(cuda_tensor(b, cuda))
+    check(host(sdb.mul_mat_q4(w, t, chain=chain)), (exact + a) * b.astype(np.float64), (mag + np.abs(a)) * np.abs(b))
+    chain.steps[0] = (sdb.STEP_MUL, *chain.steps[0][1:])
+    want = exact * a.astype(np.float64) * b
+    check(host(sdb.mul_mat_q4(w, t, chain=chain)), want, mag * np.abs(a.astype(np.float64) * b))
 
 
 def test_refusals(cuda):
