@@ -3,14 +3,15 @@
 The matrices: made numbers and scales have to be those of the formulas (restated
 here in numpy, FP32 operation by FP32 operation), bit for bit.  The products:
 sum_k x value in float64 from the numbers the matrix stands for, held to the
-linear layers' bound, oracle.K_B200 of the summed magnitudes.  The kernel takes
-x exactly (its parts sum to it) and every product exactly, so its error is that
-of FP32 sums: a running sum of s terms errs by at most s 2^-23 of the
-magnitudes with sums cut instead of rounded, s at most 8 steps of 16 products
-and three parts in a group of 128, plus the groups joined -- under 1e-6 for the
-random signs of real rows (an error of sqrt(s) steps), for which the bound was
-set.  An FP16 output adds its rounding, 2^-11 of the value (2^-25 below FP16's
-normal numbers).
+linear layers' bound, oracle.K_B200 of the summed magnitudes.  Up to 8 rows the
+kernel's sums over a group are exact and x is off by 2^-31 of a k-block's greatest
+number, so its error is that of one rounding a group and the FP32 sum over the
+groups; with more rows x is off by 2^-24 of itself and a group's sum takes at most
+16 products one after another.  A running sum of s terms errs by at most s 2^-23
+of the magnitudes with sums cut instead of rounded; for the random signs of real
+rows (an error of sqrt(s) steps) that is under 1e-6, which the bound was set for.
+An FP16 output adds its rounding, 2^-11 of the value (2^-25 below FP16's normal
+numbers).
 """
 from __future__ import annotations
 
