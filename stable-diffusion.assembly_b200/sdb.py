@@ -778,8 +778,10 @@ def _on(fn, what: str, tensors, stream, *args) -> None:
     """Calls fn(*args, stream) with the tensors' device current, on `stream` or that device's current stream."""
     index = tensors[0].get_device()
     for t in tensors:
-        if t.get_device() != index or index < 0:
-            raise SdbError(INVALID, f"{what}: the tensors are not on one CUDA device")
+        if t.get_device() != index:
+            index = -1
+    if index < 0:
+        raise SdbError(INVALID, f"{what}: the tensors are not on one CUDA device")
     if _raw_stream is None:
         _find_raw()
     if stream is None:
@@ -917,12 +919,12 @@ class Norm:
         w = b = 0
         if self.weight is not None:
             w = self.weight.data_ptr()
-            if self.weight.shape[0] != c:
-                raise SdbError(INVALID, f"a norm of {self.weight.shape[0]} numbers for rows of {c}")
+            if self.weight.numel() != c:
+                raise SdbError(INVALID, f"a norm of {self.weight.numel()} numbers for rows of {c}")
         if self.bias is not None:
             b = self.bias.data_ptr()
-            if self.bias.shape[0] != c:
-                raise SdbError(INVALID, f"a norm of {self.bias.shape[0]} numbers for rows of {c}")
+            if self.bias.numel() != c:
+                raise SdbError(INVALID, f"a norm of {self.bias.numel()} numbers for rows of {c}")
         return _NORM_FORM.pack(NORMS[self.kind], self.eps, w, b)
 
 
@@ -936,16 +938,16 @@ def _packed_operand(t, shape) -> bytes:
     if t.element_size() != 4 or not t.is_floating_point():
         raise SdbError(INVALID, "modulations are FP32")
     nb = [0, 0, 0, 0]
-    ts, st = t.shape, t.stride()
-    nd, od = len(shape), len(ts)
-    if od > nd:
+    ts = t.shape
+    if len(ts) > len(shape):
         raise SdbError(INVALID, "a modulation has more dimensions than the rows")
-    for d in range(od):
-        e = ts[od - 1 - d]
+    d = 0
+    for e, s, n in zip(reversed(ts), reversed(t.stride()), reversed(shape)):
         if e != 1:
-            if e != shape[nd - 1 - d]:
+            if e != n:
                 raise SdbError(INVALID, f"a modulation of {tuple(ts)} for rows of {tuple(shape)}")
-            nb[d] = st[od - 1 - d]
+            nb[d] = s
+        d += 1
     return _OPERAND.pack(t.data_ptr(), *nb)
 
 
@@ -970,7 +972,10 @@ def residual_norm(x, y, post: Norm | None = None, gate=None, keep: float = 1.0, 
         out = None
     elif out is None:
         out = (y if y is not None else x).new_empty(shape)
-    tensors = [t for t in (ref, y, h, out, gate, mul, add) if t is not None]
+    tensors = [ref]
+    for t in (y, h, out, gate, mul, add):
+        if t is not None:
+            tensors.append(t)
     if post is not None:
         tensors += post.tensors
     if pre is not None:
@@ -978,7 +983,9 @@ def residual_norm(x, y, post: Norm | None = None, gate=None, keep: float = 1.0, 
     c = shape[-1] if len(shape) else 0
     params = b"".join((_KEEP_SCALE.pack(keep, scale),
                        _NO_NORM if post is None else post.packed(c), _NO_NORM if pre is None else pre.packed(c),
-                       _packed_operand(gate, shape), _packed_operand(mul, shape), _packed_operand(add, shape)))
+                       _NO_OPERAND if gate is None else _packed_operand(gate, shape),
+                       _NO_OPERAND if mul is None else _packed_operand(mul, shape),
+                       _NO_OPERAND if add is None else _packed_operand(add, shape)))
     what = "residual_norm"
     _on((_lib or load()).sdb_residual_norm, what, tensors, stream,
         _packed(x, what) if x is not None else None, _packed(y, what) if y is not None else None,
