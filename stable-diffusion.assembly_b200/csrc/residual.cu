@@ -80,6 +80,11 @@ struct Stat {
     float mean, shift, rstd;
 };
 
+// 1 / sqrt(var + eps).  A rounded variance may come out below 0; a NaN stays one, so that it fills its row.
+__device__ __forceinline__ float reciprocal_root(float var, float eps) {
+    return 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);
+}
+
 // value(i) is the row's number i.
 template <typename F>
 __device__ __forceinline__ Stat row_stat(const NormForm& n, int c, F value) {
@@ -99,8 +104,7 @@ __device__ __forceinline__ Stat row_stat(const NormForm& n, int c, F value) {
     }
     t = block_sum(t);
     if (n.kind == SDB_NORM_LAYER) s.shift = t.x * inv;
-    const float var = fmaxf(t.y * inv - s.shift * s.shift, 0.0f);
-    s.rstd = 1.0f / sqrtf(var + n.eps);
+    s.rstd = reciprocal_root(t.y * inv - s.shift * s.shift, n.eps);
     return s;
 }
 
@@ -277,7 +281,7 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T, (V == 8 ? 512 : 1024) / (T 
             }
             s = row_sum<T>(s, &buffer);
             if (n.kind == SDB_NORM_LAYER) shift = s.x * inv;
-            const float rstd = 1.0f / sqrtf(fmaxf(s.y * inv - shift * shift, 0.0f) + n.eps);
+            const float rstd = reciprocal_root(s.y * inv - shift * shift, n.eps);
             each([&](int v, int e) { to[v][e] = (to[v][e] - shift) * rstd; });
             if (n.weight) with(n.weight, 1, [&](int v, int e, float w) { to[v][e] *= w; });
             if (n.bias) with(n.bias, 1, [&](int v, int e, float b) { to[v][e] += b; });

@@ -337,3 +337,30 @@ def test_modulated_block(cuda):
         cond.copy_(t(g.standard_normal((images, c)).astype(np.float32)))
         graph.replay()
         close(out)
+
+
+@pytest.mark.parametrize("where", ["post", "pre"])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("t", [np.float32, np.float16])
+@pytest.mark.parametrize("c", [3, 256, 320, 513, 1280, 2047, 4096, 5003, 8192, 16384, 20001])
+def test_a_nan_fills_its_row(cuda, c, t, kind, where):
+    """A NaN makes a norm's statistics NaN and so every number of its row, in every form of a row's width; an
+    infinity makes its own number NaN, and the others' sum of squares infinite: 0 in an RMS norm.  No other
+    row knows of either."""
+    import sdb
+
+    g = rng(c)
+    x, y = inputs(g, (4, c), t, t)
+    norm = made_norm(g, kind, c)
+    args = {where: norm_of(sdb, cuda, norm)}
+    clean = host(sdb.residual_norm(cuda_tensor(x, cuda), cuda_tensor(y, cuda), **args)[1])
+    y[1, c // 2], y[2, c - 1] = np.nan, np.inf
+    got = host(sdb.residual_norm(cuda_tensor(x, cuda), cuda_tensor(y, cuda), **args)[1])
+    assert np.isnan(got[1]).all()
+    if kind == "layer":
+        assert np.isnan(got[2]).all()
+    else:
+        assert np.isnan(got[2, c - 1])
+        want = x[2] if where == "post" else np.zeros(c, t)
+        np.testing.assert_array_equal(got[2, :c - 1], want[:c - 1])
+    np.testing.assert_array_equal(got[[0, 3]], clean[[0, 3]])
