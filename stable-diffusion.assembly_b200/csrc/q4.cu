@@ -95,7 +95,8 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const T* __restrict__ 
             zero += __shfl_xor_sync(mask, zero, o);
         }
         const bool bad = zero != 0.0f;
-        const bool empty = hi < lo;  // a group of padding
+        // A group of padding.  Its numbers do not tell: a short last group of NaN alone has no extremes either.
+        const bool empty = row >= v.n || (k0 & ~(v.group - 1)) >= k;
         __half dh = __float2half_rn(0.0f), mh = dh;
         if (!empty) {
             if (MINIMUM) {

@@ -510,3 +510,25 @@ def test_refusals(cuda):
     refused(sdb.INVALID, lambda: sdb.q4_import(torch.zeros(4, 16, device=cuda, dtype=torch.uint8),
                                                torch.zeros(4, 2, device=cuda, dtype=torch.float16)))
     refused(sdb.INVALID, lambda: sdb.q4_from_blocks(torch.zeros(4, 18, device=cuda, dtype=torch.uint8), 64))
+
+
+# ---------------------------------------------------------------- groups that hold a NaN
+
+@pytest.mark.parametrize("minimum", [False, True])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("k", [1, 33, 65, 129, 137, 300])
+def test_a_short_last_group_of_nan(cuda, k, group, dtype, minimum):
+    """Groups of nothing but NaN, short last ones and whole rows among them, stand for NaN; the others for what
+    they stand for without them."""
+    import sdb
+
+    g = rng(k + group)
+    w = g.standard_normal((20, k)).astype(dtype)
+    bad = np.zeros(w.shape, dtype=bool)
+    last = (k - 1) // group * group
+    bad[3, last:], bad[17], bad[18, last:] = True, True, True
+    w[3, last:], w[17], w[18, k - 1] = np.nan, np.nan, np.nan
+    got = host(sdb.q4_quantize(cuda_tensor(w, cuda), group, minimum).values())
+    np.testing.assert_array_equal(np.isnan(got), bad)
+    np.testing.assert_array_equal(got[~bad], quantized(np.where(bad, dtype(1), w), group, minimum)[~bad])
