@@ -809,14 +809,32 @@ class Q4:
     def __init__(self, n: int, k: int, group: int = 32, minimum: bool = False, device=None):
         import torch
 
-        size = load().sdb_q4_bytes(k, n, group, 1 if minimum else 0)
-        if size <= 0:
+        self._form = (k, n, group, 1 if minimum else 0)
+        self._size = load().sdb_q4_bytes(*self._form)
+        if self._size <= 0:
             raise SdbError(INVALID, f"no 4-bit matrix of {n} x {k} in groups of {group}")
         self.n, self.k, self.group, self.minimum = n, k, group, bool(minimum)
-        self.data = torch.empty(size, dtype=torch.uint8, device="cuda" if device is None else device)
-        if not self.data.is_cuda:
+        self.data = torch.empty(self._size, dtype=torch.uint8, device="cuda" if device is None else device)
+
+    @property
+    def data(self):
+        """The matrix's memory, uint8; another of its size may take its place."""
+        return self._data
+
+    @data.setter
+    def data(self, t):
+        import torch
+
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise SdbError(INVALID, "4-bit matrices are on a CUDA device")
-        self.struct = _Q4.pack(self.data.data_ptr(), k, n, group, 1 if minimum else 0)
+        if t.dtype != torch.uint8 or t.shape != (self._size,) or not t.is_contiguous():
+            raise SdbError(INVALID, f"a 4-bit matrix's memory is {self._size} dense bytes")
+        self._data = t
+
+    @property
+    def struct(self) -> bytes:
+        """The sdb_q4, made anew for each call: a copy of a matrix has memory of its own."""
+        return _Q4.pack(self._data.data_ptr(), *self._form)
 
     def values(self, out=None, stream=None):
         """The numbers the matrix stands for, FP32 (n, k) (sdb_q4_dequantize)."""

@@ -532,3 +532,37 @@ def test_a_short_last_group_of_nan(cuda, k, group, dtype, minimum):
     got = host(sdb.q4_quantize(cuda_tensor(w, cuda), group, minimum).values())
     np.testing.assert_array_equal(np.isnan(got), bad)
     np.testing.assert_array_equal(got[~bad], quantized(np.where(bad, dtype(1), w), group, minimum)[~bad])
+
+
+# ---------------------------------------------------------------- what a call is described by
+
+def test_copies_of_a_matrix(cuda):
+    """A copied, pickled or saved matrix reads its own memory, and one whose memory is exchanged reads the new."""
+    import copy
+    import io
+    import pickle
+
+    import sdb
+    import torch
+
+    g = rng(41)
+    q, scales, minima, values = made(g, 24, 96, 32, True)
+    w = on_device(cuda, q, scales, minima, 32)
+    x = cuda_tensor(g.standard_normal((3, 96)).astype(np.float32), cuda)
+    want = host(sdb.mul_mat_q4(w, x))
+    saved = io.BytesIO()
+    torch.save(w, saved)
+    saved.seek(0)
+    for c in (copy.deepcopy(w), pickle.loads(pickle.dumps(w)), torch.load(saved, weights_only=False)):
+        np.testing.assert_array_equal(host(c.values()), values.astype(np.float32))
+        np.testing.assert_array_equal(host(sdb.mul_mat_q4(c, x)), want)
+        c.data.zero_()
+        assert (host(c.values()) == 0).all() and (host(sdb.mul_mat_q4(c, x)) == 0).all()
+        np.testing.assert_array_equal(host(w.values()), values.astype(np.float32))
+        c.data = w.data.clone()
+        np.testing.assert_array_equal(host(sdb.mul_mat_q4(c, x)), want)
+    for bad in (w.data[:-16], w.data.cpu(), w.data.view(torch.int8), w.data[::2], None):
+        with pytest.raises(sdb.SdbError) as e:
+            w.data = bad
+        assert e.value.status == sdb.INVALID
+    np.testing.assert_array_equal(host(sdb.mul_mat_q4(w, x)), want)
