@@ -719,39 +719,43 @@ def _chain_tensors(chain: Chain | None) -> tuple:
     return tuple(found)
 
 
+def _check_operand(t, nb, shape, cols: int, rows: int) -> None:
+    """Refuses an operand that a chain would read past its memory's end."""
+    if min(nb) < 0:
+        raise SdbError(INVALID, "a chain operand's strides are not negative")
+    last = (cols - 1) * nb[0]
+    for d in range(1, len(shape)):
+        last += (shape[-1 - d] - 1) * nb[d]
+    if rows and last >= t.untyped_storage().nbytes() // 4 - t.storage_offset():
+        raise SdbError(INVALID, "a chain operand ends before the output's rows")
+
+
 def _packed_chain(chain: Chain | None, tensors: tuple, out, cols: int):
     """The sdb_chain of an operation on out's rows, `cols` columns each, as bytes (None: no chain).  Operands
     that do not reach over the rows are refused: the kernel would read past them."""
     if chain is None:
         return None
-    # A chain that is used again as it was is not described again.
-    shape = out.shape
-    key = (chain.from_redirect, cols, shape, out.stride(), out.dtype, [(kind, *nb) for kind, _, nb in chain.steps],
-           [(t.data_ptr(), t.numel()) for t in tensors])
+    shape, stride = out.shape, out.stride()
+    steps = chain.steps
+    rows = out.numel()
+    # What the kernel may touch is looked at in every call ...
+    for _, t, nb in steps:
+        if t is not None:
+            _check_operand(t, nb, shape, cols, rows)
+    r = chain.redirect_tensor
+    if r is not None and (r.dtype != out.dtype or r.shape != shape or r.stride() != stride):
+        raise SdbError(INVALID, "a chain's redirect has the output's type, extents and strides")
+    # ... and a chain that is used again as it was is not packed again.
+    key = (chain.from_redirect, [(kind, *nb) for kind, _, nb in steps], [t.data_ptr() for t in tensors], r is None)
     kept = chain.__dict__.get("_described")
     if kept is not None and kept[0] == key:
         return kept[1]
-    steps = chain.steps
     if len(steps) > MAX_STEPS:
         raise SdbError(INVALID, "chain longer than 6 steps")
     parts = [struct.pack("=i4x", len(steps))]
     for kind, t, nb in steps:
-        if t is None:
-            parts.append(_STEP.pack(kind, 0, *nb))
-            continue
-        if min(nb) < 0:
-            raise SdbError(INVALID, "a chain operand's strides are not negative")
-        last = (cols - 1) * nb[0]
-        for d in range(1, len(shape)):
-            last += (shape[-1 - d] - 1) * nb[d]
-        if last >= t.numel() and (out.numel() and
-                                  last >= t.untyped_storage().nbytes() // 4 - t.storage_offset()):
-            raise SdbError(INVALID, "a chain operand ends before the output's rows")
-        parts.append(_STEP.pack(kind, t.data_ptr(), *nb))
+        parts.append(_STEP.pack(kind, t.data_ptr() if t is not None else 0, *nb))
     parts.extend([_NO_STEP] * (MAX_STEPS - len(steps)))
-    r = chain.redirect_tensor
-    if r is not None and (r.dtype != out.dtype or r.shape != shape or r.stride() != out.stride()):
-        raise SdbError(INVALID, "a chain's redirect has the output's type, extents and strides")
     parts.append(_CHAIN_TAIL.pack(r.data_ptr() if r is not None else 0, 1 if chain.from_redirect else 0))
     packed = b"".join(parts)
     chain._described = (key, packed)

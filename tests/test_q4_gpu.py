@@ -566,3 +566,27 @@ def test_copies_of_a_matrix(cuda):
             w.data = bad
         assert e.value.status == sdb.INVALID
     np.testing.assert_array_equal(host(sdb.mul_mat_q4(w, x)), want)
+
+
+def test_a_redirect_exchanged(cuda):
+    """A chain used again with a redirect of other strides, extents or type at the same address is refused."""
+    import sdb
+    import torch
+
+    g = rng(42)
+    q, scales, minima, values = made(g, 24, 64, 32, False)
+    w = on_device(cuda, q, scales, minima, 32)
+    x = g.standard_normal((24, 64)).astype(np.float32)
+    t, r, out = cuda_tensor(x, cuda), torch.zeros(24, 24, device=cuda), torch.empty(24, 24, device=cuda)
+    exact, mag = oracle.mul_mat_exact(values, x)
+    chain = sdb.Chain().redirect(r)
+    sdb.mul_mat_q4(w, t, out=out, chain=chain)
+    check(host(r), exact, mag)
+    r.fill_(7)
+    for other in (r.t(), r.view(torch.int32), r.view(12, 48), r.view(1, 24, 24)):
+        with pytest.raises(sdb.SdbError) as e:
+            sdb.mul_mat_q4(w, t, out=out, chain=chain.redirect(other))
+        assert e.value.status == sdb.INVALID
+    assert (host(r) == 7).all()
+    sdb.mul_mat_q4(w, t, out=out, chain=chain.redirect(r))
+    check(host(r), exact, mag)

@@ -165,3 +165,33 @@ def test_binding_refuses_host_tensors(sdb):
         sdb._packed_operand(torch.zeros(3, 1, 8), (2, 5, 8))
     with pytest.raises(sdb.SdbError):
         sdb.Norm("rms", weight=torch.zeros(4)).packed(5)
+
+
+
+
+def test_operands_within_their_memory(sdb):
+    """An operand with strides of its own is held to its memory, not to its count of numbers, and again on each use."""
+    import numpy as np
+    import torch
+
+    out = torch.zeros(2, 8)
+    numbers = np.zeros(40, dtype=np.float32)
+    wide, short = torch.from_numpy(numbers)[:7], torch.from_numpy(numbers[:7])
+    assert wide.data_ptr() == short.data_ptr() and wide.numel() == short.numel()
+
+    def described(chain):
+        return sdb._packed_chain(chain, sdb._chain_tensors(chain), out, 8)
+
+    chain = sdb.Chain()
+    chain.steps.append((sdb.STEP_ADD, wide, [1, 0, 0, 0]))
+    assert len(described(chain)) == ctypes.sizeof(sdb.ChainStruct)
+    chain.steps[0] = (sdb.STEP_ADD, short, [1, 0, 0, 0])
+    # One number shown eight times, read as if there were eight of them.
+    shown = sdb.Chain()
+    shown.steps.append((sdb.STEP_ADD, torch.zeros(1).expand(8), [1, 0, 0, 0]))
+    behind = sdb.Chain()
+    behind.steps.append((sdb.STEP_ADD, wide, [-1, 0, 0, 0]))
+    for bad in (chain, shown, behind):
+        with pytest.raises(sdb.SdbError) as e:
+            described(bad)
+        assert e.value.status == sdb.INVALID
