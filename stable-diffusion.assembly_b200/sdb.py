@@ -190,16 +190,24 @@ def _stream_ptr(stream) -> int:
     return int(stream.cuda_stream)
 
 
+def _own_strides(t) -> tuple:
+    """The element strides of a chain's operand by its own extents, 0 along those of 1."""
+    own = [0 if e == 1 else s for e, s in zip(reversed(t.shape), reversed(t.stride()))]
+    return tuple((own + [0, 0, 0, 0])[:4])
+
+
 class Chain:
     """An epilogue chain (sdasm::Epilogue): steps applied in order to each output element.
 
     add(t) / mul(t): t an FP32 CUDA tensor broadcastable to the output in ggml's
-    sense (a dimension of extent 1 is broadcast); silu().  redirect(r,
+    sense (a dimension of extent 1 is broadcast), or read by explicit element
+    strides nb, dimension 0 first; silu().  redirect(r,
     from_redirect) makes the operation write into r (a residual connection).
     """
 
     def __init__(self):
-        self.steps: list[tuple[int, object, list[int]]] = []
+        # (kind, operand, strides): the operand's own strides as a tuple, explicit ones as a list.
+        self.steps: list[tuple[int, object, Sequence[int]]] = []
         self.redirect_tensor = None
         self.from_redirect = False
         self._keep: list = []
@@ -209,11 +217,7 @@ class Chain:
 
         if t.dtype != torch.float32 or not t.is_cuda:
             raise SdbError(INVALID, "chain operands are FP32 CUDA tensors")
-        if nb is None:
-            shape = list(reversed(t.shape)) + [1] * (4 - t.dim())
-            strides = list(reversed(t.stride())) + [0] * (4 - t.dim())
-            nb = [0 if shape[k] == 1 else strides[k] for k in range(4)]
-        self.steps.append((kind, t, list(nb)))
+        self.steps.append((kind, t, _own_strides(t) if nb is None else list(nb)))
         return self
 
     def add(self, t, nb=None):
@@ -720,7 +724,15 @@ def _chain_tensors(chain: Chain | None) -> tuple:
 
 
 def _check_operand(t, nb, shape, cols: int, rows: int) -> None:
-    """Refuses an operand that a chain would read past its memory's end."""
+    """Refuses an operand that is not of the output's extents or, read by explicit strides, one that a chain
+    would read past its memory's end."""
+    if type(nb) is tuple and nb == _own_strides(t):
+        d = 0
+        for e in reversed(t.shape):
+            if e != 1 and e != (cols if d == 0 else shape[-1 - d] if d < len(shape) else 1):
+                raise SdbError(INVALID, f"a chain operand of {tuple(t.shape)} for {cols} columns of {tuple(shape)}")
+            d += 1
+        return
     if min(nb) < 0:
         raise SdbError(INVALID, "a chain operand's strides are not negative")
     last = (cols - 1) * nb[0]
@@ -731,8 +743,7 @@ def _check_operand(t, nb, shape, cols: int, rows: int) -> None:
 
 
 def _packed_chain(chain: Chain | None, tensors: tuple, out, cols: int):
-    """The sdb_chain of an operation on out's rows, `cols` columns each, as bytes (None: no chain).  Operands
-    that do not reach over the rows are refused: the kernel would read past them."""
+    """The sdb_chain of an operation on out's rows, `cols` columns each, as bytes (None: no chain)."""
     if chain is None:
         return None
     shape, stride = out.shape, out.stride()

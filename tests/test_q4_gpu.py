@@ -590,3 +590,39 @@ def test_a_redirect_exchanged(cuda):
     assert (host(r) == 7).all()
     sdb.mul_mat_q4(w, t, out=out, chain=chain.redirect(r))
     check(host(r), exact, mag)
+
+
+def test_operands_of_other_extents(cuda):
+    """An operand whose extents are neither 1 nor the output's is refused, whatever lies behind it in its buffer;
+    with strides of its own it has to lie within its buffer."""
+    import sdb
+    import torch
+
+    g = rng(43)
+    q, scales, minima, values = made(g, 8, 64, 32, False)
+    w = on_device(cuda, q, scales, minima, 32)
+    x = g.standard_normal((2, 64)).astype(np.float32)
+    t = cuda_tensor(x, cuda)
+    p = g.standard_normal((100,)).astype(np.float32)
+    params = cuda_tensor(p, cuda)
+    exact, mag = oracle.mul_mat_exact(values, x)
+    for bad in (params[:7], params[:9], params[:21].view(3, 7), params[:24].view(3, 8), params[:14].view(2, 7),
+                params[:3].view(3, 1), params[:32].view(2, 2, 8)):
+        for chain in (sdb.Chain().add(bad), sdb.Chain().mul(bad)):
+            with pytest.raises(sdb.SdbError) as e:
+                sdb.mul_mat_q4(w, t, chain=chain)
+            assert e.value.status == sdb.INVALID
+    for bad in (params[:8], params[:15], params[:17]):  # the gated layer's chain has 2 N columns
+        with pytest.raises(sdb.SdbError) as e:
+            sdb.mul_mat_q4_gated(w, w, t, chain=sdb.Chain().add(bad))
+        assert e.value.status == sdb.INVALID
+    for good, b in ((params[:8], p[:8]), (params[:16].view(2, 8), p[:16].reshape(2, 8)), (params[4], p[4]),
+                    (params[:2].view(2, 1), p[:2, None]), (params[:8].view(1, 1, 1, 8), p[:8]),
+                    (params[:16:2], p[:16:2])):
+        check(host(sdb.mul_mat_q4(w, t, chain=sdb.Chain().add(good))), exact + b, mag + np.abs(b))
+    # Strides of its own: each column five apart, from any place that leaves room for them.
+    b = p[60:100:5]
+    check(host(sdb.mul_mat_q4(w, t, chain=sdb.Chain().add(params[60:61], [5, 0, 0, 0]))), exact + b, mag + np.abs(b))
+    with pytest.raises(sdb.SdbError) as e:
+        sdb.mul_mat_q4(w, t, chain=sdb.Chain().add(params[65:66], [5, 0, 0, 0]))
+    assert e.value.status == sdb.INVALID
