@@ -816,6 +816,25 @@ def _on(fn, what: str, tensors, stream, *args) -> None:
         _check(status)
 
 
+def _made(stream, device, what: str, make):
+    """make()'s new tensor or matrix for a call on `stream`, from that stream's memory: the current stream's
+    may still be written by work that has not run yet.  It is not given to others before the stream that is
+    current here is done with it either."""
+    if stream is None or device.type != "cuda":
+        return make()
+    import torch
+
+    current = torch.cuda.current_stream(device)
+    if stream == current:
+        return make()
+    if stream.device != current.device:
+        raise SdbError(INVALID, f"{what}: the stream is another device's")
+    with torch.cuda.stream(stream):
+        made = make()
+    made.data.record_stream(current)  # a matrix's memory, or the tensor's own
+    return made
+
+
 class Q4:
     """A matrix (n, k) of 4-bit numbers with group scales on the device (sdb_q4): value = d (q - 8), or with
     `minimum` d q + m, an FP16 d (and m) for every `group` numbers of a row.  Made by q4_quantize, q4_import or
@@ -856,7 +875,9 @@ class Q4:
         import torch
 
         if out is None:
-            out = torch.empty(self.n, self.k, dtype=torch.float32, device=self.data.device)
+            device = self.data.device
+            out = _made(stream, device, "Q4.values",
+                        lambda: torch.empty(self.n, self.k, dtype=torch.float32, device=device))
         _on(load().sdb_q4_dequantize, "Q4.values", (self.data, out), stream, self.struct, _packed(out, "Q4.values"))
         return out
 
@@ -865,7 +886,7 @@ def q4_quantize(w, group: int = 32, minimum: bool = False, stream=None) -> Q4:
     """w (n, k) FP32 or FP16, rows contiguous, quantized to 4 bits (sdb_q4_quantize)."""
     if w.dim() != 2:
         raise SdbError(INVALID, "q4_quantize: a matrix (n, k)")
-    q = Q4(w.shape[0], w.shape[1], group, minimum, w.device)
+    q = _made(stream, w.device, "q4_quantize", lambda: Q4(w.shape[0], w.shape[1], group, minimum, w.device))
     _on(load().sdb_q4_quantize, "q4_quantize", (w, q.data), stream, _packed(w, "q4_quantize"), q.struct)
     return q
 
@@ -877,7 +898,7 @@ def q4_import(codes, scales, minima=None, k: int | None = None, group: int = 32,
 
     k = 2 * codes.shape[-1] if k is None else k
     n, groups = codes.shape[0], -(-k // group) if group else 0
-    q = Q4(n, k, group, minima is not None, codes.device)
+    q = _made(stream, codes.device, "q4_import", lambda: Q4(n, k, group, minima is not None, codes.device))
     if codes.dtype != torch.uint8 or codes.shape != (n, (k + 1) // 2) or not codes.is_contiguous():
         raise SdbError(INVALID, "q4_import: codes must be dense uint8 (n, (k + 1) // 2)")
     tensors = [codes, scales, q.data] + ([minima] if minima is not None else [])
@@ -898,7 +919,7 @@ def q4_from_blocks(blocks, k: int, minimum: bool = False, stream=None) -> Q4:
         raise SdbError(INVALID, "q4_from_blocks: blocks must be uint8 (n, bytes of a row)")
     if k % 32 != 0 or blocks.shape[1] < k // 32 * (20 if minimum else 18):
         raise SdbError(INVALID, "q4_from_blocks: rows are k / 32 whole blocks")
-    q = Q4(blocks.shape[0], k, 32, minimum, blocks.device)
+    q = _made(stream, blocks.device, "q4_from_blocks", lambda: Q4(blocks.shape[0], k, 32, minimum, blocks.device))
     _on(load().sdb_q4_from_blocks, "q4_from_blocks", (blocks, q.data), stream, blocks.data_ptr(), blocks.stride(0),
         q.struct)
     return q
@@ -910,7 +931,8 @@ def mul_mat_q4(w: Q4, x, out=None, chain: Chain | None = None, stream=None):
     import torch
 
     if out is None:
-        out = torch.empty(*x.shape[:-1], w.n, dtype=x.dtype, device=x.device)
+        out = _made(stream, x.device, "mul_mat_q4",
+                    lambda: torch.empty(*x.shape[:-1], w.n, dtype=x.dtype, device=x.device))
     extra = _chain_tensors(chain)
     _on((_lib or load()).sdb_mul_mat_q4, "mul_mat_q4", (w.data, x, out, *extra), stream, w.struct,
         _packed(x, "mul_mat_q4"), _packed(out, "mul_mat_q4"), _packed_chain(chain, extra, out, w.n))
@@ -925,7 +947,8 @@ def mul_mat_q4_gated(w: Q4, gate: Q4, x, act: str = "gelu", out=None, chain: Cha
     if act not in GATES:
         raise SdbError(INVALID, f"mul_mat_q4_gated: no gate {act!r}")
     if out is None:
-        out = torch.empty(*x.shape[:-1], w.n, dtype=x.dtype, device=x.device)
+        out = _made(stream, x.device, "mul_mat_q4_gated",
+                    lambda: torch.empty(*x.shape[:-1], w.n, dtype=x.dtype, device=x.device))
     extra = _chain_tensors(chain)
     _on((_lib or load()).sdb_mul_mat_q4_gated, "mul_mat_q4_gated", (w.data, gate.data, x, out, *extra), stream,
         w.struct, gate.struct, _packed(x, "mul_mat_q4_gated"), _packed(out, "mul_mat_q4_gated"), GATES[act],
@@ -1000,11 +1023,11 @@ def residual_norm(x, y, post: Norm | None = None, gate=None, keep: float = 1.0, 
     if not want_h:
         h = None
     elif h is None:
-        h = ref.new_empty(shape)
+        h = _made(stream, ref.device, "residual_norm", lambda: ref.new_empty(shape))
     if not want_out:
         out = None
     elif out is None:
-        out = (y if y is not None else x).new_empty(shape)
+        out = _made(stream, ref.device, "residual_norm", lambda: (y if y is not None else x).new_empty(shape))
     tensors = [ref]
     for t in (y, h, out, gate, mul, add):
         if t is not None:

@@ -626,3 +626,42 @@ def test_operands_of_other_extents(cuda):
     with pytest.raises(sdb.SdbError) as e:
         sdb.mul_mat_q4(w, t, chain=sdb.Chain().add(params[65:66], [5, 0, 0, 0]))
     assert e.value.status == sdb.INVALID
+
+
+@pytest.mark.parametrize("call", ["quantize", "import", "blocks", "values", "linear", "gated"])
+def test_memory_made_for_another_stream(cuda, call):
+    """What a call on another stream makes is not memory that the current stream still writes."""
+    import sdb
+    import torch
+
+    g = rng(44)
+    w = cuda_tensor(g.standard_normal((256, 128)).astype(np.float32), cuda)
+    x = cuda_tensor(g.standard_normal((64, 128)).astype(np.float32), cuda)
+    q, scales, minima, _ = made(g, 256, 128, 32, False)
+    codes, scales = cuda_tensor(codes_of(q), cuda), cuda_tensor(scales, cuda)
+    blocks = cuda_tensor(g.integers(0, 60, (256, 72)).astype(np.uint8), cuda)
+    m = sdb.q4_quantize(w)
+    calls = {"quantize": lambda s: sdb.q4_quantize(w, stream=s).data,
+             "import": lambda s: sdb.q4_import(codes, scales, stream=s).data,
+             "blocks": lambda s: sdb.q4_from_blocks(blocks, 128, stream=s).data,
+             "values": lambda s: m.values(stream=s),
+             "linear": lambda s: sdb.mul_mat_q4(m, x, stream=s),
+             "gated": lambda s: sdb.mul_mat_q4_gated(m, m, x, stream=s)}
+    assert_apart(calls[call])
+
+
+def assert_apart(call):
+    """call(stream)'s tensors, made while the current stream still writes memory it has freed."""
+    import torch
+
+    tensors = lambda v: v if isinstance(v, tuple) else (v,)
+    want = [t.clone() for t in tensors(call(None))]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)
+    held = [torch.empty_like(t).fill_(1) for t in want]  # the blocks that the next such tensors would get
+    del held
+    got = tensors(call(side))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

@@ -364,3 +364,13 @@ def test_a_nan_fills_its_row(cuda, c, t, kind, where):
         want = x[2] if where == "post" else np.zeros(c, t)
         np.testing.assert_array_equal(got[2, :c - 1], want[:c - 1])
     np.testing.assert_array_equal(got[[0, 3]], clean[[0, 3]])
+
+
+def test_memory_made_for_another_stream(cuda):
+    """What a call on another stream makes is not memory that the current stream still writes."""
+    import sdb
+    from test_q4_gpu import assert_apart
+
+    x, y = inputs(rng(5), (64, 256))
+    tx, ty = cuda_tensor(x, cuda), cuda_tensor(y, cuda)
+    assert_apart(lambda s: sdb.residual_norm(tx, ty, pre=sdb.Norm("rms"), stream=s))
