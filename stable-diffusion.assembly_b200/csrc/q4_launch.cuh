@@ -66,11 +66,9 @@ int q4_launch_rows(const Q4Args& a, const Q4Plan& p, cudaStream_t st) {
     if (p.form == 2) return q4_launch_form<Q4Digits<1, GATED>, G>(a, p, st);
     if (p.form == 4) return q4_launch_form<Q4Digits<2, GATED>, G>(a, p, st);
     if (p.form == 8) return q4_launch_form<Q4Digits<4, GATED>, G>(a, p, st);
-    if (p.form == 16)
-        return a.x_half ? q4_launch_form<Q4Halves<2, true, GATED>, G>(a, p, st)
-                        : q4_launch_form<Q4Halves<2, false, GATED>, G>(a, p, st);
-    return a.x_half ? q4_launch_form<Q4Halves<4, true, GATED>, G>(a, p, st)
-                    : q4_launch_form<Q4Halves<4, false, GATED>, G>(a, p, st);
+    if (!a.x_half) return q4_launch_form<Q4Floats<2, false, GATED>, G>(a, p, st);
+    if (p.form == 16) return q4_launch_form<Q4Floats<2, true, GATED>, G>(a, p, st);
+    return q4_launch_form<Q4Floats<4, true, GATED>, G>(a, p, st);
 }
 
 template <int G>

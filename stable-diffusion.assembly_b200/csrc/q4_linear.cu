@@ -57,14 +57,16 @@ bool chain_ok(const sdb_chain* c, const sdb_tensor* dst, bool gated) {
 // With up to four rows x is cheap and the weights are all: eight warps share a tile, so that a round is a long
 // run of memory (8192 -> 28672, one row: 29.9 us; four warps 32.7, sixteen 31.1).  With more rows a CTA spends as
 // long on splitting x as on its products: the CTAs of a cluster split it between them, and few warps share a tile
-// (32 rows of 4096 -> 4096: four CTAs and one warp a tile 21.0 us, two and two 28.1, one and eight 74), but not
-// short rows (1280 -> 20160, 16 rows: no cluster and one warp a tile 20.7, two 22.9, a cluster of two and one 27;
+// (16 rows of 4096 -> 4096: four CTAs and one warp a tile 14.9 us, one and one 21.9), but not
+// short rows (1280 -> 20160, 16 rows: no cluster and one warp a tile 24.6, two 26.4, a cluster of two 28.4;
 // 8 rows: no cluster and four warps 16.7, two 17.3), and two matrices, whose sums take the registers, less so
-// (4096 -> 11008, 8 rows: two CTAs and two warps 28.4, four and one 39.0).  And where the tiles leave most SMs
+// (4096 -> 11008, 8 rows: two CTAs and two warps 28.4, four and one 39.0; 1280 -> 5120, 16 rows at a time: 16 rows
+// with two warps, 32 with one 29.8, with two 36.8).  FP32 rows, three columns each, are taken 16 at a time, FP16 rows
+// 32 (4096 -> 4096: 32 FP32 rows 22.1 us, taken at once 43.5, 77 rows 64.6 and 92.9; 77 FP16 rows 44.6).  And where the tiles leave most SMs
 // idle, more warps share one (5120 -> 1280, one row: sixteen 5.7 us, eight 6.7).
 Q4Plan plan(const Q4Args& a) {
     Q4Plan p{};
-    p.form = a.rows <= 2 ? 2 : a.rows <= 4 ? 4 : a.rows <= 8 ? 8 : a.rows <= 16 ? 16 : 32;
+    p.form = a.rows <= 2 ? 2 : a.rows <= 4 ? 4 : a.rows <= 8 ? 8 : a.rows <= 16 || !a.x_half ? 16 : 32;
     p.shared = kQ4MaxShared;
     const bool gated = a.gate != nullptr;
     const int warps = p.form <= 16 && !gated ? 16 : 8, runs = (a.rows + p.form - 1) / p.form;
@@ -74,7 +76,7 @@ Q4Plan plan(const Q4Args& a) {
         p.cluster_log = gated ? 1 : 2;
         p.wk_log = gated && p.form == 8 ? 1 : 0;
     } else {
-        p.wk_log = p.form == 8 ? (gated ? 1 : 2) : gated && p.form == 16 ? 1 : 0;
+        p.wk_log = p.form == 8 ? (gated ? 1 : 2) : gated && p.form == 16 && runs == 1 ? 1 : 0;
     }
     while ((warps >> p.wk_log) > 1 &&
            (static_cast<long long>(a.tiles / (warps >> p.wk_log)) << p.cluster_log) * runs < current_sm_count() / 2)

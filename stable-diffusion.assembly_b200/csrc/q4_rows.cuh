@@ -10,19 +10,21 @@
 //
 // Digits (up to 8 rows).  A row's 128 numbers of a k-block are scaled by a
 //   power of two to integers below 2^30 -- off by 2^-31 of the k-block's
-//   greatest number at most, an FP32 number within 2^7 of it is whole -- and
+//   greatest number at most, an FP32 number within 2^7 of it whole -- and
 //   written as four signed base-256 digits, four columns of an integer product
 //   (m16n8k32, s8 x s8).  A nibble at the top of its byte is the operand
 //   16 (q - 8): three instructions unpack eight weights.  The sum is exact; it
 //   starts from 0x4b400000, so that its bits, read as FP32, are 1.5 * 2^23 + 16 S,
 //   and one subtraction makes it a number (|16 S| <= 2^21).  A k-block that
 //   holds an infinity or a NaN makes its row's sums NaN.
-// Halves (more rows, where the digits' four columns a row cost more than the
-//   unpacking saves).  The k-block is scaled so that its greatest number comes
-//   just under 2^15, x = hi + lo in FP16 -- off by 2^-24 of x at most, or 2^-40
-//   of the greatest -- two columns of FP16 products (m16n8k16; FP16 rows are one
-//   column, as they are).  q - 8 is exact in FP16 (0x6400 | q is 1024 + q; a
-//   subtraction, or for a nibble four bits up a multiply-add, leaves q - 8).
+// Floats (more rows, where the digits' four columns a row cost more than the
+//   unpacking saves).  FP16 rows are one column each as they are; an FP32 row is
+//   the sum of three BF16 columns, whole, whatever lies beside a number: each
+//   takes the next eight of its 24 bits, and none has a range to fall out of
+//   (two FP16 columns hold 23 bits, within 2^17 of the k-block's greatest number;
+//   they took 20.8 us for 16 rows of 1280 -> 20160, three 24.7).  m16n8k16
+//   products; q - 8 is exact in both types.  Sums of 16 products at a time, the
+//   first parts' apart from the others', which are 2^-8 of them.
 //
 // A CTA has 8 or 16 working warps: WR tiles of rows side by side, WK warps to a
 // tile that share its k-blocks, and up to eight CTAs of a cluster that share
@@ -42,6 +44,7 @@
 #pragma once
 
 #include <cooperative_groups.h>
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -451,9 +454,11 @@ struct Q4Digits {
     static __device__ __forceinline__ int token_of(int c, int lane) { return 2 * c + (lane >> 1 & 1); }
 };
 
-// ---- x as FP16 halves: T products of eight rows of x, HALF: FP16 rows as they are
+// ---- x as floating-point columns: T products of eight rows of x, HALF: FP16 rows as they are
 
-// (u & MASK) ^ FLIP: two nibbles, code - 8 in four bits, made codes in FP16 numbers from 1024 on.
+// An integer below 2^m in the low bits of a number whose mantissa's last bit is worth 1 is that power of two plus
+// the integer, so a nibble becomes a number by one logic operation and a subtraction.
+// (u & MASK) ^ FLIP: two nibbles, code - 8 in four bits, made codes in such numbers.
 template <uint32_t MASK, uint32_t FLIP>
 __device__ __forceinline__ uint32_t q4_nibbles(uint32_t u) {
     uint32_t v;
@@ -461,7 +466,8 @@ __device__ __forceinline__ uint32_t q4_nibbles(uint32_t u) {
     return v;
 }
 
-__device__ __forceinline__ uint32_t q4_low(uint32_t u) {  // nibbles at bits 0 and 16: 1024 + q, less 1032
+// FP16: nibbles at bits 0 and 16: 1024 + q, less 1032.
+__device__ __forceinline__ uint32_t q4_low(uint32_t u) {
     uint32_t v;
     asm("sub.f16x2 %0, %1, %2;" : "=r"(v) : "r"(q4_nibbles<0x000f000fu, 0x64086408u>(u)), "r"(0x64086408u));
     return v;
@@ -475,30 +481,49 @@ __device__ __forceinline__ uint32_t q4_high(uint32_t u) {  // at bits 4 and 20: 
     return v;
 }
 
-// c = a b, or c += a b.
-template <bool FIRST>
+// BF16: nibbles at bits 0 and 16: 128 + q, less 136.
+__device__ __forceinline__ uint32_t q4_bf16(uint32_t u) {
+    uint32_t v;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(q4_nibbles<0x000f000fu, 0x43084308u>(u)), "r"(0x43084308u));
+    return v;
+}
+
+// c = a b, or c += a b, of FP16 (HALF) or BF16 operands.
+template <bool HALF, bool FIRST>
 __device__ __forceinline__ void q4_mma(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
-    if constexpr (FIRST)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%10, %10, %10, %10};"
-            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(0.0f));
-    else
+    if constexpr (FIRST) c[0] = c[1] = c[2] = c[3] = 0.0f;
+    if constexpr (HALF)
         asm volatile(
             "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
             "{%0, %1, %2, %3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+}
+
+// x = a[0] + a[1] + a[2] in BF16, whole: each takes the next eight bits at least.
+__device__ __forceinline__ void q4_three(float x, float y, __nv_bfloat162 (&a)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        a[i] = __floats2bfloat162_rn(x, y);
+        x -= __low2float(a[i]);
+        y -= __high2float(a[i]);
+    }
 }
 
 template <int T, bool HALF, bool GATED_>
-struct Q4Halves {
+struct Q4Floats {
     static constexpr bool GATED = GATED_;
     static constexpr int kTokens = 8 * T;
     static constexpr int kTiles = GATED ? 2 : 1;
     static constexpr int kLaneSums = 4 * T;
-    static constexpr int kProducts = HALF ? T : 2 * T;
+    static constexpr int kParts = HALF ? 1 : 3;  // columns of a row
+    static constexpr int kProducts = kParts * T;
     static constexpr int kWarps = T == 2 && !GATED ? 16 : 8;
     static constexpr int kRun = 1, kRing = GATED ? 3 : 4;
     static constexpr bool kFinisher = false;
@@ -511,22 +536,22 @@ struct Q4Halves {
     uint8_t* frags;
     float* scales;  // of a row's k-block
     float* sums;    // of a row's groups
-    __device__ __forceinline__ Q4Halves(const Q4Args& a, uint8_t* x, int) {
+    __device__ __forceinline__ Q4Floats(const Q4Args& a, uint8_t* x, int) {
         frags = x;
         scales = reinterpret_cast<float*>(x + a.chunk * (8 * kProducts * kColumn));
         sums = scales + a.chunk * kTokens;
     }
 
     // A lane's four numbers are columns 0..3 or 4..7 of the run of eight that lane t = lane / 2 % 4 of a fragment
-    // holds: a word of slice 2 (lane / 8), the even columns, and one of the next, the odd ones, of hi (a column
-    // of product 2 i) and of lo (the same column of product 2 i + 1); FP16 rows have no lo.
+    // holds: a word of slice 2 (lane / 8), the even columns, and one of the next, the odd ones, of each part (the
+    // same column of one product after another).
     template <int G, class Read>
     __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Read read) const {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
         const Q4Items it(kWarps, tokens);
         auto column = [&](int b, int m) {
-            return frags + (b * (8 * kProducts) + (HALF ? m : m / 8 * 16 + m % 8)) * kColumn;
+            return frags + (b * (8 * kProducts) + m / 8 * (8 * kParts) + m % 8) * kColumn;
         };
         auto slot = [&](int b, int m) {
             return HALF ? column(b, m) + lane * 8 : column(b, m) + (lane >> 4) * (8 * kColumn) + (lane & 15) * 16;
@@ -542,22 +567,22 @@ struct Q4Halves {
                     *reinterpret_cast<__half2*>(to + 32) = __floats2half2_rn(x.y, x.w);
                 }
             } else {
-                // top < 2^(e - 126), e its exponent field: scaled by 2^(141 - e) it is below 2^15.  The power's
-                // field is 268 - e, kept a normal number's; infinities and NaN stay what they are.
-                const int e = static_cast<int>(q4_top(x) >> 23), f = min(268 - e, 253);
-                const float up = __uint_as_float(static_cast<uint32_t>(f) << 23);
+                // Scaled by 2^24, so that the last parts of the smallest numbers too are normal ones; a k-block
+                // that reaches 2^88 by 2^-24, so that no sum overflows before its scale comes.
+                const bool great = q4_top(x) >= 0x6b800000u;
+                const float up = great ? 0x1p-24f : 0x1p24f;
                 auto put = [&](float u, float v, int at) {
-                    const __half2 hi = __floats2half2_rn(u, v);
-                    const float2 r = __half22float2(hi);
-                    const __half2 lo = __floats2half2_rn(u - r.x, v - r.y);
+                    __nv_bfloat162 parts[3];
+                    q4_three(u, v, parts);
                     if (store) {
-                        *reinterpret_cast<__half2*>(to + at) = hi;
-                        *reinterpret_cast<__half2*>(to + 8 * kColumn + at) = lo;
+#pragma unroll
+                        for (int i = 0; i < 3; ++i)
+                            *reinterpret_cast<__nv_bfloat162*>(to + i * (8 * kColumn) + at) = parts[i];
                     }
                 };
                 put(x.x * up, x.z * up, 0);
                 put(x.y * up, x.w * up, 32);
-                if (store && lane == 0) scales[b * kTokens + m] = __uint_as_float(static_cast<uint32_t>(254 - f) << 23);
+                if (store && lane == 0) scales[b * kTokens + m] = great ? 0x1p24f : 0x1p-24f;
             }
             if (a.minimum) {
                 const float s = q4_group_sum<G>(x);
@@ -579,8 +604,9 @@ struct Q4Halves {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
         const uint8_t* f = frags + at * (8 * kProducts * kColumn) + (lane >> 2) * kColumn + (lane & 3) * 8;
-        float part[kTiles][kLaneSums];  // the k-block's sums, in its rows' scales
-        float s[kTiles][T][4];          // a group's sums
+        constexpr int kSums = HALF ? 1 : 2;  // the first parts', and the others', which are far smaller
+        float part[kTiles][kLaneSums];       // the k-block's sums, in its rows' scales
+        float s[kTiles][T][kSums][4];        // a group's sums
         uint32_t w[kTiles][2][4];
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
@@ -595,20 +621,23 @@ struct Q4Halves {
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i) {
                     const uint32_t u0 = w[i][0][j] >> (8 * h), u1 = w[i][1][j] >> (8 * h);
-                    av[i][0] = q4_low(u0);
-                    av[i][1] = q4_low(u1);
-                    av[i][2] = q4_high(u0);
-                    av[i][3] = q4_high(u1);
+                    av[i][0] = HALF ? q4_low(u0) : q4_bf16(u0);
+                    av[i][1] = HALF ? q4_low(u1) : q4_bf16(u1);
+                    av[i][2] = HALF ? q4_high(u0) : q4_bf16(u0 >> 4);
+                    av[i][3] = HALF ? q4_high(u1) : q4_bf16(u1 >> 4);
                 }
+                const bool first = j % (4 / NG) == 0 && h == 0;
 #pragma unroll
-                for (int p = 0; p < kProducts; ++p) {
-                    const uint2 b = *reinterpret_cast<const uint2*>(f + (2 * j + h) * 32 + p * (8 * kColumn));
-                    const int t = HALF ? p : p / 2;
-                    const bool first = j % (4 / NG) == 0 && h == 0 && (HALF || p % 2 == 0);
+                for (int p = 0; p < kParts; ++p) {
 #pragma unroll
-                    for (int i = 0; i < kTiles; ++i) {
-                        if (first) q4_mma<true>(s[i][t], av[i], b);
-                        else q4_mma<false>(s[i][t], av[i], b);
+                    for (int t = 0; t < T; ++t) {
+                        const uint2 b = *reinterpret_cast<const uint2*>(f + (2 * j + h) * 32 +
+                                                                        (t * kParts + p) * (8 * kColumn));
+#pragma unroll
+                        for (int i = 0; i < kTiles; ++i) {
+                            if (first && p < kSums) q4_mma<HALF, true>(s[i][t][p], av[i], b);
+                            else q4_mma<HALF, false>(s[i][t][p == 0 ? 0 : kSums - 1], av[i], b);
+                        }
                     }
                 }
             }
@@ -619,7 +648,8 @@ struct Q4Halves {
                 const float2 d = Q4Stage<G>::pick(st[i].d, g);
 #pragma unroll
                 for (int c = 0; c < kLaneSums; ++c) {
-                    const float scale = c & 2 ? d.y : d.x, v = s[i][c / 4][c % 4];
+                    const float scale = c & 2 ? d.y : d.x;
+                    const float v = HALF ? s[i][c / 4][0][c % 4] : s[i][c / 4][0][c % 4] + s[i][c / 4][kSums - 1][c % 4];
                     part[i][c] = g == 0 ? scale * v : fmaf(scale, v, part[i][c]);
                 }
             }
@@ -860,7 +890,7 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
 
 // How a product is cut (q4_linear.cu).
 struct Q4Plan {
-    int form;      // rows of x a CTA takes: 2, 4 or 8 in digits; 16 or 32 in halves
+    int form;      // rows of x a CTA takes: 2, 4 or 8 in digits; 16, or 32 of FP16, in floats
     int wk_log;    // warps that share a row tile's k-blocks (fewer where their k-blocks of x do not fit)
     int cluster_log;  // CTAs that do
     int shared;    // bytes of shared memory a CTA may take

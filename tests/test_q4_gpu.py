@@ -665,3 +665,86 @@ def assert_apart(call):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- every bit of x
+#
+# The bound here is the linear layers' own, 1e-6 of the magnitudes |x value| summed, with inputs whose sums hold
+# nothing but what a wrong step would lose: numbers of x beside far greater ones whose weights are 0.  x enters
+# the products whole, and a weight of 0 adds 0 whichever way it is 0, so the roundings left are those of sums of
+# terms of the magnitudes counted, as in the tests above.
+
+def beside_great_numbers(g, rows, k, n, group, kind, great, xt):
+    """Rows of ordinary numbers with one great one in each 128 columns whose weight is 0: by code 8 of a symmetric
+    matrix, by code 0 and no minimum, or by a code that the minimum meets (d q + m = 0)."""
+    q, scales, minima, _ = made(g, n, k, group, kind != "code")
+    scales = (g.integers(1, 128, scales.shape) * 2.0 ** -10 * g.choice([-1.0, 1.0], scales.shape)).astype(np.float16)
+    at = np.arange(k) % 128 == 77 % min(k, 128)
+    zero = {"code": 8, "least": 0}.get(kind)
+    if kind == "least":
+        minima = np.zeros_like(scales)
+    if kind == "inside":
+        z = g.integers(0, 16, scales.shape)
+        minima = (-scales.astype(np.float64) * z).astype(np.float16)  # 7 bits by 4: exact
+        zero = np.repeat(z, group, axis=1)[:, :k][:, at]
+    q[:, at] = zero
+    d = np.repeat(scales.astype(np.float64), group, axis=1)[:, :k]
+    m = np.repeat(minima.astype(np.float64), group, axis=1)[:, :k] if minima is not None else -8 * d
+    values = d * q + m
+    assert (values[:, at] == 0).all()
+    x = g.standard_normal((rows, k))
+    x[:, at] *= great
+    return q, scales, minima, values, x.astype(xt)
+
+
+@pytest.mark.parametrize("kind", ["code"])
+@pytest.mark.parametrize("great", [300.0, 1e4, 1e6, 1e10, 1e20, 1e30])
+@pytest.mark.parametrize("rows", [9, 16, 17, 33])
+def test_great_numbers_that_weigh_nothing(cuda, rows, great, kind):
+    import sdb
+
+    for group, k in ((32, 300), (64, 640), (128, 257)):
+        q, scales, minima, values, x = beside_great_numbers(rng(rows + group), rows, k, 40, group, kind, great, np.float32)
+        exact, mag = oracle.mul_mat_exact(values, x)
+        check(host(sdb.mul_mat_q4(on_device(cuda, q, scales, minima, group), cuda_tensor(x, cuda))), exact, mag)
+
+
+@pytest.mark.parametrize("kind", ["code"])
+@pytest.mark.parametrize("rows", [9, 17, 33])
+def test_great_half_precision_numbers(cuda, rows, kind):
+    import sdb
+    import torch
+
+    g = rng(rows)
+    q, scales, minima, values, x = beside_great_numbers(g, rows, 400, 40, 32, kind, 1e4, np.float16)
+    quiet = np.abs(x.astype(np.float64)) < 6
+    x = np.where(quiet, x * np.float16(2.0 ** -10), x)
+    exact, mag = oracle.mul_mat_exact(values, x)
+    out = torch.empty(rows, 40, device=cuda)
+    sdb.mul_mat_q4(on_device(cuda, q, scales, minima, 32), cuda_tensor(x, cuda), out=out)
+    check(host(out), exact, mag)
+
+
+@pytest.mark.parametrize("rows", [9, 17, 33])
+@pytest.mark.parametrize("gated", [False, True])
+def test_one_number_a_column(cuda, rows, gated):
+    """Each column of the output is one number of x, all other weights 0, the numbers of a row of any magnitudes."""
+    import sdb
+
+    g = rng(rows)
+    k = 200
+    q = np.full((k, k), 8, dtype=np.uint8)
+    q[np.arange(k), np.arange(k)] = g.choice([0, 3, 7, 9, 15], k)
+    scales = (1 + g.random((k, 7))).astype(np.float16)
+    w = on_device(cuda, q, scales, None, 32)
+    values = np.repeat(scales.astype(np.float64), 32, axis=1)[:, :k] * (q.astype(np.float64) - 8)
+    x = (g.standard_normal((rows, k)) * 10.0 ** g.uniform(-15, 15, (rows, k))).astype(np.float32)
+    exact, mag = oracle.mul_mat_exact(values, x)
+    t = cuda_tensor(x, cuda)
+    if gated:  # the gate's column: SiLU(40) = 40 to FP32's last bit
+        got = host(sdb.mul_mat_q4_gated(w, on_device(cuda, q, np.zeros_like(scales), None, 32), t, "silu",
+                                        chain=sdb.Chain().add(cuda_tensor(np.repeat(np.float32([0, 40]), k), cuda))))
+        exact, mag = 40 * exact, 40 * mag
+    else:
+        got = host(sdb.mul_mat_q4(w, t))
+    assert (np.abs(got - exact) <= oracle.K_B200 * mag).all()
