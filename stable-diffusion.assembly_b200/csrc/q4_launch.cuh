@@ -25,11 +25,12 @@ int q4_launch_form(const Q4Args& args, const Q4Plan& p, cudaStream_t st) {
     const int block = F::block_bytes(std::min(a.rows, F::kTokens), 128 / G);
     const int fit = (p.shared - fixed) / block;  // k-blocks of x that fit
     // All of a CTA's k-blocks of x are held where a cluster of up to eight brings them down to what fits: else x is
-    // split again for every tile (28672 -> 8192, one row: two CTAs 31 us, one 67).
+    // split again for every tile (28672 -> 8192, one row: two CTAs 33 us, one 66).  The CTAs then stand for warps that
+    // share a tile, but for two (four rows: two 96 us, one 112).
     int wk_log = p.wk_log, cluster_log = p.cluster_log;
     while (cluster_log < 3 && ((a.kblocks - 1) >> cluster_log) + 1 > fit) {
         ++cluster_log;
-        if (wk_log > 0) --wk_log;
+        if (wk_log > 1) --wk_log;
     }
     const int cluster = 1 << cluster_log;
     a.cluster_log = static_cast<uint8_t>(cluster_log);
@@ -63,9 +64,12 @@ int q4_launch_form(const Q4Args& args, const Q4Plan& p, cudaStream_t st) {
 
 template <bool GATED, int G>
 int q4_launch_rows(const Q4Args& a, const Q4Plan& p, cudaStream_t st) {
-    if (p.form == 2) return q4_launch_form<Q4Digits<1, GATED>, G>(a, p, st);
-    if (p.form == 4) return q4_launch_form<Q4Digits<2, GATED>, G>(a, p, st);
-    if (p.form == 8) return q4_launch_form<Q4Digits<4, GATED>, G>(a, p, st);
+    if (p.form == 1) return q4_launch_form<Q4Digits<GATED>, G>(a, p, st);
+    if (p.form == 2) return q4_launch_form<Q4Pairs<1, GATED>, G>(a, p, st);
+    if (p.form == 4) return q4_launch_form<Q4Pairs<2, GATED>, G>(a, p, st);
+    if (p.form == 8)
+        return a.x_half ? q4_launch_form<Q4Floats<1, true, GATED>, G>(a, p, st)
+                        : q4_launch_form<Q4Floats<1, false, GATED>, G>(a, p, st);
     if (!a.x_half) return q4_launch_form<Q4Floats<2, false, GATED>, G>(a, p, st);
     if (p.form == 16) return q4_launch_form<Q4Floats<2, true, GATED>, G>(a, p, st);
     return q4_launch_form<Q4Floats<4, true, GATED>, G>(a, p, st);

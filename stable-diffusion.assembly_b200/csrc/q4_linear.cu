@@ -55,28 +55,32 @@ bool chain_ok(const sdb_chain* c, const sdb_tensor* dst, bool gated) {
 // Cuts the product: the rows of x a CTA takes (a form), the warps and CTAs that share a tile's k-blocks.
 //
 // With up to four rows x is cheap and the weights are all: eight warps share a tile, so that a round is a long
-// run of memory (8192 -> 28672, one row: 29.9 us; four warps 32.7, sixteen 31.1).  With more rows a CTA spends as
-// long on splitting x as on its products: the CTAs of a cluster split it between them, and few warps share a tile
-// (16 rows of 4096 -> 4096: four CTAs and one warp a tile 14.9 us, one and one 21.9), but not
-// short rows (1280 -> 20160, 16 rows: no cluster and one warp a tile 24.6, two 26.4, a cluster of two 28.4;
-// 8 rows: no cluster and four warps 16.7, two 17.3), and two matrices, whose sums take the registers, less so
-// (4096 -> 11008, 8 rows: two CTAs and two warps 28.4, four and one 39.0; 1280 -> 5120, 16 rows at a time: 16 rows
-// with two warps, 32 with one 29.8, with two 36.8).  FP32 rows, three columns each, are taken 16 at a time, FP16 rows
-// 32 (4096 -> 4096: 32 FP32 rows 22.1 us, taken at once 43.5, 77 rows 64.6 and 92.9; 77 FP16 rows 44.6).  And where the tiles leave most SMs
-// idle, more warps share one (5120 -> 1280, one row: sixteen 5.7 us, eight 6.7).
+// run of memory (8192 -> 28672, one row: 33.0 us; four warps 35.0, sixteen 34.9).  Up to eight rows likewise (five
+// rows 71.8; four CTAs and one warp 130), but where a CTA walks one or two tiles' groups the splitting of FP32 rows is
+// what it does: the CTAs of a cluster split them between them (8 rows of 4096 -> 4096: four CTAs 11.3, one 12.1; of
+// FP16 8.9 and 8.0).  So do those of more rows, with one warp a tile (16 rows of 4096 -> 4096: four CTAs 14.9, one
+// 21.9).  Short rows are no cluster's (1280 -> 20160, 16 rows: one CTA and one warp a tile 24.6, two warps 26.4, two
+// CTAs 28.4; 8 rows: four warps 17.1, eight 17.5), and two matrices, whose sums take the registers, share less
+// (1280 -> 5120, 5 rows: two warps 11.7, one 12.3, eight 12.9; 16 rows at a time: 16 rows with two warps, 32 with one
+// 29.8, with two 36.8).  FP32 rows, three columns each, are taken 16 at a time, FP16 rows 32 (4096 -> 4096: 32 FP32
+// rows 22.1 us, taken at once 43.5, 77 rows 64.6 and 92.9; 77 FP16 rows 44.1).  And where the tiles leave most SMs
+// idle, more warps share one (320 -> 1280, two rows: sixteen 4.3 us, eight 4.7).
 Q4Plan plan(const Q4Args& a) {
     Q4Plan p{};
-    p.form = a.rows <= 2 ? 2 : a.rows <= 4 ? 4 : a.rows <= 8 ? 8 : a.rows <= 16 || !a.x_half ? 16 : 32;
+    p.form = a.rows == 1 ? 1 : a.rows <= 4 && !a.x_half ? (a.rows + 1) / 2 * 2 : a.rows <= 8 ? 8 : a.rows <= 16 || !a.x_half ? 16 : 32;
     p.shared = kQ4MaxShared;
     const bool gated = a.gate != nullptr;
     const int warps = p.form <= 16 && !gated ? 16 : 8, runs = (a.rows + p.form - 1) / p.form;
     if (p.form <= 4) {
         p.wk_log = 3;
+    } else if (p.form == 8) {
+        if (a.kblocks < 16) p.wk_log = gated ? 1 : 2;
+        else if (a.x_half || gated || a.tiles > 2 * current_sm_count()) p.wk_log = 3;
+        else p.cluster_log = 2;
     } else if (a.kblocks >= 16) {
         p.cluster_log = gated ? 1 : 2;
-        p.wk_log = gated && p.form == 8 ? 1 : 0;
     } else {
-        p.wk_log = p.form == 8 ? (gated ? 1 : 2) : gated && p.form == 16 && runs == 1 ? 1 : 0;
+        p.wk_log = gated && p.form == 16 && runs == 1 ? 1 : 0;
     }
     while ((warps >> p.wk_log) > 1 &&
            (static_cast<long long>(a.tiles / (warps >> p.wk_log)) << p.cluster_log) * runs < current_sm_count() / 2)

@@ -6,41 +6,45 @@
 // The weights' bytes are the work: each is read once for up to 32 rows of x.
 // The 16 weight rows of a tile are the M of an mma and the rows of x its N; S
 // is summed over one group by the tensor core, from zero, and joins FP32 sums
-// with the group's scale.  x is taken whole in one of two forms:
+// with the group's scale.  x enters whole, to its last bit, whatever lies beside
+// a number in its row, in one of three forms:
 //
-// Digits (up to 8 rows).  A row's 128 numbers of a k-block are scaled by a
-//   power of two to integers below 2^30 -- off by 2^-31 of the k-block's
-//   greatest number at most, an FP32 number within 2^7 of it whole -- and
-//   written as four signed base-256 digits, four columns of an integer product
-//   (m16n8k32, s8 x s8).  A nibble at the top of its byte is the operand
-//   16 (q - 8): three instructions unpack eight weights.  The sum is exact; it
-//   starts from 0x4b400000, so that its bits, read as FP32, are 1.5 * 2^23 + 16 S,
-//   and one subtraction makes it a number (|16 S| <= 2^21).  A k-block that
-//   holds an infinity or a NaN makes its row's sums NaN.
-// Floats (more rows, where the digits' four columns a row cost more than the
-//   unpacking saves).  FP16 rows are one column each as they are; an FP32 row is
-//   the sum of three BF16 columns, whole, whatever lies beside a number: each
-//   takes the next eight of its 24 bits, and none has a range to fall out of
-//   (two FP16 columns hold 23 bits, within 2^17 of the k-block's greatest number;
-//   they took 20.8 us for 16 rows of 1280 -> 20160, three 24.7).  m16n8k16
-//   products; q - 8 is exact in both types.  Sums of 16 products at a time, the
-//   first parts' apart from the others', which are 2^-8 of them.
+// Digits (one row).  The row's 128 numbers of a k-block are scaled by a power of
+//   two and split into two integers of 22 bits, three signed base-256 digits
+//   each: six columns of an integer product (m16n8k32, s8 x s8).  A nibble at
+//   the top of its byte is the operand 16 (q - 8): three instructions unpack
+//   eight weights.  The sum is exact; it starts from 0x4b400000, so that its
+//   bits, read as FP32, are 1.5 * 2^23 + 16 S, and one subtraction makes it a
+//   number (|16 S| <= 2^21).  Six digits hold the numbers down to 2^-19 of the
+//   k-block's greatest; a k-block with smaller ones (0 apart), or at the ends of
+//   FP32's range, or with an infinity or a NaN, is taken as below.
+// Pairs (two to four FP32 rows).  A row is the sum of three BF16 columns, each
+//   of which takes the next eight of a number's 24 bits, and none has a range to
+//   fall out of; two rows' columns are six of a product's eight (m16n8k16).  q - 8
+//   is exact: a nibble is 128 + q in BF16, less 136.
+// Floats (more rows, and all FP16 rows but one).  FP16 rows are one column each
+//   as they are; FP32 rows three BF16 columns, in products of eight rows' first,
+//   second and third parts.  The first parts' sums are apart from the others',
+//   which are 2^-8 of them.
+//
+// (Digits unpack a weight in a third of the instructions and take one row of
+// 8192 -> 28672 in 29.3 us where a pair takes 38; two rows' twelve columns would
+// be two products, 43 us for a pair's 42.  A product of eight rows' parts for two
+// rows: 52.)
 //
 // A CTA has 8 or 16 working warps: WR tiles of rows side by side, WK warps to a
 // tile that share its k-blocks, and up to eight CTAs of a cluster that share
-// them again.  x is split once into shared memory, each column of the products
-// a run of its k-slices' fragments and 32 bytes more than a multiple of 128 to
-// the next column, so that neither a column's stores nor a slice's loads over
-// eight columns meet a bank twice, and stays there for all the row tiles the
-// CTA walks.  A product's unused columns are not stored: their lanes read what
-// lies there and their sums go nowhere.  A further warp brings the weights: a
-// round, kRun k-blocks for every working warp, is one bulk copy for each of the
-// WR tiles into one of kRing places, announced by an mbarrier and refilled when
-// the working warps have said by another that they have read it.  The working
-// warps' sums meet in shared memory and are added in one order, so a result does
-// not turn on timing; the sums of a cluster's other CTAs are read where they
-// lie.  Where there are few sums, one more warp finishes them (chain, gate,
-// store) while the others go on.
+// them again.  x is split once into shared memory, laid out so that neither a
+// column's stores nor a slice's loads over eight columns meet a bank twice, and
+// stays there for all the row tiles the CTA walks.  A product's unused columns
+// are not stored: their lanes read what lies there and their sums go nowhere.
+// A further warp brings the weights: a round, kRun k-blocks for every working
+// warp, is one bulk copy for each of the WR tiles into one of kRing places,
+// announced by an mbarrier and refilled when the working warps have said by
+// another that they have read it.  The working warps' sums meet in shared memory
+// and are added in one order, so a result does not turn on timing; the sums of a
+// cluster's other CTAs are read where they lie.  Where there are few sums, one
+// more warp finishes them (chain, gate, store) while the others go on.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -263,198 +267,7 @@ __device__ __forceinline__ uint64_t q4_fma2(uint64_t a, uint64_t b, uint64_t c) 
     return r;
 }
 
-// ---- x as digits: NT products of eight columns, 2 NT rows of x
-
-template <int NT, bool GATED_>
-struct Q4Digits {
-    static constexpr bool GATED = GATED_;
-    static constexpr int kTokens = 2 * NT;
-    static constexpr int kTiles = GATED ? 2 : 1;
-    static constexpr int kLaneSums = NT;         // of a tile, joined over the digits
-    static constexpr int kWarps = !GATED ? 16 : 8;
-    static constexpr int kRun = NT <= 2 ? 2 : 1, kRing = 3;    // k-blocks of a warp a round; rounds on their way
-    static constexpr bool kFinisher = NT <= 2;   // a warp of its own finishes the sums
-    static constexpr int kColumn = 160;          // bytes: 4 slices x 32, and a step of 8 banks
-
-    // Shared memory of `chunk` k-blocks: the columns; each column's factor; each row's sums over the groups.
-    static __host__ __device__ int columns(int tokens) { return 4 * tokens; }
-    static __host__ __device__ int block_bytes(int tokens, int ng) {
-        return columns(tokens) * (kColumn + 4) + kTokens * 4 * ng;
-    }
-    static constexpr int kTail = 8 * NT * (kColumn + 4);  // what the lanes of unused columns read past the last
-    uint8_t* frags;
-    float* factors;
-    float* sums;
-    int cols;
-    __device__ __forceinline__ Q4Digits(const Q4Args& a, uint8_t* x, int tokens) {
-        cols = columns(tokens);
-        frags = x;
-        factors = reinterpret_cast<float*>(x + (a.chunk * cols + 8 * NT) * kColumn);
-        sums = factors + a.chunk * cols + 8 * NT;
-    }
-
-    // A column's digits of a k-block are a run of 128 bytes, a lane's four numbers a word of it.
-    // read() once the numbers are on their way.
-    template <int G, class Read>
-    __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Read read) const {
-        constexpr int NG = 128 / G;
-        const int lane = threadIdx.x & 31;
-        const Q4Items it(kWarps, tokens);
-        auto slot = [&](int b, int m) {
-            return frags + (b * cols + 4 * m + (lane >> 3)) * kColumn + (lane & 7) * 16;
-        };
-        q4_fetch<false>(a, it, m0, tokens, kb0, kb1 - kb0, slot);
-        read();
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        q4_split<false>(a, it, tokens, kb1 - kb0, slot, [&](int b, int m, float4 x, bool store) {
-            // top < 2^(e - 126), e its exponent field: 2^(156 - e) x is below 2^30.  The power's field is
-            // 283 - e, kept a normal number's; of the smallest numbers a second power is what is missing.
-            const int e = static_cast<int>(q4_top(x) >> 23), f = min(283 - e, 253), more = 283 - e - f;
-            const float up = __uint_as_float(static_cast<uint32_t>(f) << 23);
-            const float up_more = __uint_as_float(static_cast<uint32_t>(127 + more) << 23);
-            // v = sum of digits 256^p: adding 128 to each of the lower three makes them v's bytes.
-            auto digits = [&](float n) {
-                return (static_cast<uint32_t>(__float2int_rn(n * up * up_more)) + 0x00808080u) ^ 0x00808080u;
-            };
-            const uint32_t v0 = digits(x.x), v1 = digits(x.y), v2 = digits(x.z), v3 = digits(x.w);
-            const uint32_t l01 = __byte_perm(v0, v1, 0x5140), l23 = __byte_perm(v2, v3, 0x5140);
-            const uint32_t h01 = __byte_perm(v0, v1, 0x7362), h23 = __byte_perm(v2, v3, 0x7362);
-            if (store) {
-                uint32_t* to = reinterpret_cast<uint32_t*>(frags + (b * cols + 4 * m) * kColumn) + lane;
-                to[0] = __byte_perm(l01, l23, 0x5410);
-                to[kColumn / 4] = __byte_perm(l01, l23, 0x7632);
-                to[kColumn / 2] = __byte_perm(h01, h23, 0x5410);
-                to[kColumn / 4 * 3] = __byte_perm(h01, h23, 0x7632);
-            }
-            if (store && lane < 4) {  // digit p's factor: 2^(8 p) of the scale's inverse, and the weights' 1 / 16
-                const float down = __uint_as_float(static_cast<uint32_t>(254 - f + 8 * lane) << 23) * 0.0625f *
-                                   __uint_as_float(static_cast<uint32_t>(127 - more) << 23);
-                factors[b * cols + 4 * m + lane] = e == 255 ? __uint_as_float(0x7fffffffu) : down;
-            }
-            if (a.minimum) {
-                const float s = q4_group_sum<G>(x);
-                if (store && lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
-            }
-        });
-    }
-
-    uint64_t acc[kTiles][NT][2];  // columns 2 t and 2 t + 1 of rows g, g + 8
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) acc[i][t][0] = acc[i][t][1] = 0;
-    }
-
-    // c = a b + (first, first, first, first), or c += a b.
-    template <bool FIRST>
-    static __device__ __forceinline__ void mma(int (&c)[4], const uint32_t (&a)[4], uint2 b) {
-        if constexpr (FIRST)
-            asm volatile(
-                "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                "{%10, %10, %10, %10};"
-                : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(0x4b400000));
-        else
-            asm volatile(
-                "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                "{%0, %1, %2, %3};"
-                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
-    }
-
-    // One k-block, the chunk's at `at`.
-    template <int G>
-    __device__ __forceinline__ void product(const Q4Stage<G> (&st)[kTiles], int at, bool minima) {
-        constexpr int NG = 128 / G, SL = 4 / NG;  // slices of 32 a group
-        const int lane = threadIdx.x & 31;
-        const uint8_t* f = frags + at * (cols * kColumn) + (lane >> 2) * kColumn + (lane & 3) * 8;
-        const uint64_t magic = q4_pair(-12582912.0f, -12582912.0f);
-        uint64_t part[kTiles][NT][2];  // the k-block's sums, in its rows' scales
-        uint32_t w[kTiles][2][4];
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-            w[i][0][0] = st[i].lo.x; w[i][0][1] = st[i].lo.y; w[i][0][2] = st[i].lo.z; w[i][0][3] = st[i].lo.w;
-            w[i][1][0] = st[i].hi.x; w[i][1][1] = st[i].hi.y; w[i][1][2] = st[i].hi.z; w[i][1][3] = st[i].hi.w;
-        }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            uint32_t av[kTiles][SL][4];
-            uint64_t d0[kTiles], d1[kTiles];
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i) {
-#pragma unroll
-                for (int s = 0; s < SL; ++s) {
-                    const uint32_t u0 = w[i][0][g * SL + s], u1 = w[i][1][g * SL + s];
-                    av[i][s][0] = u0 << 4 & 0xf0f0f0f0u;
-                    av[i][s][1] = u1 << 4 & 0xf0f0f0f0u;
-                    av[i][s][2] = u0 & 0xf0f0f0f0u;
-                    av[i][s][3] = u1 & 0xf0f0f0f0u;
-                }
-                const float2 d = Q4Stage<G>::pick(st[i].d, g);
-                d0[i] = q4_pair(d.x, d.x);
-                d1[i] = q4_pair(d.y, d.y);
-            }
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                uint2 b[SL];
-#pragma unroll
-                for (int s = 0; s < SL; ++s)
-                    b[s] = *reinterpret_cast<const uint2*>(f + t * (8 * kColumn) + (g * SL + s) * 32);
-#pragma unroll
-                for (int i = 0; i < kTiles; ++i) {
-                    int c[4];
-                    mma<true>(c, av[i][0], b[0]);
-#pragma unroll
-                    for (int s = 1; s < SL; ++s) mma<false>(c, av[i][s], b[s]);
-                    const uint64_t v0 = q4_add2(q4_pair(__int_as_float(c[0]), __int_as_float(c[1])), magic);
-                    const uint64_t v1 = q4_add2(q4_pair(__int_as_float(c[2]), __int_as_float(c[3])), magic);
-                    part[i][t][0] = g == 0 ? q4_mul2(d0[i], v0) : q4_fma2(d0[i], v0, part[i][t][0]);
-                    part[i][t][1] = g == 0 ? q4_mul2(d1[i], v1) : q4_fma2(d1[i], v1, part[i][t][1]);
-                }
-            }
-            if (minima) {
-                // (m + 8 d) sum x, to one of a row's four columns: the even lanes' first.
-                const float* xs = sums + (at * NG + g) * kTokens + (lane >> 1 & 1);
-#pragma unroll
-                for (int i = 0; i < kTiles; ++i) {
-                    const float2 d = Q4Stage<G>::pick(st[i].d, g), mn = Q4Stage<G>::pick(st[i].m, g);
-                    const float o0 = lane & 1 ? 0.0f : fmaf(8.0f, d.x, mn.x);
-                    const float o1 = lane & 1 ? 0.0f : fmaf(8.0f, d.y, mn.y);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const float v = xs[2 * t];
-                        acc[i][t][0] = q4_fma2(q4_pair(o0, 0.0f), q4_pair(v, 0.0f), acc[i][t][0]);
-                        acc[i][t][1] = q4_fma2(q4_pair(o1, 0.0f), q4_pair(v, 0.0f), acc[i][t][1]);
-                    }
-                }
-            }
-        }
-        const float* factor = factors + at * cols + (lane & 3) * 2;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const uint64_t v = *reinterpret_cast<const uint64_t*>(factor + t * 8);
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i) {
-                acc[i][t][0] = q4_fma2(v, part[i][t][0], acc[i][t][0]);
-                acc[i][t][1] = q4_fma2(v, part[i][t][1], acc[i][t][1]);
-            }
-        }
-    }
-
-    // The lane's sum c of tile i: row lane / 4 (lane odd: + 8) of row 2 c + (lane / 2) % 2 of x.
-    __device__ __forceinline__ float lane_sum(int i, int c) const {
-        const float2 a = q4_unpair(acc[i][c][0]), b = q4_unpair(acc[i][c][1]);
-        float u = a.x + a.y, v = b.x + b.y;  // two digits of the four
-        u += __shfl_xor_sync(~0u, u, 1);
-        v += __shfl_xor_sync(~0u, v, 1);
-        return threadIdx.x & 1 ? v : u;
-    }
-    static __device__ __forceinline__ int row_of(int c, int lane) { return (lane >> 2) + 8 * (lane & 1); }
-    static __device__ __forceinline__ int token_of(int c, int lane) { return 2 * c + (lane >> 1 & 1); }
-};
-
-// ---- x as floating-point columns: T products of eight rows of x, HALF: FP16 rows as they are
+// ---- operands
 
 // An integer below 2^m in the low bits of a number whose mantissa's last bit is worth 1 is that power of two plus
 // the integer, so a nibble becomes a number by one logic operation and a subtraction.
@@ -506,15 +319,458 @@ __device__ __forceinline__ void q4_mma(float (&c)[4], const uint32_t (&a)[4], ui
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
 
-// x = a[0] + a[1] + a[2] in BF16, whole: each takes the next eight bits at least.
-__device__ __forceinline__ void q4_three(float x, float y, __nv_bfloat162 (&a)[3]) {
+// The operand of 16 columns out of words of rows g and g + 8.
+__device__ __forceinline__ void q4_bf16_words(uint32_t (&a)[4], uint32_t u0, uint32_t u1) {
+    a[0] = q4_bf16(u0);
+    a[1] = q4_bf16(u1);
+    a[2] = q4_bf16(u0 >> 4);
+    a[3] = q4_bf16(u1 >> 4);
+}
+
+// An FP32 row's k-block as three BF16 columns, x = a[0] + a[1] + a[2], whole: each takes the next eight bits at
+// least.  Scaled by 2^24, so that the last parts of the smallest numbers too are normal ones; where `top`, the
+// greatest number's bits, reaches 2^88, by 2^-24, so that no sum overflows before its scale comes.
+__device__ __forceinline__ bool q4_three_great(uint32_t top) { return top >= 0x6b800000u; }
+__device__ __forceinline__ float q4_three_scale(uint32_t top) { return q4_three_great(top) ? 0x1p24f : 0x1p-24f; }
+
+// A lane's four numbers are columns 0..3 or 4..7 of the run of eight that lane t = lane / 2 % 4 of a fragment
+// holds: a word of slice 2 (lane / 8), the even columns, and one of the next, 32 bytes on, the odd ones.  `to`: the
+// first column.
+__device__ __forceinline__ int q4_float_word(int lane) { return (lane >> 3) * 64 + (lane >> 1 & 3) * 8 + (lane & 1) * 4; }
+__device__ __forceinline__ void q4_put_three(float4 x, uint32_t top, uint8_t* to, int column) {
+    to += q4_float_word(threadIdx.x & 31);
+    const float up = q4_three_great(top) ? 0x1p-24f : 0x1p24f;
+    float v[4] = {x.x * up, x.z * up, x.y * up, x.w * up};
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-        a[i] = __floats2bfloat162_rn(x, y);
-        x -= __low2float(a[i]);
-        y -= __high2float(a[i]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const __nv_bfloat162 a = __floats2bfloat162_rn(v[2 * h], v[2 * h + 1]);
+            v[2 * h] -= __low2float(a);
+            v[2 * h + 1] -= __high2float(a);
+            *reinterpret_cast<__nv_bfloat162*>(to + i * column + h * 32) = a;
+        }
     }
 }
+
+
+// ---- one row, as digits: six of a product's eight columns
+
+// 2^n as a number, n an exponent of normal numbers.
+__device__ __forceinline__ float q4_power(int n) { return __uint_as_float(static_cast<uint32_t>(n + 127) << 23); }
+
+// Adding 1.5 * 2^23 rounds a number of up to 2^22 to an integer, which it leaves in the sum's low bits.
+constexpr float kQ4Magic = 12582912.0f;
+constexpr uint32_t kQ4MagicBits = 0x4b400000u;
+
+// Three signed base-256 digits each of four such integers into three columns, a lane's word of each: adding 128 to
+// the lower two makes the digits the integer's bytes.
+__device__ __forceinline__ void q4_put_digits(const float (&n)[4], uint32_t* to) {
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (__float_as_uint(n[i]) + (0x8080u - kQ4MagicBits)) ^ 0x8080u;
+    const uint32_t l01 = __byte_perm(v[0], v[1], 0x5140), l23 = __byte_perm(v[2], v[3], 0x5140);
+    to[0] = __byte_perm(l01, l23, 0x5410);
+    to[8] = __byte_perm(l01, l23, 0x7632);
+    to[16] = __byte_perm(__byte_perm(v[0], v[1], 0x0062), __byte_perm(v[2], v[3], 0x0062), 0x5410);
+}
+
+template <bool GATED_>
+struct Q4Digits {
+    static constexpr bool GATED = GATED_;
+    static constexpr int kTokens = 1;
+    static constexpr int kTiles = GATED ? 2 : 1;
+    static constexpr int kLaneSums = 1;          // of a tile, joined over the digits
+    static constexpr int kWarps = !GATED ? 16 : 8;
+    static constexpr int kRun = 2, kRing = 3;    // k-blocks of a warp a round; rounds on their way
+    static constexpr bool kFinisher = true;      // a warp of its own finishes the sums
+    static constexpr bool kWideRows = true;      // rows that digits do not hold are three BF16 columns
+    static constexpr int kSlice = 224;           // bytes: six columns of 32 numbers, and a step of 8 banks
+    static constexpr int kRow = 4 * kSlice;      // of a k-block
+    static constexpr int kWide = 288;            // a column of a row that is not digits
+
+    // Shared memory of `chunk` k-blocks: the columns; each row's factor, twice; the scale of a row that is not digits,
+    // else 0; each row's sums over the groups.
+    static __host__ __device__ int block_bytes(int, int ng) { return kRow + 12 + 4 * ng; }
+    static constexpr int kTail = 80;             // what the lanes of columns 6 and 7 read past the last; then their factor
+    uint8_t* frags;
+    float2* factors;
+    const float2* own;  // the lane's, of columns 2 t and 2 t + 1: 0 for columns 6 and 7
+    int own_step;
+    float* scales;
+    float* sums;
+    __device__ __forceinline__ Q4Digits(const Q4Args& a, uint8_t* x, int) {
+        frags = x;
+        factors = reinterpret_cast<float2*>(x + a.chunk * kRow + kTail);
+        const bool last = (threadIdx.x & 3) == 3;
+        own = last ? factors - 1 : factors;
+        own_step = last ? 0 : 1;
+        scales = reinterpret_cast<float*>(factors + a.chunk);
+        sums = scales + a.chunk;
+    }
+
+    // A slice of 32 columns of x is the six columns of its digits, 32 bytes each, a lane's four numbers a word of each.
+    // read() once the numbers are on their way.  Returns whether the warp saw a row that is not digits.
+    template <int G, class Read>
+    __device__ __forceinline__ bool split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Read read) const {
+        constexpr int NG = 128 / G;
+        const int lane = threadIdx.x & 31;
+        const Q4Items it(kWarps, tokens);
+        bool seen = false;
+        auto slot = [&](int b, int) { return frags + b * kRow + lane * 16; };
+        q4_fetch<false>(a, it, m0, tokens, kb0, kb1 - kb0, slot);
+        if (threadIdx.x == 0) factors[-1] = make_float2(0.0f, 0.0f);
+        read();
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        q4_split<false>(a, it, tokens, kb1 - kb0, slot, [&](int b, int, float4 x, bool store) {
+            // The greatest number is below 2^(e - 126), e its exponent field: scaled by 2^(147 - e) all are below
+            // 2^21.  Their integers are three digits; what is left of each, by 2^22, is three more, and nothing is
+            // left of a number of the greatest's 2^-19 or more.
+            const uint32_t top = q4_top(x);
+            const int e = static_cast<int>(top >> 23);
+            // Not digits: smaller numbers; those whose units or sums pass the ends of FP32's range; infinities, NaN.
+            const bool out = e >= 250 || (e < 40 && top != 0);
+            const float least = q4_power(max(e, 40) - 146), up = q4_power(147 - max(e, 40));
+            const float n[4] = {x.x, x.y, x.z, x.w};
+            float first[4], second[4];
+            bool left = out;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                first[i] = fmaf(n[i], up, kQ4Magic);
+                second[i] = fmaf(fmaf(n[i], up, kQ4Magic - first[i]), 0x1p22f, kQ4Magic);
+                left |= fabsf(n[i]) < least && n[i] != 0.0f;
+            }
+            const bool wide = __any_sync(~0u, left);
+            uint8_t* row = frags + b * kRow;
+            if (store && !wide) {
+                uint32_t* to = reinterpret_cast<uint32_t*>(row + (lane >> 3) * kSlice) + (lane & 7);
+                q4_put_digits(first, to);
+                q4_put_digits(second, to + 24);
+            } else if (store) {
+                q4_put_three(x, top, row, kWide);
+            }
+            // The factor is that of column 2, with the weights' 1 / 16: 2^16 2^(e - 147) / 16.  The last two columns
+            // are not there: any bytes are integers, which count nothing, and so for a row that is not digits.
+            if (store && lane == 0) {
+                const float f = wide || top == 0 ? 0.0f : q4_power(e - 135);
+                factors[b] = make_float2(f, f);
+                scales[b] = wide ? q4_three_scale(top) : 0.0f;
+            }
+            seen |= wide;
+            if (a.minimum) {
+                const float s = q4_group_sum<G>(x);
+                if (store && lane % (G / 4) == 0) sums[b * NG + lane / (G / 4)] = s;
+            }
+        });
+        return seen;
+    }
+
+    uint64_t acc[kTiles][2];  // columns 2 t and 2 t + 1 of rows g, g + 8, in the factors' unit
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) acc[i][0] = acc[i][1] = 0;
+    }
+
+    // c = a b + (first, first, first, first), or c += a b.
+    template <bool FIRST>
+    static __device__ __forceinline__ void mma(int (&c)[4], const uint32_t (&a)[4], uint2 b) {
+        if constexpr (FIRST)
+            asm volatile(
+                "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                "{%10, %10, %10, %10};"
+                : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(0x4b400000));
+        else
+            asm volatile(
+                "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                "{%0, %1, %2, %3};"
+                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+    }
+
+    // A k-block that is not digits, its three BF16 columns one product.  Its sums, whole, take the place of column 7,
+    // lane (g, 3).
+    template <int G>
+    __device__ __forceinline__ void wide_product(const Q4Stage<G> (&st)[kTiles], int at) {
+        constexpr int NG = 128 / G, SL = 4 / NG;
+        const int lane = threadIdx.x & 31;
+        const float scale = scales[at];
+        if (scale == 0.0f) return;
+        // The lanes of columns past the third read the third's: their sums go nowhere.
+        const uint8_t* f = frags + at * kRow + min(lane >> 2, 2) * kWide + (lane & 3) * 8;
+        // Lane (g, 0) holds columns 0 and 1, lane (g, 1) column 2.
+        const float first = (lane & 3) < 2 ? scale : 0.0f, second = (lane & 3) < 1 ? scale : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+            const uint32_t u[2][4] = {{st[i].lo.x, st[i].lo.y, st[i].lo.z, st[i].lo.w},
+                                      {st[i].hi.x, st[i].hi.y, st[i].hi.z, st[i].hi.w}};
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                float c[4];
+#pragma unroll
+                for (int s = 0; s < 2 * SL; ++s) {
+                    const int j = g * SL + s / 2, h = s % 2;
+                    uint32_t av[4];
+                    q4_bf16_words(av, u[0][j] >> (8 * h), u[1][j] >> (8 * h));
+                    const uint2 b = *reinterpret_cast<const uint2*>(f + (2 * j + h) * 32);
+                    if (s == 0) q4_mma<false, true>(c, av, b);
+                    else q4_mma<false, false>(c, av, b);
+                }
+                const float2 d = Q4Stage<G>::pick(st[i].d, g);
+                sum[0] = fmaf(d.x, fmaf(first, c[0], second * c[1]), sum[0]);
+                sum[1] = fmaf(d.y, fmaf(first, c[2], second * c[3]), sum[1]);
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                sum[r] += __shfl_xor_sync(~0u, sum[r], 2);
+                sum[r] += __shfl_xor_sync(~0u, sum[r], 1);
+                const float2 v = q4_unpair(acc[i][r]);
+                acc[i][r] = q4_pair(v.x, v.y + ((lane & 3) == 3 ? sum[r] : 0.0f));
+            }
+        }
+    }
+
+    // One k-block, the chunk's at `at`.
+    template <int G>
+    __device__ __forceinline__ void product(const Q4Stage<G> (&st)[kTiles], int at, bool minima) {
+        constexpr int NG = 128 / G, SL = 4 / NG;  // slices of 32 a group
+        const int lane = threadIdx.x & 31;
+        const uint8_t* f = frags + at * kRow + lane * 8;
+        const uint64_t magic = q4_pair(-12582912.0f, -12582912.0f);
+        uint64_t part[kTiles][2];  // the k-block's sums, in its rows' scales
+        uint32_t w[kTiles][2][4];
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+            w[i][0][0] = st[i].lo.x; w[i][0][1] = st[i].lo.y; w[i][0][2] = st[i].lo.z; w[i][0][3] = st[i].lo.w;
+            w[i][1][0] = st[i].hi.x; w[i][1][1] = st[i].hi.y; w[i][1][2] = st[i].hi.z; w[i][1][3] = st[i].hi.w;
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            uint32_t av[kTiles][SL][4];
+            uint64_t d0[kTiles], d1[kTiles];
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+                for (int s = 0; s < SL; ++s) {
+                    const uint32_t u0 = w[i][0][g * SL + s], u1 = w[i][1][g * SL + s];
+                    av[i][s][0] = u0 << 4 & 0xf0f0f0f0u;
+                    av[i][s][1] = u1 << 4 & 0xf0f0f0f0u;
+                    av[i][s][2] = u0 & 0xf0f0f0f0u;
+                    av[i][s][3] = u1 & 0xf0f0f0f0u;
+                }
+                const float2 d = Q4Stage<G>::pick(st[i].d, g);
+                d0[i] = q4_pair(d.x, d.x);
+                d1[i] = q4_pair(d.y, d.y);
+            }
+            uint2 b[SL];
+#pragma unroll
+            for (int s = 0; s < SL; ++s) b[s] = *reinterpret_cast<const uint2*>(f + (g * SL + s) * kSlice);
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+                int c[4];
+                mma<true>(c, av[i][0], b[0]);
+#pragma unroll
+                for (int s = 1; s < SL; ++s) mma<false>(c, av[i][s], b[s]);
+                const uint64_t v0 = q4_add2(q4_pair(__int_as_float(c[0]), __int_as_float(c[1])), magic);
+                const uint64_t v1 = q4_add2(q4_pair(__int_as_float(c[2]), __int_as_float(c[3])), magic);
+                part[i][0] = g == 0 ? q4_mul2(d0[i], v0) : q4_fma2(d0[i], v0, part[i][0]);
+                part[i][1] = g == 0 ? q4_mul2(d1[i], v1) : q4_fma2(d1[i], v1, part[i][1]);
+            }
+            if (minima) {
+                // (m + 8 d) sum x, whole, in column 7's place.
+                const uint64_t v = q4_pair(0.0f, sums[at * NG + g]);
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) {
+                    const float2 d = Q4Stage<G>::pick(st[i].d, g), mn = Q4Stage<G>::pick(st[i].m, g);
+                    const float o0 = (lane & 3) == 3 ? fmaf(8.0f, d.x, mn.x) : 0.0f;
+                    const float o1 = (lane & 3) == 3 ? fmaf(8.0f, d.y, mn.y) : 0.0f;
+                    acc[i][0] = q4_fma2(q4_pair(0.0f, o0), v, acc[i][0]);
+                    acc[i][1] = q4_fma2(q4_pair(0.0f, o1), v, acc[i][1]);
+                }
+            }
+        }
+        const uint64_t v = *reinterpret_cast<const uint64_t*>(own + at * own_step);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+            acc[i][0] = q4_fma2(v, part[i][0], acc[i][0]);
+            acc[i][1] = q4_fma2(v, part[i][1], acc[i][1]);
+        }
+    }
+
+    // The lane's sum of tile i: row lane / 4 (lane odd: + 8).
+    __device__ __forceinline__ float lane_sum(int i, int) const {
+        // The columns' weights: 2^-16, 2^-8, 1 of the first three, 2^-22 of these of the next; what is whole.
+        const int t = threadIdx.x & 3;
+        const float lower = q4_power(t == 0 ? -16 : t == 2 ? -30 : 0);
+        const float upper = q4_power(t == 0 ? -8 : t == 1 ? -38 : t == 2 ? -22 : 0);
+        float sum[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const float2 v = q4_unpair(acc[i][r]);
+            sum[r] = fmaf(v.x, lower, v.y * upper);
+            sum[r] += __shfl_xor_sync(~0u, sum[r], 1);
+            sum[r] += __shfl_xor_sync(~0u, sum[r], 2);
+        }
+        return t & 1 ? sum[1] : sum[0];
+    }
+    static __device__ __forceinline__ int row_of(int, int lane) { return (lane >> 2) + 8 * (lane & 1); }
+    static __device__ __forceinline__ int token_of(int, int lane) { return lane >> 1 & 1; }  // lanes of a second are idle
+};
+
+// ---- a few FP32 rows: the three parts of two in each of NP products of eight columns
+
+template <int NP, bool GATED_>
+struct Q4Pairs {
+    static constexpr bool GATED = GATED_;
+    static constexpr int kTokens = 2 * NP;
+    static constexpr int kTiles = GATED ? 2 : 1;
+    static constexpr int kLaneSums = NP;
+    static constexpr int kWarps = !GATED ? 16 : 8;
+    static constexpr int kRun = NP == 1 ? 2 : 1, kRing = 3;  // k-blocks of a warp a round; rounds on their way
+    static constexpr bool kFinisher = true, kWideRows = false;
+    static constexpr int kColumn = 288;         // bytes: 8 slices x 32, and a step of 8 banks
+
+    // Column 2 p + m of a product is part p of its row m.  Held are the rows' first parts, their second and their third
+    // ones, of the rows that are there.
+    static __host__ __device__ int block_bytes(int tokens, int ng) { return tokens * 3 * kColumn + kTokens * 4 * (1 + ng); }
+    static constexpr int kTail = kColumn;  // what the lanes of a row that is not there read past the last
+    uint8_t* frags;
+    const uint8_t* column;  // the lane's, of the first product
+    int part_bytes, x_bytes;
+    float* scales;          // of a row's k-block
+    float* sums;            // of a row's groups
+    __device__ __forceinline__ Q4Pairs(const Q4Args& a, uint8_t* x, int tokens) {
+        const int lane = threadIdx.x & 31, g = lane >> 2;
+        frags = x;
+        part_bytes = tokens * kColumn;
+        x_bytes = 3 * part_bytes;
+        // The last two columns are the third parts again: their sums go nowhere.
+        column = x + min(g >> 1, 2) * part_bytes + (g & 1) * kColumn + (lane & 3) * 8;
+        scales = reinterpret_cast<float*>(x + a.chunk * x_bytes + kTail);
+        sums = scales + a.chunk * kTokens;
+    }
+
+    template <int G, class Read>
+    __device__ __forceinline__ bool split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Read read) const {
+        constexpr int NG = 128 / G;
+        const int lane = threadIdx.x & 31;
+        const Q4Items it(kWarps, tokens);
+        auto first = [&](int b, int m) { return frags + b * x_bytes + m * kColumn; };
+        auto slot = [&](int b, int m) { return first(b, m) + (lane >> 4) * part_bytes + (lane & 15) * 16; };
+        q4_fetch<false>(a, it, m0, tokens, kb0, kb1 - kb0, slot);
+        read();
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        q4_split<false>(a, it, tokens, kb1 - kb0, slot, [&](int b, int m, float4 x, bool store) {
+            const uint32_t top = q4_top(x);
+            if (store) q4_put_three(x, top, first(b, m), part_bytes);
+            if (store && lane == 0) scales[b * kTokens + m] = q4_three_scale(top);
+            if (a.minimum) {
+                const float s = q4_group_sum<G>(x);
+                if (store && lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
+            }
+        });
+        return false;
+    }
+
+    float acc[kTiles][NP][4];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+            for (int t = 0; t < NP; ++t)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[i][t][c] = 0.0f;
+    }
+
+    template <int G>
+    __device__ __forceinline__ void product(const Q4Stage<G> (&st)[kTiles], int at, bool minima) {
+        constexpr int NG = 128 / G, SL = 4 / NG;
+        const int lane = threadIdx.x & 31;
+        const uint8_t* f = column + at * x_bytes;
+        float part[kTiles][NP][4];  // the k-block's sums, in its rows' scales
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            float s[kTiles][NP][4];
+#pragma unroll
+            for (int j = g * SL; j < (g + 1) * SL; ++j) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t av[kTiles][4];
+#pragma unroll
+                    for (int i = 0; i < kTiles; ++i) {
+                        const uint32_t u0 = j == 0 ? st[i].lo.x : j == 1 ? st[i].lo.y : j == 2 ? st[i].lo.z : st[i].lo.w;
+                        const uint32_t u1 = j == 0 ? st[i].hi.x : j == 1 ? st[i].hi.y : j == 2 ? st[i].hi.z : st[i].hi.w;
+                        q4_bf16_words(av[i], u0 >> (8 * h), u1 >> (8 * h));
+                    }
+#pragma unroll
+                    for (int t = 0; t < NP; ++t) {
+                        const uint2 b = *reinterpret_cast<const uint2*>(f + (2 * j + h) * 32 + t * (2 * kColumn));
+#pragma unroll
+                        for (int i = 0; i < kTiles; ++i) {
+                            if (j == g * SL && h == 0) q4_mma<false, true>(s[i][t], av[i], b);
+                            else q4_mma<false, false>(s[i][t], av[i], b);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+                const float2 d = Q4Stage<G>::pick(st[i].d, g);
+#pragma unroll
+                for (int t = 0; t < NP; ++t)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float scale = c & 2 ? d.y : d.x;
+                        part[i][t][c] = g == 0 ? scale * s[i][t][c] : fmaf(scale, s[i][t][c], part[i][t][c]);
+                    }
+            }
+            if (minima) {
+                // (m + 8 d) sum x, in one of the lanes whose sums meet.
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) {
+                    const float2 d = Q4Stage<G>::pick(st[i].d, g), mn = Q4Stage<G>::pick(st[i].m, g);
+                    const float o0 = lane & 3 ? 0.0f : fmaf(8.0f, d.x, mn.x), o1 = lane & 3 ? 0.0f : fmaf(8.0f, d.y, mn.y);
+#pragma unroll
+                    for (int t = 0; t < NP; ++t) {
+                        const float2 v = *reinterpret_cast<const float2*>(sums + (at * NG + g) * kTokens + 2 * t);
+                        acc[i][t][0] = fmaf(o0, v.x, acc[i][t][0]);
+                        acc[i][t][1] = fmaf(o0, v.y, acc[i][t][1]);
+                        acc[i][t][2] = fmaf(o1, v.x, acc[i][t][2]);
+                        acc[i][t][3] = fmaf(o1, v.y, acc[i][t][3]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NP; ++t) {
+            const float2 v = *reinterpret_cast<const float2*>(scales + at * kTokens + 2 * t);
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[i][t][c] = fmaf(c & 1 ? v.y : v.x, part[i][t][c], acc[i][t][c]);
+        }
+    }
+    template <int G>
+    __device__ __forceinline__ void wide_product(const Q4Stage<G> (&)[kTiles], int) {}
+
+    // The lane's sum c of tile i: row lane / 4 (lane odd: + 8) of row 2 c + (lane / 2) % 2 of x, over its parts' lanes.
+    __device__ __forceinline__ float lane_sum(int i, int c) const {
+        const int lane = threadIdx.x & 31;
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[k] = (lane & 3) == 3 ? 0.0f : acc[i][c][k];
+            v[k] += __shfl_xor_sync(~0u, v[k], 2);
+            v[k] += __shfl_xor_sync(~0u, v[k], 1);
+        }
+        return lane & 2 ? (lane & 1 ? v[3] : v[1]) : (lane & 1 ? v[2] : v[0]);
+    }
+    static __device__ __forceinline__ int row_of(int, int lane) { return (lane >> 2) + 8 * (lane & 1); }
+    static __device__ __forceinline__ int token_of(int c, int lane) { return 2 * c + (lane >> 1 & 1); }
+};
+
+// ---- x as floating-point columns: T products of eight rows of x, HALF: FP16 rows as they are
 
 template <int T, bool HALF, bool GATED_>
 struct Q4Floats {
@@ -524,71 +780,64 @@ struct Q4Floats {
     static constexpr int kLaneSums = 4 * T;
     static constexpr int kParts = HALF ? 1 : 3;  // columns of a row
     static constexpr int kProducts = kParts * T;
-    static constexpr int kWarps = T == 2 && !GATED ? 16 : 8;
+    static constexpr int kWarps = T <= 2 && !GATED ? 16 : 8;
     static constexpr int kRun = 1, kRing = GATED ? 3 : 4;
-    static constexpr bool kFinisher = false;
+    static constexpr bool kFinisher = false, kWideRows = false;
+
     static constexpr int kColumn = 288;  // bytes: 8 slices x 32, and a step of 8 banks
 
-    static __host__ __device__ int block_bytes(int, int ng) {
-        return 8 * kProducts * kColumn + kTokens * 4 * (1 + ng);
+    // The columns: the eight rows' first parts of a product, their second ones, their third ones, then the next
+    // eight rows'.  Of a single product's rows only those that are there.
+    static __host__ __device__ int columns(int tokens) { return T == 1 ? kParts * tokens : 8 * kProducts; }
+    static __host__ __device__ int block_bytes(int tokens, int ng) {
+        return columns(tokens) * kColumn + kTokens * 4 * (1 + ng);
     }
-    static constexpr int kTail = 0;
+    static constexpr int kTail = T == 1 ? 8 * kColumn : 0;  // what the lanes of rows that are not there read past the last
     uint8_t* frags;
-    float* scales;  // of a row's k-block
-    float* sums;    // of a row's groups
-    __device__ __forceinline__ Q4Floats(const Q4Args& a, uint8_t* x, int) {
+    int part_bytes, x_bytes;  // from a part to the next, of a k-block
+    float* scales;            // of a row's k-block
+    float* sums;              // of a row's groups
+    __device__ __forceinline__ Q4Floats(const Q4Args& a, uint8_t* x, int tokens) {
         frags = x;
-        scales = reinterpret_cast<float*>(x + a.chunk * (8 * kProducts * kColumn));
+        part_bytes = (T == 1 ? tokens : 8) * kColumn;
+        x_bytes = columns(tokens) * kColumn;
+        scales = reinterpret_cast<float*>(x + a.chunk * x_bytes + kTail);
         sums = scales + a.chunk * kTokens;
     }
 
-    // A lane's four numbers are columns 0..3 or 4..7 of the run of eight that lane t = lane / 2 % 4 of a fragment
-    // holds: a word of slice 2 (lane / 8), the even columns, and one of the next, the odd ones, of each part (the
-    // same column of one product after another).
     template <int G, class Read>
-    __device__ __forceinline__ void split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Read read) const {
+    __device__ __forceinline__ bool split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Read read) const {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
         const Q4Items it(kWarps, tokens);
         auto column = [&](int b, int m) {
-            return frags + (b * (8 * kProducts) + m / 8 * (8 * kParts) + m % 8) * kColumn;
+            return frags + b * x_bytes + (T == 1 ? m : m / 8 * (8 * kParts) + m % 8) * kColumn;
         };
         auto slot = [&](int b, int m) {
-            return HALF ? column(b, m) + lane * 8 : column(b, m) + (lane >> 4) * (8 * kColumn) + (lane & 15) * 16;
+            return HALF ? column(b, m) + lane * 8 : column(b, m) + (lane >> 4) * part_bytes + (lane & 15) * 16;
         };
         q4_fetch<HALF>(a, it, m0, tokens, kb0, kb1 - kb0, slot);
         read();
         asm volatile("cp.async.wait_all;" ::: "memory");
         q4_split<HALF>(a, it, tokens, kb1 - kb0, slot, [&](int b, int m, float4 x, bool store) {
-            uint8_t* to = column(b, m) + (lane >> 3) * 64 + (lane >> 1 & 3) * 8 + (lane & 1) * 4;
+            uint8_t* to = column(b, m);
             if constexpr (HALF) {
+                to += q4_float_word(lane);
                 if (store) {
                     *reinterpret_cast<__half2*>(to) = __floats2half2_rn(x.x, x.z);
                     *reinterpret_cast<__half2*>(to + 32) = __floats2half2_rn(x.y, x.w);
                 }
             } else {
-                // Scaled by 2^24, so that the last parts of the smallest numbers too are normal ones; a k-block
-                // that reaches 2^88 by 2^-24, so that no sum overflows before its scale comes.
-                const bool great = q4_top(x) >= 0x6b800000u;
-                const float up = great ? 0x1p-24f : 0x1p24f;
-                auto put = [&](float u, float v, int at) {
-                    __nv_bfloat162 parts[3];
-                    q4_three(u, v, parts);
-                    if (store) {
-#pragma unroll
-                        for (int i = 0; i < 3; ++i)
-                            *reinterpret_cast<__nv_bfloat162*>(to + i * (8 * kColumn) + at) = parts[i];
-                    }
-                };
-                put(x.x * up, x.z * up, 0);
-                put(x.y * up, x.w * up, 32);
-                if (store && lane == 0) scales[b * kTokens + m] = great ? 0x1p24f : 0x1p-24f;
+                const uint32_t top = q4_top(x);
+                if (store) q4_put_three(x, top, to, part_bytes);
+                if (store && lane == 0) scales[b * kTokens + m] = q4_three_scale(top);
             }
             if (a.minimum) {
                 const float s = q4_group_sum<G>(x);
                 if (store && lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
             }
         });
+        return false;
     }
 
     float acc[kTiles][kLaneSums];
@@ -603,7 +852,7 @@ struct Q4Floats {
     __device__ __forceinline__ void product(const Q4Stage<G> (&st)[kTiles], int at, bool minima) {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
-        const uint8_t* f = frags + at * (8 * kProducts * kColumn) + (lane >> 2) * kColumn + (lane & 3) * 8;
+        const uint8_t* f = frags + at * x_bytes + (lane >> 2) * kColumn + (lane & 3) * 8;
         constexpr int kSums = HALF ? 1 : 2;  // the first parts', and the others', which are far smaller
         float part[kTiles][kLaneSums];       // the k-block's sums, in its rows' scales
         float s[kTiles][T][kSums][4];        // a group's sums
@@ -621,18 +870,22 @@ struct Q4Floats {
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i) {
                     const uint32_t u0 = w[i][0][j] >> (8 * h), u1 = w[i][1][j] >> (8 * h);
-                    av[i][0] = HALF ? q4_low(u0) : q4_bf16(u0);
-                    av[i][1] = HALF ? q4_low(u1) : q4_bf16(u1);
-                    av[i][2] = HALF ? q4_high(u0) : q4_bf16(u0 >> 4);
-                    av[i][3] = HALF ? q4_high(u1) : q4_bf16(u1 >> 4);
+                    if constexpr (HALF) {
+                        av[i][0] = q4_low(u0);
+                        av[i][1] = q4_low(u1);
+                        av[i][2] = q4_high(u0);
+                        av[i][3] = q4_high(u1);
+                    } else {
+                        q4_bf16_words(av[i], u0, u1);
+                    }
                 }
                 const bool first = j % (4 / NG) == 0 && h == 0;
 #pragma unroll
                 for (int p = 0; p < kParts; ++p) {
 #pragma unroll
                     for (int t = 0; t < T; ++t) {
-                        const uint2 b = *reinterpret_cast<const uint2*>(f + (2 * j + h) * 32 +
-                                                                        (t * kParts + p) * (8 * kColumn));
+                        const uint2 b = *reinterpret_cast<const uint2*>(f + (2 * j + h) * 32 + t * (8 * kParts * kColumn) +
+                                                                        p * (T == 1 ? part_bytes : 8 * kColumn));
 #pragma unroll
                         for (int i = 0; i < kTiles; ++i) {
                             if (first && p < kSums) q4_mma<HALF, true>(s[i][t][p], av[i], b);
@@ -681,6 +934,8 @@ struct Q4Floats {
                     acc[i][4 * t + c] = fmaf(c & 1 ? v.y : v.x, part[i][4 * t + c], acc[i][4 * t + c]);
         }
     }
+    template <int G>
+    __device__ __forceinline__ void wide_product(const Q4Stage<G> (&)[kTiles], int) {}
 
     __device__ __forceinline__ float lane_sum(int i, int c) const { return acc[i][c]; }
     static __device__ __forceinline__ int row_of(int c, int lane) { return (lane >> 2) + 4 * (c & 2); }
@@ -784,6 +1039,7 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
 
     bool started = false, held = false;  // a chunk of x, the only one, is in shared memory
     bool lost = false;                   // a bounded wait ran out
+    bool wide = false;                   // the chunk has rows that are not digits
     int parity = 0, place = 0;
     uint32_t phase = 0;
 #pragma unroll 1
@@ -795,11 +1051,12 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
             if (!held) {
                 if (started) __syncthreads();  // the chunk before has been read
                 if (worker)
-                    form.template split<G>(a, m0, tokens, kc, kc_end, [&] {
+                    wide = form.template split<G>(a, m0, tokens, kc, kc_end, [&] {
                         if (!started) asm volatile("bar.arrive 1, %0;" ::"n"(32 * (F::kWarps + 1)) : "memory");
                     });
                 started = true;
-                __syncthreads();
+                if constexpr (F::kWideRows) wide = __syncthreads_or(wide);
+                else __syncthreads();
                 held = a.chunk >= kb_end - kb_begin;
             }
             if (!worker && !bringer) continue;
@@ -814,18 +1071,27 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
                 } else {
                     const int at = kb - kc + wk * F::kRun;
                     const uint8_t* tiles = ring + place * place_bytes + warp * (F::kRun * block);
-                    auto one = [&](int i) {
+                    const int count = min(kc_end - kc - at, F::kRun);  // less than 1: none
+                    auto staged = [&](int i, auto then) {
                         Q4Stage<G> stage[F::kTiles];
 #pragma unroll
                         for (int t = 0; t < F::kTiles; ++t)
                             stage[t].read(tiles + t * (F::kWarps * F::kRun * block) + i * block, lane, minima);
-                        form.template product<G>(stage, at + i, minima);
+                        then(stage, at + i);
                     };
-                    if (F::kRun == 2 && at + 1 < kc_end - kc) {  // two k-blocks' chains of products side by side
+                    auto one = [&](int i) {
+                        staged(i, [&](auto& stage, int k) { form.template product<G>(stage, k, minima); });
+                    };
+                    if (F::kRun == 2 && count == 2) {  // two k-blocks' chains of products side by side
                         one(0);
                         one(1);
-                    } else if (at < kc_end - kc) {
+                    } else if (count > 0) {
                         one(0);
+                    }
+                    if (F::kWideRows && wide) {
+#pragma unroll 1
+                        for (int i = 0; i < count; ++i)
+                            staged(i, [&](auto& stage, int k) { form.template wide_product<G>(stage, k); });
                     }
                     __syncwarp();  // every lane has read its part
                     if (lane == 0) mbar_arrive(empty + place);
@@ -890,7 +1156,7 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
 
 // How a product is cut (q4_linear.cu).
 struct Q4Plan {
-    int form;      // rows of x a CTA takes: 2, 4 or 8 in digits; 16, or 32 of FP16, in floats
+    int form;      // rows of x a CTA takes: 1 in digits; 2 or 4 in pairs; 8, 16, or 32 of FP16, in floats
     int wk_log;    // warps that share a row tile's k-blocks (fewer where their k-blocks of x do not fit)
     int cluster_log;  // CTAs that do
     int shared;    // bytes of shared memory a CTA may take

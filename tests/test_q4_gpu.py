@@ -699,7 +699,7 @@ def beside_great_numbers(g, rows, k, n, group, kind, great, xt):
 
 @pytest.mark.parametrize("kind", ["code"])
 @pytest.mark.parametrize("great", [300.0, 1e4, 1e6, 1e10, 1e20, 1e30])
-@pytest.mark.parametrize("rows", [9, 16, 17, 33])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 7, 8, 9, 16, 17, 33])
 def test_great_numbers_that_weigh_nothing(cuda, rows, great, kind):
     import sdb
 
@@ -710,7 +710,7 @@ def test_great_numbers_that_weigh_nothing(cuda, rows, great, kind):
 
 
 @pytest.mark.parametrize("kind", ["code"])
-@pytest.mark.parametrize("rows", [9, 17, 33])
+@pytest.mark.parametrize("rows", [1, 2, 3, 8, 9, 17, 33])
 def test_great_half_precision_numbers(cuda, rows, kind):
     import sdb
     import torch
@@ -725,7 +725,7 @@ def test_great_half_precision_numbers(cuda, rows, kind):
     check(host(out), exact, mag)
 
 
-@pytest.mark.parametrize("rows", [9, 17, 33])
+@pytest.mark.parametrize("rows", [1, 2, 3, 5, 8, 9, 17, 33])
 @pytest.mark.parametrize("gated", [False, True])
 def test_one_number_a_column(cuda, rows, gated):
     """Each column of the output is one number of x, all other weights 0, the numbers of a row of any magnitudes."""
@@ -748,3 +748,25 @@ def test_one_number_a_column(cuda, rows, gated):
     else:
         got = host(sdb.mul_mat_q4(w, t))
     assert (np.abs(got - exact) <= oracle.K_B200 * mag).all()
+
+
+@pytest.mark.parametrize("minimum", [False, True])
+@pytest.mark.parametrize("rows", [1, 2, 3, 8, 9, 17, 33])
+def test_the_smallest_numbers(cuda, rows, minimum):
+    """Rows down to numbers below the normal ones, with scales that bring the sums back to normal numbers: the
+    bound holds, and 2^-143 for some sixty sums rounded to 2^-149."""
+    import sdb
+
+    g = rng(rows)
+    q, scales, minima, _ = made(g, 40, 300, 64, minimum)
+    scales = (scales * np.float16(1000)).astype(np.float16)
+    minima = (minima * np.float16(300)).astype(np.float16) if minimum else None
+    d = np.repeat(scales.astype(np.float64), 64, axis=1)[:, :300]
+    m = np.repeat(minima.astype(np.float64), 64, axis=1)[:, :300] if minimum else -8 * d
+    w = on_device(cuda, q, scales, minima, 64)
+    for scale in (1e-32, 1e-34, 3e-36, 1e-37, 1e-38, 1e-39, 1e-40):
+        x = (g.standard_normal((rows, 300)) * scale).astype(np.float32)
+        exact, mag = oracle.mul_mat_exact(d * q + m, x)
+        got = host(sdb.mul_mat_q4(w, cuda_tensor(x, cuda)))
+        worst = (np.abs(got - exact) / (oracle.K_B200 * mag + 2.0 ** -143)).max()
+        assert worst <= 1, f"{scale}: {worst:.3g} of the bound"
