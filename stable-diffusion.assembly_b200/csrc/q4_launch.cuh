@@ -1,4 +1,4 @@
-// The launches of q4_rows.cuh's kernel for one group size (a translation unit each: q4_rows_*.cu).
+// The launches of q4_rows.cuh's kernel for one group size, with minima or without (a translation unit each: q4_rows_*.cu).
 #pragma once
 
 #include <algorithm>
@@ -9,9 +9,9 @@
 
 namespace sdb {
 
-template <class F, int G>
+template <class F, int G, bool MINIMA>
 int q4_launch_form(const Q4Args& args, const Q4Plan& p, cudaStream_t st) {
-    auto kern = q4_rows_kernel<F, G>;
+    auto kern = q4_rows_kernel<F, G, MINIMA>;
     // The kernel's shared-memory limit is raised once on each device (it costs about as much as a launch).
     static std::atomic<uint64_t> raised{0};
     int dev = 0;
@@ -21,8 +21,8 @@ int q4_launch_form(const Q4Args& args, const Q4Plan& p, cudaStream_t st) {
         if (dev < 64) raised.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
     Q4Args a = args;
-    const int fixed = q4_fixed_bytes<F>(1024 + 4096 / G * (a.minimum ? 2 : 1));
-    const int block = F::block_bytes(std::min(a.rows, F::kTokens), 128 / G);
+    const int fixed = q4_fixed_bytes<F>(1024 + 4096 / G * (MINIMA ? 2 : 1));
+    const int block = F::block_bytes(std::min(a.rows, F::kTokens), MINIMA ? 128 / G : 0);
     const int fit = (p.shared - fixed) / block;  // k-blocks of x that fit
     // All of a CTA's k-blocks of x are held where a cluster of up to eight brings them down to what fits: else x is
     // split again for every tile (28672 -> 8192, one row: two CTAs 33 us, one 66).  The CTAs then stand for warps that
@@ -62,22 +62,22 @@ int q4_launch_form(const Q4Args& args, const Q4Plan& p, cudaStream_t st) {
     return SDB_OK;
 }
 
-template <bool GATED, int G>
+template <bool GATED, int G, bool MINIMA>
 int q4_launch_rows(const Q4Args& a, const Q4Plan& p, cudaStream_t st) {
-    if (p.form == 1) return q4_launch_form<Q4Digits<GATED>, G>(a, p, st);
-    if (p.form == 2) return q4_launch_form<Q4Pairs<1, GATED>, G>(a, p, st);
-    if (p.form == 4) return q4_launch_form<Q4Pairs<2, GATED>, G>(a, p, st);
+    if (p.form == 1) return q4_launch_form<Q4Digits<GATED>, G, MINIMA>(a, p, st);
+    if (p.form == 2) return q4_launch_form<Q4Pairs<1, GATED>, G, MINIMA>(a, p, st);
+    if (p.form == 4) return q4_launch_form<Q4Pairs<2, GATED>, G, MINIMA>(a, p, st);
     if (p.form == 8)
-        return a.x_half ? q4_launch_form<Q4Floats<1, true, GATED>, G>(a, p, st)
-                        : q4_launch_form<Q4Floats<1, false, GATED>, G>(a, p, st);
-    if (!a.x_half) return q4_launch_form<Q4Floats<2, false, GATED>, G>(a, p, st);
-    if (p.form == 16) return q4_launch_form<Q4Floats<2, true, GATED>, G>(a, p, st);
-    return q4_launch_form<Q4Floats<4, true, GATED>, G>(a, p, st);
+        return a.x_half ? q4_launch_form<Q4Floats<1, true, GATED>, G, MINIMA>(a, p, st)
+                        : q4_launch_form<Q4Floats<1, false, GATED>, G, MINIMA>(a, p, st);
+    if (!a.x_half) return q4_launch_form<Q4Floats<2, false, GATED>, G, MINIMA>(a, p, st);
+    if (p.form == 16) return q4_launch_form<Q4Floats<2, true, GATED>, G, MINIMA>(a, p, st);
+    return q4_launch_form<Q4Floats<4, true, GATED>, G, MINIMA>(a, p, st);
 }
 
-template <int G>
+template <int G, bool MINIMA>
 int q4_launch(const Q4Args& a, const Q4Plan& p, cudaStream_t st) {
-    return a.gate ? q4_launch_rows<true, G>(a, p, st) : q4_launch_rows<false, G>(a, p, st);
+    return a.gate ? q4_launch_rows<true, G, MINIMA>(a, p, st) : q4_launch_rows<false, G, MINIMA>(a, p, st);
 }
 
 }  // namespace sdb

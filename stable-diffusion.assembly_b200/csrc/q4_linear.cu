@@ -56,14 +56,14 @@ bool chain_ok(const sdb_chain* c, const sdb_tensor* dst, bool gated) {
 //
 // With up to four rows x is cheap and the weights are all: eight warps share a tile, so that a round is a long
 // run of memory (8192 -> 28672, one row: 33.0 us; four warps 35.0, sixteen 34.9).  Up to eight rows likewise (five
-// rows 71.8; four CTAs and one warp 130), but where a CTA walks one or two tiles' groups the splitting of FP32 rows is
+// rows 72; four CTAs and one warp 130), but where a CTA walks one or two tiles' groups the splitting of FP32 rows is
 // what it does: the CTAs of a cluster split them between them (8 rows of 4096 -> 4096: four CTAs 11.3, one 12.1; of
 // FP16 8.9 and 8.0).  So do those of more rows, with one warp a tile (16 rows of 4096 -> 4096: four CTAs 14.9, one
 // 21.9).  Short rows are no cluster's (1280 -> 20160, 16 rows: one CTA and one warp a tile 24.6, two warps 26.4, two
 // CTAs 28.4; 8 rows: four warps 17.1, eight 17.5), and two matrices, whose sums take the registers, share less
 // (1280 -> 5120, 5 rows: two warps 11.7, one 12.3, eight 12.9; 16 rows at a time: 16 rows with two warps, 32 with one
 // 29.8, with two 36.8).  FP32 rows, three columns each, are taken 16 at a time, FP16 rows 32 (4096 -> 4096: 32 FP32
-// rows 22.1 us, taken at once 43.5, 77 rows 64.6 and 92.9; 77 FP16 rows 44.1).  And where the tiles leave most SMs
+// rows 22.1 us, taken at once 43.5, 77 rows 64.6 and 92.9; 77 FP16 rows 41.5).  And where the tiles leave most SMs
 // idle, more warps share one (320 -> 1280, two rows: sixteen 4.3 us, eight 4.7).
 Q4Plan plan(const Q4Args& a) {
     Q4Plan p{};
@@ -96,7 +96,6 @@ int run(const sdb_q4* w, const sdb_q4* gate, const sdb_tensor* x, const sdb_tens
     a.gate = gate ? static_cast<const uint8_t*>(gate->data) : nullptr;
     a.tiles = v.tiles;
     a.kblocks = v.kblocks;
-    a.minimum = static_cast<uint8_t>(v.minimum);
     a.k = static_cast<int>(v.k);
     a.n = static_cast<int>(v.n);
     a.x = x->data;
@@ -119,9 +118,12 @@ int run(const sdb_q4* w, const sdb_q4* gate, const sdb_tensor* x, const sdb_tens
     a.chain = make_chain(chain);
     if (a.rows == 0) return SDB_OK;
     const Q4Plan p = plan(a);
-    if (w->group == 32) return q4_launch<32>(a, p, st);
-    if (w->group == 64) return q4_launch<64>(a, p, st);
-    return q4_launch<128>(a, p, st);
+    if (w->minimum) {
+        if (w->group == 32) return q4_launch<32, true>(a, p, st);
+        return w->group == 64 ? q4_launch<64, true>(a, p, st) : q4_launch<128, true>(a, p, st);
+    }
+    if (w->group == 32) return q4_launch<32, false>(a, p, st);
+    return w->group == 64 ? q4_launch<64, false>(a, p, st) : q4_launch<128, false>(a, p, st);
 }
 
 }  // namespace

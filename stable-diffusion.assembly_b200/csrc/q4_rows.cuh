@@ -1,7 +1,8 @@
 // The kernel of the linear layers of a few rows with 4-bit weights (q4.cuh).
 //
-//   y[m][n] = sum_g d[n][g] S + (min[n][g] + 8 d[n][g]) sum_{k in g} x[m][k],
-//   S = sum_{k in g} (q[n][k] - 8) x[m][k]
+//   y[m][n] = sum_g d[n][g] S + o[n][g] sum_{k in g} x[m][k],
+//   S = sum_{k in g} (q[n][k] - z[n][g]) x[m][k],
+// z = 8 and o = 0, or with a minimum z the code nearest to 0, o = min + d z.
 //
 // The weights' bytes are the work: each is read once for up to 32 rows of x.
 // The 16 weight rows of a tile are the M of an mma and the rows of x its N; S
@@ -13,24 +14,25 @@
 //   two and split into two integers of 22 bits, three signed base-256 digits
 //   each: six columns of an integer product (m16n8k32, s8 x s8).  A nibble at
 //   the top of its byte is the operand 16 (q - 8): three instructions unpack
-//   eight weights.  The sum is exact; it starts from 0x4b400000, so that its
+//   eight weights (8 - z times a column's sum makes them q - z).  The sum is
+//   exact; it starts from 0x4b400000, so that its
 //   bits, read as FP32, are 1.5 * 2^23 + 16 S, and one subtraction makes it a
-//   number (|16 S| <= 2^21).  Six digits hold the numbers down to 2^-19 of the
+//   number (|16 S| < 2^22).  Six digits hold the numbers down to 2^-19 of the
 //   k-block's greatest; a k-block with smaller ones (0 apart), or at the ends of
 //   FP32's range, or with an infinity or a NaN, is taken as below.
 // Pairs (two to four FP32 rows).  A row is the sum of three BF16 columns, each
 //   of which takes the next eight of a number's 24 bits, and none has a range to
-//   fall out of; two rows' columns are six of a product's eight (m16n8k16).  q - 8
-//   is exact: a nibble is 128 + q in BF16, less 136.
+//   fall out of; two rows' columns are six of a product's eight (m16n8k16).  q - z
+//   is exact: a nibble is 128 + q in BF16, less 128 + z.
 // Floats (more rows, and all FP16 rows but one).  FP16 rows are one column each
 //   as they are; FP32 rows three BF16 columns, in products of eight rows' first,
 //   second and third parts.  The first parts' sums are apart from the others',
 //   which are 2^-8 of them.
 //
 // (Digits unpack a weight in a third of the instructions and take one row of
-// 8192 -> 28672 in 29.3 us where a pair takes 38; two rows' twelve columns would
-// be two products, 43 us for a pair's 42.  A product of eight rows' parts for two
-// rows: 52.)
+// 8192 -> 28672 in 28.6 us where a pair takes 38; two rows' twelve columns would
+// be two products, 43 us for a pair's 42.  Four rows take 56 us in pairs, 70 in
+// a product of eight rows' parts.)
 //
 // A CTA has 8 or 16 working warps: WR tiles of rows side by side, WK warps to a
 // tile that share its k-blocks, and up to eight CTAs of a cluster that share
@@ -73,7 +75,6 @@ struct Q4Args {
     int chunk;                 // k-blocks of x held at a time, a multiple of WK unless all of them
     uint8_t wk_log, wr_log;    // WK = 1 << wk_log warps to a tile, WR = 1 << wr_log tiles
     uint8_t cluster_log;       // CTAs that share a tile's k-blocks
-    uint8_t minimum;
     const void* x;
     long long xnb[3];          // strides of rows in elements (dims 1..3)
     int k;
@@ -269,6 +270,28 @@ __device__ __forceinline__ uint64_t q4_fma2(uint64_t a, uint64_t b, uint64_t c) 
 
 // ---- operands
 
+// The code nearest to 0 of rows g and g + 8 of a group, z, and what remains there, o = m + d z:
+//   value = d (q - z) + o.
+// With a minimum z is -m / d rounded and held to the codes, so that |o| <= |d| / 2, or o and all d (q - z) have one
+// sign: neither term is far above the value, and a weight of 0 is two zeros.  (With 8 for all, or with d q + m as it
+// stands, a great number of x whose weight is 0 would come in twice, with opposite signs.)
+struct Q4Zero {
+    uint32_t z[2] = {8, 8};
+    float o[2] = {0.0f, 0.0f};
+    __device__ __forceinline__ void of(float2 d, float2 m) {
+        const float ds[2] = {d.x, d.y}, ms[2] = {m.x, m.y};
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float inverse;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(ds[r]));
+            // (d = 0 makes it infinite or NaN, which the bounds turn into a code)
+            const float near = fminf(fmaxf(-ms[r] * inverse, 0.0f), 15.0f) + 12582912.0f;  // its last bits an integer
+            z[r] = __float_as_uint(near) & 15u;
+            o[r] = fmaf(ds[r], near - 12582912.0f, ms[r]);
+        }
+    }
+};
+
 // An integer below 2^m in the low bits of a number whose mantissa's last bit is worth 1 is that power of two plus
 // the integer, so a nibble becomes a number by one logic operation and a subtraction.
 // (u & MASK) ^ FLIP: two nibbles, code - 8 in four bits, made codes in such numbers.
@@ -279,27 +302,31 @@ __device__ __forceinline__ uint32_t q4_nibbles(uint32_t u) {
     return v;
 }
 
-// FP16: nibbles at bits 0 and 16: 1024 + q, less 1032.
-__device__ __forceinline__ uint32_t q4_low(uint32_t u) {
+// FP16: nibbles at bits 0 and 16: 1024 + q, less 1024 + z.
+__device__ __forceinline__ uint32_t q4_low(uint32_t u, uint32_t less) {
     uint32_t v;
-    asm("sub.f16x2 %0, %1, %2;" : "=r"(v) : "r"(q4_nibbles<0x000f000fu, 0x64086408u>(u)), "r"(0x64086408u));
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(v) : "r"(q4_nibbles<0x000f000fu, 0x64086408u>(u)), "r"(less));
     return v;
 }
+__device__ __forceinline__ uint32_t q4_less_low(uint32_t z) { return 0x64006400u + z * 0x00010001u; }
 
-__device__ __forceinline__ uint32_t q4_high(uint32_t u) {  // at bits 4 and 20: (1024 + 16 q) / 16, less 72
+// At bits 4 and 20: (1024 + 16 q) / 16, less 64 + z.
+__device__ __forceinline__ uint32_t q4_high(uint32_t u, uint32_t less) {
     uint32_t v;
     asm("fma.rn.f16x2 %0, %1, %2, %3;"
         : "=r"(v)
-        : "r"(q4_nibbles<0x00f000f0u, 0x64806480u>(u)), "r"(0x2c002c00u), "r"(0xd480d480u));
+        : "r"(q4_nibbles<0x00f000f0u, 0x64806480u>(u)), "r"(0x2c002c00u), "r"(less));
     return v;
 }
+__device__ __forceinline__ uint32_t q4_less_high(uint32_t z) { return 0xd400d400u + z * 0x00100010u; }
 
-// BF16: nibbles at bits 0 and 16: 128 + q, less 136.
-__device__ __forceinline__ uint32_t q4_bf16(uint32_t u) {
+// BF16: nibbles at bits 0 and 16: 128 + q, less 128 + z.
+__device__ __forceinline__ uint32_t q4_bf16(uint32_t u, uint32_t less) {
     uint32_t v;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(q4_nibbles<0x000f000fu, 0x43084308u>(u)), "r"(0x43084308u));
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(q4_nibbles<0x000f000fu, 0x43084308u>(u)), "r"(less));
     return v;
 }
+__device__ __forceinline__ uint32_t q4_less_bf16(uint32_t z) { return 0x43004300u + z * 0x00010001u; }
 
 // c = a b, or c += a b, of FP16 (HALF) or BF16 operands.
 template <bool HALF, bool FIRST>
@@ -319,12 +346,12 @@ __device__ __forceinline__ void q4_mma(float (&c)[4], const uint32_t (&a)[4], ui
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
 
-// The operand of 16 columns out of words of rows g and g + 8.
-__device__ __forceinline__ void q4_bf16_words(uint32_t (&a)[4], uint32_t u0, uint32_t u1) {
-    a[0] = q4_bf16(u0);
-    a[1] = q4_bf16(u1);
-    a[2] = q4_bf16(u0 >> 4);
-    a[3] = q4_bf16(u1 >> 4);
+// The operand of 16 columns, q - z, out of words of rows g and g + 8.
+__device__ __forceinline__ void q4_bf16_words(uint32_t (&a)[4], uint32_t u0, uint32_t u1, const uint32_t (&less)[2]) {
+    a[0] = q4_bf16(u0, less[0]);
+    a[1] = q4_bf16(u1, less[1]);
+    a[2] = q4_bf16(u0 >> 4, less[0]);
+    a[3] = q4_bf16(u1 >> 4, less[1]);
 }
 
 // An FP32 row's k-block as three BF16 columns, x = a[0] + a[1] + a[2], whole: each takes the next eight bits at
@@ -363,16 +390,16 @@ __device__ __forceinline__ float q4_power(int n) { return __uint_as_float(static
 constexpr float kQ4Magic = 12582912.0f;
 constexpr uint32_t kQ4MagicBits = 0x4b400000u;
 
-// Three signed base-256 digits each of four such integers into three columns, a lane's word of each: adding 128 to
-// the lower two makes the digits the integer's bytes.
-__device__ __forceinline__ void q4_put_digits(const float (&n)[4], uint32_t* to) {
+// Three signed base-256 digits each of four such integers, a word of each column: adding 128 to the lower two makes
+// the digits the integer's bytes.
+__device__ __forceinline__ void q4_digits(const float (&n)[4], uint32_t* words) {
     uint32_t v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (__float_as_uint(n[i]) + (0x8080u - kQ4MagicBits)) ^ 0x8080u;
     const uint32_t l01 = __byte_perm(v[0], v[1], 0x5140), l23 = __byte_perm(v[2], v[3], 0x5140);
-    to[0] = __byte_perm(l01, l23, 0x5410);
-    to[8] = __byte_perm(l01, l23, 0x7632);
-    to[16] = __byte_perm(__byte_perm(v[0], v[1], 0x0062), __byte_perm(v[2], v[3], 0x0062), 0x5410);
+    words[0] = __byte_perm(l01, l23, 0x5410);
+    words[1] = __byte_perm(l01, l23, 0x7632);
+    words[2] = __byte_perm(__byte_perm(v[0], v[1], 0x0062), __byte_perm(v[2], v[3], 0x0062), 0x5410);
 }
 
 template <bool GATED_>
@@ -389,29 +416,32 @@ struct Q4Digits {
     static constexpr int kRow = 4 * kSlice;      // of a k-block
     static constexpr int kWide = 288;            // a column of a row that is not digits
 
-    // Shared memory of `chunk` k-blocks: the columns; each row's factor, twice; the scale of a row that is not digits,
-    // else 0; each row's sums over the groups.
-    static __host__ __device__ int block_bytes(int, int ng) { return kRow + 12 + 4 * ng; }
-    static constexpr int kTail = 80;             // what the lanes of columns 6 and 7 read past the last; then their factor
+    // Shared memory of `chunk` k-blocks: the columns; the factor, twice; the scale of a k-block that is not digits,
+    // else 0; with a minimum the sums over each group of each column's digits and of x.
+    static __host__ __device__ int block_bytes(int, int ng) { return kRow + 12 + 28 * ng; }
+    // What the lanes of columns 6 and 7 read past the last, their factor, and what aligns the sums.
+    static constexpr int kTail = 88;
     uint8_t* frags;
     float2* factors;
     const float2* own;  // the lane's, of columns 2 t and 2 t + 1: 0 for columns 6 and 7
     int own_step;
     float* scales;
+    int2* column_sums;  // of a group's three pairs of columns
     float* sums;
-    __device__ __forceinline__ Q4Digits(const Q4Args& a, uint8_t* x, int) {
+    __device__ __forceinline__ Q4Digits(const Q4Args& a, uint8_t* x, int, int ng) {
         frags = x;
-        factors = reinterpret_cast<float2*>(x + a.chunk * kRow + kTail);
+        factors = reinterpret_cast<float2*>(x + a.chunk * kRow + 80);
         const bool last = (threadIdx.x & 3) == 3;
         own = last ? factors - 1 : factors;
         own_step = last ? 0 : 1;
         scales = reinterpret_cast<float*>(factors + a.chunk);
-        sums = scales + a.chunk;
+        column_sums = reinterpret_cast<int2*>(scales + a.chunk + (a.chunk & 1));
+        sums = reinterpret_cast<float*>(column_sums + 3 * ng * a.chunk);
     }
 
     // A slice of 32 columns of x is the six columns of its digits, 32 bytes each, a lane's four numbers a word of each.
     // read() once the numbers are on their way.  Returns whether the warp saw a row that is not digits.
-    template <int G, class Read>
+    template <int G, bool MINIMA, class Read>
     __device__ __forceinline__ bool split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Read read) const {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
@@ -441,11 +471,14 @@ struct Q4Digits {
                 left |= fabsf(n[i]) < least && n[i] != 0.0f;
             }
             const bool wide = __any_sync(~0u, left);
+            uint32_t words[6];
+            q4_digits(first, words);
+            q4_digits(second, words + 3);
             uint8_t* row = frags + b * kRow;
             if (store && !wide) {
                 uint32_t* to = reinterpret_cast<uint32_t*>(row + (lane >> 3) * kSlice) + (lane & 7);
-                q4_put_digits(first, to);
-                q4_put_digits(second, to + 24);
+#pragma unroll
+                for (int c = 0; c < 6; ++c) to[8 * c] = words[c];
             } else if (store) {
                 q4_put_three(x, top, row, kWide);
             }
@@ -457,9 +490,25 @@ struct Q4Digits {
                 scales[b] = wide ? q4_three_scale(top) : 0.0f;
             }
             seen |= wide;
-            if (a.minimum) {
+            if constexpr (MINIMA) {
                 const float s = q4_group_sum<G>(x);
-                if (store && lane % (G / 4) == 0) sums[b * NG + lane / (G / 4)] = s;
+                // A sum of up to 128 digits has 15 bits: two columns' in a word.
+                int pairs[3];
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {
+                    pairs[p] = __dp4a(static_cast<int>(words[2 * p]), 0x01010101, 0) +
+                               __dp4a(static_cast<int>(words[2 * p + 1]), 0x01010101, 0) * 65536;
+                    for (int o = 1; o < G / 4; o <<= 1) pairs[p] += __shfl_xor_sync(~0u, pairs[p], o);
+                }
+                if (store && lane % (G / 4) == 0) {
+                    const int at = b * NG + lane / (G / 4);
+                    sums[at] = s;
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) {
+                        const int low = static_cast<short>(pairs[p]);
+                        column_sums[3 * at + p] = make_int2(low, (pairs[p] - low) >> 16);
+                    }
+                }
             }
         });
         return seen;
@@ -471,7 +520,8 @@ struct Q4Digits {
         for (int i = 0; i < kTiles; ++i) acc[i][0] = acc[i][1] = 0;
     }
 
-    // c = a b + (first, first, first, first), or c += a b.
+    // c = a b + (first, first, first, first), or c += a b.  With a minimum a product begins from what makes its weights
+    // q - z: 16 (8 - z) times its column's sum, exact like the rest (|16 (q - z)| <= 240 leaves |sum| < 2^22).
     template <bool FIRST>
     static __device__ __forceinline__ void mma(int (&c)[4], const uint32_t (&a)[4], uint2 b) {
         if constexpr (FIRST)
@@ -490,7 +540,7 @@ struct Q4Digits {
 
     // A k-block that is not digits, its three BF16 columns one product.  Its sums, whole, take the place of column 7,
     // lane (g, 3).
-    template <int G>
+    template <int G, bool MINIMA>
     __device__ __forceinline__ void wide_product(const Q4Stage<G> (&st)[kTiles], int at) {
         constexpr int NG = 128 / G, SL = 4 / NG;
         const int lane = threadIdx.x & 31;
@@ -507,17 +557,20 @@ struct Q4Digits {
             float sum[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
+                const float2 d = Q4Stage<G>::pick(st[i].d, g);
+                Q4Zero zero;
+                if (MINIMA) zero.of(d, Q4Stage<G>::pick(st[i].m, g));
+                const uint32_t less[2] = {q4_less_bf16(zero.z[0]), q4_less_bf16(zero.z[1])};
                 float c[4];
 #pragma unroll
                 for (int s = 0; s < 2 * SL; ++s) {
                     const int j = g * SL + s / 2, h = s % 2;
                     uint32_t av[4];
-                    q4_bf16_words(av, u[0][j] >> (8 * h), u[1][j] >> (8 * h));
+                    q4_bf16_words(av, u[0][j] >> (8 * h), u[1][j] >> (8 * h), less);
                     const uint2 b = *reinterpret_cast<const uint2*>(f + (2 * j + h) * 32);
                     if (s == 0) q4_mma<false, true>(c, av, b);
                     else q4_mma<false, false>(c, av, b);
                 }
-                const float2 d = Q4Stage<G>::pick(st[i].d, g);
                 sum[0] = fmaf(d.x, fmaf(first, c[0], second * c[1]), sum[0]);
                 sum[1] = fmaf(d.y, fmaf(first, c[2], second * c[3]), sum[1]);
             }
@@ -532,8 +585,8 @@ struct Q4Digits {
     }
 
     // One k-block, the chunk's at `at`.
-    template <int G>
-    __device__ __forceinline__ void product(const Q4Stage<G> (&st)[kTiles], int at, bool minima) {
+    template <int G, bool MINIMA>
+    __device__ __forceinline__ void product(const Q4Stage<G> (&st)[kTiles], int at) {
         constexpr int NG = 128 / G, SL = 4 / NG;  // slices of 32 a group
         const int lane = threadIdx.x & 31;
         const uint8_t* f = frags + at * kRow + lane * 8;
@@ -549,6 +602,7 @@ struct Q4Digits {
         for (int g = 0; g < NG; ++g) {
             uint32_t av[kTiles][SL][4];
             uint64_t d0[kTiles], d1[kTiles];
+            Q4Zero zero[kTiles];
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
@@ -562,6 +616,7 @@ struct Q4Digits {
                 const float2 d = Q4Stage<G>::pick(st[i].d, g);
                 d0[i] = q4_pair(d.x, d.x);
                 d1[i] = q4_pair(d.y, d.y);
+                if (MINIMA) zero[i].of(d, Q4Stage<G>::pick(st[i].m, g));
             }
             uint2 b[SL];
 #pragma unroll
@@ -569,25 +624,28 @@ struct Q4Digits {
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
                 int c[4];
-                mma<true>(c, av[i][0], b[0]);
+                if (MINIMA) {
+                    const int2 x = column_sums[3 * (at * NG + g) + min(lane & 3, 2)];
+                    const int k0 = 16 * (8 - static_cast<int>(zero[i].z[0])), k1 = 16 * (8 - static_cast<int>(zero[i].z[1]));
+                    c[0] = k0 * x.x + 0x4b400000;
+                    c[1] = k0 * x.y + 0x4b400000;
+                    c[2] = k1 * x.x + 0x4b400000;
+                    c[3] = k1 * x.y + 0x4b400000;
+                    mma<false>(c, av[i][0], b[0]);
+                    // o sum x, whole, in column 7's place.
+                    const uint64_t v = q4_pair(0.0f, sums[at * NG + g]);
+                    const bool mine = (lane & 3) == 3;
+                    acc[i][0] = q4_fma2(q4_pair(0.0f, mine ? zero[i].o[0] : 0.0f), v, acc[i][0]);
+                    acc[i][1] = q4_fma2(q4_pair(0.0f, mine ? zero[i].o[1] : 0.0f), v, acc[i][1]);
+                } else {
+                    mma<true>(c, av[i][0], b[0]);
+                }
 #pragma unroll
                 for (int s = 1; s < SL; ++s) mma<false>(c, av[i][s], b[s]);
                 const uint64_t v0 = q4_add2(q4_pair(__int_as_float(c[0]), __int_as_float(c[1])), magic);
                 const uint64_t v1 = q4_add2(q4_pair(__int_as_float(c[2]), __int_as_float(c[3])), magic);
                 part[i][0] = g == 0 ? q4_mul2(d0[i], v0) : q4_fma2(d0[i], v0, part[i][0]);
                 part[i][1] = g == 0 ? q4_mul2(d1[i], v1) : q4_fma2(d1[i], v1, part[i][1]);
-            }
-            if (minima) {
-                // (m + 8 d) sum x, whole, in column 7's place.
-                const uint64_t v = q4_pair(0.0f, sums[at * NG + g]);
-#pragma unroll
-                for (int i = 0; i < kTiles; ++i) {
-                    const float2 d = Q4Stage<G>::pick(st[i].d, g), mn = Q4Stage<G>::pick(st[i].m, g);
-                    const float o0 = (lane & 3) == 3 ? fmaf(8.0f, d.x, mn.x) : 0.0f;
-                    const float o1 = (lane & 3) == 3 ? fmaf(8.0f, d.y, mn.y) : 0.0f;
-                    acc[i][0] = q4_fma2(q4_pair(0.0f, o0), v, acc[i][0]);
-                    acc[i][1] = q4_fma2(q4_pair(0.0f, o1), v, acc[i][1]);
-                }
             }
         }
         const uint64_t v = *reinterpret_cast<const uint64_t*>(own + at * own_step);
@@ -627,7 +685,7 @@ struct Q4Pairs {
     static constexpr int kTiles = GATED ? 2 : 1;
     static constexpr int kLaneSums = NP;
     static constexpr int kWarps = !GATED ? 16 : 8;
-    static constexpr int kRun = NP == 1 ? 2 : 1, kRing = 3;  // k-blocks of a warp a round; rounds on their way
+    static constexpr int kRun = 2, kRing = 3;   // k-blocks of a warp a round; rounds on their way
     static constexpr bool kFinisher = true, kWideRows = false;
     static constexpr int kColumn = 288;         // bytes: 8 slices x 32, and a step of 8 banks
 
@@ -640,7 +698,7 @@ struct Q4Pairs {
     int part_bytes, x_bytes;
     float* scales;          // of a row's k-block
     float* sums;            // of a row's groups
-    __device__ __forceinline__ Q4Pairs(const Q4Args& a, uint8_t* x, int tokens) {
+    __device__ __forceinline__ Q4Pairs(const Q4Args& a, uint8_t* x, int tokens, int) {
         const int lane = threadIdx.x & 31, g = lane >> 2;
         frags = x;
         part_bytes = tokens * kColumn;
@@ -651,7 +709,7 @@ struct Q4Pairs {
         sums = scales + a.chunk * kTokens;
     }
 
-    template <int G, class Read>
+    template <int G, bool MINIMA, class Read>
     __device__ __forceinline__ bool split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Read read) const {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
@@ -665,7 +723,7 @@ struct Q4Pairs {
             const uint32_t top = q4_top(x);
             if (store) q4_put_three(x, top, first(b, m), part_bytes);
             if (store && lane == 0) scales[b * kTokens + m] = q4_three_scale(top);
-            if (a.minimum) {
+            if constexpr (MINIMA) {
                 const float s = q4_group_sum<G>(x);
                 if (store && lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
             }
@@ -683,8 +741,8 @@ struct Q4Pairs {
                 for (int c = 0; c < 4; ++c) acc[i][t][c] = 0.0f;
     }
 
-    template <int G>
-    __device__ __forceinline__ void product(const Q4Stage<G> (&st)[kTiles], int at, bool minima) {
+    template <int G, bool MINIMA>
+    __device__ __forceinline__ void product(const Q4Stage<G> (&st)[kTiles], int at) {
         constexpr int NG = 128 / G, SL = 4 / NG;
         const int lane = threadIdx.x & 31;
         const uint8_t* f = column + at * x_bytes;
@@ -692,6 +750,14 @@ struct Q4Pairs {
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             float s[kTiles][NP][4];
+            Q4Zero zero[kTiles];
+            uint32_t less[kTiles][2];
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+                if (MINIMA) zero[i].of(Q4Stage<G>::pick(st[i].d, g), Q4Stage<G>::pick(st[i].m, g));
+                less[i][0] = q4_less_bf16(zero[i].z[0]);
+                less[i][1] = q4_less_bf16(zero[i].z[1]);
+            }
 #pragma unroll
             for (int j = g * SL; j < (g + 1) * SL; ++j) {
 #pragma unroll
@@ -701,7 +767,7 @@ struct Q4Pairs {
                     for (int i = 0; i < kTiles; ++i) {
                         const uint32_t u0 = j == 0 ? st[i].lo.x : j == 1 ? st[i].lo.y : j == 2 ? st[i].lo.z : st[i].lo.w;
                         const uint32_t u1 = j == 0 ? st[i].hi.x : j == 1 ? st[i].hi.y : j == 2 ? st[i].hi.z : st[i].hi.w;
-                        q4_bf16_words(av[i], u0 >> (8 * h), u1 >> (8 * h));
+                        q4_bf16_words(av[i], u0 >> (8 * h), u1 >> (8 * h), less[i]);
                     }
 #pragma unroll
                     for (int t = 0; t < NP; ++t) {
@@ -725,12 +791,11 @@ struct Q4Pairs {
                         part[i][t][c] = g == 0 ? scale * s[i][t][c] : fmaf(scale, s[i][t][c], part[i][t][c]);
                     }
             }
-            if (minima) {
-                // (m + 8 d) sum x, in one of the lanes whose sums meet.
+            if (MINIMA) {
+                // o sum x, in one of the lanes whose sums meet.
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i) {
-                    const float2 d = Q4Stage<G>::pick(st[i].d, g), mn = Q4Stage<G>::pick(st[i].m, g);
-                    const float o0 = lane & 3 ? 0.0f : fmaf(8.0f, d.x, mn.x), o1 = lane & 3 ? 0.0f : fmaf(8.0f, d.y, mn.y);
+                    const float o0 = lane & 3 ? 0.0f : zero[i].o[0], o1 = lane & 3 ? 0.0f : zero[i].o[1];
 #pragma unroll
                     for (int t = 0; t < NP; ++t) {
                         const float2 v = *reinterpret_cast<const float2*>(sums + (at * NG + g) * kTokens + 2 * t);
@@ -751,7 +816,7 @@ struct Q4Pairs {
                 for (int c = 0; c < 4; ++c) acc[i][t][c] = fmaf(c & 1 ? v.y : v.x, part[i][t][c], acc[i][t][c]);
         }
     }
-    template <int G>
+    template <int G, bool MINIMA>
     __device__ __forceinline__ void wide_product(const Q4Stage<G> (&)[kTiles], int) {}
 
     // The lane's sum c of tile i: row lane / 4 (lane odd: + 8) of row 2 c + (lane / 2) % 2 of x, over its parts' lanes.
@@ -781,7 +846,7 @@ struct Q4Floats {
     static constexpr int kParts = HALF ? 1 : 3;  // columns of a row
     static constexpr int kProducts = kParts * T;
     static constexpr int kWarps = T <= 2 && !GATED ? 16 : 8;
-    static constexpr int kRun = 1, kRing = GATED ? 3 : 4;
+    static constexpr int kRun = T == 1 && HALF ? 2 : 1, kRing = kRun == 2 || GATED ? 3 : 4;
     static constexpr bool kFinisher = false, kWideRows = false;
 
     static constexpr int kColumn = 288;  // bytes: 8 slices x 32, and a step of 8 banks
@@ -797,7 +862,7 @@ struct Q4Floats {
     int part_bytes, x_bytes;  // from a part to the next, of a k-block
     float* scales;            // of a row's k-block
     float* sums;              // of a row's groups
-    __device__ __forceinline__ Q4Floats(const Q4Args& a, uint8_t* x, int tokens) {
+    __device__ __forceinline__ Q4Floats(const Q4Args& a, uint8_t* x, int tokens, int) {
         frags = x;
         part_bytes = (T == 1 ? tokens : 8) * kColumn;
         x_bytes = columns(tokens) * kColumn;
@@ -805,7 +870,7 @@ struct Q4Floats {
         sums = scales + a.chunk * kTokens;
     }
 
-    template <int G, class Read>
+    template <int G, bool MINIMA, class Read>
     __device__ __forceinline__ bool split(const Q4Args& a, int m0, int tokens, int kb0, int kb1, Read read) const {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
@@ -832,7 +897,7 @@ struct Q4Floats {
                 if (store) q4_put_three(x, top, to, part_bytes);
                 if (store && lane == 0) scales[b * kTokens + m] = q4_three_scale(top);
             }
-            if (a.minimum) {
+            if constexpr (MINIMA) {
                 const float s = q4_group_sum<G>(x);
                 if (store && lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
             }
@@ -848,14 +913,16 @@ struct Q4Floats {
             for (int c = 0; c < kLaneSums; ++c) acc[i][c] = 0.0f;
     }
 
-    template <int G>
-    __device__ __forceinline__ void product(const Q4Stage<G> (&st)[kTiles], int at, bool minima) {
+    template <int G, bool MINIMA>
+    __device__ __forceinline__ void product(const Q4Stage<G> (&st)[kTiles], int at) {
         constexpr int NG = 128 / G;
         const int lane = threadIdx.x & 31;
         const uint8_t* f = frags + at * x_bytes + (lane >> 2) * kColumn + (lane & 3) * 8;
         constexpr int kSums = HALF ? 1 : 2;  // the first parts', and the others', which are far smaller
         float part[kTiles][kLaneSums];       // the k-block's sums, in its rows' scales
         float s[kTiles][T][kSums][4];        // a group's sums
+        Q4Zero zero[kTiles];
+        uint32_t less[kTiles][2], less_high[kTiles][2];
         uint32_t w[kTiles][2][4];
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
@@ -864,6 +931,18 @@ struct Q4Floats {
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            if (j % (4 / NG) == 0 && (j == 0 || MINIMA)) {
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) {
+                    const int g = j / (4 / NG);
+                    if (MINIMA) zero[i].of(Q4Stage<G>::pick(st[i].d, g), Q4Stage<G>::pick(st[i].m, g));
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        less[i][r] = HALF ? q4_less_low(zero[i].z[r]) : q4_less_bf16(zero[i].z[r]);
+                        if (HALF) less_high[i][r] = q4_less_high(zero[i].z[r]);
+                    }
+                }
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t av[kTiles][4];
@@ -871,12 +950,12 @@ struct Q4Floats {
                 for (int i = 0; i < kTiles; ++i) {
                     const uint32_t u0 = w[i][0][j] >> (8 * h), u1 = w[i][1][j] >> (8 * h);
                     if constexpr (HALF) {
-                        av[i][0] = q4_low(u0);
-                        av[i][1] = q4_low(u1);
-                        av[i][2] = q4_high(u0);
-                        av[i][3] = q4_high(u1);
+                        av[i][0] = q4_low(u0, less[i][0]);
+                        av[i][1] = q4_low(u1, less[i][1]);
+                        av[i][2] = q4_high(u0, less_high[i][0]);
+                        av[i][3] = q4_high(u1, less_high[i][1]);
                     } else {
-                        q4_bf16_words(av[i], u0, u1);
+                        q4_bf16_words(av[i], u0, u1, less[i]);
                     }
                 }
                 const bool first = j % (4 / NG) == 0 && h == 0;
@@ -906,12 +985,11 @@ struct Q4Floats {
                     part[i][c] = g == 0 ? scale * v : fmaf(scale, v, part[i][c]);
                 }
             }
-            if (minima) {
+            if (MINIMA) {
                 const float* xs = sums + (at * NG + g) * kTokens + (lane & 3) * 2;
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i) {
-                    const float2 d = Q4Stage<G>::pick(st[i].d, g), mn = Q4Stage<G>::pick(st[i].m, g);
-                    const float o0 = fmaf(8.0f, d.x, mn.x), o1 = fmaf(8.0f, d.y, mn.y);
+                    const float o0 = zero[i].o[0], o1 = zero[i].o[1];
 #pragma unroll
                     for (int t = 0; t < T; ++t) {
                         const float2 v = *reinterpret_cast<const float2*>(xs + t * 8);
@@ -934,7 +1012,7 @@ struct Q4Floats {
                     acc[i][4 * t + c] = fmaf(c & 1 ? v.y : v.x, part[i][4 * t + c], acc[i][4 * t + c]);
         }
     }
-    template <int G>
+    template <int G, bool MINIMA>
     __device__ __forceinline__ void wide_product(const Q4Stage<G> (&)[kTiles], int) {}
 
     __device__ __forceinline__ float lane_sum(int i, int c) const { return acc[i][c]; }
@@ -974,7 +1052,9 @@ int q4_fixed_bytes(int block) {
            F::kTail;
 }
 
-template <class F, int G>
+// MINIMA: compiled for itself, so that the products of two k-blocks lie side by side without a branch between (one
+// row of 8192 -> 28672 without a minimum 28.6 us, with the choice made in the loop 31.8).
+template <class F, int G, bool MINIMA>
 __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __grid_constant__ Q4Args a) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
@@ -984,16 +1064,15 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
     const int groups = a.groups, group0 = blockIdx.x >> a.cluster_log, group_step = gridDim.x >> a.cluster_log;
     const int kb_begin = rank * a.range, kb_end = min(kb_begin + a.range, a.kblocks);
     const int m0 = blockIdx.y * F::kTokens, tokens = min(F::kTokens, a.rows - m0);
-    const bool minima = a.minimum != 0;
-    const int block = 1024 + 4096 / G * (minima ? 2 : 1);  // bytes of a tile
-    const int place_bytes = F::kWarps * F::kTiles * F::kRun * block;
+    constexpr int block = 1024 + 4096 / G * (MINIMA ? 2 : 1);  // bytes of a tile
+    constexpr int place_bytes = F::kWarps * F::kTiles * F::kRun * block;
 
     float* red = reinterpret_cast<float*>(smem);
     uint8_t* ring = reinterpret_cast<uint8_t*>(red + q4_red_buffers<F>() * q4_red_floats<F>());
     uint64_t* full = reinterpret_cast<uint64_t*>(ring + F::kRing * place_bytes);
     uint64_t* empty = full + F::kRing;
     volatile int* abort = reinterpret_cast<volatile int*>(empty + F::kRing);
-    F form(a, reinterpret_cast<uint8_t*>(empty + F::kRing) + 16, tokens);
+    F form(a, reinterpret_cast<uint8_t*>(empty + F::kRing) + 16, tokens, MINIMA ? 128 / G : 0);
 
     // The rounds in order: over the row tiles, the chunks of x and their k-blocks.
     int next_group = group0, next_kc = kb_begin, next_kb = kb_begin, brought = 0;
@@ -1051,7 +1130,7 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
             if (!held) {
                 if (started) __syncthreads();  // the chunk before has been read
                 if (worker)
-                    wide = form.template split<G>(a, m0, tokens, kc, kc_end, [&] {
+                    wide = form.template split<G, MINIMA>(a, m0, tokens, kc, kc_end, [&] {
                         if (!started) asm volatile("bar.arrive 1, %0;" ::"n"(32 * (F::kWarps + 1)) : "memory");
                     });
                 started = true;
@@ -1076,11 +1155,11 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
                         Q4Stage<G> stage[F::kTiles];
 #pragma unroll
                         for (int t = 0; t < F::kTiles; ++t)
-                            stage[t].read(tiles + t * (F::kWarps * F::kRun * block) + i * block, lane, minima);
+                            stage[t].read(tiles + t * (F::kWarps * F::kRun * block) + i * block, lane, MINIMA);
                         then(stage, at + i);
                     };
                     auto one = [&](int i) {
-                        staged(i, [&](auto& stage, int k) { form.template product<G>(stage, k, minima); });
+                        staged(i, [&](auto& stage, int k) { form.template product<G, MINIMA>(stage, k); });
                     };
                     if (F::kRun == 2 && count == 2) {  // two k-blocks' chains of products side by side
                         one(0);
@@ -1091,7 +1170,7 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
                     if (F::kWideRows && wide) {
 #pragma unroll 1
                         for (int i = 0; i < count; ++i)
-                            staged(i, [&](auto& stage, int k) { form.template wide_product<G>(stage, k); });
+                            staged(i, [&](auto& stage, int k) { form.template wide_product<G, MINIMA>(stage, k); });
                     }
                     __syncwarp();  // every lane has read its part
                     if (lane == 0) mbar_arrive(empty + place);
@@ -1162,8 +1241,8 @@ struct Q4Plan {
     int shared;    // bytes of shared memory a CTA may take
 };
 
-// Launches the kernel for rows in FP16 or FP32, plain or gated, groups of G.
-template <int G>
+// Launches the kernel for rows in FP16 or FP32, plain or gated, groups of G with MINIMA or without.
+template <int G, bool MINIMA>
 int q4_launch(const Q4Args& a, const Q4Plan& p, cudaStream_t st);
 
 }  // namespace sdb

@@ -697,7 +697,7 @@ def beside_great_numbers(g, rows, k, n, group, kind, great, xt):
     return q, scales, minima, values, x.astype(xt)
 
 
-@pytest.mark.parametrize("kind", ["code"])
+@pytest.mark.parametrize("kind", ["code", "least", "inside"])
 @pytest.mark.parametrize("great", [300.0, 1e4, 1e6, 1e10, 1e20, 1e30])
 @pytest.mark.parametrize("rows", [1, 2, 3, 4, 7, 8, 9, 16, 17, 33])
 def test_great_numbers_that_weigh_nothing(cuda, rows, great, kind):
@@ -709,7 +709,7 @@ def test_great_numbers_that_weigh_nothing(cuda, rows, great, kind):
         check(host(sdb.mul_mat_q4(on_device(cuda, q, scales, minima, group), cuda_tensor(x, cuda))), exact, mag)
 
 
-@pytest.mark.parametrize("kind", ["code"])
+@pytest.mark.parametrize("kind", ["code", "least", "inside"])
 @pytest.mark.parametrize("rows", [1, 2, 3, 8, 9, 17, 33])
 def test_great_half_precision_numbers(cuda, rows, kind):
     import sdb
