@@ -746,30 +746,39 @@ def _packed_chain(chain: Chain | None, tensors: tuple, out, cols: int):
     """The sdb_chain of an operation on out's rows, `cols` columns each, as bytes (None: no chain)."""
     if chain is None:
         return None
-    shape, stride = out.shape, out.stride()
-    steps = chain.steps
-    rows = out.numel()
-    # What the kernel may touch is looked at in every call ...
-    for _, t, nb in steps:
-        if t is not None:
-            _check_operand(t, nb, shape, cols, rows)
-    r = chain.redirect_tensor
-    if r is not None and (r.dtype != out.dtype or r.shape != shape or r.stride() != stride):
+    shape = out.shape
+    steps, r = chain.steps, chain.redirect_tensor
+    if r is not None and (r.dtype != out.dtype or r.shape != shape or r.stride() != out.stride()):
         raise SdbError(INVALID, "a chain's redirect has the output's type, extents and strides")
-    # ... and a chain that is used again as it was is not packed again.
-    key = (chain.from_redirect, [(kind, *nb) for kind, _, nb in steps], [t.data_ptr() for t in tensors], r is None)
+    # A chain that is used again as it was is not described again: the key is all that the checks of operands with
+    # their own strides look at.  The memory behind explicit strides is looked at in every call.
+    own = True
+    places = []
+    for kind, t, nb in steps:
+        if t is None:
+            places.append(kind)
+        elif type(nb) is tuple:
+            places.append((kind, nb, t.data_ptr(), t.shape, t.stride()))
+        else:
+            own = False
+            places.append((kind, *nb, t.data_ptr()))
+    key = (places, cols, shape, None if r is None else r.data_ptr(), chain.from_redirect)
     kept = chain.__dict__.get("_described")
-    if kept is not None and kept[0] == key:
+    if own and kept is not None and kept[0] == key:
         return kept[1]
     if len(steps) > MAX_STEPS:
         raise SdbError(INVALID, "chain longer than 6 steps")
+    rows = out.numel()
     parts = [struct.pack("=i4x", len(steps))]
     for kind, t, nb in steps:
+        if t is not None:
+            _check_operand(t, nb, shape, cols, rows)
+            own = own and nb == _own_strides(t)
         parts.append(_STEP.pack(kind, t.data_ptr() if t is not None else 0, *nb))
     parts.extend([_NO_STEP] * (MAX_STEPS - len(steps)))
-    parts.append(_CHAIN_TAIL.pack(r.data_ptr() if r is not None else 0, 1 if chain.from_redirect else 0))
+    parts.append(_CHAIN_TAIL.pack(key[3] or 0, 1 if chain.from_redirect else 0))
     packed = b"".join(parts)
-    chain._described = (key, packed)
+    chain._described = (key, packed) if own else None
     return packed
 
 
@@ -863,12 +872,15 @@ class Q4:
             raise SdbError(INVALID, "4-bit matrices are on a CUDA device")
         if t.dtype != torch.uint8 or t.shape != (self._size,) or not t.is_contiguous():
             raise SdbError(INVALID, f"a 4-bit matrix's memory is {self._size} dense bytes")
-        self._data = t
+        self._data, self._at = t, None
 
     @property
     def struct(self) -> bytes:
-        """The sdb_q4, made anew for each call: a copy of a matrix has memory of its own."""
-        return _Q4.pack(self._data.data_ptr(), *self._form)
+        """The sdb_q4 of the memory the matrix has now: a copy of a matrix has memory of its own."""
+        at = self._data.data_ptr()
+        if at != self._at:
+            self._packed, self._at = _Q4.pack(at, *self._form), at
+        return self._packed
 
     def values(self, out=None, stream=None):
         """The numbers the matrix stands for, FP32 (n, k) (sdb_q4_dequantize)."""
