@@ -202,7 +202,8 @@ __device__ __forceinline__ float2 row_sum(float2 v, int* buffer) {
 // numbers, aligned), else one by one.  A thread's numbers lie T (runs) apart.
 template <typename TX, typename TY, int V, int T, bool VEC>
 // Registers for 1024 threads an SM: 64 a thread (rows of 8193 to 16384 numbers: 128), more rows at once being worth
-// more than the few words that spill (8 x 4096 x 320 35.7 us, unbounded 40.0; 2 x 4096 x 1280 30.1 and 30.8).
+// more than what spills -- with VEC 24 bytes at most, number by number 8 to 32, 120 (513 to 1280 numbers of FP16) and
+// 192 (4097 to 8192) -- 8 x 4096 x 320 35.7 us, unbounded 40.0; 2 x 4096 x 1280 30.1 and 30.8.
 __global__ void __launch_bounds__(T == 32 ? 256 : T, (V == 8 ? 512 : 1024) / (T == 32 ? 256 : T)) residual_kernel(const __grid_constant__ ResidualArgs a) {
     const int t = T == 32 ? threadIdx.x & 31 : threadIdx.x;
     constexpr int kRows = T == 32 ? 8 : 1;
@@ -340,7 +341,7 @@ void launch(const ResidualArgs& a, bool vec, cudaStream_t st) {
     else if (a.c <= 16384) launch_rows<TX, TY, 8, 512>(a, vec, st);
     else
         residual_rows_kernel<TX, TY>
-            <<<static_cast<unsigned>(std::min<long long>(a.rows, 148LL * 32)), kRowThreads, 0, st>>>(a);
+            <<<static_cast<unsigned>(std::min<long long>(a.rows, current_sm_count() * 32LL)), kRowThreads, 0, st>>>(a);
 }
 
 bool rows_of(const sdb_tensor* t, bool written) {
