@@ -356,8 +356,9 @@ __device__ __forceinline__ void q4_bf16_words(uint32_t (&a)[4], uint32_t u0, uin
 
 // An FP32 row's k-block as three BF16 columns, x = a[0] + a[1] + a[2], whole: each takes the next eight bits at
 // least.  Scaled by 2^24, so that the last parts of the smallest numbers too are normal ones; where `top`, the
-// greatest number's bits, reaches 2^88, by 2^-24, so that no sum overflows before its scale comes.
-__device__ __forceinline__ bool q4_three_great(uint32_t top) { return top >= 0x6b800000u; }
+// greatest number's bits, reaches 2^72, by 2^-24: 128 numbers below 2^72 by codes and a scale of 2^16 sum to less than
+// 2^123 either way, and what lies below 2^-86 beside a number of 2^72 may lose bits.
+__device__ __forceinline__ bool q4_three_great(uint32_t top) { return top >= 0x63800000u; }
 __device__ __forceinline__ float q4_three_scale(uint32_t top) { return q4_three_great(top) ? 0x1p24f : 0x1p-24f; }
 
 // A lane's four numbers are columns 0..3 or 4..7 of the run of eight that lane t = lane / 2 % 4 of a fragment

@@ -770,3 +770,21 @@ def test_the_smallest_numbers(cuda, rows, minimum):
         got = host(sdb.mul_mat_q4(w, cuda_tensor(x, cuda)))
         worst = (np.abs(got - exact) / (oracle.K_B200 * mag + 2.0 ** -143)).max()
         assert worst <= 1, f"{scale}: {worst:.3g} of the bound"
+
+
+@pytest.mark.parametrize("minimum", [False, True])
+@pytest.mark.parametrize("rows", [1, 2, 3, 8, 9, 17, 33])
+def test_sums_near_the_end_of_the_range(cuda, rows, minimum):
+    """Great numbers and great scales: no sum on the way overflows where the output does not."""
+    import sdb
+
+    g = rng(rows)
+    q, scales, minima, _ = made(g, 40, 256, 128, minimum)
+    scales = (np.sign(scales) * g.uniform(20000, 60000, scales.shape)).astype(np.float16)
+    d = np.repeat(scales.astype(np.float64), 128, axis=1)
+    m = np.repeat(minima.astype(np.float64), 128, axis=1) if minimum else -8 * d
+    w = on_device(cuda, q, scales, minima, 128)
+    for exponent in (60, 70, 71, 72, 76, 84, 87, 88, 96):
+        x = np.clip(g.standard_normal((rows, 256)), -1.9, 1.9).astype(np.float32) * np.float32(2.0 ** exponent)
+        exact, mag = oracle.mul_mat_exact(d * q + m, x)
+        check(host(sdb.mul_mat_q4(w, cuda_tensor(x, cuda))), exact, mag)
