@@ -232,10 +232,10 @@ __device__ __forceinline__ uint32_t q4_top(float4 x) {
     return __reduce_max_sync(~0u, max(a, b));
 }
 
-// The sums of a warp's numbers over its groups of G, in every lane.
+// The sums of a warp's numbers, times `up`, over its groups of G, in every lane.
 template <int G>
-__device__ __forceinline__ float q4_group_sum(float4 x) {
-    float s = (x.x + x.y) + (x.z + x.w);
+__device__ __forceinline__ float q4_group_sum(float4 x, float up) {
+    float s = (x.x * up + x.y * up) + (x.z * up + x.w * up);
 #pragma unroll
     for (int o = 1; o < G / 4; o <<= 1) s += __shfl_xor_sync(~0u, s, o);
     return s;
@@ -359,6 +359,7 @@ __device__ __forceinline__ void q4_bf16_words(uint32_t (&a)[4], uint32_t u0, uin
 // greatest number's bits, reaches 2^72, by 2^-24: 128 numbers below 2^72 by codes and a scale of 2^16 sum to less than
 // 2^123 either way, and what lies below 2^-86 beside a number of 2^72 may lose bits.
 __device__ __forceinline__ bool q4_three_great(uint32_t top) { return top >= 0x63800000u; }
+__device__ __forceinline__ float q4_three_up(uint32_t top) { return q4_three_great(top) ? 0x1p-24f : 0x1p24f; }
 __device__ __forceinline__ float q4_three_scale(uint32_t top) { return q4_three_great(top) ? 0x1p24f : 0x1p-24f; }
 
 // A lane's four numbers are columns 0..3 or 4..7 of the run of eight that lane t = lane / 2 % 4 of a fragment
@@ -367,7 +368,7 @@ __device__ __forceinline__ float q4_three_scale(uint32_t top) { return q4_three_
 __device__ __forceinline__ int q4_float_word(int lane) { return (lane >> 3) * 64 + (lane >> 1 & 3) * 8 + (lane & 1) * 4; }
 __device__ __forceinline__ void q4_put_three(float4 x, uint32_t top, uint8_t* to, int column) {
     to += q4_float_word(threadIdx.x & 31);
-    const float up = q4_three_great(top) ? 0x1p-24f : 0x1p24f;
+    const float up = q4_three_up(top);
     float v[4] = {x.x * up, x.z * up, x.y * up, x.w * up};
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
@@ -418,8 +419,9 @@ struct Q4Digits {
     static constexpr int kWide = 288;            // a column of a row that is not digits
 
     // Shared memory of `chunk` k-blocks: the columns; the factor, twice; the scale of a k-block that is not digits,
-    // else 0; with a minimum the sums over each group of each column's digits and of x.
-    static __host__ __device__ int block_bytes(int, int ng) { return kRow + 12 + 28 * ng; }
+    // else 0; with a minimum the sums over each group of each column's digits and of x, of a k-block that is not digits
+    // in that scale, apart from the others'.
+    static __host__ __device__ int block_bytes(int, int ng) { return kRow + 12 + 32 * ng; }
     // What the lanes of columns 6 and 7 read past the last, their factor, and what aligns the sums.
     static constexpr int kTail = 88;
     uint8_t* frags;
@@ -429,6 +431,7 @@ struct Q4Digits {
     float* scales;
     int2* column_sums;  // of a group's three pairs of columns
     float* sums;
+    float* wide_sums;
     __device__ __forceinline__ Q4Digits(const Q4Args& a, uint8_t* x, int, int ng) {
         frags = x;
         factors = reinterpret_cast<float2*>(x + a.chunk * kRow + 80);
@@ -438,6 +441,7 @@ struct Q4Digits {
         scales = reinterpret_cast<float*>(factors + a.chunk);
         column_sums = reinterpret_cast<int2*>(scales + a.chunk + (a.chunk & 1));
         sums = reinterpret_cast<float*>(column_sums + 3 * ng * a.chunk);
+        wide_sums = sums + ng * a.chunk;
     }
 
     // A slice of 32 columns of x is the six columns of its digits, 32 bytes each, a lane's four numbers a word of each.
@@ -460,7 +464,7 @@ struct Q4Digits {
             const uint32_t top = q4_top(x);
             const int e = static_cast<int>(top >> 23);
             // Not digits: smaller numbers; those whose units or sums pass the ends of FP32's range; infinities, NaN.
-            const bool out = e >= 250 || (e < 40 && top != 0);
+            const bool out = e >= 240 || (e < 40 && top != 0);
             const float least = q4_power(max(e, 40) - 146), up = q4_power(147 - max(e, 40));
             const float n[4] = {x.x, x.y, x.z, x.w};
             float first[4], second[4];
@@ -492,7 +496,7 @@ struct Q4Digits {
             }
             seen |= wide;
             if constexpr (MINIMA) {
-                const float s = q4_group_sum<G>(x);
+                const float s = q4_group_sum<G>(x, wide ? q4_three_up(top) : 1.0f);
                 // A sum of up to 128 digits has 15 bits: two columns' in a word.
                 int pairs[3];
 #pragma unroll
@@ -503,7 +507,8 @@ struct Q4Digits {
                 }
                 if (store && lane % (G / 4) == 0) {
                     const int at = b * NG + lane / (G / 4);
-                    sums[at] = s;
+                    sums[at] = wide ? 0.0f : s;
+                    wide_sums[at] = s;
 #pragma unroll
                     for (int p = 0; p < 3; ++p) {
                         const int low = static_cast<short>(pairs[p]);
@@ -549,8 +554,6 @@ struct Q4Digits {
         if (scale == 0.0f) return;
         // The lanes of columns past the third read the third's: their sums go nowhere.
         const uint8_t* f = frags + at * kRow + min(lane >> 2, 2) * kWide + (lane & 3) * 8;
-        // Lane (g, 0) holds columns 0 and 1, lane (g, 1) column 2.
-        const float first = (lane & 3) < 2 ? scale : 0.0f, second = (lane & 3) < 1 ? scale : 0.0f;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
             const uint32_t u[2][4] = {{st[i].lo.x, st[i].lo.y, st[i].lo.z, st[i].lo.w},
@@ -572,15 +575,19 @@ struct Q4Digits {
                     if (s == 0) q4_mma<false, true>(c, av, b);
                     else q4_mma<false, false>(c, av, b);
                 }
-                sum[0] = fmaf(d.x, fmaf(first, c[0], second * c[1]), sum[0]);
-                sum[1] = fmaf(d.y, fmaf(first, c[2], second * c[3]), sum[1]);
+                // Lane (g, 0) holds columns 0 and 1, lane (g, 1) column 2, lane (g, 3) what the minima add.
+                const int t = lane & 3;
+                const float part[2] = {t == 0 ? c[0] + c[1] : t == 1 ? c[0] : 0.0f, t == 0 ? c[2] + c[3] : t == 1 ? c[2] : 0.0f};
+                const float x = MINIMA && t == 3 ? wide_sums[at * NG + g] : 0.0f;
+                sum[0] = fmaf(d.x, part[0], fmaf(zero.o[0], x, sum[0]));
+                sum[1] = fmaf(d.y, part[1], fmaf(zero.o[1], x, sum[1]));
             }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 sum[r] += __shfl_xor_sync(~0u, sum[r], 2);
                 sum[r] += __shfl_xor_sync(~0u, sum[r], 1);
                 const float2 v = q4_unpair(acc[i][r]);
-                acc[i][r] = q4_pair(v.x, v.y + ((lane & 3) == 3 ? sum[r] : 0.0f));
+                acc[i][r] = q4_pair(v.x, (lane & 3) == 3 ? fmaf(scale, sum[r], v.y) : v.y);
             }
         }
     }
@@ -698,7 +705,7 @@ struct Q4Pairs {
     const uint8_t* column;  // the lane's, of the first product
     int part_bytes, x_bytes;
     float* scales;          // of a row's k-block
-    float* sums;            // of a row's groups
+    float* sums;            // of a row's groups, in its scale
     __device__ __forceinline__ Q4Pairs(const Q4Args& a, uint8_t* x, int tokens, int) {
         const int lane = threadIdx.x & 31, g = lane >> 2;
         frags = x;
@@ -725,7 +732,7 @@ struct Q4Pairs {
             if (store) q4_put_three(x, top, first(b, m), part_bytes);
             if (store && lane == 0) scales[b * kTokens + m] = q4_three_scale(top);
             if constexpr (MINIMA) {
-                const float s = q4_group_sum<G>(x);
+                const float s = q4_group_sum<G>(x, q4_three_up(top));
                 if (store && lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
             }
         });
@@ -800,10 +807,10 @@ struct Q4Pairs {
 #pragma unroll
                     for (int t = 0; t < NP; ++t) {
                         const float2 v = *reinterpret_cast<const float2*>(sums + (at * NG + g) * kTokens + 2 * t);
-                        acc[i][t][0] = fmaf(o0, v.x, acc[i][t][0]);
-                        acc[i][t][1] = fmaf(o0, v.y, acc[i][t][1]);
-                        acc[i][t][2] = fmaf(o1, v.x, acc[i][t][2]);
-                        acc[i][t][3] = fmaf(o1, v.y, acc[i][t][3]);
+                        part[i][t][0] = fmaf(o0, v.x, part[i][t][0]);
+                        part[i][t][1] = fmaf(o0, v.y, part[i][t][1]);
+                        part[i][t][2] = fmaf(o1, v.x, part[i][t][2]);
+                        part[i][t][3] = fmaf(o1, v.y, part[i][t][3]);
                     }
                 }
             }
@@ -862,7 +869,7 @@ struct Q4Floats {
     uint8_t* frags;
     int part_bytes, x_bytes;  // from a part to the next, of a k-block
     float* scales;            // of a row's k-block
-    float* sums;              // of a row's groups
+    float* sums;              // of a row's groups, in its scale
     __device__ __forceinline__ Q4Floats(const Q4Args& a, uint8_t* x, int tokens, int) {
         frags = x;
         part_bytes = (T == 1 ? tokens : 8) * kColumn;
@@ -887,6 +894,7 @@ struct Q4Floats {
         asm volatile("cp.async.wait_all;" ::: "memory");
         q4_split<HALF>(a, it, tokens, kb1 - kb0, slot, [&](int b, int m, float4 x, bool store) {
             uint8_t* to = column(b, m);
+            float up = 1.0f;
             if constexpr (HALF) {
                 to += q4_float_word(lane);
                 if (store) {
@@ -895,11 +903,12 @@ struct Q4Floats {
                 }
             } else {
                 const uint32_t top = q4_top(x);
+                up = q4_three_up(top);
                 if (store) q4_put_three(x, top, to, part_bytes);
                 if (store && lane == 0) scales[b * kTokens + m] = q4_three_scale(top);
             }
             if constexpr (MINIMA) {
-                const float s = q4_group_sum<G>(x);
+                const float s = q4_group_sum<G>(x, up);
                 if (store && lane % (G / 4) == 0) sums[(b * NG + lane / (G / 4)) * kTokens + m] = s;
             }
         });
@@ -994,10 +1003,10 @@ struct Q4Floats {
 #pragma unroll
                     for (int t = 0; t < T; ++t) {
                         const float2 v = *reinterpret_cast<const float2*>(xs + t * 8);
-                        acc[i][4 * t] = fmaf(o0, v.x, acc[i][4 * t]);
-                        acc[i][4 * t + 1] = fmaf(o0, v.y, acc[i][4 * t + 1]);
-                        acc[i][4 * t + 2] = fmaf(o1, v.x, acc[i][4 * t + 2]);
-                        acc[i][4 * t + 3] = fmaf(o1, v.y, acc[i][4 * t + 3]);
+                        part[i][4 * t] = fmaf(o0, v.x, part[i][4 * t]);
+                        part[i][4 * t + 1] = fmaf(o0, v.y, part[i][4 * t + 1]);
+                        part[i][4 * t + 2] = fmaf(o1, v.x, part[i][4 * t + 2]);
+                        part[i][4 * t + 3] = fmaf(o1, v.y, part[i][4 * t + 3]);
                     }
                 }
             }

@@ -788,3 +788,28 @@ def test_sums_near_the_end_of_the_range(cuda, rows, minimum):
         x = np.clip(g.standard_normal((rows, 256)), -1.9, 1.9).astype(np.float32) * np.float32(2.0 ** exponent)
         exact, mag = oracle.mul_mat_exact(d * q + m, x)
         check(host(sdb.mul_mat_q4(w, cuda_tensor(x, cuda))), exact, mag)
+
+
+@pytest.mark.parametrize("kind", ["code", "inside", "below"])
+@pytest.mark.parametrize("rows", [1, 2, 3, 8, 9, 17, 33])
+def test_the_greatest_numbers(cuda, rows, kind):
+    """Numbers up to FP32's greatest, with scales that bring the sums back: no sum of x alone overflows, whether its
+    weight is 0 (no minimum or one that a code meets) or not."""
+    import sdb
+
+    g = rng(rows)
+    n, k, group = 40, 300, 64
+    q, scales, minima, _ = made(g, n, k, group, kind != "code")
+    scales = (g.integers(1, 128, scales.shape) * 2.0 ** -20).astype(np.float16)
+    if kind == "inside":
+        minima = (-scales.astype(np.float64) * g.integers(0, 16, scales.shape)).astype(np.float16)
+    elif kind == "below":
+        minima = (-scales.astype(np.float64) * 24).astype(np.float16)
+    d = np.repeat(scales.astype(np.float64), group, axis=1)[:, :k]
+    m = np.repeat(minima.astype(np.float64), group, axis=1)[:, :k] if minima is not None else -8 * d
+    w = on_device(cuda, q, scales, minima, group)
+    for exponent in (112, 113, 114, 120, 126, 127):
+        x = (g.uniform(1, 1.99, (rows, k)) * g.choice([1.0, 1.0, -1.0], (rows, k)) * 2.0 ** exponent).astype(np.float32)
+        exact, mag = oracle.mul_mat_exact(d * q + m, x)
+        assert mag.max() < 2.0 ** 127
+        check(host(sdb.mul_mat_q4(w, cuda_tensor(x, cuda))), exact, mag)
