@@ -63,19 +63,21 @@ bool chain_ok(const sdb_chain* c, const sdb_tensor* dst, bool gated) {
 // CTAs 28.4; 8 rows: four warps 17.1, eight 17.5), and two matrices, whose sums take the registers, share less
 // (1280 -> 5120, 5 rows: two warps 11.7, one 12.3, eight 12.9; 16 rows at a time: 16 rows with two warps, 32 with one
 // 29.8, with two 36.8).  FP32 rows, three columns each, are taken 16 at a time, FP16 rows 32 (4096 -> 4096: 32 FP32
-// rows 22.1 us, taken at once 43.5, 77 rows 64.6 and 92.9; 77 FP16 rows 41.5).  And where the tiles leave most SMs
+// rows 22.1 us, taken at once 43.5, 77 rows 64.6 and 92.9; 77 FP16 rows 41.5); but 9 to 16 FP32 rows of two long
+// matrices in two runs of eight, whose CTAs hold more of x (4096 -> 11008: 16 rows 62 us, at once 77).  And where the tiles leave most SMs
 // idle, more warps share one (320 -> 1280, two rows: sixteen 4.3 us, eight 4.7).
 Q4Plan plan(const Q4Args& a) {
     Q4Plan p{};
-    p.form = a.rows == 1 ? 1 : a.rows <= 4 && !a.x_half ? (a.rows + 1) / 2 * 2 : a.rows <= 8 ? 8 : a.rows <= 16 || !a.x_half ? 16 : 32;
-    p.shared = kQ4MaxShared;
     const bool gated = a.gate != nullptr;
+    p.form = a.rows == 1 ? 1 : a.rows <= 4 && !a.x_half ? (a.rows + 1) / 2 * 2 : a.rows <= 8 ? 8 : a.rows <= 16 || !a.x_half ? 16 : 32;
+    if (p.form == 16 && gated && !a.x_half && a.rows <= 16 && a.kblocks >= 16) p.form = 8;
+    p.shared = kQ4MaxShared;
     const int warps = p.form <= 16 && !gated ? 16 : 8, runs = (a.rows + p.form - 1) / p.form;
     if (p.form <= 4) {
         p.wk_log = 3;
     } else if (p.form == 8) {
         if (a.kblocks < 16) p.wk_log = gated ? 1 : 2;
-        else if (a.x_half || gated || a.tiles > 2 * current_sm_count()) p.wk_log = 3;
+        else if (a.x_half || gated || a.tiles > 2 * current_sm_count()) p.wk_log = runs > 1 ? 2 : 3;
         else p.cluster_log = 2;
     } else if (a.kblocks >= 16) {
         p.cluster_log = gated ? 1 : 2;

@@ -813,3 +813,46 @@ def test_the_greatest_numbers(cuda, rows, kind):
         exact, mag = oracle.mul_mat_exact(d * q + m, x)
         assert mag.max() < 2.0 ** 127
         check(host(sdb.mul_mat_q4(w, cuda_tensor(x, cuda))), exact, mag)
+
+
+# ---------------------------------------------------------------- rows that are held in parts
+
+@pytest.mark.parametrize("minimum", [False, True])
+@pytest.mark.parametrize("xt", [np.float32, np.float16])
+@pytest.mark.parametrize("rows,k", [(1, 150001), (2, 90000), (2, 28672), (4, 60001), (7, 30000), (8, 28672)])
+def test_long_rows(cuda, rows, k, xt, minimum):
+    """Rows longer than the CTAs of a cluster hold at once, some k-blocks of one row with numbers of 1e-9 beside those
+    of 1: digits and other k-blocks in one sum."""
+    import sdb
+    import torch
+
+    g = rng(k)
+    q, scales, minima, values = made(g, 20, k, 128, minimum)
+    x = g.standard_normal((rows, k))
+    x[:, ::1000] *= 1e-9 if xt == np.float32 else 1e-4
+    x = x.astype(xt)
+    out = torch.full((rows, 20), float("nan"), device=cuda)
+    sdb.mul_mat_q4(on_device(cuda, q, scales, minima, 128), cuda_tensor(x, cuda), out=out)
+    exact, mag = oracle.mul_mat_exact(values, x)
+    check(host(out), exact, mag)
+
+
+@pytest.mark.parametrize("minimum", [False, True])
+@pytest.mark.parametrize("xt", [np.float32, np.float16])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 6, 8, 9, 13, 16])
+def test_gated_long_rows(cuda, rows, xt, minimum):
+    """Two matrices of 16 k-blocks and more: the plan's other side for each form."""
+    import sdb
+    import torch
+
+    g = rng(rows)
+    k, half, group = 2100, 70, 64
+    qa, qb = made(g, half, k, group, minimum), made(g, half, k, group, minimum)
+    x = (g.standard_normal((rows, k)) / np.sqrt(k)).astype(xt)
+    out = torch.full((rows, half), float("nan"), device=cuda)
+    sdb.mul_mat_q4_gated(on_device(cuda, *qa[:3], group), on_device(cuda, *qb[:3], group), cuda_tensor(x, cuda), "silu",
+                         out=out)
+    a, ma = oracle.mul_mat_exact(qa[3], x)
+    b, mb = oracle.mul_mat_exact(qb[3], x)
+    act = b / (1 + np.exp(-b))
+    check(host(out), a * act, ma * np.abs(act) + np.abs(a) * 1.13 * mb)
