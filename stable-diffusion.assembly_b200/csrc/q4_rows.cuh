@@ -19,7 +19,8 @@
 //   bits, read as FP32, are 1.5 * 2^23 + 16 S, and one subtraction makes it a
 //   number (|16 S| < 2^22).  Six digits hold the numbers down to 2^-19 of the
 //   k-block's greatest; a k-block with smaller ones (0 apart), or at the ends of
-//   FP32's range, or with an infinity or a NaN, is taken as below.
+//   FP32's range, or with an infinity or a NaN, is three BF16 columns as below
+//   (a row of nothing else: 8192 -> 28672 45.6 us, of digits 27.3).
 // Pairs (two to four FP32 rows).  A row is the sum of three BF16 columns, each
 //   of which takes the next eight of a number's 24 bits, and none has a range to
 //   fall out of; two rows' columns are six of a product's eight (m16n8k16).  q - z
@@ -30,7 +31,7 @@
 //   which are 2^-8 of them.
 //
 // (Digits unpack a weight in a third of the instructions and take one row of
-// 8192 -> 28672 in 28.6 us where a pair takes 38; two rows' twelve columns would
+// 8192 -> 28672 in 27.6 us where a pair takes 38; two rows' twelve columns would
 // be two products, 43 us for a pair's 42.  Four rows take 56 us in pairs, 70 in
 // a product of eight rows' parts.)
 //
@@ -420,8 +421,8 @@ struct Q4Digits {
 
     // Shared memory of `chunk` k-blocks: the columns; the factor, twice; the scale of a k-block that is not digits,
     // else 0; with a minimum the sums over each group of each column's digits and of x, of a k-block that is not digits
-    // in that scale, apart from the others'.
-    static __host__ __device__ int block_bytes(int, int ng) { return kRow + 12 + 32 * ng; }
+    // in that scale.
+    static __host__ __device__ int block_bytes(int, int ng) { return kRow + 12 + 28 * ng; }
     // What the lanes of columns 6 and 7 read past the last, their factor, and what aligns the sums.
     static constexpr int kTail = 88;
     uint8_t* frags;
@@ -431,7 +432,6 @@ struct Q4Digits {
     float* scales;
     int2* column_sums;  // of a group's three pairs of columns
     float* sums;
-    float* wide_sums;
     __device__ __forceinline__ Q4Digits(const Q4Args& a, uint8_t* x, int, int ng) {
         frags = x;
         factors = reinterpret_cast<float2*>(x + a.chunk * kRow + 80);
@@ -441,7 +441,6 @@ struct Q4Digits {
         scales = reinterpret_cast<float*>(factors + a.chunk);
         column_sums = reinterpret_cast<int2*>(scales + a.chunk + (a.chunk & 1));
         sums = reinterpret_cast<float*>(column_sums + 3 * ng * a.chunk);
-        wide_sums = sums + ng * a.chunk;
     }
 
     // A slice of 32 columns of x is the six columns of its digits, 32 bytes each, a lane's four numbers a word of each.
@@ -487,10 +486,10 @@ struct Q4Digits {
             } else if (store) {
                 q4_put_three(x, top, row, kWide);
             }
-            // The factor is that of column 2, with the weights' 1 / 16: 2^16 2^(e - 147) / 16.  The last two columns
-            // are not there: any bytes are integers, which count nothing, and so for a row that is not digits.
+            // The factor is that of column 2, with the weights' 1 / 16: 2^16 2^(e - 147) / 16.  (The last two columns
+            // are not there: any bytes are integers, and theirs count nothing.)
             if (store && lane == 0) {
-                const float f = wide || top == 0 ? 0.0f : q4_power(e - 135);
+                const float f = out || top == 0 ? 0.0f : q4_power(e - 135);
                 factors[b] = make_float2(f, f);
                 scales[b] = wide ? q4_three_scale(top) : 0.0f;
             }
@@ -507,8 +506,7 @@ struct Q4Digits {
                 }
                 if (store && lane % (G / 4) == 0) {
                     const int at = b * NG + lane / (G / 4);
-                    sums[at] = wide ? 0.0f : s;
-                    wide_sums[at] = s;
+                    sums[at] = s;
 #pragma unroll
                     for (int p = 0; p < 3; ++p) {
                         const int low = static_cast<short>(pairs[p]);
@@ -544,6 +542,8 @@ struct Q4Digits {
                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
     }
 
+    __device__ __forceinline__ bool wide(int at) const { return scales[at] != 0.0f; }
+
     // A k-block that is not digits, its three BF16 columns one product.  Its sums, whole, take the place of column 7,
     // lane (g, 3).
     template <int G, bool MINIMA>
@@ -551,7 +551,6 @@ struct Q4Digits {
         constexpr int NG = 128 / G, SL = 4 / NG;
         const int lane = threadIdx.x & 31;
         const float scale = scales[at];
-        if (scale == 0.0f) return;
         // The lanes of columns past the third read the third's: their sums go nowhere.
         const uint8_t* f = frags + at * kRow + min(lane >> 2, 2) * kWide + (lane & 3) * 8;
 #pragma unroll
@@ -578,7 +577,7 @@ struct Q4Digits {
                 // Lane (g, 0) holds columns 0 and 1, lane (g, 1) column 2, lane (g, 3) what the minima add.
                 const int t = lane & 3;
                 const float part[2] = {t == 0 ? c[0] + c[1] : t == 1 ? c[0] : 0.0f, t == 0 ? c[2] + c[3] : t == 1 ? c[2] : 0.0f};
-                const float x = MINIMA && t == 3 ? wide_sums[at * NG + g] : 0.0f;
+                const float x = MINIMA && t == 3 ? sums[at * NG + g] : 0.0f;
                 sum[0] = fmaf(d.x, part[0], fmaf(zero.o[0], x, sum[0]));
                 sum[1] = fmaf(d.y, part[1], fmaf(zero.o[1], x, sum[1]));
             }
@@ -824,6 +823,7 @@ struct Q4Pairs {
                 for (int c = 0; c < 4; ++c) acc[i][t][c] = fmaf(c & 1 ? v.y : v.x, part[i][t][c], acc[i][t][c]);
         }
     }
+    __device__ __forceinline__ bool wide(int) const { return false; }
     template <int G, bool MINIMA>
     __device__ __forceinline__ void wide_product(const Q4Stage<G> (&)[kTiles], int) {}
 
@@ -1022,6 +1022,7 @@ struct Q4Floats {
                     acc[i][4 * t + c] = fmaf(c & 1 ? v.y : v.x, part[i][4 * t + c], acc[i][4 * t + c]);
         }
     }
+    __device__ __forceinline__ bool wide(int) const { return false; }
     template <int G, bool MINIMA>
     __device__ __forceinline__ void wide_product(const Q4Stage<G> (&)[kTiles], int) {}
 
@@ -1063,7 +1064,7 @@ int q4_fixed_bytes(int block) {
 }
 
 // MINIMA: compiled for itself, so that the products of two k-blocks lie side by side without a branch between (one
-// row of 8192 -> 28672 without a minimum 28.6 us, with the choice made in the loop 31.8).
+// row of 8192 -> 28672 without a minimum 27.6 us, with the choice made in the loop 31.8).
 template <class F, int G, bool MINIMA>
 __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __grid_constant__ Q4Args a) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -1171,16 +1172,17 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
                     auto one = [&](int i) {
                         staged(i, [&](auto& stage, int k) { form.template product<G, MINIMA>(stage, k); });
                     };
-                    if (F::kRun == 2 && count == 2) {  // two k-blocks' chains of products side by side
+                    if (F::kWideRows && wide) {
+#pragma unroll 1
+                        for (int i = 0; i < count; ++i) {
+                            if (!form.wide(at + i)) one(i);
+                            else staged(i, [&](auto& stage, int k) { form.template wide_product<G, MINIMA>(stage, k); });
+                        }
+                    } else if (F::kRun == 2 && count == 2) {  // two k-blocks' chains of products side by side
                         one(0);
                         one(1);
                     } else if (count > 0) {
                         one(0);
-                    }
-                    if (F::kWideRows && wide) {
-#pragma unroll 1
-                        for (int i = 0; i < count; ++i)
-                            staged(i, [&](auto& stage, int k) { form.template wide_product<G, MINIMA>(stage, k); });
                     }
                     __syncwarp();  // every lane has read its part
                     if (lane == 0) mbar_arrive(empty + place);
