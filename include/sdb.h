@@ -122,7 +122,7 @@ int64_t sdb_q4_bytes(int64_t k, int64_t n, int32_t group, int32_t minimum);
  *   minimum: d = f16((max - min) / 15), m = f16(min),
  *     q = clamp(floor((w - m) / d + 0.5), 0, 15), 0 where d = 0;
  * in FP32, each operation rounded; d and m saturate at FP16's range.  A group
- * that holds an infinity or a NaN stands for NaN. */
+ * that holds an infinity or a NaN, a short last one too, stands for NaN. */
 int sdb_q4_quantize(const sdb_tensor *w, const sdb_q4 *q, void *stream);
 /* From 4-bit numbers and their scales: codes [n][(k + 1) / 2] bytes, the even
  * column in the low half; scales (and minima, else NULL) [n][ceil(k / group)]
@@ -137,10 +137,13 @@ int sdb_q4_dequantize(const sdb_q4 *q, const sdb_tensor *w, void *stream);
 /* dst[m][n] = sum_k x[m][k] value[n][k], then the chain: sdb_mul_mat for 4-bit
  * weights and few rows (for hundreds of rows, sdb_q4_dequantize once and
  * sdb_mul_mat).  x [K, ...] and dst [N, ...] FP32 or FP16, each row contiguous,
- * rows (at most 2^20) over dimensions 1..3 at any strides; x and dst do not overlap.  Products
- * and sums are FP32 whatever the types (x to its last bit), dst rounded once.
- * A row of x that holds an infinity or a NaN gives numbers that are not finite,
- * and no other row does.  A chain's redirect needs an FP32 dst.  No rows: nothing is done.  No device
+ * rows (at most 2^20) over dimensions 1..3 at any strides; x and dst do not
+ * overlap.  x enters the products to its last bit, whatever its row holds (but
+ * that in 128 numbers that reach 2^72, those below 2^-86 may lose bits), and a
+ * weight of 0 adds 0; sums are FP32 whatever the types, dst rounded once: off by
+ * at most 1e-6 of the summed magnitudes |x value|.  A row of x that holds an
+ * infinity or a NaN gives numbers that are not finite, and no other row does.  A
+ * chain's redirect needs an FP32 dst.  No rows: nothing is done.  No device
  * memory is allocated and none is shared between calls. */
 int sdb_mul_mat_q4_supported(const sdb_q4 *w, const sdb_tensor *x, const sdb_tensor *dst);
 int sdb_mul_mat_q4(const sdb_q4 *w, const sdb_tensor *x, const sdb_tensor *dst, const sdb_chain *chain,
@@ -251,7 +254,8 @@ int sdb_mul_mat_gated_layer_normed(const sdb_tensor *w, const sdb_tensor *x, con
  * [C, ...], FP32 or FP16, h of x's type and out of y's, rows contiguous at any
  * strides.  h and out may be the very memory of x or y (same type and strides);
  * they overlap nothing else.  Arithmetic in FP32, a row's statistics over the
- * numbers themselves (out is made from h before h is rounded). */
+ * numbers themselves (out is made from h before h is rounded); a NaN in a row
+ * makes all of its norm NaN, and no other row's. */
 enum { SDB_NORM_NONE = 0, SDB_NORM_LAYER = 1, SDB_NORM_RMS = 2 };
 /* (v - mean) / sqrt(variance + eps), or v / sqrt(mean of v^2 + eps); then
  * weight [C] and bias [C], each unless NULL. */

@@ -12,7 +12,8 @@ normalised magnitudes.  Sums over a row are FP32, at most a few hundred numbers
 a thread and a tree: the variance's error, random in sign, is far inside the 16.
 A LayerNorm's mean is off by a number of its own, which counts where a number is
 near the mean: a sum of c numbers d of depth s (c / 256 numbers a thread and the
-tree over a CTA, or c / 32 <= 40 and the tree over a warp) errs by at most
+tree over a CTA where a row is read again, at most 32 numbers and the tree over a
+warp or a CTA where it is in registers) errs by at most
 s u sum |d|, the mean so by s u mean |d| <= s u sigma: s u of the normalised
 numbers, s = max(48, c / 256 + 16).  A half precision output adds 2^-11 of its
 value (2^-25 below the normal numbers).
