@@ -15,12 +15,12 @@
 //   each: six columns of an integer product (m16n8k32, s8 x s8).  A nibble at
 //   the top of its byte is the operand 16 (q - 8): three instructions unpack
 //   eight weights (8 - z times a column's sum makes them q - z).  The sum is
-//   exact; it starts from 0x4b400000, so that its
-//   bits, read as FP32, are 1.5 * 2^23 + 16 S, and one subtraction makes it a
-//   number (|16 S| < 2^22).  Six digits hold the numbers down to 2^-19 of the
-//   k-block's greatest; a k-block with smaller ones (0 apart), or at the ends of
-//   FP32's range, or with an infinity or a NaN, is three BF16 columns as below
-//   (a row of nothing else: 8192 -> 28672 45.6 us, of digits 27.3).
+//   exact; it starts from 0x4b400000, so that its bits, read as FP32, are
+//   1.5 * 2^23 + 16 S, and one subtraction makes it a number (|16 S| < 2^22).
+//   Six digits hold the numbers down to 2^-19 of the k-block's greatest; a
+//   k-block with smaller ones (0 apart), or at the ends of FP32's range, or with
+//   an infinity or a NaN, is three BF16 columns as below (a row of nothing else:
+//   8192 -> 28672 45.6 us, of digits 27.3).
 // Pairs (two to four FP32 rows).  A row is the sum of three BF16 columns, each
 //   of which takes the next eight of a number's 24 bits, and none has a range to
 //   fall out of; two rows' columns are six of a product's eight (m16n8k16).  q - z
@@ -382,7 +382,6 @@ __device__ __forceinline__ void q4_put_three(float4 x, uint32_t top, uint8_t* to
         }
     }
 }
-
 
 // ---- one row, as digits: six of a product's eight columns
 
@@ -823,10 +822,6 @@ struct Q4Pairs {
                 for (int c = 0; c < 4; ++c) acc[i][t][c] = fmaf(c & 1 ? v.y : v.x, part[i][t][c], acc[i][t][c]);
         }
     }
-    __device__ __forceinline__ bool wide(int) const { return false; }
-    template <int G, bool MINIMA>
-    __device__ __forceinline__ void wide_product(const Q4Stage<G> (&)[kTiles], int) {}
-
     // The lane's sum c of tile i: row lane / 4 (lane odd: + 8) of row 2 c + (lane / 2) % 2 of x, over its parts' lanes.
     __device__ __forceinline__ float lane_sum(int i, int c) const {
         const int lane = threadIdx.x & 31;
@@ -1022,10 +1017,6 @@ struct Q4Floats {
                     acc[i][4 * t + c] = fmaf(c & 1 ? v.y : v.x, part[i][4 * t + c], acc[i][4 * t + c]);
         }
     }
-    __device__ __forceinline__ bool wide(int) const { return false; }
-    template <int G, bool MINIMA>
-    __device__ __forceinline__ void wide_product(const Q4Stage<G> (&)[kTiles], int) {}
-
     __device__ __forceinline__ float lane_sum(int i, int c) const { return acc[i][c]; }
     static __device__ __forceinline__ int row_of(int c, int lane) { return (lane >> 2) + 4 * (c & 2); }
     static __device__ __forceinline__ int token_of(int c, int lane) { return c / 4 * 8 + (lane & 3) * 2 + (c & 1); }
@@ -1172,16 +1163,19 @@ __global__ void __launch_bounds__(q4_threads<F>(), 1) q4_rows_kernel(const __gri
                     auto one = [&](int i) {
                         staged(i, [&](auto& stage, int k) { form.template product<G, MINIMA>(stage, k); });
                     };
-                    if (F::kWideRows && wide) {
+                    bool apart = false;  // each k-block by itself
+                    if constexpr (F::kWideRows) {
+                        apart = wide;
 #pragma unroll 1
-                        for (int i = 0; i < count; ++i) {
+                        for (int i = 0; apart && i < count; ++i) {
                             if (!form.wide(at + i)) one(i);
                             else staged(i, [&](auto& stage, int k) { form.template wide_product<G, MINIMA>(stage, k); });
                         }
-                    } else if (F::kRun == 2 && count == 2) {  // two k-blocks' chains of products side by side
+                    }
+                    if (!apart && F::kRun == 2 && count == 2) {  // two k-blocks' chains of products side by side
                         one(0);
                         one(1);
-                    } else if (count > 0) {
+                    } else if (!apart && count > 0) {
                         one(0);
                     }
                     __syncwarp();  // every lane has read its part
