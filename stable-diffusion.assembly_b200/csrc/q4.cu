@@ -2,7 +2,7 @@
 // scales, or from ggml's Q4_0 / Q4_1 blocks, and turned back into FP32.
 //
 // All four are one pass over the matrix, a lane to a word of eight columns
-// (q4.cuh), bound by memory.
+// (q4.cuh), bound by memory; quantizing by its instructions.
 #include <cuda_runtime.h>
 
 #include <algorithm>
